@@ -52,11 +52,14 @@ enum trc_hip_status {
 /* ggml type ids used by this ABI (include/traincpp/trc_types.h:11-49). */
 enum trc_hip_type {
     TRC_HIP_TYPE_F32  = 0,
+    TRC_HIP_TYPE_F16  = 1,
     TRC_HIP_TYPE_Q4_0 = 2,
     TRC_HIP_TYPE_Q4_1 = 3,
     TRC_HIP_TYPE_Q5_0 = 6,
     TRC_HIP_TYPE_Q5_1 = 7,
-    TRC_HIP_TYPE_Q8_0 = 8
+    TRC_HIP_TYPE_Q8_0 = 8,
+    TRC_HIP_TYPE_I32  = 26,
+    TRC_HIP_TYPE_BF16 = 30
 };
 
 /* Largest activation batch (columns of src1) the fused quantized matvec takes
@@ -291,6 +294,130 @@ int trc_hip_acc_f32(const trc_hip_tensor* a, const trc_hip_tensor* b, const trc_
  * each output is summed from 0 in a's linear element order, so the result is
  * bit-identical to the CPU's. F32 only. */
 int trc_hip_repeat_back_f32(const trc_hip_tensor* a, const trc_hip_tensor* dst, void* stream);
+
+/* ------------------------------------------------------------------ tuning
+ *
+ * What it takes to tune low-rank adapters on weights that stay as they were loaded:
+ * the adapters beside a projection and their gradients, the preference loss and its
+ * gradient, and the step that updates the tensors. The reference trains through
+ * graphs of single ops and has no counterpart of the first two; the step is its AdamW. */
+
+/* Largest rank of an adapter. */
+#define TRC_HIP_LORA_MAX_RANK 256
+
+/* n adapters of one projection and the requests of one batch that use them. */
+typedef struct trc_hip_lora_set {
+    trc_hip_tensor a;       /* [K, R, n] F32, F16 or BF16; nb[0] is the element size, nb[1] and nb[2] any */
+    trc_hip_tensor b;       /* [R, M, n] of a's type, likewise                                             */
+    trc_hip_tensor scale;   /* [n] F32, contiguous: the factor on each adapter's product                   */
+    trc_hip_tensor start;   /* [requests + 1] I32, contiguous: request q holds tokens start[q] up to
+                             * start[q+1] - 1 (none, where they are equal); from 0 to the number of tokens,
+                             * never falling                                                               */
+    trc_hip_tensor adapter; /* [requests] I32, contiguous: the adapter of each request; outside 0 .. n-1: none */
+} trc_hip_lora_set;
+
+/* Adapters of many requests at once, added to the output of the projection they share:
+ *   h[:,t] = A x[:,t]      dst[:,t] = base[:,t] + scale B h[:,t]
+ * with A, B and scale of the adapter of token t's request. x is [K, T], base and dst
+ * [M, T], h [R, T] contiguous; all F32 with nb[0] = 4 and rows at any 4-byte aligned stride
+ * that keeps the written ones apart. base may be NULL (zeros) or dst itself. A token without
+ * an adapter gets dst = base and h = 0. h is what trc_hip_lora_back needs of this call.
+ * Sums are in 32 bits on the F32 matrix instructions, adapters in 16 bits widened, in an order
+ * that only the sizes decide: the same from run to run. A batch of few tokens keeps partial sums in the
+ * stream's workspace of trc_hip_qmatvec, which the first such call on a stream
+ * allocates (make it before capturing that stream in global mode). start and adapter are read
+ * on the device; wrong values in them give wrong results, and no access outside the tensors. */
+int trc_hip_lora(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc_hip_tensor* base,
+                 const trc_hip_tensor* h, const trc_hip_tensor* dst, void* stream);
+
+/* The gradients of trc_hip_lora for dy [M, T], with x and h of that call:
+ *   g[:,t] = scale B^T dy[:,t]      dx[:,t] = base[:,t] + A^T g[:,t]
+ *   da = sum over an adapter's tokens of g x^T ([K, R, n]), db = scale sum of dy h^T ([R, M, n])
+ * g is [R, T] contiguous and scratch of the caller's. base (the gradient through the shared
+ * projection) may be NULL (zeros) or dx itself; dx may be NULL where nothing before the
+ * projection is trained (then base has to be NULL too). da and db are F32 whatever the adapters'
+ * type, with nb[0] = 4; accumulate != 0 adds to them, as a graph's gradient accumulators
+ * want it, 0 overwrites them. An adapter without tokens has gradients of 0. The sums' order is
+ * fixed by the sizes and requests: no atomics. */
+int trc_hip_lora_back(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc_hip_tensor* h,
+                      const trc_hip_tensor* dy, const trc_hip_tensor* g, const trc_hip_tensor* base,
+                      const trc_hip_tensor* dx, const trc_hip_tensor* da, const trc_hip_tensor* db,
+                      int accumulate, void* stream);
+
+/* The loss that ranks a chosen answer above a rejected one, for P pairs of sequences.
+ * logits is [V, T] of F32, F16 or BF16 (nb[0] the element size, rows at any aligned
+ * stride), labels [T] I32: the token each row predicts; a negative label is not counted
+ * (a prompt's token, padding), and its row is not read. Sequence s is rows start[s]
+ * up to start[s+1] - 1 of start [2P + 1] I32; pair i is sequences 2i (chosen) and 2i + 1
+ * (rejected). ref [2P] F32 holds the reference model's logp. Then
+ *   lse[t] = log sum_v exp(logits[v,t])              logp[s] = sum of logits[label,t] - lse[t]
+ *   z_i = beta ((logp - ref)[2i] - (logp - ref)[2i+1])
+ *   loss[0] = mean_i -(1 - smoothing) log sigma(z_i) - smoothing log sigma(-z_i)
+ * and slope [P] is the loss's derivative by each z, before the mean. lse is [T] F32 (0 for
+ * rows not counted), logp [2P], slope [P], loss [1]; lse and slope are what trc_hip_preference_loss_back
+ * needs. All vectors contiguous. smoothing is in 0 .. 1. Rows are summed in 32 bits, sequences and
+ * pairs in 64, in a fixed order. A logit of -inf is a token that cannot occur; a label of V or
+ * more makes the loss NaN. Few rows keep partial sums in the stream's workspace (see
+ * trc_hip_lora). */
+int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* start,
+                            const trc_hip_tensor* ref, float beta, float smoothing, const trc_hip_tensor* lse,
+                            const trc_hip_tensor* logp, const trc_hip_tensor* slope, const trc_hip_tensor* loss,
+                            void* stream);
+
+/* The logits' gradient of trc_hip_preference_loss, for dloss [1] F32:
+ *   dlogits[v,t] = dloss (+-beta / P) slope_i (1[v = label_t] - exp(logits[v,t] - lse[t]))
+ * (+ for the chosen sequence), and 0 for rows that are not counted or in no sequence, whatever
+ * their logits hold. dlogits has logits' type and shape and may be logits itself. */
+int trc_hip_preference_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels,
+                                 const trc_hip_tensor* start, const trc_hip_tensor* lse,
+                                 const trc_hip_tensor* slope, const trc_hip_tensor* dloss, float beta,
+                                 const trc_hip_tensor* dlogits, void* stream);
+
+/* Elements that share a scale where AdamW's moments are held in 8 bits. */
+#define TRC_HIP_ADAMW_BLOCK 256
+
+/* One tensor of an AdamW step: n contiguous elements. */
+typedef struct trc_hip_adamw_tensor {
+    float*      param;
+    const void* grad;
+    void*       m;         /* moments: float with 32 bits; with 8, int8_t (m) and uint8_t (v), n of each */
+    void*       v;
+    float*      m_scale;   /* with 8 bits: ceil(n / TRC_HIP_ADAMW_BLOCK) scales each; else unused       */
+    float*      v_scale;
+    float*      m_out;     /* where trc_hip_adamw_moments writes n floats each, or NULL                 */
+    float*      v_out;
+    int64_t     n;         /* 0 is allowed                                                              */
+    float       decay;     /* factor on the weight decay: 1, or 0 for biases and norms                  */
+    int32_t     grad_type; /* TRC_HIP_TYPE_F32, _F16 or _BF16                                           */
+} trc_hip_adamw_tensor;
+
+typedef struct trc_hip_adamw_hyper {
+    double  lr, beta1, beta2, eps, weight_decay;
+    double  grad_scale; /* every gradient is multiplied by it first (1, or what unscales or clips it) */
+    int64_t step;       /* counts from 1 */
+} trc_hip_adamw_hyper;
+
+/* A plan of AdamW steps over `count` tensors, with moments of 32 or 8 bits. The
+ * descriptions are copied to the current device, the tensors stay the caller's: their
+ * addresses must hold until trc_hip_adamw_destroy, and no two may overlap. Moments start as
+ * zeros (scales too). Allocates; not for a stream under capture. */
+int trc_hip_adamw_create(const trc_hip_adamw_tensor* tensors, int64_t count, int bits, void** plan);
+
+/* One step over every tensor of the plan, in one launch:
+ *   m = beta1 m + (1 - beta1) g          v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * The step of the reference's AdamW (src/optim/trc_optim.cpp). With 8 bits, the parameters
+ * are updated from this step's moments in 32 bits, which are then held as codes of a block's
+ * largest magnitude: m = m_scale sign(c) (c / 127)^2 and sqrt(v) = v_scale (c / 255)^2, rounded to
+ * nearest and never to 0 where v is above 0. A block that meets a value that is not finite stays so.
+ * A captured step keeps its hyper-parameters, the step's number among them. */
+int trc_hip_adamw_step(void* plan, const trc_hip_adamw_hyper* hyper, void* stream);
+
+/* The moments of every tensor as floats (m and v, not sqrt(v)), into m_out and v_out. */
+int trc_hip_adamw_moments(void* plan, void* stream);
+
+/* Frees the plan (not the tensors), after its work: synchronize first. NULL is allowed. */
+int trc_hip_adamw_destroy(void* plan);
 
 #ifdef __cplusplus
 }

@@ -34,8 +34,8 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
-# Per-file extras. Dequantization must round every * and + on its own.
-HIP_FILE_FLAGS = {"dequant.hip": ["-ffp-contract=off"]}
+# Per-file extras. Dequantization and the optimizer's step must round every * and + on its own.
+HIP_FILE_FLAGS = {"dequant.hip": ["-ffp-contract=off"], "adamw.hip": ["-ffp-contract=off"]}
 
 CXX = os.environ.get("CXX", "g++")
 # -ffp-contract=off: the host dequantizer (core/gguf.cpp) rounds d*q and +m on their own.

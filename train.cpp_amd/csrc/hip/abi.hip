@@ -1,12 +1,14 @@
 // extern "C" entry points of libtrc_hip.so (declared in include/trc_hip_abi.h):
 // argument validation, error reporting and the HIP runtime calls. Kernels live
-// in dequant.hip, qmatvec.hip, qmm.hip, mul_mat.hip, elementwise.hip and copy.hip.
+// in dequant.hip, qmatvec.hip, qmm.hip, mul_mat.hip, elementwise.hip, copy.hip, lora.hip,
+// preference.hip and adamw.hip.
 #include "common.h"
 
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <new>
 
 namespace trc_hip {
 
@@ -406,6 +408,251 @@ int trc_hip_repeat_back_f32(const trc_hip_tensor* a, const trc_hip_tensor* dst, 
     if (a == nullptr || dst == nullptr) return fail(TRC_HIP_E_INVALID, "trc_hip_repeat_back_f32: NULL tensor");
     if (a->data == nullptr || dst->data == nullptr) return fail(TRC_HIP_E_INVALID, "trc_hip_repeat_back_f32: NULL data");
     return launch_repeat_back_f32(*a, *dst, (hipStream_t) stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+// The bytes a tensor covers, from its first element to its last.
+struct Span {
+    uintptr_t lo, hi;
+};
+Span span_of(const trc_hip_tensor& t) {
+    Span s{(uintptr_t) t.data, (uintptr_t) t.data + basic_type_size(t.type)};
+    for (int i = 0; i < 4; ++i) s.hi += (uintptr_t) (t.ne[i] - 1) * t.nb[i];
+    return s;
+}
+
+// A tensor of `type` and shape ne0 x ne1 x ne2 x 1, its elements side by side along ne0;
+// `apart`: its rows and planes do not overlap (it is written).
+int check_shape(const char* who, const char* name, const trc_hip_tensor* t, int type, int64_t ne0, int64_t ne1, int64_t ne2,
+                bool apart) {
+    if (t == nullptr) return fail(TRC_HIP_E_INVALID, "%s: %s is NULL", who, name);
+    const size_t es = basic_type_size(type);
+    if (t->type != type) return fail(TRC_HIP_E_INVALID, "%s: %s has type %d, not %d", who, name, t->type, type);
+    if (t->ne[0] != ne0 || t->ne[1] != ne1 || t->ne[2] != ne2 || t->ne[3] != 1) {
+        return fail(TRC_HIP_E_SHAPE, "%s: %s is [%lld,%lld,%lld,%lld], not [%lld,%lld,%lld,1]", who, name,
+                    (long long) t->ne[0], (long long) t->ne[1], (long long) t->ne[2], (long long) t->ne[3], (long long) ne0,
+                    (long long) ne1, (long long) ne2);
+    }
+    if (t->data == nullptr || (uintptr_t) t->data % es != 0) {
+        return fail(TRC_HIP_E_ALIGN, "%s: %s's data must be non-NULL and %zu-byte aligned", who, name, es);
+    }
+    if ((ne0 > 1 && t->nb[0] != es) || (ne1 > 1 && t->nb[1] % es != 0) || (ne2 > 1 && t->nb[2] % es != 0)) {
+        return fail(TRC_HIP_E_ALIGN, "%s: %s's strides must be whole elements, and neighbours along ne[0]", who, name);
+    }
+    if (apart && ((ne1 > 1 && t->nb[1] < (size_t) ne0 * es) || (ne2 > 1 && t->nb[2] < (size_t) (ne1 - 1) * t->nb[1] + (size_t) ne0 * es))) {
+        return fail(TRC_HIP_E_SHAPE, "%s: rows of %s overlap", who, name);
+    }
+    return TRC_HIP_OK;
+}
+
+// What is written may share no byte with another operand, unless they are the same view.
+int check_apart(const char* who, const trc_hip_tensor* out, const char* name, const trc_hip_tensor* other,
+                const char* other_name, bool same_is_fine) {
+    if (out == nullptr || other == nullptr) return TRC_HIP_OK;
+    const Span a = span_of(*out), b = span_of(*other);
+    if (a.lo >= b.hi || b.lo >= a.hi) return TRC_HIP_OK;
+    if (same_is_fine && out->data == other->data && (out->ne[1] == 1 || out->nb[1] == other->nb[1])) return TRC_HIP_OK;
+    return fail(TRC_HIP_E_SHAPE, "%s: %s overlaps %s", who, name, other_name);
+}
+
+#define TRC_TRY(call)                             \
+    do {                                          \
+        const int trc_rc = (call);                \
+        if (trc_rc != TRC_HIP_OK) return trc_rc;  \
+    } while (0)
+
+bool is_float(int type) {
+    return type == TRC_HIP_TYPE_F32 || type == TRC_HIP_TYPE_F16 || type == TRC_HIP_TYPE_BF16;
+}
+
+// The rules that trc_hip_lora and trc_hip_lora_back share; T is the batch's tokens.
+int check_lora_set(const char* who, const trc_hip_lora_set* set, int64_t T) {
+    const trc_hip_tensor &a = set->a, &b = set->b;
+    if (!is_float(a.type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of a is not F32, F16 or BF16", who, a.type);
+    const int64_t K = a.ne[0], R = a.ne[1], n = a.ne[2], M = b.ne[1], requests = set->adapter.ne[0];
+    if (K <= 0 || M <= 0 || T <= 0 || n <= 0 || n > 65535 || requests <= 0 || R <= 0 || R > TRC_HIP_LORA_MAX_RANK ||
+        requests > INT32_MAX || T > INT32_MAX || K > INT32_MAX || M > ((int64_t) 1 << 24) || K > ((int64_t) 1 << 24)) {
+        return fail(TRC_HIP_E_SHAPE,
+                    "%s: K = %lld, M = %lld, T = %lld, rank %lld (at most %d), %lld adapters, %lld requests", who,
+                    (long long) K, (long long) M, (long long) T, (long long) R, TRC_HIP_LORA_MAX_RANK, (long long) n,
+                    (long long) requests);
+    }
+    TRC_TRY(check_shape(who, "a", &a, a.type, K, R, n, false));
+    TRC_TRY(check_shape(who, "b", &b, a.type, R, M, n, false));
+    TRC_TRY(check_shape(who, "scale", &set->scale, TRC_HIP_TYPE_F32, n, 1, 1, false));
+    TRC_TRY(check_shape(who, "start", &set->start, TRC_HIP_TYPE_I32, requests + 1, 1, 1, false));
+    return check_shape(who, "adapter", &set->adapter, TRC_HIP_TYPE_I32, requests, 1, 1, false);
+}
+
+int check_lora_out(const char* who, const trc_hip_lora_set* set, const trc_hip_tensor* out, const char* name) {
+    TRC_TRY(check_apart(who, out, name, &set->a, "a", false));
+    TRC_TRY(check_apart(who, out, name, &set->b, "b", false));
+    TRC_TRY(check_apart(who, out, name, &set->scale, "scale", false));
+    TRC_TRY(check_apart(who, out, name, &set->start, "start", false));
+    return check_apart(who, out, name, &set->adapter, "adapter", false);
+}
+
+// A contiguous vector or matrix: rows back to back.
+int check_packed(const char* who, const char* name, const trc_hip_tensor* t) {
+    if (t->ne[1] > 1 && t->nb[1] != (size_t) t->ne[0] * basic_type_size(t->type)) {
+        return fail(TRC_HIP_E_SHAPE, "%s: %s must be contiguous", who, name);
+    }
+    return TRC_HIP_OK;
+}
+
+// The rules that the preference loss and its gradient share.
+int check_preference(const char* who, const trc_hip_tensor* logits, const trc_hip_tensor* labels,
+                     const trc_hip_tensor* start, const trc_hip_tensor* lse, const trc_hip_tensor* slope, float beta) {
+    if (logits == nullptr || slope == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL tensor", who);
+    if (!is_float(logits->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of logits is not F32, F16 or BF16", who, logits->type);
+    const int64_t V = logits->ne[0], T = logits->ne[1], P = slope->ne[0];
+    if (V <= 0 || V > INT32_MAX || T <= 0 || T > INT32_MAX || P <= 0 || P > INT32_MAX / 2) {
+        return fail(TRC_HIP_E_SHAPE, "%s: V = %lld, T = %lld, %lld pairs", who, (long long) V, (long long) T, (long long) P);
+    }
+    if (!(beta == beta)) return fail(TRC_HIP_E_INVALID, "%s: beta is NaN", who);
+    TRC_TRY(check_shape(who, "logits", logits, logits->type, V, T, 1, false));
+    TRC_TRY(check_shape(who, "labels", labels, TRC_HIP_TYPE_I32, T, 1, 1, false));
+    TRC_TRY(check_shape(who, "start", start, TRC_HIP_TYPE_I32, 2 * P + 1, 1, 1, false));
+    TRC_TRY(check_shape(who, "lse", lse, TRC_HIP_TYPE_F32, T, 1, 1, false));
+    return check_shape(who, "slope", slope, TRC_HIP_TYPE_F32, P, 1, 1, false);
+}
+
+}  // namespace
+
+extern "C" {
+
+int trc_hip_lora(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc_hip_tensor* base, const trc_hip_tensor* h,
+                 const trc_hip_tensor* dst, void* stream) {
+    const char* const who = "trc_hip_lora";
+    TRC_FORCED("trc_hip_lora");
+    if (set == nullptr || x == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL argument", who);
+    const int64_t K = set->a.ne[0], R = set->a.ne[1], M = set->b.ne[1], T = x->ne[1];
+    TRC_TRY(check_lora_set(who, set, T));
+    TRC_TRY(check_shape(who, "x", x, TRC_HIP_TYPE_F32, K, T, 1, false));
+    TRC_TRY(check_shape(who, "h", h, TRC_HIP_TYPE_F32, R, T, 1, true));
+    TRC_TRY(check_packed(who, "h", h));
+    TRC_TRY(check_shape(who, "dst", dst, TRC_HIP_TYPE_F32, M, T, 1, true));
+    if (base != nullptr) TRC_TRY(check_shape(who, "base", base, TRC_HIP_TYPE_F32, M, T, 1, false));
+    TRC_TRY(check_lora_out(who, set, h, "h"));
+    TRC_TRY(check_lora_out(who, set, dst, "dst"));
+    TRC_TRY(check_apart(who, h, "h", x, "x", false));
+    TRC_TRY(check_apart(who, h, "h", base, "base", false));
+    TRC_TRY(check_apart(who, dst, "dst", x, "x", false));
+    TRC_TRY(check_apart(who, dst, "dst", h, "h", false));
+    TRC_TRY(check_apart(who, dst, "dst", base, "base", true));
+    return launch_lora(*set, *x, base, *h, *dst, (hipStream_t) stream);
+}
+
+int trc_hip_lora_back(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc_hip_tensor* h, const trc_hip_tensor* dy,
+                      const trc_hip_tensor* g, const trc_hip_tensor* base, const trc_hip_tensor* dx, const trc_hip_tensor* da,
+                      const trc_hip_tensor* db, int accumulate, void* stream) {
+    const char* const who = "trc_hip_lora_back";
+    TRC_FORCED("trc_hip_lora_back");
+    if (set == nullptr || x == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL argument", who);
+    const int64_t K = set->a.ne[0], R = set->a.ne[1], n = set->a.ne[2], M = set->b.ne[1], T = x->ne[1];
+    TRC_TRY(check_lora_set(who, set, T));
+    TRC_TRY(check_shape(who, "x", x, TRC_HIP_TYPE_F32, K, T, 1, false));
+    TRC_TRY(check_shape(who, "h", h, TRC_HIP_TYPE_F32, R, T, 1, false));
+    TRC_TRY(check_packed(who, "h", h));
+    TRC_TRY(check_shape(who, "dy", dy, TRC_HIP_TYPE_F32, M, T, 1, false));
+    TRC_TRY(check_shape(who, "g", g, TRC_HIP_TYPE_F32, R, T, 1, true));
+    TRC_TRY(check_packed(who, "g", g));
+    if (dx != nullptr) TRC_TRY(check_shape(who, "dx", dx, TRC_HIP_TYPE_F32, K, T, 1, true));
+    if (base != nullptr) {
+        if (dx == nullptr) return fail(TRC_HIP_E_INVALID, "%s: base without dx", who);
+        TRC_TRY(check_shape(who, "base", base, TRC_HIP_TYPE_F32, K, T, 1, false));
+    }
+    TRC_TRY(check_shape(who, "da", da, TRC_HIP_TYPE_F32, K, R, n, true));
+    TRC_TRY(check_shape(who, "db", db, TRC_HIP_TYPE_F32, R, M, n, true));
+    const trc_hip_tensor* const outs[4] = {g, dx, da, db};
+    const char* const names[4] = {"g", "dx", "da", "db"};
+    for (int i = 0; i < 4; ++i) {
+        if (outs[i] == nullptr) continue;
+        TRC_TRY(check_lora_out(who, set, outs[i], names[i]));
+        TRC_TRY(check_apart(who, outs[i], names[i], x, "x", false));
+        TRC_TRY(check_apart(who, outs[i], names[i], h, "h", false));
+        TRC_TRY(check_apart(who, outs[i], names[i], dy, "dy", false));
+        TRC_TRY(check_apart(who, outs[i], names[i], base, "base", outs[i] == dx));
+        for (int j = i + 1; j < 4; ++j) TRC_TRY(check_apart(who, outs[i], names[i], outs[j], names[j], false));
+    }
+    return launch_lora_back(*set, *x, *h, *dy, *g, base, dx, *da, *db, accumulate != 0, (hipStream_t) stream);
+}
+
+int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* start,
+                            const trc_hip_tensor* ref, float beta, float smoothing, const trc_hip_tensor* lse,
+                            const trc_hip_tensor* logp, const trc_hip_tensor* slope, const trc_hip_tensor* loss,
+                            void* stream) {
+    const char* const who = "trc_hip_preference_loss";
+    TRC_FORCED("trc_hip_preference_loss");
+    TRC_TRY(check_preference(who, logits, labels, start, lse, slope, beta));
+    const int64_t P = slope->ne[0];
+    if (!(smoothing >= 0.f && smoothing <= 1.f)) return fail(TRC_HIP_E_INVALID, "%s: smoothing %g is not in 0 .. 1", who, smoothing);
+    TRC_TRY(check_shape(who, "ref", ref, TRC_HIP_TYPE_F32, 2 * P, 1, 1, false));
+    TRC_TRY(check_shape(who, "logp", logp, TRC_HIP_TYPE_F32, 2 * P, 1, 1, false));
+    TRC_TRY(check_shape(who, "loss", loss, TRC_HIP_TYPE_F32, 1, 1, 1, false));
+    const trc_hip_tensor* const all[8] = {lse, logp, slope, loss, logits, labels, start, ref};
+    const char* const names[8] = {"lse", "logp", "slope", "loss", "logits", "labels", "start", "ref"};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = i + 1; j < 8; ++j) TRC_TRY(check_apart(who, all[i], names[i], all[j], names[j], false));
+    }
+    return launch_preference_loss(*logits, (const int32_t*) labels->data, (const int32_t*) start->data, P,
+                                  (const float*) ref->data, beta, smoothing, (float*) lse->data, (float*) logp->data,
+                                  (float*) slope->data, (float*) loss->data, (hipStream_t) stream);
+}
+
+int trc_hip_preference_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* start,
+                                 const trc_hip_tensor* lse, const trc_hip_tensor* slope, const trc_hip_tensor* dloss,
+                                 float beta, const trc_hip_tensor* dlogits, void* stream) {
+    const char* const who = "trc_hip_preference_loss_back";
+    TRC_FORCED("trc_hip_preference_loss_back");
+    TRC_TRY(check_preference(who, logits, labels, start, lse, slope, beta));
+    TRC_TRY(check_shape(who, "dloss", dloss, TRC_HIP_TYPE_F32, 1, 1, 1, false));
+    TRC_TRY(check_shape(who, "dlogits", dlogits, logits->type, logits->ne[0], logits->ne[1], 1, true));
+    const trc_hip_tensor* const all[6] = {logits, labels, start, lse, slope, dloss};
+    const char* const names[6] = {"logits", "labels", "start", "lse", "slope", "dloss"};
+    for (int j = 0; j < 6; ++j) TRC_TRY(check_apart(who, dlogits, "dlogits", all[j], names[j], j == 0));
+    return launch_preference_loss_back(*logits, (const int32_t*) labels->data, (const int32_t*) start->data, slope->ne[0],
+                                       (const float*) lse->data, (const float*) slope->data, (const float*) dloss->data, beta,
+                                       *dlogits, (hipStream_t) stream);
+}
+
+int trc_hip_adamw_create(const trc_hip_adamw_tensor* tensors, int64_t count, int bits, void** plan) {
+    const char* const who = "trc_hip_adamw_create";
+    if (plan == nullptr) return fail(TRC_HIP_E_INVALID, "%s: plan is NULL", who);
+    *plan = nullptr;
+    TRC_FORCED("trc_hip_adamw_create");
+    if (count < 0 || (count > 0 && tensors == nullptr)) return fail(TRC_HIP_E_INVALID, "%s: no tensors", who);
+    if (bits != 32 && bits != 8) return fail(TRC_HIP_E_INVALID, "%s: moments of %d bits (32 or 8)", who, bits);
+    try {
+        return adamw_create(tensors, count, bits, plan);
+    } catch (const std::bad_alloc&) {
+        return fail((int) hipErrorOutOfMemory, "%s: out of host memory", who);
+    }
+}
+
+int trc_hip_adamw_step(void* plan, const trc_hip_adamw_hyper* hyper, void* stream) {
+    const char* const who = "trc_hip_adamw_step";
+    TRC_FORCED("trc_hip_adamw_step");
+    if (plan == nullptr || hyper == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL argument", who);
+    if (hyper->step < 1) return fail(TRC_HIP_E_INVALID, "%s: step %lld (they count from 1)", who, (long long) hyper->step);
+    if (!(hyper->beta1 >= 0.0 && hyper->beta1 < 1.0) || !(hyper->beta2 >= 0.0 && hyper->beta2 < 1.0) || !(hyper->eps >= 0.0)) {
+        return fail(TRC_HIP_E_INVALID, "%s: beta1 = %g, beta2 = %g, eps = %g", who, hyper->beta1, hyper->beta2, hyper->eps);
+    }
+    return adamw_step(plan, *hyper, (hipStream_t) stream);
+}
+
+int trc_hip_adamw_moments(void* plan, void* stream) {
+    TRC_FORCED("trc_hip_adamw_moments");
+    if (plan == nullptr) return fail(TRC_HIP_E_INVALID, "trc_hip_adamw_moments: plan is NULL");
+    return adamw_moments(plan, (hipStream_t) stream);
+}
+
+int trc_hip_adamw_destroy(void* plan) {
+    TRC_FORCED("trc_hip_adamw_destroy");
+    return plan != nullptr ? adamw_destroy(plan) : TRC_HIP_OK;
 }
 
 }  // extern "C"

@@ -171,6 +171,23 @@ int launch_acc_f32(const trc_hip_tensor& a, const trc_hip_tensor& b, const trc_h
                    size_t nb3, size_t offset, int inplace, hipStream_t stream);
 int launch_repeat_back_f32(const trc_hip_tensor& a, const trc_hip_tensor& d, hipStream_t stream);
 int launch_fill_f32(float* dst, float value, int64_t count, hipStream_t stream);
+// Adapters (lora.hip): contract, then expand; base and dx may be null.
+int launch_lora(const trc_hip_lora_set& set, const trc_hip_tensor& x, const trc_hip_tensor* base, const trc_hip_tensor& h,
+                const trc_hip_tensor& dst, hipStream_t stream);
+int launch_lora_back(const trc_hip_lora_set& set, const trc_hip_tensor& x, const trc_hip_tensor& h, const trc_hip_tensor& dy,
+                     const trc_hip_tensor& g, const trc_hip_tensor* base, const trc_hip_tensor* dx, const trc_hip_tensor& da,
+                     const trc_hip_tensor& db, bool accumulate, hipStream_t stream);
+int launch_preference_loss(const trc_hip_tensor& logits, const int32_t* labels, const int32_t* start, int64_t pairs,
+                           const float* ref, float beta, float smoothing, float* lse, float* logp, float* slope,
+                           float* loss, hipStream_t stream);
+int launch_preference_loss_back(const trc_hip_tensor& logits, const int32_t* labels, const int32_t* start, int64_t pairs,
+                                const float* lse, const float* slope, const float* dloss, float beta,
+                                const trc_hip_tensor& dlogits, hipStream_t stream);
+// AdamW plans (adamw.hip). adamw_create may throw std::bad_alloc.
+int adamw_create(const trc_hip_adamw_tensor* tensors, int64_t count, int bits, void** plan);
+int adamw_step(void* plan, const trc_hip_adamw_hyper& hyper, hipStream_t stream);
+int adamw_moments(void* plan, hipStream_t stream);
+int adamw_destroy(void* plan);
 int launch_cpy(const trc_hip_tensor& src, const trc_hip_tensor& dst, size_t elem_size,
                hipStream_t stream);
 

@@ -13,9 +13,12 @@ LIB_DIR = Path(__file__).resolve().parent / "lib"
 LIB_PATH = LIB_DIR / "libtrc_hip.so"
 
 TYPE_F32, TYPE_Q4_0, TYPE_Q4_1, TYPE_Q5_0, TYPE_Q5_1, TYPE_Q8_0 = 0, 2, 3, 6, 7, 8
+TYPE_F16, TYPE_I32, TYPE_BF16 = 1, 26, 30
 QUANT_TYPES = {"q4_0": TYPE_Q4_0, "q4_1": TYPE_Q4_1, "q5_0": TYPE_Q5_0, "q5_1": TYPE_Q5_1, "q8_0": TYPE_Q8_0}
 BLOCK_BYTES = {TYPE_Q4_0: 18, TYPE_Q4_1: 20, TYPE_Q5_0: 22, TYPE_Q5_1: 24, TYPE_Q8_0: 34}
 QMATVEC_MAX_N = 64
+LORA_MAX_RANK = 256
+ADAMW_BLOCK = 256
 
 OK, E_INVALID, E_SHAPE, E_ALIGN, E_NO_DEVICE, E_FORCED = 0, -1, -2, -3, -4, -5
 
@@ -26,6 +29,8 @@ EXPORTS = (
     "trc_hip_add_f32", "trc_hip_acc_f32", "trc_hip_repeat_back_f32", "trc_hip_qmatvec_noalloc",
     "trc_hip_mul_f32", "trc_hip_repeat_f32", "trc_hip_sum_f32", "trc_hip_qmatvec_release_stream",
     "trc_hip_mul_mat_acc_f32", "trc_hip_sqr_f32", "trc_hip_scale_f32",
+    "trc_hip_lora", "trc_hip_lora_back", "trc_hip_preference_loss", "trc_hip_preference_loss_back",
+    "trc_hip_adamw_create", "trc_hip_adamw_step", "trc_hip_adamw_moments", "trc_hip_adamw_destroy",
 )
 
 
@@ -41,6 +46,25 @@ class Tensor(C.Structure):
     _fields_ = [
         ("data", C.c_void_p), ("type", C.c_int32), ("flags", C.c_int32),
         ("ne", C.c_int64 * 4), ("nb", C.c_size_t * 4),
+    ]
+
+
+class LoraSet(C.Structure):
+    _fields_ = [("a", Tensor), ("b", Tensor), ("scale", Tensor), ("start", Tensor), ("adapter", Tensor)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+        ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("m_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("n", C.c_int64), ("decay", C.c_float), ("grad_type", C.c_int32),
+    ]
+
+
+class AdamWHyper(C.Structure):
+    _fields_ = [
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+        ("weight_decay", C.c_double), ("grad_scale", C.c_double), ("step", C.c_int64),
     ]
 
 
@@ -106,6 +130,14 @@ def load() -> C.CDLL:
         "trc_hip_mul_f32": ([C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor), P], I),
         "trc_hip_repeat_f32": ([C.POINTER(Tensor), C.POINTER(Tensor), P], I),
         "trc_hip_sum_f32": ([C.POINTER(Tensor), C.POINTER(Tensor), P], I),
+        "trc_hip_lora": ([C.POINTER(LoraSet)] + [C.POINTER(Tensor)] * 4 + [P], I),
+        "trc_hip_lora_back": ([C.POINTER(LoraSet)] + [C.POINTER(Tensor)] * 8 + [I, P], I),
+        "trc_hip_preference_loss": ([C.POINTER(Tensor)] * 4 + [F, F] + [C.POINTER(Tensor)] * 4 + [P], I),
+        "trc_hip_preference_loss_back": ([C.POINTER(Tensor)] * 6 + [F, C.POINTER(Tensor), P], I),
+        "trc_hip_adamw_create": ([C.POINTER(AdamWTensor), I64, I, C.POINTER(P)], I),
+        "trc_hip_adamw_step": ([P, C.POINTER(AdamWHyper), P], I),
+        "trc_hip_adamw_moments": ([P, P], I),
+        "trc_hip_adamw_destroy": ([P], I),
     }
     for name, (args, ret) in sig.items():
         fn = getattr(lib, name)
@@ -211,6 +243,74 @@ def sum_f32(a: Tensor, d: Tensor, stream: int | None = None) -> None:
 
 def fill_f32(ptr: int, value: float, count: int, stream: int | None = None) -> None:
     check(load().trc_hip_fill_f32(ptr, value, count, stream))
+
+
+def lora_set(a: Tensor, b: Tensor, scale: Tensor, start: Tensor, adapter: Tensor) -> LoraSet:
+    """The adapters of a projection and a batch's requests (trc_hip_lora_set)."""
+    return LoraSet(a, b, scale, start, adapter)
+
+
+def _ref(t):
+    return None if t is None else C.byref(t)
+
+
+def lora(s: LoraSet, x: Tensor, base: Tensor | None, h: Tensor, d: Tensor, stream: int | None = None) -> None:
+    """h = A x, d = base + scale B h (trc_hip_lora)."""
+    check(load().trc_hip_lora(C.byref(s), C.byref(x), _ref(base), C.byref(h), C.byref(d), stream))
+
+
+def lora_back(s: LoraSet, x: Tensor, h: Tensor, dy: Tensor, g: Tensor, base: Tensor | None, dx: Tensor | None,
+              da: Tensor, db: Tensor, accumulate: bool = False, stream: int | None = None) -> None:
+    """The gradients of lora() (trc_hip_lora_back)."""
+    check(load().trc_hip_lora_back(C.byref(s), C.byref(x), C.byref(h), C.byref(dy), C.byref(g), _ref(base), _ref(dx),
+                                   C.byref(da), C.byref(db), 1 if accumulate else 0, stream))
+
+
+def preference_loss(logits: Tensor, labels: Tensor, start: Tensor, ref: Tensor, beta: float, smoothing: float,
+                    lse: Tensor, logp: Tensor, slope: Tensor, loss: Tensor, stream: int | None = None) -> None:
+    check(load().trc_hip_preference_loss(C.byref(logits), C.byref(labels), C.byref(start), C.byref(ref), beta, smoothing,
+                                         C.byref(lse), C.byref(logp), C.byref(slope), C.byref(loss), stream))
+
+
+def preference_loss_back(logits: Tensor, labels: Tensor, start: Tensor, lse: Tensor, slope: Tensor, dloss: Tensor,
+                         beta: float, dlogits: Tensor, stream: int | None = None) -> None:
+    check(load().trc_hip_preference_loss_back(C.byref(logits), C.byref(labels), C.byref(start), C.byref(lse),
+                                              C.byref(slope), C.byref(dloss), beta, C.byref(dlogits), stream))
+
+
+class AdamW:
+    """A plan of AdamW steps (trc_hip_adamw_create). Each tensor is a dict of
+    trc_hip_adamw_tensor's fields (device addresses, n, decay, grad_type)."""
+
+    def __init__(self, tensors, bits: int = 32):
+        self.plan = None
+        ts = (AdamWTensor * max(len(tensors), 1))()
+        for t, fields in zip(ts, tensors):
+            t.decay = 1.0
+            for k, v in fields.items():
+                setattr(t, k, v)
+        p = C.c_void_p()
+        check(load().trc_hip_adamw_create(ts, len(tensors), bits, C.byref(p)))
+        self.plan = p
+
+    def step(self, lr: float, step: int, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
+             weight_decay: float = 0.0, grad_scale: float = 1.0, stream: int | None = None) -> None:
+        h = AdamWHyper(lr, beta1, beta2, eps, weight_decay, grad_scale, step)
+        check(load().trc_hip_adamw_step(self.plan, C.byref(h), stream))
+
+    def moments(self, stream: int | None = None) -> None:
+        check(load().trc_hip_adamw_moments(self.plan, stream))
+
+    def destroy(self) -> None:
+        if self.plan is not None:
+            plan, self.plan = self.plan, None
+            check(load().trc_hip_adamw_destroy(plan))
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
 
 
 class DeviceBuffer:
