@@ -320,7 +320,7 @@ typedef struct trc_hip_lora_set {
  *   h[:,t] = A x[:,t]      dst[:,t] = base[:,t] + scale B h[:,t]
  * with A, B and scale of the adapter of token t's request. x is [K, T], base and dst
  * [M, T], h [R, T] contiguous; all F32 with nb[0] = 4 and rows at any 4-byte aligned stride
- * that keeps the written ones apart. base may be NULL (zeros) or dst itself. A token without
+ * up to 128 MiB (16 MiB for the adapters') that keeps the written ones apart. base may be NULL (zeros) or dst itself. A token without
  * an adapter gets dst = base and h = 0. h is what trc_hip_lora_back needs of this call.
  * Sums are in 32 bits on the F32 matrix instructions, adapters in 16 bits widened, in an order
  * that only the sizes decide: the same from run to run. A batch of few tokens keeps partial sums in the

@@ -482,6 +482,9 @@ int check_lora_set(const char* who, const trc_hip_lora_set* set, int64_t T) {
     }
     TRC_TRY(check_shape(who, "a", &a, a.type, K, R, n, false));
     TRC_TRY(check_shape(who, "b", &b, a.type, R, M, n, false));
+    if ((R > 1 && a.nb[1] > ((size_t) 1 << 24)) || (M > 1 && b.nb[1] > ((size_t) 1 << 24))) {
+        return fail(TRC_HIP_E_SHAPE, "%s: rows of a or b over 16 MiB apart", who);
+    }
     TRC_TRY(check_shape(who, "scale", &set->scale, TRC_HIP_TYPE_F32, n, 1, 1, false));
     TRC_TRY(check_shape(who, "start", &set->start, TRC_HIP_TYPE_I32, requests + 1, 1, 1, false));
     return check_shape(who, "adapter", &set->adapter, TRC_HIP_TYPE_I32, requests, 1, 1, false);
@@ -493,6 +496,14 @@ int check_lora_out(const char* who, const trc_hip_lora_set* set, const trc_hip_t
     TRC_TRY(check_apart(who, out, name, &set->scale, "scale", false));
     TRC_TRY(check_apart(who, out, name, &set->start, "start", false));
     return check_apart(who, out, name, &set->adapter, "adapter", false);
+}
+
+// The kernels address a tile's rows of an activation through 32-bit offsets.
+int check_row_stride(const char* who, const char* name, const trc_hip_tensor* t) {
+    if (t != nullptr && t->ne[1] > 1 && t->nb[1] > ((size_t) 1 << 27)) {
+        return fail(TRC_HIP_E_SHAPE, "%s: rows of %s over 128 MiB apart", who, name);
+    }
+    return TRC_HIP_OK;
 }
 
 // A contiguous vector or matrix: rows back to back.
@@ -536,6 +547,9 @@ int trc_hip_lora(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc
     TRC_TRY(check_packed(who, "h", h));
     TRC_TRY(check_shape(who, "dst", dst, TRC_HIP_TYPE_F32, M, T, 1, true));
     if (base != nullptr) TRC_TRY(check_shape(who, "base", base, TRC_HIP_TYPE_F32, M, T, 1, false));
+    TRC_TRY(check_row_stride(who, "x", x));
+    TRC_TRY(check_row_stride(who, "base", base));
+    TRC_TRY(check_row_stride(who, "dst", dst));
     TRC_TRY(check_lora_out(who, set, h, "h"));
     TRC_TRY(check_lora_out(who, set, dst, "dst"));
     TRC_TRY(check_apart(who, h, "h", x, "x", false));
@@ -567,6 +581,10 @@ int trc_hip_lora_back(const trc_hip_lora_set* set, const trc_hip_tensor* x, cons
     }
     TRC_TRY(check_shape(who, "da", da, TRC_HIP_TYPE_F32, K, R, n, true));
     TRC_TRY(check_shape(who, "db", db, TRC_HIP_TYPE_F32, R, M, n, true));
+    TRC_TRY(check_row_stride(who, "x", x));
+    TRC_TRY(check_row_stride(who, "dy", dy));
+    TRC_TRY(check_row_stride(who, "base", base));
+    TRC_TRY(check_row_stride(who, "dx", dx));
     const trc_hip_tensor* const outs[4] = {g, dx, da, db};
     const char* const names[4] = {"g", "dx", "da", "db"};
     for (int i = 0; i < 4; ++i) {

@@ -6,13 +6,17 @@
 //   g_t  = s_a B_a^T dy_t       dx_t = base_t + A_a^T g_t
 //   dA_a = sum_t g_t x_t^T      dB_a = s_a sum_t dy_t h_t^T
 //
-// Three kernels serve all six, on v_mfma_f32_16x16x4_f32 (F32 products as exact as
-// float FMAs; adapters in 16 bits are widened):
-//   k_contract  h and g: a wide activation times a matrix of R rows or columns
-//   k_expand    y and dx: base plus a matrix times h or g
-//   k_outer     dA and dB: sums over tokens of outer products
-// A workgroup of the first two takes 16 tokens of one request, so a request of one token
-// costs one reading of its adapter and a long one reads it once per 16 tokens, from the L2.
+// Three steps make all six, on v_mfma_f32_16x16x4_f32 (products as exact as float
+// FMAs; adapters in 16 bits are widened):
+//   contract  h and g: a wide activation times a matrix of R rows or columns
+//   expand    y and dx: base plus a matrix times h or g
+//   outer     dA and dB: sums over tokens of outer products
+// The first two take 16 tokens of one request at a time, so a request of one token costs one
+// reading of its adapter, and a long one reads it once per 16 tokens, from the L2.
+//
+// In that instruction lane l holds A[i][k] and B[k][j] at i = j = l % 16, k = l / 16, and
+// the sums at i = 4 (l / 16) + v, j = l % 16. The order of a sum's terms is free, so a lane takes
+// four neighbours of the long axis with one load and feeds them to four instructions.
 #include <algorithm>
 #include <type_traits>
 
@@ -22,35 +26,83 @@ namespace trc_hip {
 
 namespace {
 
-constexpr int LT = 16;           // tokens of a tile
-constexpr int LC_THREADS = 512;  // k_contract: 8 waves split the long axis
-constexpr int LE_THREADS = 256;  // k_expand
-constexpr int LE_COLS = 512;     // outputs of a workgroup's tokens
-constexpr int LO_THREADS = 512;  // k_outer: 8 waves split the tokens
-constexpr int LR = 64;           // rank of one pass, at most
+constexpr int LT = 16;             // tokens of a tile
+constexpr int LO_WAVES = 16;       // waves of a workgroup of the backward pass
+constexpr int LE_THREADS = 256;    // k_expand
+constexpr int LE_COLS = 64;        // outputs a wave makes of each token at a time
+constexpr int LO_COLS = 32;        // outer: columns of a workgroup
+constexpr int LR = 64;             // rank that is summed at a time, at most
 constexpr int L_MAX_RANK = TRC_HIP_LORA_MAX_RANK;
 
-// four elements whose address is only as aligned as one
+// Registers for four waves a SIMD: with fewer, the loads in flight do not fill memory's latency.
+#define L_FOUR_WAVES __attribute__((amdgpu_waves_per_eu(4)))
+
+typedef float f4v __attribute__((ext_vector_type(4), may_alias));
+typedef uint16_t h4 __attribute__((ext_vector_type(4)));
+// elements whose address is only as aligned as one
+typedef float f2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t h2u __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
 
+// Weights as they are loaded, four or fewer at a time; they are widened where they are
+// multiplied, so that nothing waits for a load before.
 template <int TYPE>
 struct Wt {
     typedef uint16_t Elem;
+    template <int N>
+    using Raw = std::conditional_t<N == 1, uint16_t, std::conditional_t<N == 2, h2u, h4u>>;
     static __device__ __forceinline__ float get(Elem x) {
         return TYPE == TRC_HIP_TYPE_F16 ? half_bits_to_float(x) : __builtin_bit_cast(float, (uint32_t) x << 16);
-    }
-    static __device__ __forceinline__ f4 get4(const Elem* p) {
-        const h4u h = *(const h4u*) p;
-        return f4{get(h[0]), get(h[1]), get(h[2]), get(h[3])};
     }
 };
 template <>
 struct Wt<TRC_HIP_TYPE_F32> {
     typedef float Elem;
+    template <int N>
+    using Raw = std::conditional_t<N == 1, float, std::conditional_t<N == 2, f2u, f4u>>;
     static __device__ __forceinline__ float get(Elem x) { return x; }
-    static __device__ __forceinline__ f4 get4(const Elem* p) { return *(const f4u*) p; }
 };
+template <class R>
+__device__ __forceinline__ auto element(const R& r, int i) {
+    if constexpr (std::is_arithmetic_v<R>) {
+        return r;
+    } else {
+        return r[i];
+    }
+}
+
+// A value of another lane by data-parallel primitives, which need no LDS: 0 where there is no such lane.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int from_lane(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR8 = 0x128;  // (quads permuted; a row of 16 rotated by 8)
+constexpr int DPP_SHR = 0x110, DPP_BCAST15 = 0x142, DPP_BCAST31 = 0x143;
+// Lane ^ MASK among each 32 lanes, MASK under 32.
+template <int MASK>
+__device__ __forceinline__ float swizzle_xor(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, x), MASK << 10 | 0x1f));
+}
+
+// 16 bytes at any address that is whole elements.
+struct __attribute__((packed, aligned(2))) v16u {
+    f4v v;
+};
+
+// Keeps the loads before it where they are: without it the compiler moves the loads of a loop's next
+// round behind the products of this one, and every round waits for memory.
+__device__ __forceinline__ void loads_stay() { asm volatile("" ::: "memory"); }
+// A wave's LDS operations run in order; this keeps the compiler from changing it.
+__device__ __forceinline__ void lds_in_order() { asm volatile("" ::: "memory"); }
+
+// A load at a base all lanes share, kept in scalar registers, and a lane's 32-bit offset.
+template <class V>
+__device__ __forceinline__ V load_at(const void* base, uint32_t offset) {
+    return *(const V*) ((const uint8_t*) base + offset);
+}
 
 struct Batch {
     const int32_t* start;
@@ -61,39 +113,46 @@ struct Batch {
 };
 
 struct Tile {
-    int64_t lo;   // first token
+    int lo;       // first token
     int tokens;   // 0: none
     int adapter;  // -1: none
 };
 
 // Tile `index` of the batch, requests in order and each in tiles of LT tokens. Every lane
-// of a wave has to be here. What start holds is only compared and clamped, so
-// no value of it leads out of the T tokens.
-__device__ __forceinline__ Tile find_tile(const Batch& b, int64_t index) {
-    const int lane = (int) threadIdx.x & 63;
+// of a wave has to be here; the result is the same in all and held in scalar registers. What start
+// holds is only compared and clamped, so no value of it leads out of the T tokens.
+__device__ __forceinline__ Tile find_tile(const Batch& b, int index) {
+    const int lane = (int) threadIdx.x & 63, T = (int) b.T;
     for (int q0 = 0; q0 < b.requests; q0 += 64) {
         const int q = q0 + lane;
-        int64_t lo = 0, hi = 0;
+        int lo = 0, hi = 0, id = -1;
         if (q < b.requests) {
-            lo = min(max((int64_t) b.start[q], (int64_t) 0), b.T);
-            hi = min(max((int64_t) b.start[q + 1], lo), b.T);
+            lo = min(max(b.start[q], 0), T);
+            hi = min(max(b.start[q + 1], lo), T);
+            id = b.ids[q];
         }
-        const int64_t mine = (hi - lo + LT - 1) / LT;
-        int64_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t v = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += v;
-        }
-        const uint64_t in = __ballot(index < upto);
+        const int mine = (int) (((uint32_t) (hi - lo) + LT - 1) / LT);
+        // tiles of the requests up to this lane's (wrong starts may overflow it; what comes of that is clamped below)
+        uint32_t sum = (uint32_t) mine;
+        sum += (uint32_t) from_lane<DPP_SHR + 1>((int) sum);
+        sum += (uint32_t) from_lane<DPP_SHR + 2>((int) sum);
+        sum += (uint32_t) from_lane<DPP_SHR + 4>((int) sum);
+        sum += (uint32_t) from_lane<DPP_SHR + 8>((int) sum);
+        sum += (uint32_t) from_lane<DPP_BCAST15, 0xa>((int) sum);
+        sum += (uint32_t) from_lane<DPP_BCAST31, 0xc>((int) sum);
+        const int upto = (int) sum;
+        const uint64_t in = __ballot(index < upto && mine > 0);
         if (in != 0) {
             const int src = __ffsll((unsigned long long) in) - 1;
-            const int64_t first = __shfl(lo, src, 64) + (index - __shfl(upto - mine, src, 64)) * LT;
-            const int64_t end = __shfl(hi, src, 64);
-            const int id = b.ids[q0 + src];
-            return {first, (int) min(end - first, (int64_t) LT), id >= 0 && id < b.adapters ? id : -1};
+            lo = __builtin_amdgcn_readlane(lo, src);
+            hi = __builtin_amdgcn_readlane(hi, src);
+            id = __builtin_amdgcn_readlane(id, src);
+            const int before = __builtin_amdgcn_readlane((int) ((uint32_t) upto - (uint32_t) mine), src);
+            const int64_t first = lo + ((int64_t) index - before) * LT;
+            if (first < lo || first >= hi) return {0, 0, -1};
+            return {(int) first, min(hi - (int) first, LT), id >= 0 && id < b.adapters ? id : -1};
         }
-        index -= __shfl(upto, 63, 64);
+        index = (int) ((uint32_t) index - (uint32_t) __builtin_amdgcn_readlane(upto, 63));
     }
     return {0, 0, -1};
 }
@@ -105,233 +164,905 @@ struct Matrix {
     int64_t row, adapter;  // strides in elements
 };
 
-// out[t][r] = scale sum_n x[t][n] W(n, r), where W(n, r) is w[r][n] (A) or, with OUTER,
-// w[n][r] (B). Blocks: (tile, 64 of the rank, part of n); part p goes to out + p * T * R.
-// A lane of the x operand holds token lane % 16 and of each 16 of n the four from
-// 4 * (lane / 16) on, one per instruction; the weights' lanes hold column r = lane % 16 the
-// same way, so the four products of a lane's vector need no shuffle. Lanes past the
-// tile's tokens or past R read the last one and are not stored.
-template <int TYPE, bool OUTER, int RT>
-__global__ __launch_bounds__(LC_THREADS) void k_contract(const uint8_t* __restrict__ x, size_t x_nb1, int64_t N, Matrix wm,
-                                                          int R, Batch b, bool scaled, int64_t part_len,
-                                                          float* __restrict__ out) {
-    typedef Wt<TYPE> W;
-    constexpr int WAVES = LC_THREADS / 64;
-    const Tile t = find_tile(b, blockIdx.x);
-    if (t.tokens == 0) return;
-    out += (int64_t) blockIdx.z * b.T * R;
-    const int r0 = (int) blockIdx.y * LR;
-    if (t.adapter < 0) {
-        for (int i = (int) threadIdx.x; i < t.tokens * LR; i += LC_THREADS) {
-            const int r = r0 + i % LR;
-            if (r < R) out[(t.lo + i / LR) * R + r] = 0.f;
-        }
-        return;
-    }
-    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    const float* const xt = (const float*) (x + (t.lo + min(col, t.tokens - 1)) * x_nb1);
-    const typename W::Elem* const w = (const typename W::Elem*) wm.p + t.adapter * wm.adapter;
-    const typename W::Elem* wr[RT];
+struct Rows {
+    const uint8_t* p;
+    size_t nb1;
+    int64_t n;  // elements of a row
+};
+
+template <int WAVES, int RT>
+using Partial = f4[WAVES][RT][64];
+
+// Element e = (j * 64 + lane) * 4 + v of the waves' sums, added in order.
+template <int WAVES, int RT>
+__device__ __forceinline__ float joined(const Partial<WAVES, RT>& part, int e) {
+    const float* const p = (const float*) part + e;
+    float x[WAVES];
 #pragma unroll
-    for (int j = 0; j < RT; ++j) wr[j] = w + (int64_t) min(r0 + 16 * j + col, R - 1) * (OUTER ? 1 : wm.row);
+    for (int w = 0; w < WAVES; ++w) x[w] = p[w * RT * 256];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) x[0] += x[w];
+    return x[0];
+}
+
+// Both operands of the instruction want neighbouring lanes in different rows, and a load whose
+// neighbouring lanes are not neighbours in memory is split up lane by lane (64 tag lookups
+// instead of 16 for 1 KB; that, not HBM, bounded these kernels at first). So 16 rows are loaded
+// along the rows and turned through LDS, each wave in a piece of its own: its LDS
+// operations run in order, so no barrier is needed.
+//
+// Rows16: 16 rows of CN elements, as loaded: lane l of load i has 16 bytes (or four elements) of
+// row i * RPI + l / LPR. Rows in LDS are 16 bytes longer than CN elements, which spreads 16 rows at one
+// column over all banks.
+template <class Elem, int CN>
+struct Rows16 {
+    static constexpr int ES = sizeof(Elem), LPR = CN * ES / 16, RPI = 64 / LPR, LOADS = 16 / RPI;
+    static constexpr int PITCH = CN * ES + 16, BYTES = 16 * PITCH;
+    static_assert(LOADS >= 1, "a load has 16 rows at most");
+    f4v raw[LOADS];
+    // row(i): the byte offset of row i, for its lane
+    template <class RowOffset>
+    static __device__ __forceinline__ void offsets(uint32_t (&o)[LOADS], RowOffset&& row) {
+        const int lane = (int) threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) o[i] = row(i * RPI + lane / LPR) + 16 * (lane % LPR);
+    }
+    __device__ __forceinline__ void load(const uint8_t* base, const uint32_t (&o)[LOADS]) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) raw[i] = load_at<v16u>(base, o[i]).v;
+    }
+    __device__ __forceinline__ void stage(uint8_t* lds) const {
+        const int lane = (int) threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) *(f4v*) (lds + (i * RPI + lane / LPR) * PITCH + 16 * (lane % LPR)) = raw[i];
+    }
+    // Elements 16 u + 4 (lane / 16) .. + 3 of row lane % 16.
+    typedef std::conditional_t<ES == 4, f4, h4> Four;
+    static __device__ __forceinline__ Four four(const uint8_t* lds, int u) {
+        const int lane = (int) threadIdx.x & 63;
+        return *(const Four*) (lds + (lane & 15) * PITCH + (16 * u + 4 * (lane >> 4)) * ES);
+    }
+};
+
+constexpr int L_CHUNK = 32;  // elements of the long axis that a wave takes at a time
+// a wave's piece of LDS for contract_tile: x, then 16 columns of the weights
+template <class Elem>
+constexpr int contract_lds = Rows16<float, L_CHUNK>::BYTES + Rows16<Elem, L_CHUNK>::BYTES;
+
+// sum_n x[t][n] W(n, r) for the tile's tokens, n in lo .. hi-1 and r in r0 .. r0 + 16 RT - 1,
+// where W(n, r) is w[r][n] (A) or, with OUTER, w[n][r] (B); each sum goes to
+// sink(token, r, sum). Columns of the weights past R read others again and do not reach
+// the sink, as tokens past the tile's. The waves take chunks of the long axis in turn, each with
+// the loads of the next chunk under way. part may be the memory that is staged through.
+template <int TYPE, bool OUTER, int WAVES, int RT, class Sink>
+__device__ __forceinline__ void contract_tile(const Tile& t, const Rows& x, const Matrix& wm, int R, int r0, int64_t lo,
+                                              int64_t hi, uint8_t* lds, Partial<WAVES, RT>& part, Sink&& sink) {
+    typedef Wt<TYPE> W;
+    typedef typename W::Elem Elem;
+    constexpr int CN = L_CHUNK, U = CN / 16;
+    constexpr int ES = sizeof(Elem);
+    typedef Rows16<float, CN> X;
+    typedef Rows16<Elem, CN> A;
+    const int lane = (int) threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    uint8_t* const xs = lds + wave * contract_lds<Elem>;
+    uint8_t* const ws = xs + X::BYTES;
+    const uint8_t* const xb = x.p + (int64_t) t.lo * x.nb1;
+    const uint32_t wrow = (uint32_t) wm.row * ES;
+    const uint8_t* const wb = (const uint8_t*) wm.p + (t.adapter * wm.adapter + (OUTER ? 0 : r0 * wm.row)) * ES;
+    uint32_t xo[X::LOADS], ao[OUTER ? 1 : RT][A::LOADS], bo = 0;
+    X::offsets(xo, [&](int row) { return (uint32_t) min(row, t.tokens - 1) * (uint32_t) x.nb1; });
+    // A: tile j's column is r0 + 16 j + col. B: columns side by side, r0 + RT col + j, so that one
+    // load has a lane's columns of all tiles; the last ones are moved back into the row (R >= RT).
+    if constexpr (OUTER) {
+        bo = 4 * quad * wrow + (uint32_t) min(r0 + RT * col, R - RT) * ES;
+    } else {
+#pragma unroll
+        for (int j = 0; j < RT; ++j) A::offsets(ao[j], [&](int row) { return (uint32_t) min(16 * j + row, R - 1 - r0) * wrow; });
+    }
     f4 acc[RT];
 #pragma unroll
     for (int j = 0; j < RT; ++j) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
-    const int64_t lo = (int64_t) blockIdx.z * part_len, hi = min(lo + part_len, N);
-    auto weights = [&](int j, int64_t n) {
-        if (!OUTER) return W::get4(wr[j] + n);
-        f4 v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = W::get(wr[j][(n + k) * wm.row]);
-        return v;
+    // Whether a chunk's weights are loaded with its x, a chunk ahead; else 16 columns ahead, which takes
+    // fewer registers.
+    constexpr bool AHEAD = RT * ES <= 4;
+    struct Chunk {
+        X x;
+        A a[OUTER || !AHEAD ? 1 : RT];
+        typename W::template Raw<RT> b[OUTER ? U : 1][4];
     };
-    constexpr int U = 4;  // groups of 16 that are loaded together
-    int64_t n = lo + wave * (16 * U) + 4 * quad;
-    const int64_t whole = lo + (hi - lo) / (16 * U) * (16 * U);
-    for (; n - 4 * quad < whole; n += WAVES * 16 * U) {
-        f4 xv[U], wv[U][RT];
+    auto load = [&](Chunk& c, int64_t i) {  // the wave's chunk i
+        const int64_t n = lo + (wave + i * WAVES) * CN;
+        c.x.load(xb + n * 4, xo);
+        if constexpr (OUTER) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            xv[u] = *(const f4u*) (xt + n + 16 * u);
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < RT; ++j) wv[u][j] = weights(j, n + 16 * u);
+                for (int k = 0; k < 4; ++k)
+                    c.b[u][k] = load_at<typename W::template Raw<RT>>(wb + (n + 16 * u + k) * (int64_t) wrow, bo);
+        } else if constexpr (AHEAD) {
+#pragma unroll
+            for (int j = 0; j < RT; ++j) c.a[j].load(wb + n * ES, ao[j]);
         }
+    };
+    auto multiply = [&](const Chunk& c, int64_t i) {
+        const int64_t n = lo + (wave + i * WAVES) * CN;
+        A ring[2];
+        if constexpr (!OUTER && !AHEAD) ring[0].load(wb + n * ES, ao[0]);
+        c.x.stage(xs);
+        lds_in_order();
+        f4 xv[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) xv[u] = X::four(xs, u);
+        if constexpr (OUTER) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < RT; ++j) acc[j] = mfma(xv[u][k], wv[u][j][k], acc[j]);
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) acc[j] = mfma(xv[u][k], W::get(element(c.b[u][k], j)), acc[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                if constexpr (AHEAD) {
+                    c.a[j].stage(ws);
+                } else {
+                    if (j + 1 < RT) ring[(j + 1) & 1].load(wb + n * ES, ao[j + 1 < RT ? j + 1 : 0]);
+                    loads_stay();
+                    ring[j & 1].stage(ws);
+                }
+                lds_in_order();
+                typename A::Four wv[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) wv[u] = A::four(ws, u);
+                lds_in_order();
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[j] = mfma(xv[u][k], W::get(wv[u][k]), acc[j]);
+            }
+        }
+        lds_in_order();
+    };
+    const int64_t chunks = (hi - lo) / CN;
+    // Two chunks in turn and no branch around the loads, so that what is waited for is counted in order
+    // and nothing is copied.
+    const int64_t mine = wave < chunks ? (chunks - wave + WAVES - 1) / WAVES : 0;
+    if (mine > 0) {
+        Chunk c0, c1;
+        load(c0, 0);
+        int64_t i = 0;
+        for (; i + 2 < mine; i += 2) {
+            load(c1, i + 1);
+            loads_stay();
+            multiply(c0, i);
+            load(c0, i + 2);
+            loads_stay();
+            multiply(c1, i + 1);
+        }
+        if (i + 1 < mine) {
+            load(c1, i + 1);
+            loads_stay();
+            multiply(c0, i);
+            multiply(c1, i + 1);
+        } else {
+            multiply(c0, i);
+        }
     }
-    // the rest, in groups of 16: both operands are 0 past the end, so nothing there counts
-    for (n = whole + wave * 16; n < hi; n += WAVES * 16) {
+    // the rest, in groups of 16 and element by element: both operands are 0 past the end
+    for (int64_t n = lo + chunks * CN + wave * 16; n < hi; n += WAVES * 16) {
+        const uint32_t xt = (uint32_t) min(col, t.tokens - 1) * (uint32_t) x.nb1;
+        float xk[4], wk[4][RT];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int64_t at = n + 4 * quad + k;
-            const float xk = at < hi ? xt[at] : 0.f;
+            const uint32_t at = (uint32_t) min((int64_t) (4 * quad + k), hi - 1 - n);
+            xk[k] = load_at<float>(xb + n * 4, xt + 4 * at);
 #pragma unroll
-            for (int j = 0; j < RT; ++j) acc[j] = mfma(xk, at < hi ? W::get(wr[j][OUTER ? at * wm.row : at]) : 0.f, acc[j]);
+            for (int j = 0; j < RT; ++j) {
+                const uint32_t o = OUTER ? at * wrow + (uint32_t) (min(r0 + RT * col, R - RT) + j) * ES
+                                         : (uint32_t) min(16 * j + col, R - 1 - r0) * wrow + at * ES;
+                wk[k][j] = W::get(load_at<Elem>(OUTER ? wb + n * (int64_t) wrow : wb + n * ES, o));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool in = n + 4 * quad + k < hi;
+#pragma unroll
+            for (int j = 0; j < RT; ++j) acc[j] = mfma(in ? xk[k] : 0.f, in ? wk[k][j] : 0.f, acc[j]);
         }
     }
-    __shared__ f4 part[WAVES][RT][64];
+    __syncthreads();  // (part may lie over what is staged)
 #pragma unroll
     for (int j = 0; j < RT; ++j) part[wave][j][lane] = acc[j];
     __syncthreads();
-    const float s = scaled ? b.scale[t.adapter] : 1.f;
-    for (int i = (int) threadIdx.x; i < RT * 64; i += LC_THREADS) {
-        const int j = i >> 6, l = i & 63, r = r0 + 16 * j + (l & 15);
-        f4 sum = part[0][j][l];
+    for (int e = (int) threadIdx.x; e < RT * 256; e += WAVES * 64) {
+        const float sum = joined<WAVES, RT>(part, e);
+        const int j = e >> 8, l = (e >> 2) & 63, tok = 4 * (l >> 4) + (e & 3), own = r0 + RT * (l & 15);
+        // (a moved column's sums belong to the lane whose own column it is)
+        const int r = OUTER ? min(own, R - RT) + j : r0 + 16 * j + (l & 15);
+        if (r < R && (!OUTER || r >= own) && tok < t.tokens) sink(tok, r, sum);
+    }
+}
+
+// The same of one token and A, without the matrix instructions, which would do 16 tokens' work: each
+// lane multiplies eight neighbours of n, a wave takes eight columns r at a time, and as many
+// waves as there are share a column's 512-element chunks. red: [wave][8].
+template <int TYPE, int WAVES, class Sink>
+__device__ __forceinline__ void contract_one(const Tile& t, const Rows& x, const Matrix& wm, int R, int64_t lo, int64_t hi,
+                                             float* red, Sink&& sink) {
+    typedef Wt<TYPE> W;
+    typedef typename W::Elem Elem;
+    constexpr int ES = sizeof(Elem);
+    const int lane = (int) threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    const uint8_t* const xb = x.p + (int64_t) t.lo * x.nb1;
+    const uint8_t* const wb = (const uint8_t*) wm.p + t.adapter * wm.adapter * ES;
+    const int groups = (R + 7) / 8;
+    for (int g0 = 0; g0 < groups; g0 += WAVES) {
+        const int here = min(groups - g0, WAVES), per = WAVES / here;  // waves that share a group
+        const int g = g0 + wave % here, sub = wave / here;
+        float acc[8];
 #pragma unroll
-        for (int v = 1; v < WAVES; ++v) sum += part[v][j][l];
-        if (r >= R) continue;
+        for (int r = 0; r < 8; ++r) acc[r] = 0.f;
+        if (sub < per) {
+            for (int64_t n = lo + sub * 512; n < hi; n += per * 512) {
+                const int left = (int) min((int64_t) 8, max((int64_t) 0, hi - n - 8 * lane));
+                if (left == 8) {
+                    const f4u x0 = load_at<f4u>(xb + n * 4, 32 * lane), x1 = load_at<f4u>(xb + n * 4, 32 * lane + 16);
+                    typename W::template Raw<4> w0[8], w1[8];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int tok = 4 * (l >> 4) + v;
-            if (tok < t.tokens) out[(t.lo + tok) * R + r] = sum[v] * s;
+                    for (int r = 0; r < 8; ++r) {
+                        const uint8_t* const row = wb + (min(8 * g + r, R - 1) * wm.row + n) * ES;
+                        w0[r] = load_at<typename W::template Raw<4>>(row, 8 * ES * lane);
+                        w1[r] = load_at<typename W::template Raw<4>>(row, 8 * ES * lane + 4 * ES);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            acc[r] = fmaf(x1[k], W::get(w1[r][k]), fmaf(x0[k], W::get(w0[r][k]), acc[r]));
+                } else {
+                    for (int k = 0; k < left; ++k) {
+                        const float xk = load_at<float>(xb + n * 4, 32 * lane + 4 * k);
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            const uint8_t* const row = wb + (min(8 * g + r, R - 1) * wm.row + n) * ES;
+                            acc[r] = fmaf(xk, W::get(load_at<Elem>(row, (8 * lane + k) * ES)), acc[r]);
+                        }
+                    }
+                }
+            }
+        }
+        // Eight sums over 64 lanes: three rounds that halve the sums a lane keeps, three that add up.
+        // What lane bits 0, 1 and 3 keep apart, and so a lane's column: bits 2, 1 and 0 of it.
+        const bool b0 = (lane & 1) != 0, b1 = (lane & 2) != 0, b3 = (lane & 8) != 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = (b0 ? acc[r + 4] : acc[r]) + from_lane<DPP_XOR1>(b0 ? acc[r] : acc[r + 4]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) acc[r] = (b1 ? acc[r + 2] : acc[r]) + from_lane<DPP_XOR2>(b1 ? acc[r] : acc[r + 2]);
+        float s = (b3 ? acc[1] : acc[0]) + from_lane<DPP_XOR8>(b3 ? acc[0] : acc[1]);
+        s += swizzle_xor<4>(s);
+        s += swizzle_xor<16>(s);
+        s += __shfl_xor(s, 32, 64);
+        __syncthreads();
+        if ((lane & 52) == 0) red[wave * 8 + (b0 ? 4 : 0) + (b1 ? 2 : 0) + (b3 ? 1 : 0)] = s;
+        __syncthreads();
+        for (int i = (int) threadIdx.x; i < here * 8; i += WAVES * 64) {
+            const int r = 8 * (g0 + i / 8) + i % 8;
+            float sum = 0.f;
+            for (int k = 0; k < per; ++k) sum += red[(k * here + i / 8) * 8 + i % 8];
+            if (r < R) sink(0, r, sum);
         }
     }
 }
 
-// out[t][n] = base[t][n] + scale sum_r h[t][r] W(n, r): W(n, r) is w[n][r] (B) or, with
-// OUTER, w[r][n] (A). Blocks: (tile, LE_COLS of n). h comes in `parts` parts that are
-// summed here; where there is more than one, the workgroups of the first columns store the sum.
-// The weights are the first operand, so a lane's four sums are neighbours in n of one token.
-template <int TYPE, bool OUTER>
-__global__ __launch_bounds__(LE_THREADS) void k_expand(const float* __restrict__ h, int parts, Matrix wm, int R, Batch b,
-                                                        bool scaled, const uint8_t* base, size_t base_nb1, int64_t N,
-                                                        uint8_t* out, size_t out_nb1, float* __restrict__ h_sum) {
+// out[t][n] = base[t][n] + sum_r hs[t][r] W(n, r) for n in n_lo .. n_hi-1: W(n, r) is w[n][r] (B)
+// or, with OUTER, w[r][n] (A). hs has rows of Rp + 4 floats with zeros from R to Rp, R
+// rounded up to 16 RT. A wave makes 64 columns of the 16 tokens at a time; column
+// 4 (l % 16) + c of the 64 is tile c's, so a lane has four neighbours of each of its four
+// tokens, and base and out are read and written in runs of 256 bytes.
+template <int TYPE, bool OUTER, int WAVES, int RT>
+struct Expand {
     typedef Wt<TYPE> W;
-    const Tile t = find_tile(b, blockIdx.x);
-    if (t.tokens == 0) return;
-    const int64_t n_lo = (int64_t) blockIdx.y * LE_COLS, n_hi = min(n_lo + LE_COLS, N);
-    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    const int Rp = (R + 15) / 16 * 16;
-    // h of the tile, [token][r] with a row of 4 more floats than Rp: 16-byte rows that start on other banks
-    __shared__ __attribute__((aligned(16))) float hs[LT * (L_MAX_RANK + 4)];
-    const int hrow = Rp + 4;
-    const float s = t.adapter >= 0 && scaled ? b.scale[t.adapter] : 1.f;
-    for (int i = (int) threadIdx.x; i < LT * Rp; i += LE_THREADS) {
+    typedef typename W::Elem Elem;
+    typedef typename W::template Raw<4> Raw4;
+    static constexpr int ES = sizeof(Elem);
+    // 16 of the rank, as loaded. A: [k] is row r0 + 4 quad + k, columns 4 col .. + 3. B: [i] is row
+    // 16 i + lane / 4 of the 64, r0 + 4 (lane % 4) .. + 3; it is turned through LDS.
+    struct Weights {
+        Raw4 w[4];
+    };
+    // B in LDS: row n of the 64 is (n % 4, n / 4), since a lane reads rows 4 col + c; the
+    // paddings spread both the rows of a store and those of a read over the banks.
+    static constexpr int PITCH = ES == 4 ? 80 : 40, BLOCK = 16 * PITCH + (ES == 4 ? 64 : 32);
+    static constexpr int LDS = OUTER ? 0 : 4 * BLOCK;  // bytes of a wave
+    struct Base {
+        f4u b[4];
+    };
+    const Tile& t;
+    const uint8_t *w, *bp, *op;
+    uint32_t wrow;
+    uint8_t* lds;
+    int R, lane, col, quad, wave;
+    bool based;
+    int64_t N, n_lo, steps;  // steps: whole ones
+    uint32_t bo[4], oo[4];
+    Base first;
+
+    __device__ __forceinline__ Expand(const Tile& t, const Matrix& wm, int R, const uint8_t* base, size_t base_nb1, int64_t N,
+                                      uint8_t* out, size_t out_nb1, int64_t n_lo, int64_t n_hi, uint8_t* all_lds)
+        : t(t), R(R), based(base != nullptr), N(min(n_hi, N)), n_lo(n_lo) {
+        lane = (int) threadIdx.x & 63;
+        col = lane & 15;
+        quad = lane >> 4;
+        wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+        lds = all_lds + wave * LDS;
+        w = (const uint8_t*) wm.p + max(t.adapter, 0) * wm.adapter * ES;
+        wrow = (uint32_t) wm.row * ES;
+        bp = base + (int64_t) t.lo * base_nb1;
+        op = out + (int64_t) t.lo * out_nb1;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {  // (tokens past the tile's read the last one's base and are not stored)
+            const uint32_t tok = (uint32_t) min(4 * quad + v, t.tokens - 1);
+            bo[v] = tok * (uint32_t) base_nb1 + 16 * col;
+            oo[v] = tok * (uint32_t) out_nb1 + 16 * col;
+        }
+        steps = (this->N - n_lo) / LE_COLS;
+    }
+    // Whether weights are loaded in fours of r; of the fours past R the last one is read again.
+    __device__ __forceinline__ bool fours() const { return R % 4 == 0; }
+    // Whether this is a tile of 16 tokens with all that the pipelined loop takes for granted.
+    __device__ __forceinline__ bool full() const { return t.tokens == LT && t.adapter >= 0 && based && fours(); }
+
+    __device__ __forceinline__ void load(Weights& s, int64_t n0, int r0) const {
+        const uint32_t r = (uint32_t) min(r0 + 4 * (OUTER ? quad : lane & 3), R - 4);
+        const uint32_t o = OUTER ? r * wrow + 4 * col * ES : (lane >> 2) * wrow + r * ES;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s.w[k] = load_at<Raw4>(OUTER ? w + n0 * ES + k * (int64_t) wrow : w + (n0 + 16 * k) * wrow, o);
+    }
+    __device__ __forceinline__ void load(Base& s, int64_t n0) const {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s.b[v] = load_at<f4u>(bp + n0 * 4, bo[v]);
+    }
+    // A full tile's base is read and its outputs are written once, past the caches: 4096 x 4096 outputs in 44 us
+    // where plain accesses take 50.
+    __device__ __forceinline__ void stream(Base& s, int64_t n0) const {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s.b[v] = __builtin_nontemporal_load((const f4u*) (bp + n0 * 4 + bo[v]));
+    }
+    // The first columns' base, long before run() where there are registers for it.
+    static constexpr bool EARLY = RT == 1;
+    __device__ __forceinline__ void start() {
+        if (EARLY && full() && wave < steps) stream(first, n_lo + wave * LE_COLS);
+    }
+    // zeros past R, whatever was read there
+    __device__ __forceinline__ void multiply(const Weights& s, const float* hrow, int r0, f4 (&acc)[4]) const {
+        typedef std::conditional_t<ES == 4, f4, h4> Four;
+        const f4 hv = *(const f4*) (hrow + r0);
+        const bool in = r0 + 16 <= R || r0 + 4 * quad < R;
+        Four v[4];
+        if constexpr (!OUTER) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = 16 * i + (lane >> 2);
+                *(Four*) (lds + (n & 3) * BLOCK + (n >> 2) * PITCH + 4 * (lane & 3) * ES) = (Four) s.w[i];
+            }
+            lds_in_order();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = *(const Four*) (lds + c * BLOCK + col * PITCH + 4 * quad * ES);
+            lds_in_order();
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float x = W::get(OUTER ? s.w[k][c] : v[c][k]);
+                acc[c] = mfma(hv[k], in ? x : 0.f, acc[c]);
+            }
+        }
+    }
+    // All of the rank: the first RT blocks of 16 with the next one's loads under way (and `last` after
+    // the last of them), then the others.
+    template <class Last>
+    __device__ __forceinline__ void product(const float* hrow, int64_t n0, f4 (&acc)[4], Last&& last) const {
+        Weights s[2];
+        load(s[0], n0, 0);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            if (j + 1 < RT) load(s[(j + 1) & 1], n0, 16 * (j + 1));
+            if (j + 2 == RT || RT == 1) last();
+            loads_stay();
+            multiply(s[j & 1], hrow, 16 * j, acc);
+        }
+        for (int r0 = 16 * RT; r0 < R; r0 += 16) {
+            load(s[0], n0, r0);
+            multiply(s[0], hrow, r0, acc);
+        }
+    }
+    static __device__ __forceinline__ f4 row(const f4 (&acc)[4], int v) { return f4{acc[0][v], acc[1][v], acc[2][v], acc[3][v]}; }
+
+    // One step of a full tile, the next one's base (at next, or none) under way behind its weights, since
+    // loads arrive in the order they are waited for. Its stores have no branch around them, so that the
+    // wait for the loads behind them is counted and does not wait for the stores.
+    template <bool NEXT>
+    __device__ __forceinline__ void step(const Base& b, const float* hrow, int64_t n0, Base& next, int64_t n_next) const {
+        f4 acc[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
+        product(hrow, n0, acc, [&] {
+            if (NEXT) stream(next, n_next);
+        });
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const f4u sum = row(acc, v) + b.b[v];
+            __builtin_nontemporal_store(sum, (f4u*) ((uint8_t*) op + n0 * 4 + oo[v]));
+        }
+    }
+    __device__ __forceinline__ void whole_steps(const float* hrow) const {
+        constexpr int64_t S = WAVES * LE_COLS;
+        int64_t n0 = n_lo + wave * LE_COLS, left = (steps - 1 - wave) / WAVES;
+        Base b0, b1;
+        if constexpr (EARLY) {
+            b0 = first;
+        } else {
+            stream(b0, n0);
+        }
+        for (; left > 1; left -= 2) {
+            step<true>(b0, hrow, n0, b1, n0 + S);
+            step<true>(b1, hrow, n0 + S, b0, n0 + 2 * S);
+            n0 += 2 * S;
+        }
+        if (left > 0) {
+            step<true>(b0, hrow, n0, b1, n0 + S);
+            step<false>(b1, hrow, n0 + S, b0, 0);
+        } else {
+            step<false>(b0, hrow, n0, b1, 0);
+        }
+    }
+    // Weights one by one, for ranks that are not whole fours and for the last columns.
+    __device__ __forceinline__ void singly(const float* hrow, int64_t n0, f4 (&acc)[4]) const {
+        const uint8_t* const wn = w + n0 * (OUTER ? (int64_t) ES : (int64_t) wrow);
+        uint32_t nc[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) nc[c] = (uint32_t) min((int64_t) (4 * col + c), N - 1 - n0) * (OUTER ? ES : wrow);
+        for (int r0 = 0; r0 < R; r0 += 4) {  // four of r, one for each quad
+            const int r = r0 + quad;
+            const uint32_t rc = (uint32_t) min(r, R - 1) * (OUTER ? wrow : ES);
+            const float hv = hrow[r0 - 3 * quad];
+            Elem x[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[c] = load_at<Elem>(wn, nc[c] + rc);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = mfma(hv, r < R ? W::get(x[c]) : 0.f, acc[c]);
+        }
+    }
+    // One step of any tile and any columns.
+    __device__ __forceinline__ void any_step(const float* hrow, int64_t n0) const {
+        const bool whole = n0 + LE_COLS <= N;
+        Base b;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) b.b[v] = f4{0.f, 0.f, 0.f, 0.f};
+        if (based && whole) load(b, n0);
+        if (based && !whole) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int back = (int) min((int64_t) (4 * col + k), N - 1 - n0) - 4 * col;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) b.b[v][k] = load_at<float>(bp + n0 * 4, (uint32_t) ((int) bo[v] + 4 * back));
+            }
+        }
+        f4 acc[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
+        if (t.adapter >= 0) {
+            if (whole && fours()) {
+                product(hrow, n0, acc, [] {});
+            } else {
+                singly(hrow, n0, acc);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            if (4 * quad + v >= t.tokens) continue;
+            const f4 sum = row(acc, v) + b.b[v];
+            uint8_t* const p = (uint8_t*) op + n0 * 4 + oo[v];
+            if (whole) {
+                *(f4u*) p = sum;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n0 + 4 * col + k < N) *(float*) (p + 4 * k) = sum[k];
+            }
+        }
+    }
+    __device__ __forceinline__ void run(const float* hs) const {
+        const float* const hrow = hs + col * ((R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4) + 4 * quad;
+        int64_t i = wave;
+        if (full() && i < steps) {
+            whole_steps(hrow);
+            i += ((steps - 1 - wave) / WAVES + 1) * WAVES;
+        }
+        for (; n_lo + i * LE_COLS < N; i += WAVES) any_step(hrow, n_lo + i * LE_COLS);
+    }
+};
+
+// The same of one token and B, without the matrix instructions. 16 bytes of a row of B are a lane's,
+// G lanes (a power of two) make one output together, so a wave reads 1 KB of rows side by side at a time.
+template <int TYPE, int WAVES>
+struct ExpandOne {
+    typedef Wt<TYPE> W;
+    typedef typename W::Elem Elem;
+    static constexpr int ES = sizeof(Elem), E = 16 / ES, U = 4;
+    const uint8_t* w;
+    uint32_t wrow;
+    const float* bt;
+    float* ot;
+    int R, lane, G, logG, r0, per;  // per: outputs of a wave at a time
+    int64_t n_lo, n_hi;
+    f4v raw[U];
+    float b[U];
+
+    __device__ __forceinline__ ExpandOne(const Tile& t, const Matrix& wm, int R, const uint8_t* base, size_t base_nb1, int64_t N,
+                                         uint8_t* out, size_t out_nb1, int64_t lo, int64_t hi)
+        : R(R), lane((int) threadIdx.x & 63), G(1), logG(0) {
+        while (G * E < R) G <<= 1, ++logG;
+        r0 = (lane & (G - 1)) * E;
+        per = 64 >> logG;
+        w = (const uint8_t*) wm.p + t.adapter * wm.adapter * ES;
+        wrow = (uint32_t) wm.row * ES;
+        bt = base != nullptr ? (const float*) (base + (int64_t) t.lo * base_nb1) : nullptr;
+        ot = (float*) (out + (int64_t) t.lo * out_nb1);
+        n_lo = lo + __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6) * (per * U);
+        n_hi = min(hi, N);
+    }
+    __device__ __forceinline__ uint32_t output(int u, int64_t n0) const {
+        return (uint32_t) min((int64_t) (u * per + (lane >> logG)), n_hi - 1 - n0);
+    }
+    __device__ __forceinline__ void load(int64_t n0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = output(u, n0);
+            if (R % E == 0) raw[u] = load_at<v16u>(w + n0 * (int64_t) wrow, i * wrow + (uint32_t) min(r0, R - E) * ES).v;
+            b[u] = bt != nullptr ? load_at<float>(bt + n0, 4 * i) : 0.f;
+        }
+    }
+    // The first outputs' loads, which may be long before run().
+    __device__ __forceinline__ void start() {
+        if (n_lo < n_hi) load(n_lo);
+    }
+    __device__ __forceinline__ void run(const float* hs) {
+        float hv[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) hv[e] = r0 + e < R ? hs[r0 + e] : 0.f;
+        for (int64_t n0 = n_lo; n0 < n_hi; n0 += WAVES * per * U) {
+            if (n0 != n_lo) load(n0);
+            float sum[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Elem x[E];
+                if (R % E == 0) {
+                    __builtin_memcpy(x, &raw[u], 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        x[e] = load_at<Elem>(w + n0 * (int64_t) wrow, output(u, n0) * wrow + (uint32_t) min(r0 + e, R - 1) * ES);
+                }
+                sum[u] = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[u] = fmaf(hv[e], r0 + e < R ? W::get(x[e]) : 0.f, sum[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (G > 1) sum[u] += from_lane<DPP_XOR1>(sum[u]);
+                if (G > 2) sum[u] += from_lane<DPP_XOR2>(sum[u]);
+                if (G > 4) sum[u] += swizzle_xor<4>(sum[u]);
+                if (G > 8) sum[u] += from_lane<DPP_XOR8>(sum[u]);
+                if (G > 16) sum[u] += swizzle_xor<16>(sum[u]);
+                if (G > 32) sum[u] += __shfl_xor(sum[u], 32, 64);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t n = n0 + u * per + (lane >> logG);
+                if ((lane & (G - 1)) == 0 && n < n_hi) ot[n] = b[u] + sum[u];
+            }
+        }
+    }
+};
+
+// The tile's h as Expand wants it: the sum of its parts times s.
+template <int RT>
+__device__ __forceinline__ void stage_h(const Tile& t, const float* __restrict__ h, int parts, int64_t T, int R, float s,
+                                        float* __restrict__ h_sum, float* hs, int threads) {
+    const int Rp = (R + 16 * RT - 1) / (16 * RT) * (16 * RT);
+    for (int i = (int) threadIdx.x; i < LT * Rp; i += threads) {
         const int tok = i / Rp, r = i % Rp;
         float v = 0.f;
         if (tok < t.tokens && r < R && t.adapter >= 0) {
-            for (int p = 0; p < parts; ++p) v += h[((int64_t) p * b.T + t.lo + tok) * R + r];
+            const float* const p = h + (int64_t) (t.lo + tok) * R + r;
+            int k = 0;
+            for (; k + 4 <= parts; k += 4) {
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = p[(k + j) * T * R];
+                v += ((x[0] + x[1]) + x[2]) + x[3];
+            }
+            for (; k < parts; ++k) v += p[k * T * R];
         }
-        if (h_sum != nullptr && blockIdx.y == 0 && tok < t.tokens && r < R) h_sum[(t.lo + tok) * R + r] = v;
-        hs[tok * hrow + r] = v * s;
+        if (h_sum != nullptr && tok < t.tokens && r < R) h_sum[(int64_t) (t.lo + tok) * R + r] = v;
+        hs[tok * (Rp + 4) + r] = v * s;
     }
     __syncthreads();
-    const bool here = col < t.tokens;
-    const int64_t tok = t.lo + (here ? col : 0);
-    const float* const bt = base != nullptr ? (const float*) (base + tok * base_nb1) : nullptr;
-    float* const ot = (float*) (out + tok * out_nb1);
-    const typename W::Elem* const w = t.adapter >= 0 ? (const typename W::Elem*) wm.p + t.adapter * wm.adapter : nullptr;
-    for (int64_t n0 = n_lo + wave * 16; n0 < n_hi; n0 += LE_THREADS / 64 * 16) {
-        const int64_t n = n0 + 4 * quad;  // the first of this lane's four outputs
-        f4 acc = {0.f, 0.f, 0.f, 0.f};
-        f4 bv = acc;
-        if (bt != nullptr && here) {
-            if (n + 4 <= N) {
-                bv = *(const f4u*) (bt + n);
-            } else {
-                for (int k = 0; n + k < N; ++k) bv[k] = bt[n + k];
-            }
-        }
-        if (w != nullptr) {
-            const int64_t nw = min(n0 + col, N - 1);  // this lane's row of weights
-            for (int r = 4 * quad; r < Rp; r += 16) {
-                const f4 hv = *(const f4*) (hs + col * hrow + r);
-                f4 wv;
-                if (!OUTER && r + 4 <= R) {
-                    wv = W::get4(w + nw * wm.row + r);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        wv[k] = r + k < R ? W::get(OUTER ? w[(int64_t) (r + k) * wm.row + nw] : w[nw * wm.row + r + k]) : 0.f;
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc = mfma(wv[k], hv[k], acc);
-            }
-        }
-        if (!here) continue;
-        acc += bv;
-        if (n + 4 <= N) {
-            *(f4u*) (ot + n) = acc;
-        } else {
-            for (int k = 0; n + k < N; ++k) ot[n + k] = acc[k];
-        }
+}
+
+__device__ __forceinline__ void zero_h(const Tile& t, int R, int r0, int rn, float* out, int threads) {
+    for (int i = (int) threadIdx.x; i < t.tokens * rn; i += threads) {
+        const int r = r0 + i % rn;
+        if (r < R) out[(int64_t) (t.lo + i / rn) * R + r] = 0.f;
     }
 }
 
-// d(n, r) (+)= scale sum_t x[t][n] h[t][r] over the tokens of one adapter's requests:
-// d(n, r) is d[n][r] (dB), or d[r][n] with ROWS (dA). Blocks: (64 of n, 64 of the rank,
-// adapter). Each wave takes four tokens at a time; a lane of x holds the four columns
-// 4 * (lane % 16) .. + 3 of one token, which feed four accumulators.
-template <bool ROWS, int RT>
-__global__ __launch_bounds__(LO_THREADS) void k_outer(const uint8_t* __restrict__ x, size_t x_nb1, int64_t N,
-                                                       const float* __restrict__ h, int R, Batch b, bool scaled, float* d,
-                                                       int64_t d_row, int64_t d_adapter, bool accumulate) {
-    constexpr int WAVES = LO_THREADS / 64;
-    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-    const int64_t n0 = (int64_t) blockIdx.x * 64;
-    const int r0 = (int) blockIdx.y * LR, adapter = (int) blockIdx.z;
-    const int64_t n = n0 + 4 * col;  // this lane's columns of x
-    f4 acc[4][RT];
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int j = 0; j < RT; ++j) acc[c][j] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int q = 0; q < b.requests; ++q) {
-        if (b.ids[q] != adapter) continue;
-        const int64_t lo = min(max((int64_t) b.start[q], (int64_t) 0), b.T);
-        const int64_t hi = min(max((int64_t) b.start[q + 1], lo), b.T);
-        for (int64_t t0 = lo + 4 * wave; t0 < hi; t0 += 4 * WAVES) {
-            const int64_t t = t0 + quad;
-            f4 xv = {0.f, 0.f, 0.f, 0.f};
-            float hv[RT];
-#pragma unroll
-            for (int j = 0; j < RT; ++j) hv[j] = 0.f;
-            if (t < hi) {
-                const float* const xt = (const float*) (x + t * x_nb1);
-                if (n + 4 <= N) {
-                    xv = *(const f4u*) (xt + n);
-                } else {
-                    for (int k = 0; n + k < N; ++k) xv[k] = xt[n + k];
-                }
-#pragma unroll
-                for (int j = 0; j < RT; ++j) hv[j] = h[t * R + min(r0 + 16 * j + col, R - 1)];
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int j = 0; j < RT; ++j) acc[c][j] = mfma(xv[c], hv[j], acc[c][j]);
+template <int TYPE, int WAVES, int RT>
+union ContractLds {
+    __attribute__((aligned(16))) uint8_t stage[WAVES * contract_lds<typename Wt<TYPE>::Elem>];
+    Partial<WAVES, RT> part;
+};
+// floats of a tile's h in LDS
+template <int RT>
+constexpr int h_floats = LT * ((RT == 4 ? L_MAX_RANK : 16 * RT) + 4);
+
+// h (or g, scaled) alone. Blocks: (tile, 16 RT of the rank, part of the long axis); part p
+// goes to out + p T R.
+template <int TYPE, bool OUTER, int WAVES, int RT>
+__device__ __forceinline__ void contract_block(int tile, int rank_block, int part_index, const Rows& x, const Matrix& wm,
+                                               int R, const Batch& b, bool scaled, int64_t part_len, float* out,
+                                               ContractLds<TYPE, WAVES, RT>& lds) {
+    const Tile t = find_tile(b, tile);
+    if (t.tokens == 0) return;
+    out += (int64_t) part_index * b.T * R;
+    const int r0 = rank_block * (16 * RT);
+    if (t.adapter < 0) {
+        zero_h(t, R, r0, 16 * RT, out, WAVES * 64);
+        return;
+    }
+    const float s = scaled ? b.scale[t.adapter] : 1.f;
+    const int64_t lo = (int64_t) part_index * part_len, hi = min(lo + part_len, x.n);
+    auto sink = [&](int tok, int r, float v) { out[(int64_t) (t.lo + tok) * R + r] = v * s; };
+    if (!OUTER && t.tokens == 1) {
+        if (rank_block == 0) contract_one<TYPE, WAVES>(t, x, wm, R, lo, hi, (float*) lds.stage, sink);
+    } else {
+        contract_tile<TYPE, OUTER, WAVES, RT>(t, x, wm, R, r0, lo, hi, lds.stage, lds.part, sink);
+    }
+}
+
+template <int TYPE, int RT>
+__global__ __launch_bounds__(512) L_FOUR_WAVES void k_contract(Rows x, Matrix wm, int R, Batch b, int64_t part_len, float* __restrict__ out) {
+    __shared__ ContractLds<TYPE, 8, RT> lds;
+    contract_block<TYPE, false, 8, RT>((int) blockIdx.x, (int) blockIdx.y, (int) blockIdx.z, x, wm, R, b, false, part_len, out,
+                                       lds);
+}
+
+// y of a tile's columns blockIdx.y * cols .. from h in parts; the first columns' workgroups
+// store the sum of more than one part.
+template <int TYPE, int RT>
+__global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float* __restrict__ h, int parts, Matrix wm, int R, Batch b,
+                                                        const uint8_t* base, size_t base_nb1, int64_t N, uint8_t* out,
+                                                        size_t out_nb1, float* __restrict__ h_sum, int cols) {
+    // Workgroups are dealt out to the 8 XCDs in turn: an XCD has every eighth slice of the columns, so that its
+    // L2 holds that part of the adapters alone.
+    const int tiles = (int) gridDim.x, slices = (int) gridDim.y, id = (int) (blockIdx.y * gridDim.x + blockIdx.x);
+    int tile = (int) blockIdx.x, slice = (int) blockIdx.y;
+    if (id < slices / 8 * 8 * tiles) {
+        tile = id / 8 % tiles;
+        slice = id / 8 / tiles * 8 + id % 8;
+    }
+    const Tile t = find_tile(b, tile);
+    if (t.tokens == 0) return;
+    typedef Expand<TYPE, false, LE_THREADS / 64, RT> E;
+    __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[LE_THREADS / 64 * E::LDS];
+    const int64_t n_lo = (int64_t) slice * cols;
+    const float s = t.adapter >= 0 ? b.scale[t.adapter] : 1.f;
+    float* const sums = n_lo == 0 ? h_sum : nullptr;
+    if (t.tokens == 1 && t.adapter >= 0) {
+        ExpandOne<TYPE, LE_THREADS / 64> e(t, wm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols);
+        e.start();
+        stage_h<RT>(t, h, parts, b.T, R, s, sums, hs, LE_THREADS);
+        e.run(hs);
+    } else {
+        E e(t, wm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols, stage);
+        e.start();
+        stage_h<RT>(t, h, parts, b.T, R, s, sums, hs, LE_THREADS);
+        e.run(hs);
+    }
+}
+
+// Both in one launch: a workgroup makes h of its tile for itself, then y of `cols` columns.
+template <int TYPE, int WAVES, int RT>
+__global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix am, Matrix bm, int R, Batch b, const uint8_t* base,
+                                                      size_t base_nb1, int64_t N, uint8_t* out, size_t out_nb1,
+                                                      float* __restrict__ h, int cols) {
+    const Tile t = find_tile(b, (int) blockIdx.x);
+    if (t.tokens == 0) return;
+    typedef Expand<TYPE, false, WAVES, RT> E;
+    __shared__ union {
+        ContractLds<TYPE, WAVES, RT> contract;
+        __attribute__((aligned(16))) uint8_t expand[WAVES * E::LDS];
+    } lds;
+    __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
+    const int hrow = (R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4;
+    const int64_t n_lo = (int64_t) blockIdx.y * cols;
+    const float s = t.adapter >= 0 ? b.scale[t.adapter] : 1.f;
+    auto sink = [&](int tok, int r, float v) {
+        hs[tok * hrow + r] = v * s;
+        if (blockIdx.y == 0) h[(int64_t) (t.lo + tok) * R + r] = v;
+    };
+    if (t.tokens == 1 && t.adapter >= 0) {
+        ExpandOne<TYPE, WAVES> e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols);
+        e.start();
+        contract_one<TYPE, WAVES>(t, x, am, R, 0, x.n, (float*) lds.contract.stage, sink);
+        __syncthreads();
+        e.run(hs);
+        return;
+    }
+    E e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols, lds.expand);
+    e.start();
+    if (t.adapter < 0) {
+        if (blockIdx.y == 0) zero_h(t, R, 0, R, h, WAVES * 64);
+    } else {
+        for (int i = (int) threadIdx.x; i < LT * hrow; i += WAVES * 64) hs[i] = 0.f;
+        __syncthreads();
+        for (int r0 = 0; r0 < R; r0 += 16 * RT) {
+            contract_tile<TYPE, false, WAVES, RT>(t, x, am, R, r0, 0, x.n, lds.contract.stage, lds.contract.part, sink);
+            __syncthreads();
         }
     }
-    // the waves' sums, joined in order, one accumulator of every wave at a time
-    __shared__ f4 part[WAVES][RT][64];
-    const float s = scaled ? b.scale[adapter] : 1.f;
-    d += adapter * d_adapter;
+    e.run(hs);
+}
+
+// d(n, r) (+)= scale sum_t x[t][n] h[t][r] over the tokens of one adapter's requests:
+// d(n, r) is d[n][r] (dB), or d[r][n] with ROWS (dA).
+struct Outer {
+    Rows x;
+    const float* h;
+    float* d;
+    int64_t d_row, d_adapter;
+    bool scaled, accumulate;
+    int col_blocks, rank_blocks, splits;  // blocks: columns fastest, then ranks, adapters, splits
+    int64_t split_len;                    // tokens
+    float* parts;                         // [split][adapter][n][r] where there is more than one split
+    int64_t blocks(int adapters) const { return (int64_t) col_blocks * rank_blocks * adapters * splits; }
+};
+
+// Each wave takes four tokens at a time; a lane holds two neighbouring columns of one
+// token, which feed two accumulators. The waves' sums are joined in order.
+template <bool ROWS, int RT>
+__device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R, const Batch& b, Partial<LO_WAVES, RT>& part) {
+    const int lane = (int) threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    const int64_t n0 = block % o.col_blocks * LO_COLS;
+    block /= o.col_blocks;
+    const int r0 = (int) (block % o.rank_blocks) * 16 * RT;
+    block /= o.rank_blocks;
+    const int adapter = (int) (block % b.adapters), split = (int) (block / b.adapters);
+    const int64_t t_lo = split * o.split_len, t_hi = min(t_lo + o.split_len, b.T);
+    const int64_t N = o.x.n;
+    const bool whole = n0 + LO_COLS <= N;
+    f4 acc[2][RT];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[c][j] = f4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 4;  // tokens of a lane that are loaded together
+    for (int q = 0; q < b.requests; ++q) {
+        if (b.ids[q] != adapter) continue;
+        const int64_t lo = max(min(max((int64_t) b.start[q], (int64_t) 0), b.T), t_lo);
+        const int64_t hi = min(max((int64_t) b.start[q + 1], lo), t_hi);
+        for (int64_t t0 = lo + 4 * U * wave; t0 < hi; t0 += 4 * U * LO_WAVES) {
+            // tokens past the last read it again, as zeros; columns past N read the last one
+            float xv[U][2], hv[U][RT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t t = (uint32_t) min((int64_t) (4 * u + quad), hi - 1 - t0);
+                const uint8_t* const xb = o.x.p + t0 * o.x.nb1 + n0 * 4;
+                if (whole) {
+                    const f2u v = load_at<f2u>(xb, t * (uint32_t) o.x.nb1 + 8 * col);
+                    xv[u][0] = v[0], xv[u][1] = v[1];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        xv[u][c] = load_at<float>(xb, t * (uint32_t) o.x.nb1 + 4 * (uint32_t) min((int64_t) (2 * col + c), N - 1 - n0));
+                }
+#pragma unroll
+                for (int j = 0; j < RT; ++j) hv[u][j] = load_at<float>(o.h + t0 * R, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
+            }
+            if (t0 + 4 * U > hi) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool in = t0 + 4 * u + quad < hi;
+                    xv[u][0] = in ? xv[u][0] : 0.f, xv[u][1] = in ? xv[u][1] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) hv[u][j] = in ? hv[u][j] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) acc[c][j] = mfma(xv[u][c], hv[u][j], acc[c][j]);
+        }
+    }
+    const float s = o.scaled ? b.scale[adapter] : 1.f;
+    float* const d = o.d + adapter * o.d_adapter;
+    float* const p = o.parts + ((int64_t) split * b.adapters + adapter) * N * R;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < RT; ++j) part[wave][j][lane] = acc[c][j];
         __syncthreads();
-        for (int i = (int) threadIdx.x; i < RT * 64; i += LO_THREADS) {
-            const int j = i >> 6, l = i & 63, r = r0 + 16 * j + (l & 15);
-            f4 sum = part[0][j][l];
-#pragma unroll
-            for (int v = 1; v < WAVES; ++v) sum += part[v][j][l];
-            if (r >= R) continue;
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int64_t at = n0 + 4 * (4 * (l >> 4) + v) + c;
-                if (at >= N) continue;
-                float* const p = d + (ROWS ? r * d_row + at : at * d_row + r);
-                *p = accumulate ? *p + sum[v] * s : sum[v] * s;
+        for (int e = (int) threadIdx.x; e < RT * 256; e += LO_WAVES * 64) {
+            const float sum = joined<LO_WAVES, RT>(part, e);
+            const int l = (e >> 2) & 63, r = r0 + 16 * (e >> 8) + (l & 15);
+            const int64_t at = n0 + 2 * (4 * (l >> 4) + (e & 3)) + c;
+            if (r >= R || at >= N) continue;
+            if (o.splits > 1) {
+                p[at * R + r] = sum;
+            } else {
+                float* const q = d + (ROWS ? r * o.d_row + at : at * o.d_row + r);
+                *q = o.accumulate ? *q + sum * s : sum * s;
             }
         }
     }
+}
+
+// The first launch of the backward pass: dB, then g.
+template <int TYPE, int RT>
+__global__ __launch_bounds__(LO_WAVES * 64) void k_back_b(Outer o, int outers, Rows dy, Matrix bm, int R, Batch b,
+                                                           float* __restrict__ g) {
+    __shared__ ContractLds<TYPE, LO_WAVES, RT> lds;
+    if ((int) blockIdx.x < outers) {
+        outer_block<false, RT>(blockIdx.x, o, R, b, lds.part);
+    } else {
+        const int i = (int) blockIdx.x - outers, rank_blocks = (R + 16 * RT - 1) / (16 * RT);
+        contract_block<TYPE, true, LO_WAVES, RT>(i / rank_blocks, i % rank_blocks, 0, dy, bm, R, b, true, dy.n, g, lds);
+    }
+}
+
+// The second: dA, then dx.
+template <int TYPE, int RT>
+__global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, const float* __restrict__ g, Matrix am, int R,
+                                                           Batch b, const uint8_t* base, size_t base_nb1, int64_t N,
+                                                           uint8_t* dx, size_t dx_nb1, int cols) {
+    __shared__ union {
+        Partial<LO_WAVES, RT> part;
+        float hs[h_floats<RT>];
+    } lds;
+    if ((int) blockIdx.x < outers) {
+        outer_block<true, RT>(blockIdx.x, o, R, b, lds.part);
+    } else {
+        const int i = (int) blockIdx.x - outers, slices = (int) ((N + cols - 1) / cols);
+        const Tile t = find_tile(b, i / slices);
+        if (t.tokens == 0) return;
+        const int64_t n_lo = (int64_t) (i % slices) * cols;
+        Expand<TYPE, true, LO_WAVES, RT> e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
+        e.start();
+        stage_h<RT>(t, g, 1, b.T, R, 1.f, nullptr, lds.hs, LO_WAVES * 64);
+        e.run(lds.hs);
+    }
+}
+
+// Gradients whose tokens were split: the parts in order.
+__global__ __launch_bounds__(256) void k_back_join(Outer o, bool rows, int R, Batch b) {
+    const int64_t N = o.x.n, per = N * R, all = per * b.adapters;
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= all) return;
+    float sum = 0.f;
+    for (int k = 0; k < o.splits; ++k) sum += o.parts[k * all + i];
+    const int64_t a = i / per, n = i % per / R, r = i % R;
+    if (o.scaled) sum *= b.scale[a];
+    float* const e = o.d + a * o.d_adapter + (rows ? r * o.d_row + n : n * o.d_row + r);
+    *e = o.accumulate ? *e + sum : sum;
 }
 
 struct Call {
@@ -352,79 +1083,85 @@ Call call_of(const trc_hip_lora_set& q, int64_t T, hipStream_t s) {
             q.a.type, (int) q.a.ne[1], s};
 }
 
+Rows rows_of(const trc_hip_tensor& t) { return {(const uint8_t*) t.data, t.nb[1], t.ne[0]}; }
+
+template <class F>
+void with_type(int type, F&& f) {
+    if (type == TRC_HIP_TYPE_F32) f(std::integral_constant<int, TRC_HIP_TYPE_F32>());
+    if (type == TRC_HIP_TYPE_F16) f(std::integral_constant<int, TRC_HIP_TYPE_F16>());
+    if (type == TRC_HIP_TYPE_BF16) f(std::integral_constant<int, TRC_HIP_TYPE_BF16>());
+}
+// f with the tiles of 16 that a rank is summed in at a time
+template <class F>
+void with_rank(int R, F&& f) {
+    if (R <= 16) return f(std::integral_constant<int, 1>());
+    if (R <= 32) return f(std::integral_constant<int, 2>());
+    f(std::integral_constant<int, 4>());
+}
+int rank_blocks(int R) { return R <= 16 ? 1 : R <= 32 ? 1 : (R + LR - 1) / LR; }
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
 // The long axis in parts where the tiles leave CUs idle, of 1024 or more each; the
 // parts' sums are kept in the stream's workspace.
 int64_t contract_parts(const Call& c, int64_t N) {
-    const int64_t blocks = c.tiles() * ((c.R + LR - 1) / LR);
+    const int64_t blocks = c.tiles() * rank_blocks(c.R);
     int64_t parts = std::min(device_cus() / std::max(blocks, (int64_t) 1), N / 1024);
     const int64_t room = (int64_t) (qm_workspace_bytes() / sizeof(float)) / (c.batch.T * c.R);
     parts = std::min(parts, std::min(room, (int64_t) 16));
     return std::max(parts, (int64_t) 1);
 }
 
-template <bool OUTER>
-int contract(const Call& c, const trc_hip_tensor& x, const Matrix& w, bool scaled, int64_t parts, float* out) {
-    const int64_t N = x.ne[0];
-    const int64_t len = parts > 1 ? ((N + parts - 1) / parts + 63) / 64 * 64 : N;
-    const dim3 grid((unsigned) c.tiles(), (unsigned) ((c.R + LR - 1) / LR), (unsigned) parts);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(LC_THREADS), 0, c.s, (const uint8_t*) x.data, x.nb[1], N, w, c.R, c.batch, scaled,
-                           len, out);
-    };
-    auto ranks = [&](auto type) {
-        constexpr int TYPE = decltype(type)::value;
-        if (c.R <= 16) return go(k_contract<TYPE, OUTER, 1>);
-        if (c.R <= 32) return go(k_contract<TYPE, OUTER, 2>);
-        return go(k_contract<TYPE, OUTER, 4>);
-    };
-    if (c.type == TRC_HIP_TYPE_F32) ranks(std::integral_constant<int, TRC_HIP_TYPE_F32>());
-    if (c.type == TRC_HIP_TYPE_F16) ranks(std::integral_constant<int, TRC_HIP_TYPE_F16>());
-    if (c.type == TRC_HIP_TYPE_BF16) ranks(std::integral_constant<int, TRC_HIP_TYPE_BF16>());
-    return check_launch("lora (contract)");
-}
-
-template <bool OUTER>
-int expand(const Call& c, const float* h, int64_t parts, const Matrix& w, bool scaled, const trc_hip_tensor* base,
-           const trc_hip_tensor& out, float* h_sum) {
-    const int64_t N = out.ne[0];
-    const dim3 grid((unsigned) c.tiles(), (unsigned) ((N + LE_COLS - 1) / LE_COLS));
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(LE_THREADS), 0, c.s, h, (int) parts, w, c.R, c.batch, scaled,
-                           base != nullptr ? (const uint8_t*) base->data : nullptr, base != nullptr ? base->nb[1] : (size_t) 0, N,
-                           (uint8_t*) out.data, out.nb[1], parts > 1 ? h_sum : nullptr);
-    };
-    if (c.type == TRC_HIP_TYPE_F32) go(k_expand<TRC_HIP_TYPE_F32, OUTER>);
-    if (c.type == TRC_HIP_TYPE_F16) go(k_expand<TRC_HIP_TYPE_F16, OUTER>);
-    if (c.type == TRC_HIP_TYPE_BF16) go(k_expand<TRC_HIP_TYPE_BF16, OUTER>);
+int forward_apart(const Call& c, const trc_hip_tensor& x, const trc_hip_tensor* base, const trc_hip_tensor& h,
+                  const trc_hip_tensor& dst) {
+    const int64_t K = x.ne[0], M = dst.ne[0], parts = contract_parts(c, K);
+    const int64_t len = parts > 1 ? round_up((K + parts - 1) / parts, 64) : K;
+    float* sums = (float*) h.data;
+    if (parts > 1) {
+        uint8_t* ws = nullptr;
+        const int rc = qm_stream_workspace(c.s, &ws);
+        if (rc != TRC_HIP_OK) return rc;
+        sums = (float*) ws;
+    }
+    with_type(c.type, [&](auto type) {
+        with_rank(c.R, [&](auto rt) {
+            hipLaunchKernelGGL((k_contract<decltype(type)::value, decltype(rt)::value>),
+                               dim3((unsigned) c.tiles(), (unsigned) rank_blocks(c.R), (unsigned) parts), dim3(512), 0, c.s,
+                               rows_of(x), c.a, c.R, c.batch, len, sums);
+        });
+    });
+    int rc = check_launch("lora (contract)");
+    if (rc != TRC_HIP_OK) return rc;
+    // four workgroups a CU at a time, of at least 256 columns (a step of each wave)
+    const int64_t slices = std::max(std::min(4 * device_cus() / c.tiles(), (M + 255) / 256), (int64_t) 1);
+    const int cols = (int) round_up((M + slices - 1) / slices, 256);
+    with_type(c.type, [&](auto type) {
+        with_rank(c.R, [&](auto rt) {
+            hipLaunchKernelGGL((k_expand<decltype(type)::value, decltype(rt)::value>),
+                               dim3((unsigned) c.tiles(), (unsigned) ((M + cols - 1) / cols)), dim3(LE_THREADS), 0, c.s, sums,
+                               (int) parts, c.b, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
+                               base != nullptr ? base->nb[1] : (size_t) 0, M, (uint8_t*) dst.data, dst.nb[1],
+                               parts > 1 ? (float*) h.data : nullptr, cols);
+        });
+    });
     return check_launch("lora (expand)");
 }
 
-template <bool ROWS>
-int outer(const Call& c, const trc_hip_tensor& x, const float* h, bool scaled, const trc_hip_tensor& d, bool accumulate) {
-    const int64_t N = x.ne[0];
-    const dim3 grid((unsigned) ((N + 63) / 64), (unsigned) ((c.R + LR - 1) / LR), (unsigned) c.batch.adapters);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(LO_THREADS), 0, c.s, (const uint8_t*) x.data, x.nb[1], N, h, c.R, c.batch, scaled,
-                           (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), accumulate);
-    };
-    if (c.R <= 16) {
-        go(k_outer<ROWS, 1>);
-    } else if (c.R <= 32) {
-        go(k_outer<ROWS, 2>);
-    } else {
-        go(k_outer<ROWS, 4>);
+// How a gradient's blocks are laid out: tokens split where there are few column blocks, 512
+// or more each, while the parts fit into `room` floats at `ws`.
+Outer outer_of(const Call& c, const trc_hip_tensor& x, const float* h, const trc_hip_tensor& d, bool scaled, bool accumulate,
+               float* ws, int64_t room) {
+    Outer o{rows_of(x), h, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate, 0, 0, 1, c.batch.T, ws};
+    o.col_blocks = (int) ((x.ne[0] + LO_COLS - 1) / LO_COLS);
+    o.rank_blocks = rank_blocks(c.R);
+    const int64_t blocks = o.blocks(c.batch.adapters), T = c.batch.T;
+    int64_t n = std::min((int64_t) device_cus() / blocks, T / 512);
+    n = std::min(n, room / (x.ne[0] * c.R * c.batch.adapters));
+    if (n > 1) {
+        o.split_len = round_up((T + n - 1) / n, 64);
+        o.splits = (int) ((T + o.split_len - 1) / o.split_len);
     }
-    return check_launch("lora (gradients)");
-}
-
-int parts_of(const Call& c, int64_t N, float* whole, int64_t* parts, float** out) {
-    *parts = contract_parts(c, N);
-    *out = whole;
-    if (*parts == 1) return TRC_HIP_OK;
-    uint8_t* ws = nullptr;
-    const int rc = qm_stream_workspace(c.s, &ws);
-    *out = (float*) ws;
-    return rc;
+    return o;
 }
 
 }  // namespace
@@ -432,29 +1169,74 @@ int parts_of(const Call& c, int64_t N, float* whole, int64_t* parts, float** out
 int launch_lora(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hip_tensor* base, const trc_hip_tensor& h,
                 const trc_hip_tensor& dst, hipStream_t s) {
     const Call c = call_of(q, x.ne[1], s);
-    int64_t parts = 1;
-    float* sums = nullptr;
-    int rc = parts_of(c, x.ne[0], (float*) h.data, &parts, &sums);
-    if (rc != TRC_HIP_OK) return rc;
-    rc = contract<false>(c, x, c.a, false, parts, sums);
-    if (rc != TRC_HIP_OK) return rc;
-    return expand<false>(c, sums, parts, c.b, true, base, dst, (float*) h.data);
+    const int64_t K = x.ne[0], M = dst.ne[0], tiles = c.tiles();
+    // One launch, every workgroup of a tile making h for itself, unless that is much to read.
+    const int64_t slices = std::max(std::min(device_cus() / tiles, (M + 255) / 256), (int64_t) 1);
+    const int64_t again = K * (c.R * (c.type == TRC_HIP_TYPE_F32 ? 4 : 2) + LT * 4);
+    if (slices > 1 && again > ((int64_t) 1 << 19)) return forward_apart(c, x, base, h, dst);
+    const int cols = (int) round_up((M + slices - 1) / slices, LE_COLS);
+    with_type(c.type, [&](auto type) {
+        with_rank(c.R, [&](auto rt) {
+            constexpr int TYPE = decltype(type)::value, RT = decltype(rt)::value;
+            auto go = [&](auto kernel, int threads) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned) tiles, (unsigned) ((M + cols - 1) / cols)), dim3((unsigned) threads), 0, s,
+                                   rows_of(x), c.a, c.b, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
+                                   base != nullptr ? base->nb[1] : (size_t) 0, M, (uint8_t*) dst.data, dst.nb[1], (float*) h.data,
+                                   cols);
+            };
+            go(k_lora<TYPE, 16, RT>, 1024);
+        });
+    });
+    return check_launch("lora");
 }
 
 int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hip_tensor& h, const trc_hip_tensor& dy,
                      const trc_hip_tensor& g, const trc_hip_tensor* base, const trc_hip_tensor* dx, const trc_hip_tensor& da,
                      const trc_hip_tensor& db, bool accumulate, hipStream_t s) {
     const Call c = call_of(q, x.ne[1], s);
-    // (g has to be whole before dA reads it, so the long axis is never in parts here)
-    int rc = contract<true>(c, dy, c.b, true, 1, (float*) g.data);
-    if (rc != TRC_HIP_OK) return rc;
-    if (dx != nullptr) {
-        rc = expand<true>(c, (const float*) g.data, 1, c.a, false, base, *dx, nullptr);
+    const int64_t K = x.ne[0], tiles = c.tiles();
+    const int64_t half = (int64_t) (qm_workspace_bytes() / sizeof(float)) / 2;
+    Outer ob = outer_of(c, dy, (const float*) h.data, db, true, accumulate, nullptr, half);
+    Outer oa = outer_of(c, x, (const float*) g.data, da, false, accumulate, nullptr, half);
+    if (ob.splits > 1 || oa.splits > 1) {
+        uint8_t* ws = nullptr;
+        const int rc = qm_stream_workspace(s, &ws);
         if (rc != TRC_HIP_OK) return rc;
+        ob.parts = (float*) ws;
+        oa.parts = (float*) ws + half;
     }
-    rc = outer<false>(c, dy, (const float*) h.data, true, db, accumulate);
+    const int64_t nb = ob.blocks(c.batch.adapters), na = oa.blocks(c.batch.adapters), ng = tiles * rank_blocks(c.R);
+    const int64_t slices = std::max(std::min(2 * device_cus() / tiles, (K + 1023) / 1024), (int64_t) 1);
+    const int cols = (int) round_up((K + slices - 1) / slices, LE_COLS);
+    const int64_t nx = dx != nullptr ? tiles * ((K + cols - 1) / cols) : 0;
+    if (nb + ng > max_groups(LO_WAVES * 64) || na + nx > max_groups(LO_WAVES * 64)) {
+        return fail(TRC_HIP_E_SHAPE, "trc_hip_lora_back: %lld workgroups", (long long) std::max(nb + ng, na + nx));
+    }
+    with_type(c.type, [&](auto type) {
+        with_rank(c.R, [&](auto rt) {
+            hipLaunchKernelGGL((k_back_b<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (nb + ng)), dim3(LO_WAVES * 64), 0, s,
+                               ob, (int) nb, rows_of(dy), c.b, c.R, c.batch, (float*) g.data);
+        });
+    });
+    int rc = check_launch("lora_back (g, dB)");
     if (rc != TRC_HIP_OK) return rc;
-    return outer<true>(c, x, (const float*) g.data, false, da, accumulate);
+    with_type(c.type, [&](auto type) {
+        with_rank(c.R, [&](auto rt) {
+            hipLaunchKernelGGL((k_back_a<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (na + nx)), dim3(LO_WAVES * 64), 0, s,
+                               oa, (int) na, (const float*) g.data, c.a, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
+                               base != nullptr ? base->nb[1] : (size_t) 0, K, dx != nullptr ? (uint8_t*) dx->data : nullptr,
+                               dx != nullptr ? dx->nb[1] : (size_t) 0, cols);
+        });
+    });
+    rc = check_launch("lora_back (dx, dA)");
+    for (int k = 0; k < 2 && rc == TRC_HIP_OK; ++k) {
+        const Outer& o = k == 0 ? ob : oa;
+        if (o.splits == 1) continue;
+        hipLaunchKernelGGL(k_back_join, dim3((unsigned) ((o.x.n * c.R * c.batch.adapters + 255) / 256)), dim3(256), 0, s, o, k == 1,
+                           c.R, c.batch);
+        rc = check_launch("lora_back (join)");
+    }
+    return rc;
 }
 
 }  // namespace trc_hip
