@@ -30,13 +30,14 @@ namespace {
 
 constexpr int AW_BLOCK = TRC_HIP_ADAMW_BLOCK;  // a wave: 64 lanes of four elements
 constexpr int AW_THREADS = 256;
-constexpr int AW_CHUNK = 4096;  // elements of one workgroup
+constexpr int AW_CHUNK = 2048;  // elements of one workgroup
 static_assert(AW_BLOCK == 64 * 4 && AW_CHUNK % (AW_THREADS * 4) == 0, "a wave per block");
 
 // vectors whose address is only as aligned as one element
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint8_t b4u __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32u __attribute__((aligned(1)));
 
 struct AwTensor {
     float* p;
@@ -63,6 +64,14 @@ struct Plan {
     AwTensor* tensors;  // device
     uint32_t* owner;    // device: the tensor of each chunk
 };
+
+// A step reads and writes everything once, past the caches: the 243 million elements of a 4096-wide layer take
+// 1200 us, and 1270 with plain accesses.
+__device__ __forceinline__ f4u once(const f4u* p) { return __builtin_nontemporal_load(p); }
+__device__ __forceinline__ h4u once(const h4u* p) { return __builtin_nontemporal_load(p); }
+__device__ __forceinline__ uint32_t once(const u32u* p) { return __builtin_nontemporal_load(p); }
+__device__ __forceinline__ void store_once(f4u* p, f4 x) { __builtin_nontemporal_store(x, p); }
+__device__ __forceinline__ void store_once(u32u* p, uint32_t x) { __builtin_nontemporal_store(x, p); }
 
 __device__ __forceinline__ f4 load_grad(const void* g, int type, int64_t i) {
     if (type == TRC_HIP_TYPE_F32) return *(const f4u*) ((const float*) g + i);
@@ -101,7 +110,7 @@ __global__ __launch_bounds__(AW_THREADS) void k_adamw(const AwTensor* __restrict
     for (int it = 0; it < AW_CHUNK / (AW_THREADS * 4); ++it) {
         const int64_t i = base + (it * AW_THREADS + (int) threadIdx.x) * 4;
         if (i + 4 <= t.n) {
-            f4 p = *(const f4u*) (t.p + i), m = *(const f4u*) (pm + i), v = *(const f4u*) (pv + i);
+            f4 p = once((const f4u*) (t.p + i)), m = once((const f4u*) (pm + i)), v = once((const f4u*) (pv + i));
             const f4 g = load_grad(t.g, t.gtype, i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -111,9 +120,9 @@ __global__ __launch_bounds__(AW_THREADS) void k_adamw(const AwTensor* __restrict
                 m[k] = mk;
                 v[k] = vk;
             }
-            *(f4u*) (t.p + i) = p;
-            *(f4u*) (pm + i) = m;
-            *(f4u*) (pv + i) = v;
+            store_once((f4u*) (t.p + i), p);
+            store_once((f4u*) (pm + i), m);
+            store_once((f4u*) (pv + i), v);
         } else {
             for (int64_t j = i; j < t.n; ++j) {
                 float u;
@@ -125,13 +134,19 @@ __global__ __launch_bounds__(AW_THREADS) void k_adamw(const AwTensor* __restrict
 
 // The largest of a wave's values, in every lane. Magnitudes compare as their bits,
 // with infinities and NaNs above all others.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t max_with(uint32_t x) {
+    const uint32_t y = (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, CTRL, ROWS, 0xf, true);
+    return x > y ? x : y;
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint32_t y = (uint32_t) __shfl_xor((int) x, d, 64);
-        x = x > y ? x : y;
-    }
-    return (uint32_t) __builtin_amdgcn_readfirstlane((int) x);
+    x = max_with<0x111, 0xf>(x);  // from the lane before in the row of 16, then 2, 4 and 8 before
+    x = max_with<0x112, 0xf>(x);
+    x = max_with<0x114, 0xf>(x);
+    x = max_with<0x118, 0xf>(x);
+    x = max_with<0x142, 0xa>(x);  // the last lanes of rows 0 and 2 to rows 1 and 3, of row 1 to rows 2 and 3
+    x = max_with<0x143, 0xc>(x);
+    return (uint32_t) __builtin_amdgcn_readlane((int) x, 63);
 }
 
 __device__ __forceinline__ float inverse_scale(float s) {
@@ -149,79 +164,175 @@ __device__ __forceinline__ float decode_u(uint8_t c, float s) {
     return (x * x * s) * U_UNIT;
 }
 
+// One block of up to 256 elements by a wave, with every operation as it is defined.
+__device__ __forceinline__ void exact_block(const AwTensor& t, const AwHyper& h, float decay, int64_t at) {
+    const int lane = (int) threadIdx.x & 63;
+    int8_t* const pm = (int8_t*) t.m;
+    uint8_t* const pv = (uint8_t*) t.v;
+    const int64_t i = at + lane * 4;
+    const float sm = t.ms[at / AW_BLOCK], su = t.vs[at / AW_BLOCK];
+    float p[4], g[4], m[4], u[4];
+    int8_t cm[4];
+    uint8_t cv[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // (elements past the end read the last one and are not stored)
+        const int64_t j = min(i + k, t.n - 1);
+        p[k] = t.p[j];
+        g[k] = load_grad1(t.g, t.gtype, j);
+        cm[k] = pm[j];
+        cv[k] = pv[j];
+    }
+    uint32_t top_m = 0, top_u = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = decode_m(cm[k], sm);
+        u[k] = decode_u(cv[k], su);
+        float v = u[k] * u[k];
+        update(h, decay, p[k], g[k], m[k], v, u[k]);
+        if (i + k < t.n) {
+            top_m = max(top_m, __builtin_bit_cast(uint32_t, m[k]) & 0x7fffffffu);
+            top_u = max(top_u, __builtin_bit_cast(uint32_t, u[k]) & 0x7fffffffu);
+        }
+    }
+    float nm = __builtin_bit_cast(float, wave_max(top_m)), nu = __builtin_bit_cast(float, wave_max(top_u));
+    const float im = inverse_scale(nm), iu = inverse_scale(nu);
+    if (im == 0.f && nm < 1.f) nm = 0.f;
+    if (iu == 0.f && nu < 1.f) nu = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float rm = rintf(sqrtf(fabsf(m[k]) * im) * 127.f), ru = u[k] * iu;
+        const float rv = fmaxf(rintf(sqrtf(ru) * 255.f), ceilf(ru));  // (1 at least, where ru is above 0)
+        if (i + k >= t.n) continue;
+        t.p[i + k] = p[k];
+        pm[i + k] = (int8_t) (int) copysignf(rm, m[k]);
+        pv[i + k] = (uint8_t) (int) rv;
+    }
+    if (lane == 0) {
+        t.ms[at / AW_BLOCK] = nm;
+        t.vs[at / AW_BLOCK] = nu;
+    }
+}
+
+// What a lane has of a whole block.
+struct Block8 {
+    f4u p;
+    f4u g32;
+    h4u g16;
+    uint32_t m, v;
+    float sm, su;
+};
+
+template <int GTYPE>
+__device__ __forceinline__ void load_block(Block8& b, const AwTensor& t, int64_t at) {
+    const int64_t i = at + ((int) threadIdx.x & 63) * 4;
+    b.p = once((const f4u*) (t.p + i));
+    if (GTYPE == TRC_HIP_TYPE_F32) {
+        b.g32 = once((const f4u*) ((const float*) t.g + i));
+    } else {
+        b.g16 = once((const h4u*) ((const uint16_t*) t.g + i));
+    }
+    b.m = once((const u32u*) ((const uint8_t*) t.m + i));
+    b.v = once((const u32u*) ((const uint8_t*) t.v + i));
+    b.sm = t.ms[at / AW_BLOCK];
+    b.su = t.vs[at / AW_BLOCK];
+}
+
+// The square root of 0, of an infinity or NaN, or of 2^-96 and more, correctly rounded: the instruction's is
+// one unit off at most, and the signs of two residues tell which neighbour is nearest.
+__device__ __forceinline__ float sqrt_from_2em96(float x) {
+    const float s = __builtin_amdgcn_sqrtf(x);
+    const float lower = __builtin_bit_cast(float, __builtin_bit_cast(int, s) - 1);
+    const float upper = __builtin_bit_cast(float, __builtin_bit_cast(int, s) + 1);
+    const float dl = __builtin_fmaf(-lower, s, x), du = __builtin_fmaf(-upper, s, x);
+    float r = dl <= 0.f ? lower : s;
+    return du > 0.f ? upper : r;
+}
+
+// A whole block. The arithmetic bounds this kernel, not memory, so it takes what is as good as the exact
+// operations wherever that can be told: the square roots of the codes come from the instruction alone, within
+// 2 units of the last place, which decides a code unless it is within 1e-4 of the middle of two. A wave that
+// meets one such code, or a v above 0 and under 2^-96, leaves the block to exact_block()
+// (returns whether it has to be left to that).
+template <int GTYPE>
+__device__ __forceinline__ bool fast_block(const Block8& b, const AwTensor& t, const AwHyper& h, float decay, int64_t at) {
+    const int lane = (int) threadIdx.x & 63;
+    const int64_t i = at + lane * 4;
+    f4 p, m, u;
+    uint32_t top_m = 0, top_u = 0, least = 0xffffffffu;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float g = GTYPE == TRC_HIP_TYPE_F32   ? b.g32[k]
+                  : GTYPE == TRC_HIP_TYPE_F16 ? half_bits_to_float(b.g16[k])
+                                              : __builtin_bit_cast(float, (uint32_t) b.g16[k] << 16);
+        float mk = decode_m((int8_t) (b.m >> 8 * k), b.sm), uk = decode_u((uint8_t) (b.v >> 8 * k), b.su);
+        // (update(), but for the square root)
+        g = g * h.gscale;
+        mk = mk * h.b1 + g * h.c1;
+        const float vk = (uk * uk) * h.b2 + (g * g) * h.c2;
+        least = min(least, __builtin_bit_cast(uint32_t, vk) - 1u);  // 0 is above all others here
+        uk = sqrt_from_2em96(vk);
+        p[k] = b.p[k] * decay - (mk / (uk * h.root + h.eps)) * h.rate;
+        m[k] = mk;
+        u[k] = uk;
+        top_m = max(top_m, __builtin_bit_cast(uint32_t, mk) & 0x7fffffffu);
+        top_u = max(top_u, __builtin_bit_cast(uint32_t, uk) & 0x7fffffffu);
+    }
+    float nm = __builtin_bit_cast(float, wave_max(top_m)), nu = __builtin_bit_cast(float, wave_max(top_u));
+    const float im = inverse_scale(nm), iu = inverse_scale(nu);
+    if (im == 0.f && nm < 1.f) nm = 0.f;
+    if (iu == 0.f && nu < 1.f) nu = 0.f;
+    float off = 0.f;  // the largest distance of a ratio from its code
+    int cm[4];
+    uint32_t cv = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float tm = __builtin_amdgcn_sqrtf(fabsf(m[k]) * im) * 127.f, rm = __builtin_rintf(tm);
+        const float ru = u[k] * iu, tu = __builtin_amdgcn_sqrtf(ru) * 255.f, rv = __builtin_rintf(tu);
+        off = fmaxf(off, fmaxf(fabsf(tm - rm), fabsf(tu - rv)));
+        cm[k] = (int) __builtin_copysignf(rm, m[k]);
+        cv = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(rv, __builtin_ceilf(ru)), k, cv);
+    }
+    // (a NaN or an infinity is left to the exact operations too)
+    const bool doubt = !(off < 0.4999f) || least < 0x0f7fffffu || top_u >= 0x7f800000u || top_m >= 0x7f800000u;
+    if (__any(doubt)) return true;
+    store_once((f4u*) (t.p + i), p);
+    const uint32_t lo = __builtin_amdgcn_perm((uint32_t) cm[1], (uint32_t) cm[0], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm((uint32_t) cm[3], (uint32_t) cm[2], 0x04000c0cu);
+    store_once((u32u*) ((uint8_t*) t.m + i), lo | hi);
+    store_once((u32u*) ((uint8_t*) t.v + i), cv);
+    if (lane == 0) {
+        t.ms[at / AW_BLOCK] = nm;
+        t.vs[at / AW_BLOCK] = nu;
+    }
+    return false;
+}
+
+// A wave's two blocks; returns which of them are left.
+template <int GTYPE>
+__device__ __forceinline__ int chunk8(const AwTensor& t, const AwHyper& h, float decay, int64_t at) {
+    constexpr int STEP = AW_THREADS * 4;
+    static_assert(AW_CHUNK == 2 * STEP, "two blocks a wave");
+    if (at + AW_BLOCK > t.n) return 3;
+    Block8 b0, b1;
+    load_block<GTYPE>(b0, t, at);
+    if (at + STEP + AW_BLOCK > t.n) return fast_block<GTYPE>(b0, t, h, decay, at) ? 3 : 2;
+    load_block<GTYPE>(b1, t, at + STEP);
+    const bool left = fast_block<GTYPE>(b0, t, h, decay, at);
+    return (left ? 1 : 0) | (fast_block<GTYPE>(b1, t, h, decay, at + STEP) ? 2 : 0);
+}
+
 __global__ __launch_bounds__(AW_THREADS) void k_adamw8(const AwTensor* __restrict__ tensors,
                                                         const uint32_t* __restrict__ owner, AwHyper h) {
     const AwTensor t = tensors[owner[blockIdx.x]];
     const float decay = (float) (1.0 - h.decay * (double) t.decay);
-    const int lane = (int) threadIdx.x & 63;
-    const int64_t base = ((int64_t) blockIdx.x - t.first) * AW_CHUNK + ((int) threadIdx.x >> 6) * AW_BLOCK;
-    int8_t* const pm = (int8_t*) t.m;
-    uint8_t* const pv = (uint8_t*) t.v;
-    for (int it = 0; it < AW_CHUNK / (AW_THREADS * 4); ++it) {
-        const int64_t at = base + it * (AW_THREADS * 4);  // the wave's block
-        if (at >= t.n) break;
-        const int64_t i = at + lane * 4;
-        const int here = t.n - i >= 4 ? 4 : t.n > i ? (int) (t.n - i) : 0;
-        const float sm = t.ms[at / AW_BLOCK], su = t.vs[at / AW_BLOCK];
-        f4 p = {0.f, 0.f, 0.f, 0.f}, g = p;
-        b4u cm = {0, 0, 0, 0}, cv = cm;
-        if (here == 4) {
-            p = *(const f4u*) (t.p + i);
-            g = load_grad(t.g, t.gtype, i);
-            cm = *(const b4u*) (pm + i);
-            cv = *(const b4u*) (pv + i);
-        } else {
-            for (int k = 0; k < here; ++k) {
-                p[k] = t.p[i + k];
-                g[k] = load_grad1(t.g, t.gtype, i + k);
-                cm[k] = (uint8_t) pm[i + k];
-                cv[k] = pv[i + k];
-            }
-        }
-        f4 m, u;
-        uint32_t top_m = 0, top_u = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float pk = p[k], mk = decode_m((int8_t) cm[k], sm), uk = decode_u(cv[k], su);
-            float vk = uk * uk;
-            update(h, decay, pk, g[k], mk, vk, uk);
-            // lanes past the end hold zeros, but eps may be 0: keep them out of the maxima
-            if (k >= here) mk = uk = 0.f;
-            p[k] = pk;
-            m[k] = mk;
-            u[k] = uk;
-            const uint32_t bm = __builtin_bit_cast(uint32_t, mk) & 0x7fffffffu, bu = __builtin_bit_cast(uint32_t, uk) & 0x7fffffffu;
-            top_m = bm > top_m ? bm : top_m;
-            top_u = bu > top_u ? bu : top_u;
-        }
-        float nm = __builtin_bit_cast(float, wave_max(top_m)), nu = __builtin_bit_cast(float, wave_max(top_u));
-        const float im = inverse_scale(nm), iu = inverse_scale(nu);
-        if (im == 0.f && nm < 1.f) nm = 0.f;
-        if (iu == 0.f && nu < 1.f) nu = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float rm = rintf(sqrtf(fabsf(m[k]) * im) * 127.f);
-            cm[k] = (uint8_t) (int8_t) (m[k] < 0.f ? -rm : rm);
-            const float ru = u[k] * iu;
-            float c = rintf(sqrtf(ru) * 255.f);
-            if (ru > 0.f && c < 1.f) c = 1.f;
-            cv[k] = (uint8_t) c;
-        }
-        if (here == 4) {
-            *(f4u*) (t.p + i) = p;
-            *(b4u*) (pm + i) = cm;
-            *(b4u*) (pv + i) = cv;
-        } else {
-            for (int k = 0; k < here; ++k) {
-                t.p[i + k] = p[k];
-                pm[i + k] = (int8_t) cm[k];
-                pv[i + k] = cv[k];
-            }
-        }
-        if (lane == 0) {
-            t.ms[at / AW_BLOCK] = nm;
-            t.vs[at / AW_BLOCK] = nu;
-        }
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    const int64_t at = ((int64_t) blockIdx.x - t.first) * AW_CHUNK + wave * AW_BLOCK;
+    const int left = t.gtype == TRC_HIP_TYPE_F32   ? chunk8<TRC_HIP_TYPE_F32>(t, h, decay, at)
+                     : t.gtype == TRC_HIP_TYPE_F16 ? chunk8<TRC_HIP_TYPE_F16>(t, h, decay, at)
+                                                   : chunk8<TRC_HIP_TYPE_BF16>(t, h, decay, at);
+    for (int k = 0; k < 2; ++k) {
+        const int64_t block = at + k * (AW_THREADS * 4);
+        if ((left >> k & 1) != 0 && block < t.n) exact_block(t, h, decay, block);
     }
 }
 
@@ -250,8 +361,8 @@ __global__ __launch_bounds__(AW_THREADS) void k_adamw_moments(const AwTensor* __
                 m[k] = decode_m((int8_t) cm[k], sm);
                 v[k] = u * u;
             }
-            *(f4u*) (t.mf + i) = m;
-            *(f4u*) (t.vf + i) = v;
+            store_once((f4u*) (t.mf + i), m);
+            store_once((f4u*) (t.vf + i), v);
         } else {
             for (int64_t j = i; j < t.n; ++j) {
                 const float u = decode_u(((const uint8_t*) t.v)[j], su);

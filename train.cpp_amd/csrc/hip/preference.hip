@@ -11,6 +11,8 @@
 // sum), one workgroup over the pairs, and the gradient (each row read and written once).
 // All three are bound by memory; the gradient cannot begin before the pair's last row is
 // summed, so the logits are read twice.
+#include <cfloat>
+
 #include "common.h"
 
 namespace trc_hip {
@@ -18,8 +20,10 @@ namespace trc_hip {
 namespace {
 
 constexpr int PF_THREADS = 256;
-constexpr int PF_JOIN_THREADS = 1024;
-constexpr int PF_MAX_PARTS = 64;  // parts of a row, at most
+constexpr int PF_WAVES = 16;       // of the join
+constexpr int PF_MAX_PARTS = 64;   // parts of a row: a lane each where they are joined
+constexpr int PF_LOADS = 4;        // 16-byte loads that a thread has under way
+constexpr int64_t PF_MAX_ROWS = (int64_t) 1 << 20;  // their log-probabilities fit the stream's workspace
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // 16 bytes of a row whose address is only as aligned as one element
@@ -43,7 +47,7 @@ struct Row<TRC_HIP_TYPE_F32> {
         f4u v;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) v[k] = x[k];
-        *(f4u*) p = v;
+        __builtin_nontemporal_store(v, (f4u*) p);
     }
 };
 template <int TYPE>
@@ -67,7 +71,7 @@ struct Row16 {
         h8u v;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) v[k] = put(x[k]);
-        *(h8u*) p = v;
+        __builtin_nontemporal_store(v, (h8u*) p);
     }
 };
 template <>
@@ -77,9 +81,9 @@ struct Row<TRC_HIP_TYPE_BF16> : Row16<TRC_HIP_TYPE_BF16> {};
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
-// A maximum and the sum of exponentials taken from it. A maximum of -inf (nothing yet,
-// or only -inf) is subtracted as 0, so that exp(-inf - m) is 0 and not NaN; infinities
-// and NaNs reach the sum.
+// A maximum and the sum of exponentials taken from it (the difference first: its product with LOG2E cannot
+// overflow where logits are the type's lowest value). A maximum of -inf (nothing yet, or only -inf)
+// is subtracted as 0, so that exp(-inf - m) is 0 and not NaN; infinities and NaNs reach the sum.
 struct Soft {
     float m, s;
 };
@@ -93,122 +97,187 @@ __device__ __forceinline__ Soft wave_join(Soft a) {
     for (int d = 32; d > 0; d >>= 1) a = join(a, {__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)});
     return a;
 }
+__device__ __forceinline__ float lse_of(Soft a) { return a.m + logf(a.s); }
 
-// Rows whose label is negative are not counted: they are not read, and their lse is 0.
-// gridDim.y parts of `len` elements each; one part writes lse, more write (m, s) to parts.
+template <int N>
+__device__ __forceinline__ void take(Soft& a, const float (&x)[N]) {
+    float m = a.m;
+#pragma unroll
+    for (int k = 0; k < N; ++k) m = fmaxf(m, x[k]);
+    const float base = base_of(m);
+    float s = a.s * exp_of(a.m - base);
+#pragma unroll
+    for (int k = 0; k < N; ++k) s += exp_of(x[k] - base);
+    a = {m, s};
+}
+
+// A thread's share of n elements at p, with the running maximum: 4 KB of a wave's loads under way together.
+template <int TYPE>
+__device__ __forceinline__ Soft careful_share(const typename Row<TYPE>::Elem* p, int n) {
+    typedef Row<TYPE> R;
+    constexpr int VEC = R::VEC, STEP = PF_THREADS * VEC;
+    const int whole = n / VEC * VEC;
+    Soft a = {-INFINITY, 0.f};
+    for (int i = (int) threadIdx.x * VEC; i < whole; i += STEP) {
+        float x[VEC];
+        R::load(p + i, x);
+        take(a, x);
+    }
+    if (whole + (int) threadIdx.x < n) a = join(a, {R::get(p[whole + threadIdx.x]), 1.f});
+    return a;
+}
+
+// The same, with the exponentials taken from the largest of the thread's first elements rather than from a
+// running maximum: their sum is as exact from any point that does not overflow, and an element costs a
+// multiply-add, an exponential and an add.
+// Sums that are not finite, or a start that is not, go the careful way.
+template <int TYPE>
+__device__ __forceinline__ Soft share(const typename Row<TYPE>::Elem* p, int n) {
+    typedef Row<TYPE> R;
+    constexpr int VEC = R::VEC, U = PF_LOADS, STEP = PF_THREADS * VEC;
+    const int whole = n / VEC * VEC;
+    int i = (int) threadIdx.x * VEC;
+    if (i + (U - 1) * STEP >= whole) return careful_share<TYPE>(p, n);
+    float x[U * VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) R::load(p + i + u * STEP, x + u * VEC);
+    float m = x[0];
+#pragma unroll
+    for (int k = 1; k < U * VEC; ++k) m = fmaxf(m, x[k]);
+    const float unit = m * LOG2E;
+    float s = 0.f;
+    auto add = [&] {
+#pragma unroll
+        for (int k = 0; k < U * VEC; ++k) s += __builtin_amdgcn_exp2f(fmaf(x[k], LOG2E, -unit));
+    };
+    add();
+    for (i += U * STEP; i + (U - 1) * STEP < whole; i += U * STEP) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) R::load(p + i + u * STEP, x + u * VEC);
+        add();
+    }
+#pragma unroll
+    for (int k = 0; k < U * VEC; ++k) x[k] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (i + u * STEP < whole) R::load(p + i + u * STEP, x + u * VEC);
+    if (whole + (int) threadIdx.x < n) x[U * VEC - 1] = R::get(p[whole + threadIdx.x]);
+    add();
+    if (!(s <= FLT_MAX) || !(fabsf(unit) <= FLT_MAX)) return careful_share<TYPE>(p, n);
+    // what rounding m LOG2E left out, taken back
+    return {m, s * exp_of(fmaf(m, LOG2E, -unit) * -(1.f / LOG2E))};
+}
+
+// Rows whose label is negative are not counted: they are not read, and their lse and log-probability are 0.
+// gridDim.y parts of `len` elements each; one part writes lse and the label's log-probability lp, more
+// write (m, s) to parts, and lp is the label's logit until they are joined.
 template <int TYPE>
 __global__ __launch_bounds__(PF_THREADS) void k_pref_rows(const uint8_t* __restrict__ logits, size_t nb1, int64_t V,
                                                            const int32_t* __restrict__ labels, int64_t len,
-                                                           float* __restrict__ lse, Soft* __restrict__ parts) {
+                                                           float* __restrict__ lse, float* __restrict__ lp,
+                                                           Soft* __restrict__ parts) {
     typedef Row<TYPE> R;
-    constexpr int VEC = R::VEC, U = 4;
     const int64_t row = blockIdx.x;
-    if (labels[row] < 0) {
-        if (blockIdx.y == 0 && threadIdx.x == 0) lse[row] = 0.f;
+    const int32_t y = labels[row];
+    if (y < 0) {
+        if (blockIdx.y == 0 && threadIdx.x == 0) lse[row] = lp[row] = 0.f;
         return;
     }
-    const typename R::Elem* const p = (const typename R::Elem*) (logits + row * nb1);
-    const int64_t lo = (int64_t) blockIdx.y * len, hi = lo + len < V ? lo + len : V;
-    Soft a = {-INFINITY, 0.f};
-    int64_t i = lo + (int) threadIdx.x * VEC;
-    for (; i + (U - 1) * PF_THREADS * VEC + VEC <= hi; i += U * PF_THREADS * VEC) {
-        float x[U][VEC];
-#pragma unroll
-        for (int u = 0; u < U; ++u) R::load(p + i + u * PF_THREADS * VEC, x[u]);
-        float m = a.m;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) m = fmaxf(m, x[u][k]);
-        const float base = base_of(m);
-        float s = a.s * exp_of(a.m - base);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) s += exp_of(x[u][k] - base);
-        a = {m, s};
-    }
-    for (; i < hi; i += PF_THREADS * VEC) {
-        if (i + VEC <= hi) {
-            float x[VEC], m = a.m;
-            R::load(p + i, x);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) m = fmaxf(m, x[k]);
-            const float base = base_of(m);
-            float s = a.s * exp_of(a.m - base);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) s += exp_of(x[k] - base);
-            a = {m, s};
-        } else {
-            for (int64_t j = i; j < hi; ++j) a = join(a, {R::get(p[j]), 1.f});
-        }
-    }
+    const typename R::Elem* const all = (const typename R::Elem*) (logits + row * nb1);
+    const int64_t lo = (int64_t) blockIdx.y * len;
+    const float ly = y < V ? R::get(all[y]) : NAN;
+    Soft a = share<TYPE>(all + lo, (int) (min(lo + len, V) - lo));
     __shared__ Soft w[PF_THREADS / 64];
     a = wave_join(a);
     if (((int) threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = a;
     __syncthreads();
     if (threadIdx.x != 0) return;
+#pragma unroll
     for (int k = 1; k < PF_THREADS / 64; ++k) a = join(a, w[k]);
     if (gridDim.y == 1) {
-        lse[row] = a.m + logf(a.s);
+        const float e = lse_of(a);
+        lse[row] = e;
+        lp[row] = ly - e;
     } else {
         parts[row * gridDim.y + blockIdx.y] = a;
+        if (blockIdx.y == 0) lp[row] = ly;
     }
 }
 
-// One workgroup: the rows' parts joined where there are any, then a wave for each pair.
-// The tokens' log-probabilities and the pair's terms are summed in 64 bits, each
-// sum in one order: a sequence's sum is far larger than the ratios that come of it.
-template <int TYPE>
-__global__ __launch_bounds__(PF_JOIN_THREADS) void k_pref_pairs(
-    const uint8_t* __restrict__ logits, size_t nb1, int64_t V, int64_t T, const int32_t* __restrict__ labels,
-    const int32_t* __restrict__ start, int64_t pairs, const float* __restrict__ ref, float beta, float smooth, int n_parts,
-    const Soft* __restrict__ parts, float* lse, float* __restrict__ logp, float* __restrict__ slope, float* __restrict__ loss) {
-    typedef Row<TYPE> R;
+// One workgroup: the rows' parts joined where there are any, a wave a row, then a wave for each sequence.
+// The tokens' log-probabilities and the pairs' terms are summed in 64 bits, each sum in one
+// order: a sequence's sum is far larger than the ratios that come of it.
+__global__ __launch_bounds__(PF_WAVES * 64) void k_pref_pairs(int64_t T, const int32_t* __restrict__ labels,
+                                                               const int32_t* __restrict__ start, int64_t pairs,
+                                                               const float* __restrict__ ref, float beta, float smooth,
+                                                               int n_parts, const Soft* __restrict__ parts, float* lse,
+                                                               float* lp, float* __restrict__ logp,
+                                                               float* __restrict__ slope, float* __restrict__ loss) {
+    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6;
     if (n_parts > 1) {
-        for (int64_t t = threadIdx.x; t < T; t += PF_JOIN_THREADS) {
-            if (labels[t] < 0) continue;
-            Soft a = parts[t * n_parts];
-            for (int k = 1; k < n_parts; ++k) a = join(a, parts[t * n_parts + k]);
-            lse[t] = a.m + logf(a.s);
+        for (int64_t t0 = wave; t0 < T; t0 += 4 * PF_WAVES) {
+            Soft a[4];
+            int32_t y[4];
+            float l[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t t = min(t0 + k * PF_WAVES, T - 1);
+                y[k] = labels[t];
+                l[k] = lp[t];
+                a[k] = parts[t * n_parts + min(lane, n_parts - 1)];  // (of rows not counted: whatever is there)
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t t = t0 + k * PF_WAVES;
+                const Soft all = wave_join(lane < n_parts ? a[k] : Soft{-INFINITY, 0.f});
+                if (lane == 0 && t < T && y[k] >= 0) {
+                    const float e = lse_of(all);
+                    lse[t] = e;
+                    lp[t] = l[k] - e;
+                }
+            }
         }
         __syncthreads();
     }
-    __shared__ double total[PF_JOIN_THREADS / 64];
-    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6;
+    __shared__ double L[PF_WAVES], terms[PF_WAVES / 2];
     double mine = 0.0;
-    for (int64_t i = wave; i < pairs; i += PF_JOIN_THREADS / 64) {
-        double L[2];
-        for (int k = 0; k < 2; ++k) {
-            const int64_t lo = min(max((int64_t) start[2 * i + k], (int64_t) 0), T);
-            const int64_t hi = min(max((int64_t) start[2 * i + k + 1], lo), T);
+    for (int64_t s0 = 0; s0 < 2 * pairs; s0 += PF_WAVES) {
+        if (s0 + wave < 2 * pairs) {
+            const int64_t lo = min(max((int64_t) start[s0 + wave], (int64_t) 0), T);
+            const int64_t hi = min(max((int64_t) start[s0 + wave + 1], lo), T);
             double sum = 0.0;
-            for (int64_t t = lo + lane; t < hi; t += 64) {
-                const int32_t y = labels[t];
-                if (y < 0) continue;
-                const float l = y < V ? R::get(((const typename R::Elem*) (logits + t * nb1))[y]) : NAN;
-                sum += (double) l - (double) lse[t];
+            for (int64_t t = lo + lane; t < hi; t += 8 * 64) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = t + 64 * k < hi ? lp[t + 64 * k] : 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += (double) x[k];
             }
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-            L[k] = sum;
+            if (lane == 0) {
+                L[wave] = sum;
+                logp[s0 + wave] = (float) sum;
+            }
         }
-        if (lane == 0) {
-            logp[2 * i] = (float) L[0];
-            logp[2 * i + 1] = (float) L[1];
-            const double z = (double) beta * ((L[0] - (double) ref[2 * i]) - (L[1] - (double) ref[2 * i + 1]));
-            const double e = (double) smooth, tail = log1p(exp(-fabs(z)));
+        __syncthreads();
+        const int64_t i = s0 / 2 + threadIdx.x;
+        if (threadIdx.x < PF_WAVES / 2 && i < pairs) {
+            const double z = (double) beta * ((L[2 * threadIdx.x] - (double) ref[2 * i]) - (L[2 * threadIdx.x + 1] - (double) ref[2 * i + 1]));
+            const double e = (double) smooth, small = exp(-fabs(z)), tail = log1p(small);
             const double up = fmax(-z, 0.0) + tail, down = fmax(z, 0.0) + tail;  // -log sigma(z), -log sigma(-z)
-            // (e = 0 takes no part of an infinite term)
-            mine += z != z ? z : (1.0 - e) * up + (e == 0.0 ? 0.0 : e * down);
-            slope[i] = (float) (e / (1.0 + exp(-z)) - (1.0 - e) / (1.0 + exp(z)));
+            // (a weight of 0 takes no part of an infinite term)
+            mine += z != z ? z : (e == 1.0 ? 0.0 : (1.0 - e) * up) + (e == 0.0 ? 0.0 : e * down);
+            const double near = 1.0 / (1.0 + small), far = small / (1.0 + small);  // sigma(|z|), sigma(-|z|)
+            slope[i] = (float) (z != z ? z : z >= 0.0 ? e * near - (1.0 - e) * far : e * far - (1.0 - e) * near);
         }
+        __syncthreads();
     }
-    if (lane == 0) total[wave] = mine;
+    if (threadIdx.x < PF_WAVES / 2) terms[threadIdx.x] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
         double sum = 0.0;
-        for (int k = 0; k < PF_JOIN_THREADS / 64; ++k) sum += total[k];
+        for (int k = 0; k < PF_WAVES / 2; ++k) sum += terms[k];
         loss[0] = (float) (sum / (double) pairs);
     }
 }
@@ -236,53 +305,59 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_back(const uint8_t* logits,
                                                            const float* __restrict__ dloss, float beta, int64_t len,
                                                            uint8_t* dlogits, size_t dnb1) {
     typedef Row<TYPE> R;
-    constexpr int VEC = R::VEC, U = 4;
-    const int64_t row = blockIdx.x;
+    constexpr int VEC = R::VEC, U = PF_LOADS, STEP = PF_THREADS * VEC;
+    // The last rows first: they are what the caches still hold of the forward pass. With stores that do not stay
+    // there either, 8192 rows of 32000 in 16 bits take 227 us both ways, and 275 in order with plain stores.
+    const int64_t row = gridDim.x - 1 - blockIdx.x, lo = (int64_t) blockIdx.y * len;
     const int32_t y = labels[row];
     const int64_t seq = y < 0 ? -1 : sequence_of(start, 2 * pairs, row);
-    const typename R::Elem* const p = (const typename R::Elem*) (logits + row * nb1);
-    typename R::Elem* const d = (typename R::Elem*) (dlogits + row * dnb1);
-    const int64_t lo = (int64_t) blockIdx.y * len, hi = lo + len < V ? lo + len : V;
-    int64_t i = lo + (int) threadIdx.x * VEC;
+    const typename R::Elem* const p = (const typename R::Elem*) (logits + row * nb1) + lo;
+    typename R::Elem* const d = (typename R::Elem*) (dlogits + row * dnb1) + lo;
+    const int n = (int) (min(lo + len, V) - lo), whole = n / VEC * VEC;
+    int i = (int) threadIdx.x * VEC;
     if (seq < 0) {  // not counted: zeros, whatever the logits hold
         float z[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) z[k] = 0.f;
-        for (; i < hi; i += PF_THREADS * VEC) {
-            if (i + VEC <= hi) {
-                R::store(d + i, z);
-            } else {
-                for (int64_t j = i; j < hi; ++j) d[j] = R::put(0.f);
-            }
-        }
+        for (; i < whole; i += STEP) R::store(d + i, z);
+        if (whole + (int) threadIdx.x < n) d[whole + threadIdx.x] = R::put(0.f);
         return;
     }
     const float w = (float) ((double) slope[seq >> 1] * (double) beta / (double) pairs) * dloss[0] * ((seq & 1) ? -1.f : 1.f);
     const float base = lse[row];
-    auto grad = [&](float l, int64_t v) { return w * ((v == y ? 1.f : 0.f) - exp_of(l - base)); };
-    for (; i + (U - 1) * PF_THREADS * VEC + VEC <= hi; i += U * PF_THREADS * VEC) {
+    const int64_t label = y - lo;  // in this part
+    // -w exp(l - lse), and w more at the label
+    auto store = [&](int at, float* x) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[k] = exp_of(x[k] - base);
+        if (label >= at && label < at + VEC) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[k] = (label == at + k ? 1.f : 0.f) - x[k];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[k] *= w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[k] *= -w;
+        }
+        R::store(d + at, x);
+    };
+    for (; i + (U - 1) * STEP < whole; i += U * STEP) {
         float x[U][VEC];
 #pragma unroll
-        for (int u = 0; u < U; ++u) R::load(p + i + u * PF_THREADS * VEC, x[u]);
+        for (int u = 0; u < U; ++u) R::load(p + i + u * STEP, x[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t at = i + u * PF_THREADS * VEC;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) x[u][k] = grad(x[u][k], at + k);
-            R::store(d + at, x[u]);
-        }
+        for (int u = 0; u < U; ++u) store(i + u * STEP, x[u]);
     }
-    for (; i < hi; i += PF_THREADS * VEC) {
-        if (i + VEC <= hi) {
-            float x[VEC];
-            R::load(p + i, x);
+    float x[U][VEC];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[k] = grad(x[k], i + k);
-            R::store(d + i, x);
-        } else {
-            for (int64_t j = i; j < hi; ++j) d[j] = R::put(grad(R::get(p[j]), j));
-        }
-    }
+    for (int u = 0; u < U - 1; ++u)
+        if (i + u * STEP < whole) R::load(p + i + u * STEP, x[u]);
+    const int last = whole + (int) threadIdx.x;
+    if (last < n) x[U - 1][0] = R::get(p[last]);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (i + u * STEP < whole) store(i + u * STEP, x[u]);
+    if (last < n) d[last] = R::put(w * ((label == last ? 1.f : 0.f) - exp_of(x[U - 1][0] - base)));
 }
 
 // Parts of a row, and their length: whole rows while there are rows for every CU
@@ -300,23 +375,21 @@ template <int TYPE>
 int forward(const trc_hip_tensor& l, const int32_t* labels, const int32_t* start, int64_t pairs, const float* ref, float beta,
             float smooth, float* lse, float* logp, float* slope, float* loss, hipStream_t s) {
     const int64_t V = l.ne[0], T = l.ne[1];
-    int64_t len = part_length(V, T);
-    int64_t n = (V + len - 1) / len;
+    const int64_t len = part_length(V, T), n = (V + len - 1) / len;  // (n T is about 8 CUs: little of the workspace)
     uint8_t* ws = nullptr;
-    if (n > 1) {
-        const int rc = qm_stream_workspace(s, &ws);
-        if (rc != TRC_HIP_OK) return rc;
-        if ((size_t) (n * T) * sizeof(Soft) > qm_workspace_bytes()) {  // rows enough without parts
-            len = V;
-            n = 1;
-        }
+    int rc = qm_stream_workspace(s, &ws);
+    if (rc != TRC_HIP_OK) return rc;
+    float* const lp = (float*) ws;
+    Soft* const parts = (Soft*) (ws + (size_t) (T + 1) / 2 * 8);
+    if ((size_t) (T + 1) / 2 * 8 + (n > 1 ? (size_t) (n * T) * sizeof(Soft) : 0) > qm_workspace_bytes()) {
+        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss: %lld rows in %lld parts", (long long) T, (long long) n);
     }
     hipLaunchKernelGGL(k_pref_rows<TYPE>, dim3((unsigned) T, (unsigned) n), dim3(PF_THREADS), 0, s, (const uint8_t*) l.data,
-                       l.nb[1], V, labels, len, lse, (Soft*) ws);
-    const int rc = check_launch("preference_loss (rows)");
+                       l.nb[1], V, labels, len, lse, lp, parts);
+    rc = check_launch("preference_loss (rows)");
     if (rc != TRC_HIP_OK) return rc;
-    hipLaunchKernelGGL(k_pref_pairs<TYPE>, dim3(1), dim3(PF_JOIN_THREADS), 0, s, (const uint8_t*) l.data, l.nb[1], V, T, labels,
-                       start, pairs, ref, beta, smooth, (int) n, (const Soft*) ws, lse, logp, slope, loss);
+    hipLaunchKernelGGL(k_pref_pairs, dim3(1), dim3(PF_WAVES * 64), 0, s, T, labels, start, pairs, ref, beta, smooth, (int) n,
+                       parts, lse, lp, logp, slope, loss);
     return check_launch("preference_loss (pairs)");
 }
 
@@ -335,8 +408,8 @@ int backward(const trc_hip_tensor& l, const int32_t* labels, const int32_t* star
 int launch_preference_loss(const trc_hip_tensor& l, const int32_t* labels, const int32_t* start, int64_t pairs,
                            const float* ref, float beta, float smooth, float* lse, float* logp, float* slope, float* loss,
                            hipStream_t s) {
-    if (l.ne[1] > max_groups(PF_THREADS)) {
-        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss: %lld rows", (long long) l.ne[1]);
+    if (l.ne[1] > PF_MAX_ROWS) {
+        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss: %lld rows (at most %lld)", (long long) l.ne[1], (long long) PF_MAX_ROWS);
     }
     auto* const f = l.type == TRC_HIP_TYPE_F32   ? forward<TRC_HIP_TYPE_F32>
                     : l.type == TRC_HIP_TYPE_F16 ? forward<TRC_HIP_TYPE_F16>
@@ -347,8 +420,9 @@ int launch_preference_loss(const trc_hip_tensor& l, const int32_t* labels, const
 int launch_preference_loss_back(const trc_hip_tensor& l, const int32_t* labels, const int32_t* start, int64_t pairs,
                                 const float* lse, const float* slope, const float* dloss, float beta,
                                 const trc_hip_tensor& d, hipStream_t s) {
-    if (l.ne[1] > max_groups(PF_THREADS)) {
-        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss_back: %lld rows", (long long) l.ne[1]);
+    if (l.ne[1] > PF_MAX_ROWS) {
+        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss_back: %lld rows (at most %lld)", (long long) l.ne[1],
+                    (long long) PF_MAX_ROWS);
     }
     auto* const f = l.type == TRC_HIP_TYPE_F32   ? backward<TRC_HIP_TYPE_F32>
                     : l.type == TRC_HIP_TYPE_F16 ? backward<TRC_HIP_TYPE_F16>
