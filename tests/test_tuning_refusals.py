@@ -202,3 +202,10 @@ def test_forced_errors(entry, call):
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=str(ROOT / "tests"), timeout=120,
                        env={**os.environ, "TRC_HIP_FORCE_ERROR": entry})
     assert r.returncode == 0 and r.stdout.strip() == "-5", r.stdout + r.stderr
+
+
+def test_tensors_outside_of_hip_buffers_abort():
+    r = subprocess.run([str(ROOT / "tests" / "cpp" / "bin" / "test_tuning"), "--abort-host"], capture_output=True, text=True,
+                       timeout=60)
+    assert r.returncode != 0
+    assert "not in a HIP buffer" in r.stderr

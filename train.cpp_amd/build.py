@@ -6,7 +6,7 @@
                         Device/BufferType/Buffer implementation, linked against
                         libtrc_hip.so (g++)
 
-Outputs go to train.cpp_amd/lib/. Every call rebuilds from source.
+and the programs of examples/ on top of both. The libraries go to train.cpp_amd/lib/. Every call rebuilds from source.
 """
 from __future__ import annotations
 
@@ -24,6 +24,7 @@ HIP_SRC = PKG / "csrc" / "hip"
 CORE_SRC = PKG / "csrc" / "core"
 BACKEND_SRC = PKG / "csrc" / "backend"
 INCLUDE = ROOT / "include"
+EXAMPLES = ROOT / "examples"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("TRC_HIP_ARCH", "gfx950")
@@ -92,10 +93,22 @@ def build_core(verbose: bool = False, jobs: int = 8) -> Path | None:
     return out
 
 
+def build_examples(verbose: bool = False) -> list[Path]:
+    """examples/*.cpp, each a program of its own in examples/bin/."""
+    out = []
+    (EXAMPLES / "bin").mkdir(exist_ok=True)
+    for s in sorted(EXAMPLES.glob("*.cpp")):
+        out.append(EXAMPLES / "bin" / s.stem)
+        _run([CXX, "-std=c++20", "-O2", "-Wall", "-Wextra", f"-I{INCLUDE}", str(s), f"-L{LIB}", "-ltraincpp_hip", "-ltrc_hip",
+              "-Wl,-rpath,$ORIGIN/../../train.cpp_amd/lib", "-o", str(out[-1])], verbose)
+    return out
+
+
 def build_all(verbose: bool = False) -> None:
     LIB.mkdir(parents=True, exist_ok=True)
     build_hip(verbose)
     build_core(verbose)
+    build_examples(verbose)
 
 
 if __name__ == "__main__":

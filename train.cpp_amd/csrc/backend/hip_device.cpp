@@ -703,4 +703,185 @@ bool hip_dequant_host(Type type, const void* host_blocks, int64_t n_blocks, floa
     return true;
 }
 
+// ---- adapters, preference loss, AdamW ----
+
+namespace {
+
+HipBuffer* buffer_of(const Tensor* t, const char* what) {
+    HipBuffer* b = t != nullptr ? hip_buffer_of(t) : nullptr;
+    if (b == nullptr) {
+        std::fprintf(stderr, "[traincpp-hip][FATAL] %s: tensor %s is not in a HIP buffer\n", what,
+                     t != nullptr ? t->name : "(null)");
+        std::abort();
+    }
+    return b;
+}
+
+// The descriptors of a call's tensors, which have to be on one device; selects that device.
+class Operands {
+public:
+    explicit Operands(const char* what) : what_(what) {}
+    trc_hip_tensor operator()(const Tensor* t) {
+        HipBuffer* b = buffer_of(t, what_);
+        if (ordinal_ < 0) {
+            ordinal_ = b->ordinal();
+            check(trc_hip_init(ordinal_, nullptr), "select device");
+        } else if (ordinal_ != b->ordinal()) {
+            std::fprintf(stderr, "[traincpp-hip][FATAL] %s: tensor %s is on another device\n", what_, t->name);
+            std::abort();
+        }
+        return describe(t, b);
+    }
+
+private:
+    const char* what_;
+    int ordinal_ = -1;
+};
+
+trc_hip_lora_set lora_set(const HipLoraSet& s, Operands& at) {
+    return {at(s.a), at(s.b), at(s.scale), at(s.start), at(s.adapter)};
+}
+
+}  // namespace
+
+void hip_lora(const HipLoraSet& set, const Tensor* x, const Tensor* base, Tensor* h, Tensor* dst) {
+    Operands at("hip_lora");
+    const trc_hip_lora_set s = lora_set(set, at);
+    const trc_hip_tensor tx = at(x), th = at(h), td = at(dst);
+    trc_hip_tensor tb{};
+    if (base != nullptr) tb = at(base);
+    check(trc_hip_lora(&s, &tx, base != nullptr ? &tb : nullptr, &th, &td, nullptr), "hip_lora");
+}
+
+void hip_lora_back(const HipLoraSet& set, const Tensor* x, const Tensor* h, const Tensor* dy, Tensor* g, const Tensor* base,
+                   Tensor* dx, Tensor* da, Tensor* db, bool accumulate) {
+    Operands at("hip_lora_back");
+    const trc_hip_lora_set s = lora_set(set, at);
+    const trc_hip_tensor tx = at(x), th = at(h), ty = at(dy), tg = at(g), ta = at(da), tb = at(db);
+    trc_hip_tensor tbase{}, tdx{};
+    if (base != nullptr) tbase = at(base);
+    if (dx != nullptr) tdx = at(dx);
+    check(trc_hip_lora_back(&s, &tx, &th, &ty, &tg, base != nullptr ? &tbase : nullptr, dx != nullptr ? &tdx : nullptr, &ta, &tb,
+                            accumulate ? 1 : 0, nullptr),
+          "hip_lora_back");
+}
+
+void hip_preference_loss(const HipPreference& p) {
+    Operands at("hip_preference_loss");
+    const trc_hip_tensor l = at(p.logits), y = at(p.labels), s = at(p.start), r = at(p.ref), e = at(p.lse), lp = at(p.logp),
+                         sl = at(p.slope), lo = at(p.loss);
+    check(trc_hip_preference_loss(&l, &y, &s, &r, p.beta, p.smoothing, &e, &lp, &sl, &lo, nullptr), "hip_preference_loss");
+}
+
+void hip_preference_loss_back(const HipPreference& p, const Tensor* dloss, Tensor* dlogits) {
+    Operands at("hip_preference_loss_back");
+    const trc_hip_tensor l = at(p.logits), y = at(p.labels), s = at(p.start), e = at(p.lse), sl = at(p.slope), d = at(dloss),
+                         dl = at(dlogits);
+    check(trc_hip_preference_loss_back(&l, &y, &s, &e, &sl, &d, p.beta, &dl, nullptr), "hip_preference_loss_back");
+}
+
+struct HipAdamW::State {
+    std::vector<trc_hip_adamw_tensor> tensors;
+    int bits = 32;
+    int ordinal = 0;
+    uint8_t* moments = nullptr;  // device: every tensor's moments and scales
+    size_t bytes = 0;
+    void* plan = nullptr;
+    int64_t steps = 0;
+    void select() const { check(trc_hip_init(ordinal, nullptr), "select device"); }
+};
+
+HipAdamW::HipAdamW(Tensor* const* params, Tensor* const* grads, size_t count, int bits, const float* decay)
+    : s_(new State) {
+    const char* const what = "HipAdamW";
+    Operands at(what);
+    s_->bits = bits;
+    // one allocation, each piece of it at a multiple of 256 bytes
+    std::vector<size_t> offsets;
+    for (size_t i = 0; i < count; ++i) {
+        const trc_hip_tensor p = at(params[i]), g = at(grads[i]);
+        const int64_t n = tensor_nelements(params[i]);
+        if (params[i]->type != TYPE_F32 || !tensor_is_contiguous(params[i]) || !tensor_is_contiguous(grads[i]) ||
+            tensor_nelements(grads[i]) != n) {
+            std::fprintf(stderr, "[traincpp-hip][FATAL] %s: tensor %s is not a contiguous F32 tensor of its gradient's size\n",
+                         what, params[i]->name);
+            std::abort();
+        }
+        s_->ordinal = hip_buffer_of(params[i])->ordinal();
+        trc_hip_adamw_tensor t{};
+        t.param = (float*) p.data;
+        t.grad = g.data;
+        t.grad_type = g.type;
+        t.n = n;
+        t.decay = decay != nullptr ? decay[i] : 1.f;
+        s_->tensors.push_back(t);
+        const size_t state = (size_t) n * (bits == 8 ? 1 : sizeof(float));
+        const size_t scales = bits == 8 ? (size_t) ((n + TRC_HIP_ADAMW_BLOCK - 1) / TRC_HIP_ADAMW_BLOCK) * sizeof(float) : 0;
+        for (size_t b : {state, state, scales, scales}) {
+            offsets.push_back(s_->bytes);
+            s_->bytes += (b + 255) / 256 * 256;
+        }
+    }
+    if (s_->bytes > 0) {
+        void* p = nullptr;
+        check(trc_hip_malloc(&p, s_->bytes), "HipAdamW (moments)");
+        s_->moments = (uint8_t*) p;
+        check(trc_hip_memset(p, 0, s_->bytes, nullptr), "HipAdamW (moments)");
+    }
+    for (size_t i = 0; i < count; ++i) {
+        trc_hip_adamw_tensor& t = s_->tensors[i];
+        t.m = s_->moments + offsets[4 * i];
+        t.v = s_->moments + offsets[4 * i + 1];
+        t.m_scale = (float*) (s_->moments + offsets[4 * i + 2]);
+        t.v_scale = (float*) (s_->moments + offsets[4 * i + 3]);
+    }
+    check(trc_hip_adamw_create(s_->tensors.data(), (int64_t) count, bits, &s_->plan), what);
+}
+
+HipAdamW::~HipAdamW() {
+    trc_hip_init(s_->ordinal, nullptr);
+    trc_hip_sync(nullptr);
+    trc_hip_adamw_destroy(s_->plan);
+    trc_hip_free(s_->moments);
+    delete s_;
+}
+
+void HipAdamW::step(const HipAdamWParams& p) {
+    s_->select();
+    const trc_hip_adamw_hyper h{p.lr, p.beta1, p.beta2, p.eps, p.weight_decay, p.grad_scale, ++s_->steps};
+    check(trc_hip_adamw_step(s_->plan, &h, nullptr), "HipAdamW::step");
+}
+
+int64_t HipAdamW::steps() const { return s_->steps; }
+
+void HipAdamW::moments(size_t i, float* m, float* v) const {
+    s_->select();
+    trc_hip_adamw_tensor t = s_->tensors.at(i);
+    if (t.n == 0) return;
+    const size_t bytes = (size_t) t.n * sizeof(float);
+    StagingBuffer out(2 * bytes);
+    t.m_out = (float*) out.p;
+    t.v_out = (float*) out.p + t.n;
+    void* plan = nullptr;
+    check(trc_hip_adamw_create(&t, 1, s_->bits, &plan), "HipAdamW::moments");
+    check(trc_hip_adamw_moments(plan, nullptr), "HipAdamW::moments");
+    if (m != nullptr) check(trc_hip_d2h(m, t.m_out, bytes, nullptr), "HipAdamW::moments");
+    if (v != nullptr) check(trc_hip_d2h(v, t.v_out, bytes, nullptr), "HipAdamW::moments");
+    check(trc_hip_sync(nullptr), "HipAdamW::moments");
+    check(trc_hip_adamw_destroy(plan), "HipAdamW::moments");
+}
+
+size_t HipAdamW::state_bytes() const { return s_->bytes; }
+
+void HipAdamW::get_state(void* state) const {
+    s_->select();
+    check(trc_hip_d2h(state, s_->moments, s_->bytes, nullptr), "HipAdamW::get_state");
+}
+
+void HipAdamW::set_state(const void* state, int64_t steps) {
+    s_->select();
+    check(trc_hip_h2d(s_->moments, state, s_->bytes, nullptr), "HipAdamW::set_state");
+    s_->steps = steps;
+}
+
 }  // namespace traincpp
