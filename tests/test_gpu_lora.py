@@ -230,6 +230,14 @@ def test_many_tokens(hip):
     check_backward(Problem("f32", 260, 520, 32, [3000, 1, 1100], [1, 0, 2]))
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradients_of_one_small_adapter_over_many_tokens(hip, accumulate):
+    """Few columns and thousands of tokens: the gradients' tokens are split, and the parts joined."""
+    announce(f"lora one adapter, many tokens, accumulate {accumulate}")
+    check_backward(Problem("bf16", 70, 40, 6, [4500, 1, 1710], [0, 0, 0], n=1), accumulate=accumulate)
+    check_backward(Problem("f32", 35, 33, 17, [4097], [0], n=1), accumulate=accumulate, use_dx=False)
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 def test_values_that_are_not_finite_stay_with_their_token(hip, bad):
     """... and with their adapter: a token without one only passes its base on, and a neighbour in

@@ -224,10 +224,12 @@ struct Rows16 {
     }
 };
 
-constexpr int L_CHUNK = 32;  // elements of the long axis that a wave takes at a time
-// a wave's piece of LDS for contract_tile: x, then 16 columns of the weights
-template <class Elem>
-constexpr int contract_lds = Rows16<float, L_CHUNK>::BYTES + Rows16<Elem, L_CHUNK>::BYTES;
+// elements of the long axis that a wave takes at a time: more where the weights' registers allow it
+template <bool OUTER, int RT>
+constexpr int chunk_of = OUTER && RT == 1 ? 64 : 32;
+// a wave's piece of LDS for contract_tile: x, then 16 columns of A
+template <class Elem, bool OUTER, int RT>
+constexpr int contract_lds = Rows16<float, chunk_of<OUTER, RT>>::BYTES + (OUTER ? 0 : Rows16<Elem, chunk_of<OUTER, RT>>::BYTES);
 
 // sum_n x[t][n] W(n, r) for the tile's tokens, n in lo .. hi-1 and r in r0 .. r0 + 16 RT - 1,
 // where W(n, r) is w[r][n] (A) or, with OUTER, w[n][r] (B); each sum goes to
@@ -239,13 +241,13 @@ __device__ __forceinline__ void contract_tile(const Tile& t, const Rows& x, cons
                                               int64_t hi, uint8_t* lds, Partial<WAVES, RT>& part, Sink&& sink) {
     typedef Wt<TYPE> W;
     typedef typename W::Elem Elem;
-    constexpr int CN = L_CHUNK, U = CN / 16;
+    constexpr int CN = chunk_of<OUTER, RT>, U = CN / 16;
     constexpr int ES = sizeof(Elem);
     typedef Rows16<float, CN> X;
     typedef Rows16<Elem, CN> A;
     const int lane = (int) threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    uint8_t* const xs = lds + wave * contract_lds<Elem>;
+    uint8_t* const xs = lds + wave * contract_lds<Elem, OUTER, RT>;
     uint8_t* const ws = xs + X::BYTES;
     const uint8_t* const xb = x.p + (int64_t) t.lo * x.nb1;
     const uint32_t wrow = (uint32_t) wm.row * ES;
@@ -409,18 +411,20 @@ __device__ __forceinline__ void contract_one(const Tile& t, const Rows& x, const
                 const int left = (int) min((int64_t) 8, max((int64_t) 0, hi - n - 8 * lane));
                 if (left == 8) {
                     const f4u x0 = load_at<f4u>(xb + n * 4, 32 * lane), x1 = load_at<f4u>(xb + n * 4, 32 * lane + 16);
-                    typename W::template Raw<4> w0[8], w1[8];
+                    f4v raw[8][ES / 2];
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
                         const uint8_t* const row = wb + (min(8 * g + r, R - 1) * wm.row + n) * ES;
-                        w0[r] = load_at<typename W::template Raw<4>>(row, 8 * ES * lane);
-                        w1[r] = load_at<typename W::template Raw<4>>(row, 8 * ES * lane + 4 * ES);
+#pragma unroll
+                        for (int k = 0; k < ES / 2; ++k) raw[r][k] = load_at<v16u>(row, 8 * ES * lane + 16 * k).v;
                     }
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
+                    for (int r = 0; r < 8; ++r) {
+                        Elem w[8];
+                        __builtin_memcpy(w, raw[r], sizeof(w));
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            acc[r] = fmaf(x1[k], W::get(w1[r][k]), fmaf(x0[k], W::get(w0[r][k]), acc[r]));
+                        for (int k = 0; k < 4; ++k) acc[r] = fmaf(x1[k], W::get(w[4 + k]), fmaf(x0[k], W::get(w[k]), acc[r]));
+                    }
                 } else {
                     for (int k = 0; k < left; ++k) {
                         const float xk = load_at<float>(xb + n * 4, 32 * lane + 4 * k);
@@ -449,8 +453,11 @@ __device__ __forceinline__ void contract_one(const Tile& t, const Rows& x, const
         __syncthreads();
         for (int i = (int) threadIdx.x; i < here * 8; i += WAVES * 64) {
             const int r = 8 * (g0 + i / 8) + i % 8;
-            float sum = 0.f;
-            for (int k = 0; k < per; ++k) sum += red[(k * here + i / 8) * 8 + i % 8];
+            float part[WAVES], sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k) part[k] = red[min(k * here + i / 8, WAVES - 1) * 8 + i % 8];
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k) sum += k < per ? part[k] : 0.f;
             if (r < R) sink(0, r, sum);
         }
     }
@@ -461,7 +468,7 @@ __device__ __forceinline__ void contract_one(const Tile& t, const Rows& x, const
 // rounded up to 16 RT. A wave makes 64 columns of the 16 tokens at a time; column
 // 4 (l % 16) + c of the 64 is tile c's, so a lane has four neighbours of each of its four
 // tokens, and base and out are read and written in runs of 256 bytes.
-template <int TYPE, bool OUTER, int WAVES, int RT>
+template <int TYPE, bool OUTER, int WAVES, int RT, bool EARLY = false>
 struct Expand {
     typedef Wt<TYPE> W;
     typedef typename W::Elem Elem;
@@ -530,8 +537,7 @@ struct Expand {
 #pragma unroll
         for (int v = 0; v < 4; ++v) s.b[v] = __builtin_nontemporal_load((const f4u*) (bp + n0 * 4 + bo[v]));
     }
-    // The first columns' base, long before run() where there are registers for it.
-    static constexpr bool EARLY = RT == 1;
+    // With EARLY, the first columns' base is loaded here, long before run().
     __device__ __forceinline__ void start() {
         if (EARLY && full() && wave < steps) stream(first, n_lo + wave * LE_COLS);
     }
@@ -801,44 +807,33 @@ __device__ __forceinline__ void zero_h(const Tile& t, int R, int r0, int rn, flo
     }
 }
 
-template <int TYPE, int WAVES, int RT>
+template <int TYPE, bool OUTER, int WAVES, int RT>
 union ContractLds {
-    __attribute__((aligned(16))) uint8_t stage[WAVES * contract_lds<typename Wt<TYPE>::Elem>];
+    __attribute__((aligned(16))) uint8_t stage[WAVES * contract_lds<typename Wt<TYPE>::Elem, OUTER, RT>];
     Partial<WAVES, RT> part;
 };
 // floats of a tile's h in LDS
 template <int RT>
 constexpr int h_floats = LT * ((RT == 4 ? L_MAX_RANK : 16 * RT) + 4);
 
-// h (or g, scaled) alone. Blocks: (tile, 16 RT of the rank, part of the long axis); part p
-// goes to out + p T R.
-template <int TYPE, bool OUTER, int WAVES, int RT>
-__device__ __forceinline__ void contract_block(int tile, int rank_block, int part_index, const Rows& x, const Matrix& wm,
-                                               int R, const Batch& b, bool scaled, int64_t part_len, float* out,
-                                               ContractLds<TYPE, WAVES, RT>& lds) {
-    const Tile t = find_tile(b, tile);
-    if (t.tokens == 0) return;
-    out += (int64_t) part_index * b.T * R;
-    const int r0 = rank_block * (16 * RT);
-    if (t.adapter < 0) {
-        zero_h(t, R, r0, 16 * RT, out, WAVES * 64);
-        return;
-    }
-    const float s = scaled ? b.scale[t.adapter] : 1.f;
-    const int64_t lo = (int64_t) part_index * part_len, hi = min(lo + part_len, x.n);
-    auto sink = [&](int tok, int r, float v) { out[(int64_t) (t.lo + tok) * R + r] = v * s; };
-    if (!OUTER && t.tokens == 1) {
-        if (rank_block == 0) contract_one<TYPE, WAVES>(t, x, wm, R, lo, hi, (float*) lds.stage, sink);
-    } else {
-        contract_tile<TYPE, OUTER, WAVES, RT>(t, x, wm, R, r0, lo, hi, lds.stage, lds.part, sink);
-    }
-}
-
+// h alone. Blocks: (tile, 16 RT of the rank, part of the long axis); part p goes to out + p T R.
 template <int TYPE, int RT>
-__global__ __launch_bounds__(512) L_FOUR_WAVES void k_contract(Rows x, Matrix wm, int R, Batch b, int64_t part_len, float* __restrict__ out) {
-    __shared__ ContractLds<TYPE, 8, RT> lds;
-    contract_block<TYPE, false, 8, RT>((int) blockIdx.x, (int) blockIdx.y, (int) blockIdx.z, x, wm, R, b, false, part_len, out,
-                                       lds);
+__global__ __launch_bounds__(512) L_FOUR_WAVES void k_contract(Rows x, Matrix wm, int R, Batch b, int64_t part_len,
+                                                                float* __restrict__ out) {
+    const Tile t = find_tile(b, (int) blockIdx.x);
+    if (t.tokens == 0) return;
+    __shared__ ContractLds<TYPE, false, 8, RT> lds;
+    out += (int64_t) blockIdx.z * b.T * R;
+    const int r0 = (int) blockIdx.y * (16 * RT);
+    const int64_t lo = (int64_t) blockIdx.z * part_len, hi = min(lo + part_len, x.n);
+    auto sink = [&](int tok, int r, float v) { out[(int64_t) (t.lo + tok) * R + r] = v; };
+    if (t.adapter < 0) {
+        zero_h(t, R, r0, 16 * RT, out, 512);
+    } else if (t.tokens == 1) {
+        if (r0 == 0) contract_one<TYPE, 8>(t, x, wm, R, lo, hi, (float*) lds.stage, sink);
+    } else {
+        contract_tile<TYPE, false, 8, RT>(t, x, wm, R, r0, lo, hi, lds.stage, lds.part, sink);
+    }
 }
 
 // y of a tile's columns blockIdx.y * cols .. from h in parts; the first columns' workgroups
@@ -857,7 +852,7 @@ __global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float*
     }
     const Tile t = find_tile(b, tile);
     if (t.tokens == 0) return;
-    typedef Expand<TYPE, false, LE_THREADS / 64, RT> E;
+    typedef Expand<TYPE, false, LE_THREADS / 64, RT, RT == 1> E;
     __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
     __shared__ __attribute__((aligned(16))) uint8_t stage[LE_THREADS / 64 * E::LDS];
     const int64_t n_lo = (int64_t) slice * cols;
@@ -883,9 +878,9 @@ __global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix
                                                       float* __restrict__ h, int cols) {
     const Tile t = find_tile(b, (int) blockIdx.x);
     if (t.tokens == 0) return;
-    typedef Expand<TYPE, false, WAVES, RT> E;
+    typedef Expand<TYPE, false, WAVES, RT, RT == 1> E;  // (there are registers for it)
     __shared__ union {
-        ContractLds<TYPE, WAVES, RT> contract;
+        ContractLds<TYPE, false, WAVES, RT> contract;
         __attribute__((aligned(16))) uint8_t expand[WAVES * E::LDS];
     } lds;
     __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
@@ -1016,40 +1011,50 @@ __device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R
     }
 }
 
-// The first launch of the backward pass: dB, then g.
+// The first launch of the backward pass: dB, then g = s B^T dy.
 template <int TYPE, int RT>
 __global__ __launch_bounds__(LO_WAVES * 64) void k_back_b(Outer o, int outers, Rows dy, Matrix bm, int R, Batch b,
                                                            float* __restrict__ g) {
-    __shared__ ContractLds<TYPE, LO_WAVES, RT> lds;
+    __shared__ ContractLds<TYPE, true, LO_WAVES, RT> lds;
     if ((int) blockIdx.x < outers) {
         outer_block<false, RT>(blockIdx.x, o, R, b, lds.part);
-    } else {
-        const int i = (int) blockIdx.x - outers, rank_blocks = (R + 16 * RT - 1) / (16 * RT);
-        contract_block<TYPE, true, LO_WAVES, RT>(i / rank_blocks, i % rank_blocks, 0, dy, bm, R, b, true, dy.n, g, lds);
+        return;
     }
+    const int i = (int) blockIdx.x - outers, rank_blocks = (R + 16 * RT - 1) / (16 * RT);
+    const Tile t = find_tile(b, i / rank_blocks);
+    if (t.tokens == 0) return;
+    const int r0 = i % rank_blocks * (16 * RT);
+    if (t.adapter < 0) {
+        zero_h(t, R, r0, 16 * RT, g, LO_WAVES * 64);
+        return;
+    }
+    const float s = b.scale[t.adapter];
+    contract_tile<TYPE, true, LO_WAVES, RT>(t, dy, bm, R, r0, 0, dy.n, lds.stage, lds.part,
+                                            [&](int tok, int r, float v) { g[(int64_t) (t.lo + tok) * R + r] = v * s; });
 }
 
-// The second: dA, then dx.
+// The second: dA, then dx, `cols` columns of it a workgroup.
 template <int TYPE, int RT>
 __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, const float* __restrict__ g, Matrix am, int R,
                                                            Batch b, const uint8_t* base, size_t base_nb1, int64_t N,
                                                            uint8_t* dx, size_t dx_nb1, int cols) {
     __shared__ union {
         Partial<LO_WAVES, RT> part;
-        float hs[h_floats<RT>];
+        __attribute__((aligned(16))) float hs[h_floats<RT>];
     } lds;
     if ((int) blockIdx.x < outers) {
         outer_block<true, RT>(blockIdx.x, o, R, b, lds.part);
-    } else {
-        const int i = (int) blockIdx.x - outers, slices = (int) ((N + cols - 1) / cols);
-        const Tile t = find_tile(b, i / slices);
-        if (t.tokens == 0) return;
-        const int64_t n_lo = (int64_t) (i % slices) * cols;
-        Expand<TYPE, true, LO_WAVES, RT> e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
-        e.start();
-        stage_h<RT>(t, g, 1, b.T, R, 1.f, nullptr, lds.hs, LO_WAVES * 64);
-        e.run(lds.hs);
+        return;
     }
+    const int i = (int) blockIdx.x - outers, slices = (int) ((N + cols - 1) / cols);
+    const Tile t = find_tile(b, i / slices);
+    if (t.tokens == 0) return;
+    const int64_t n_lo = (int64_t) (i % slices) * cols;
+    typedef Expand<TYPE, true, LO_WAVES, RT, RT == 1> E;
+    E e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
+    e.start();
+    stage_h<RT>(t, g, 1, b.T, R, 1.f, nullptr, lds.hs, LO_WAVES * 64);
+    e.run(lds.hs);
 }
 
 // Gradients whose tokens were split: the parts in order.
@@ -1147,15 +1152,16 @@ int forward_apart(const Call& c, const trc_hip_tensor& x, const trc_hip_tensor* 
     return check_launch("lora (expand)");
 }
 
-// How a gradient's blocks are laid out: tokens split where there are few column blocks, 512
-// or more each, while the parts fit into `room` floats at `ws`.
+// How a gradient's blocks are laid out: tokens split where there are few column blocks and an adapter has
+// 2048 tokens or more for each part (a launch to join them costs what some 1000 tokens take), while the parts fit
+// into `room` floats at `ws`.
 Outer outer_of(const Call& c, const trc_hip_tensor& x, const float* h, const trc_hip_tensor& d, bool scaled, bool accumulate,
                float* ws, int64_t room) {
     Outer o{rows_of(x), h, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate, 0, 0, 1, c.batch.T, ws};
     o.col_blocks = (int) ((x.ne[0] + LO_COLS - 1) / LO_COLS);
     o.rank_blocks = rank_blocks(c.R);
     const int64_t blocks = o.blocks(c.batch.adapters), T = c.batch.T;
-    int64_t n = std::min((int64_t) device_cus() / blocks, T / 512);
+    int64_t n = std::min((int64_t) device_cus() / blocks, T / (2048 * c.batch.adapters));
     n = std::min(n, room / (x.ne[0] * c.R * c.batch.adapters));
     if (n > 1) {
         o.split_len = round_up((T + n - 1) / n, 64);
@@ -1205,7 +1211,8 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
         ob.parts = (float*) ws;
         oa.parts = (float*) ws + half;
     }
-    const int64_t nb = ob.blocks(c.batch.adapters), na = oa.blocks(c.batch.adapters), ng = tiles * rank_blocks(c.R);
+    const int64_t nb = ob.blocks(c.batch.adapters), na = oa.blocks(c.batch.adapters);
+    const int64_t ng = tiles * rank_blocks(c.R);
     const int64_t slices = std::max(std::min(2 * device_cus() / tiles, (K + 1023) / 1024), (int64_t) 1);
     const int cols = (int) round_up((K + slices - 1) / slices, LE_COLS);
     const int64_t nx = dx != nullptr ? tiles * ((K + cols - 1) / cols) : 0;
@@ -1218,7 +1225,7 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
                                ob, (int) nb, rows_of(dy), c.b, c.R, c.batch, (float*) g.data);
         });
     });
-    int rc = check_launch("lora_back (g, dB)");
+    int rc = check_launch("lora_back (dB, g)");
     if (rc != TRC_HIP_OK) return rc;
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
@@ -1228,7 +1235,7 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
                                dx != nullptr ? dx->nb[1] : (size_t) 0, cols);
         });
     });
-    rc = check_launch("lora_back (dx, dA)");
+    rc = check_launch("lora_back (dA, dx)");
     for (int k = 0; k < 2 && rc == TRC_HIP_OK; ++k) {
         const Outer& o = k == 0 ? ob : oa;
         if (o.splits == 1) continue;
