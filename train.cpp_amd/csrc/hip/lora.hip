@@ -7,7 +7,9 @@
 //   dA_a = sum_t g_t x_t^T      dB_a = s_a sum_t dy_t h_t^T
 //
 // Three steps make all six, on v_mfma_f32_16x16x4_f32 (products as exact as float
-// FMAs; adapters in 16 bits are widened):
+// FMAs; adapters in 16 bits are widened). h and y of bfloat16 adapters are made on the bfloat16
+// instructions instead, the other factor in three parts, which is exact as well and takes a fifth of
+// the time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 43 us, 54 with the FP32 instructions.
 //   contract  h and g: a wide activation times a matrix of R rows or columns
 //   expand    y and dx: base plus a matrix times h or g
 //   outer     dA and dB: sums over tokens of outer products
@@ -224,6 +226,42 @@ struct Rows16 {
     }
 };
 
+// N floats, each the sum of three in bfloat16 that hold 8 bits of it each (down to 2^-126; an infinity or NaN
+// is in the first alone), so that products with numbers in bfloat16 are exact.
+template <int N>
+struct Thirds {
+    typedef uint32_t Bits __attribute__((ext_vector_type(N / 2)));
+    Bits hi, mid, lo;
+    __device__ __forceinline__ explicit Thirds(const float (&x)[N]) {
+        uint32_t a[N], b[N], c[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            a[k] = __builtin_bit_cast(uint32_t, x[k]);
+            const bool finite = __builtin_fabsf(x[k]) < __builtin_inff();
+            const float rest = finite ? x[k] - __builtin_bit_cast(float, a[k] & 0xffff0000u) : 0.f;
+            b[k] = __builtin_bit_cast(uint32_t, rest);
+            c[k] = __builtin_bit_cast(uint32_t, rest - __builtin_bit_cast(float, b[k] & 0xffff0000u));
+        }
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) {  // (the upper halves of two)
+            hi[k] = __builtin_amdgcn_perm(a[2 * k + 1], a[2 * k], 0x07060302u);
+            mid[k] = __builtin_amdgcn_perm(b[2 * k + 1], b[2 * k], 0x07060302u);
+            lo[k] = __builtin_amdgcn_perm(c[2 * k + 1], c[2 * k], 0x07060302u);
+        }
+    }
+};
+// Products of bfloat16, 4 or 8 to a lane: sums over 16 or 32
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f4 mfma_bf16(u2 a, u2 b, f4 c) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f4 mfma_bf16(u4 a, u4 b, f4 c) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
 // elements of the long axis that a wave takes at a time: more where the weights' registers allow it
 template <bool OUTER, int RT>
 constexpr int chunk_of = OUTER && RT == 1 ? 64 : 32;
@@ -304,6 +342,9 @@ __device__ __forceinline__ void contract_tile(const Tile& t, const Rows& x, cons
 #pragma unroll
                     for (int j = 0; j < RT; ++j) acc[j] = mfma(xv[u][k], W::get(element(c.b[u][k], j)), acc[j]);
         } else {
+            static_assert(U == 2, "a chunk is 32 elements here, 8 to a lane");
+            const float x8[8] = {xv[0][0], xv[0][1], xv[0][2], xv[0][3], xv[1][0], xv[1][1], xv[1][2], xv[1][3]};
+            const Thirds<8> x3(x8);
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
                 if constexpr (AHEAD) {
@@ -318,6 +359,13 @@ __device__ __forceinline__ void contract_tile(const Tile& t, const Rows& x, cons
 #pragma unroll
                 for (int u = 0; u < U; ++u) wv[u] = A::four(ws, u);
                 lds_in_order();
+                if constexpr (TYPE == TRC_HIP_TYPE_BF16) {
+                    const u4 w8 = __builtin_bit_cast(u4, __builtin_shufflevector(wv[0], wv[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    acc[j] = mfma_bf16(x3.lo, w8, acc[j]);
+                    acc[j] = mfma_bf16(x3.mid, w8, acc[j]);
+                    acc[j] = mfma_bf16(x3.hi, w8, acc[j]);
+                    continue;
+                }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -463,28 +511,44 @@ __device__ __forceinline__ void contract_one(const Tile& t, const Rows& x, const
     }
 }
 
+// A row's first byte up to 2^31 on; what lies further is neither read (0 comes back) nor stored
+// to. Nothing is, with no memory.
+constexpr uint32_t L_RSRC_WORD3 = 0x00020000u;  // gfx9 buffer resource: raw 32-bit dwords
+constexpr uint32_t L_SPAN = 0x80000000u, L_OUTSIDE = 0xffffff00u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t span(const uint8_t* p, bool memory) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*) p, (short) 0, memory ? (int) L_SPAN : 0, L_RSRC_WORD3);
+}
+
 // out[t][n] = base[t][n] + sum_r hs[t][r] W(n, r) for n in n_lo .. n_hi-1: W(n, r) is w[n][r] (B)
 // or, with OUTER, w[r][n] (A). hs has rows of Rp + 4 floats with zeros from R to Rp, R
 // rounded up to 16 RT. A wave makes 64 columns of the 16 tokens at a time; column
 // 4 (l % 16) + c of the 64 is tile c's, so a lane has four neighbours of each of its four
-// tokens, and base and out are read and written in runs of 256 bytes.
-template <int TYPE, bool OUTER, int WAVES, int RT, bool EARLY = false>
+// tokens, and base and out are read and written in runs of 256 bytes. Tokens past the tile's are left out
+// by their offsets, so no tile has a branch around its loads and stores: with one, a wait for
+// loads waits for all that is under way.
+constexpr int NOTHING = 0, BASE = 1, ALL = 2;  // what is loaded early
+template <int TYPE, bool OUTER, int WAVES, int RT, bool WIDE = false, int EARLY = NOTHING>
 struct Expand {
     typedef Wt<TYPE> W;
     typedef typename W::Elem Elem;
-    typedef typename W::template Raw<4> Raw4;
     static constexpr int ES = sizeof(Elem);
-    // 16 of the rank, as loaded. A: [k] is row r0 + 4 quad + k, columns 4 col .. + 3. B: [i] is row
-    // 16 i + lane / 4 of the 64, r0 + 4 (lane % 4) .. + 3; it is turned through LDS.
+    // A block is KB of the rank, as loaded. A: [k] is row r0 + 4 quad + k, columns 4 col .. + 3. B: [i] is row
+    // 16 i + lane / 4 of the 64, r0 + F (lane % 4) .. + F-1; it is turned through LDS. A lane's F elements are
+    // 16 bytes for F32 and WIDE, else 8: a row's 64 bytes side by side are read at twice the rate of 32.
+    static constexpr int F = WIDE ? 8 : 4, KB = 4 * F;
+    typedef Elem Four __attribute__((ext_vector_type(F)));
+    typedef Elem FourU __attribute__((ext_vector_type(F), aligned(ES)));
     struct Weights {
-        Raw4 w[4];
+        Four w[4];
     };
+    // such blocks that are under way ahead of the one that is multiplied (in 32 registers at most)
+    static constexpr int NB = 16 * RT / KB, D = NB < 32 / (F * ES) ? NB : 32 / (F * ES);
     // B in LDS: row n of the 64 is (n % 4, n / 4), since a lane reads rows 4 col + c; the
     // paddings spread both the rows of a store and those of a read over the banks.
-    static constexpr int PITCH = ES == 4 ? 80 : 40, BLOCK = 16 * PITCH + (ES == 4 ? 64 : 32);
+    static constexpr int PITCH = 5 * F * ES, BLOCK = 16 * PITCH + 4 * F * ES;
     static constexpr int LDS = OUTER ? 0 : 4 * BLOCK;  // bytes of a wave
     struct Base {
-        f4u b[4];
+        f4 b[4];
     };
     const Tile& t;
     const uint8_t *w, *bp, *op;
@@ -494,7 +558,8 @@ struct Expand {
     bool based;
     int64_t N, n_lo, steps;  // steps: whole ones
     uint32_t bo[4], oo[4];
-    Base first;
+    Weights window[D];
+    Base b;
 
     __device__ __forceinline__ Expand(const Tile& t, const Matrix& wm, int R, const uint8_t* base, size_t base_nb1, int64_t N,
                                       uint8_t* out, size_t out_nb1, int64_t n_lo, int64_t n_hi, uint8_t* all_lds)
@@ -509,121 +574,140 @@ struct Expand {
         bp = base + (int64_t) t.lo * base_nb1;
         op = out + (int64_t) t.lo * out_nb1;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {  // (tokens past the tile's read the last one's base and are not stored)
-            const uint32_t tok = (uint32_t) min(4 * quad + v, t.tokens - 1);
-            bo[v] = tok * (uint32_t) base_nb1 + 16 * col;
-            oo[v] = tok * (uint32_t) out_nb1 + 16 * col;
+        for (int v = 0; v < 4; ++v) {
+            const uint32_t tok = (uint32_t) (4 * quad + v);
+            bo[v] = (int) tok < t.tokens ? tok * (uint32_t) base_nb1 + 16 * col : L_OUTSIDE;
+            oo[v] = (int) tok < t.tokens ? tok * (uint32_t) out_nb1 + 16 * col : L_OUTSIDE;
         }
         steps = (this->N - n_lo) / LE_COLS;
     }
-    // Whether weights are loaded in fours of r; of the fours past R the last one is read again.
-    __device__ __forceinline__ bool fours() const { return R % 4 == 0; }
-    // Whether this is a tile of 16 tokens with all that the pipelined loop takes for granted.
-    __device__ __forceinline__ bool full() const { return t.tokens == LT && t.adapter >= 0 && based && fours(); }
+    // Whether weights are loaded in blocks; of the lanes' elements past R the last ones are read again.
+    __device__ __forceinline__ bool fours() const { return t.adapter >= 0 && R % F == 0; }
 
     __device__ __forceinline__ void load(Weights& s, int64_t n0, int r0) const {
-        const uint32_t r = (uint32_t) min(r0 + 4 * (OUTER ? quad : lane & 3), R - 4);
+        const uint32_t r = (uint32_t) min(r0 + F * (OUTER ? quad : lane & 3), R - F);
         const uint32_t o = OUTER ? r * wrow + 4 * col * ES : (lane >> 2) * wrow + r * ES;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s.w[k] = load_at<Raw4>(OUTER ? w + n0 * ES + k * (int64_t) wrow : w + (n0 + 16 * k) * wrow, o);
+        for (int k = 0; k < 4; ++k) s.w[k] = load_at<FourU>(OUTER ? w + n0 * ES + k * (int64_t) wrow : w + (n0 + 16 * k) * wrow, o);
     }
+    // base is read and the outputs are written once, past the caches (auxiliary bit 1): 4096 x 4096 outputs in 44 us
+    // where plain accesses take 50
     __device__ __forceinline__ void load(Base& s, int64_t n0) const {
+        const __amdgpu_buffer_rsrc_t m = span(bp + n0 * 4, based);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s.b[v] = load_at<f4u>(bp + n0 * 4, bo[v]);
+        for (int v = 0; v < 4; ++v) s.b[v] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(m, bo[v], 0, 2));
     }
-    // A full tile's base is read and its outputs are written once, past the caches: 4096 x 4096 outputs in 44 us
-    // where plain accesses take 50.
-    __device__ __forceinline__ void stream(Base& s, int64_t n0) const {
+    __device__ __forceinline__ void store(const f4 (&sum)[4], int64_t n0) const {
+        const __amdgpu_buffer_rsrc_t m = span(op + n0 * 4, true);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) s.b[v] = __builtin_nontemporal_load((const f4u*) (bp + n0 * 4 + bo[v]));
+        for (int v = 0; v < 4; ++v) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, sum[v]), m, oo[v], 0, 2);
     }
-    // With EARLY, the first columns' base is loaded here, long before run().
-    __device__ __forceinline__ void start() {
-        if (EARLY && full() && wave < steps) stream(first, n_lo + wave * LE_COLS);
-    }
-    // zeros past R, whatever was read there
-    __device__ __forceinline__ void multiply(const Weights& s, const float* hrow, int r0, f4 (&acc)[4]) const {
-        typedef std::conditional_t<ES == 4, f4, h4> Four;
-        const f4 hv = *(const f4*) (hrow + r0);
-        const bool in = r0 + 16 <= R || r0 + 4 * quad < R;
+    // zeros past R, whatever was read there; `loaded` once s may be loaded again
+    template <class Then>
+    __device__ __forceinline__ void multiply(const Weights& s, const float* hrow, int r0, f4 (&acc)[4], Then&& loaded) const {
+        float hv[F];
+#pragma unroll
+        for (int k = 0; k < F; k += 4) {
+            const f4 x = *(const f4*) (hrow + r0 + k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) hv[k + i] = x[i];
+        }
+        const bool in = r0 + KB <= R || r0 + F * quad < R;
         Four v[4];
         if constexpr (!OUTER) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int n = 16 * i + (lane >> 2);
-                *(Four*) (lds + (n & 3) * BLOCK + (n >> 2) * PITCH + 4 * (lane & 3) * ES) = (Four) s.w[i];
+                *(Four*) (lds + (n & 3) * BLOCK + (n >> 2) * PITCH + (lane & 3) * F * ES) = s.w[i];
             }
             lds_in_order();
+            loaded();
+            auto turned = [&](int c) { return *(const Four*) (lds + c * BLOCK + col * PITCH + quad * F * ES); };
+            if constexpr (TYPE == TRC_HIP_TYPE_BF16) {
+                typedef typename Thirds<F>::Bits Bits;
+                const Thirds<F> h3(hv);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = *(const Four*) (lds + c * BLOCK + col * PITCH + 4 * quad * ES);
+                for (int c = 0; c < 4; ++c) {
+                    const Bits x = in ? __builtin_bit_cast(Bits, turned(c)) : Bits(0);
+                    acc[c] = mfma_bf16(h3.lo, x, acc[c]);
+                    acc[c] = mfma_bf16(h3.mid, x, acc[c]);
+                    acc[c] = mfma_bf16(h3.hi, x, acc[c]);
+                }
+                lds_in_order();
+                return;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = turned(c);
             lds_in_order();
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < F; ++k) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const float x = W::get(OUTER ? s.w[k][c] : v[c][k]);
                 acc[c] = mfma(hv[k], in ? x : 0.f, acc[c]);
             }
         }
+        if (OUTER) loaded();
     }
-    // All of the rank: the first RT blocks of 16 with the next one's loads under way (and `last` after
-    // the last of them), then the others.
-    template <class Last>
-    __device__ __forceinline__ void product(const float* hrow, int64_t n0, f4 (&acc)[4], Last&& last) const {
-        Weights s[2];
-        load(s[0], n0, 0);
-#pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            if (j + 1 < RT) load(s[(j + 1) & 1], n0, 16 * (j + 1));
-            if (j + 2 == RT || RT == 1) last();
-            loads_stay();
-            multiply(s[j & 1], hrow, 16 * j, acc);
-        }
-        for (int r0 = 16 * RT; r0 < R; r0 += 16) {
-            load(s[0], n0, r0);
-            multiply(s[0], hrow, r0, acc);
-        }
-    }
-    static __device__ __forceinline__ f4 row(const f4 (&acc)[4], int v) { return f4{acc[0][v], acc[1][v], acc[2][v], acc[3][v]}; }
-
-    // One step of a full tile, the next one's base (at next, or none) under way behind its weights, since
-    // loads arrive in the order they are waited for. Its stores have no branch around them, so that the
-    // wait for the loads behind them is counted and does not wait for the stores.
-    template <bool NEXT>
-    __device__ __forceinline__ void step(const Base& b, const float* hrow, int64_t n0, Base& next, int64_t n_next) const {
-        f4 acc[4];
+    static __device__ __forceinline__ void clear(f4 (&acc)[4]) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
-        product(hrow, n0, acc, [&] {
-            if (NEXT) stream(next, n_next);
-        });
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const f4u sum = row(acc, v) + b.b[v];
-            __builtin_nontemporal_store(sum, (f4u*) ((uint8_t*) op + n0 * 4 + oo[v]));
-        }
     }
-    __device__ __forceinline__ void whole_steps(const float* hrow) const {
+    static __device__ __forceinline__ void add(Base& b, const f4 (&acc)[4]) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) b.b[v] += f4{acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
+    }
+
+    // The wave's first columns: weights, then base, since loads arrive in the order they are waited for. All of
+    // it is loaded long before run(), or base alone, or nothing, by the registers that there are.
+    template <bool WEIGHTS, bool FIRST_BASE>
+    __device__ __forceinline__ void begin() {
+        const int64_t n0 = n_lo + wave * LE_COLS;
+#pragma unroll
+        for (int j = 0; WEIGHTS && j < D; ++j) load(window[j], n0, KB * j);
+        if (FIRST_BASE) load(b, n0);
+    }
+    __device__ __forceinline__ bool begins() const { return fours() && wave < steps; }
+    __device__ __forceinline__ void start() {
+        if (EARLY != NOTHING && begins()) begin<EARLY == ALL, true>();
+    }
+    // 64 columns. A block's registers are loaded with the block D further on, of the next columns in the end; then
+    // base of those.
+    template <bool NEXT>
+    __device__ __forceinline__ void step(const float* hrow, int64_t n0, int64_t n_next) {
+        f4 acc[4];
+        clear(acc);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            Weights& s = window[j % D];
+            multiply(s, hrow, KB * j, acc, [&] {
+                if (j + D < NB) load(s, n0, KB * (j + D));
+                else if (NEXT) load(s, n_next, KB * (j + D - NB));
+                loads_stay();
+            });
+        }
+        for (int r0 = KB * NB; r0 < R; r0 += KB) {
+            Weights s;
+            load(s, n0, r0);
+            multiply(s, hrow, r0, acc, [] {});
+        }
+        add(b, acc);
+        f4 sum[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sum[v] = b.b[v];
+        if (NEXT) {
+            load(b, n_next);
+            loads_stay();
+        }
+        store(sum, n0);
+    }
+    __device__ __forceinline__ void whole_steps(const float* hrow) {
         constexpr int64_t S = WAVES * LE_COLS;
-        int64_t n0 = n_lo + wave * LE_COLS, left = (steps - 1 - wave) / WAVES;
-        Base b0, b1;
-        if constexpr (EARLY) {
-            b0 = first;
-        } else {
-            stream(b0, n0);
-        }
-        for (; left > 1; left -= 2) {
-            step<true>(b0, hrow, n0, b1, n0 + S);
-            step<true>(b1, hrow, n0 + S, b0, n0 + 2 * S);
-            n0 += 2 * S;
-        }
-        if (left > 0) {
-            step<true>(b0, hrow, n0, b1, n0 + S);
-            step<false>(b1, hrow, n0 + S, b0, 0);
-        } else {
-            step<false>(b0, hrow, n0, b1, 0);
-        }
+        int64_t n0 = n_lo + wave * LE_COLS;
+        begin<EARLY != ALL, EARLY == NOTHING>();
+        for (int64_t left = (steps - 1 - wave) / WAVES; left > 0; --left, n0 += S) step<true>(hrow, n0, n0 + S);
+        step<false>(hrow, n0, 0);
     }
     // Weights one by one, for ranks that are not whole fours and for the last columns.
     __device__ __forceinline__ void singly(const float* hrow, int64_t n0, f4 (&acc)[4]) const {
@@ -634,7 +718,7 @@ struct Expand {
         for (int r0 = 0; r0 < R; r0 += 4) {  // four of r, one for each quad
             const int r = r0 + quad;
             const uint32_t rc = (uint32_t) min(r, R - 1) * (OUTER ? wrow : ES);
-            const float hv = hrow[r0 - 3 * quad];
+            const float hv = hrow[r0 + quad - F * quad];
             Elem x[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) x[c] = load_at<Elem>(wn, nc[c] + rc);
@@ -642,49 +726,38 @@ struct Expand {
             for (int c = 0; c < 4; ++c) acc[c] = mfma(hv, r < R ? W::get(x[c]) : 0.f, acc[c]);
         }
     }
-    // One step of any tile and any columns.
-    __device__ __forceinline__ void any_step(const float* hrow, int64_t n0) const {
-        const bool whole = n0 + LE_COLS <= N;
-        Base b;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) b.b[v] = f4{0.f, 0.f, 0.f, 0.f};
-        if (based && whole) load(b, n0);
-        if (based && !whole) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int back = (int) min((int64_t) (4 * col + k), N - 1 - n0) - 4 * col;
-#pragma unroll
-                for (int v = 0; v < 4; ++v) b.b[v][k] = load_at<float>(bp + n0 * 4, (uint32_t) ((int) bo[v] + 4 * back));
-            }
-        }
+    // One step of any rank and any columns, with or without an adapter.
+    __device__ __forceinline__ void any_step(const float* hrow, int64_t n0) {
         f4 acc[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
-        if (t.adapter >= 0) {
-            if (whole && fours()) {
-                product(hrow, n0, acc, [] {});
-            } else {
-                singly(hrow, n0, acc);
-            }
+        clear(acc);
+        if (t.adapter >= 0) singly(hrow, n0, acc);
+        if (n0 + LE_COLS <= N) {
+            load(b, n0);
+            add(b, acc);
+            store(b.b, n0);
+            return;
         }
+        const __amdgpu_buffer_rsrc_t from = span(bp + n0 * 4, based), to = span(op + n0 * 4, true);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            if (4 * quad + v >= t.tokens) continue;
-            const f4 sum = row(acc, v) + b.b[v];
-            uint8_t* const p = (uint8_t*) op + n0 * 4 + oo[v];
-            if (whole) {
-                *(f4u*) p = sum;
-            } else {
+        for (int k = 0; k < 4; ++k) {
+            const bool in = n0 + 4 * col + k < N;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (n0 + 4 * col + k < N) *(float*) (p + 4 * k) = sum[k];
-            }
+            for (int v = 0; v < 4; ++v)
+                b.b[v][k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(from, in ? bo[v] + 4 * k : L_OUTSIDE, 0, 0));
+        }
+        add(b, acc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool in = n0 + 4 * col + k < N;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float) b.b[v][k]), to, in ? oo[v] + 4 * k : L_OUTSIDE, 0, 0);
         }
     }
-    __device__ __forceinline__ void run(const float* hs) const {
-        const float* const hrow = hs + col * ((R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4) + 4 * quad;
+    __device__ __forceinline__ void run(const float* hs) {
+        const float* const hrow = hs + col * ((R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4) + F * quad;
         int64_t i = wave;
-        if (full() && i < steps) {
+        if (begins()) {
             whole_steps(hrow);
             i += ((steps - 1 - wave) / WAVES + 1) * WAVES;
         }
@@ -745,9 +818,10 @@ struct ExpandOne {
             float sum[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                Elem x[E];
+                typedef Elem Piece __attribute__((ext_vector_type(E)));
+                Piece x;
                 if (R % E == 0) {
-                    __builtin_memcpy(x, &raw[u], 16);
+                    x = __builtin_bit_cast(Piece, raw[u]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < E; ++e)
@@ -836,6 +910,22 @@ __global__ __launch_bounds__(512) L_FOUR_WAVES void k_contract(Rows x, Matrix wm
     }
 }
 
+// Whether 16-bit adapters are expanded 16 bytes of a row at a time
+template <int TYPE, int RT>
+constexpr bool may_be_wide = TYPE != TRC_HIP_TYPE_F32 && RT > 1;
+template <int TYPE, int RT, class Body>
+__device__ __forceinline__ void either_width(int R, Body&& body) {
+    if constexpr (may_be_wide<TYPE, RT>) {
+        if (R % 8 == 0) {
+            body(std::true_type{});
+            return;
+        }
+    }
+    body(std::false_type{});
+}
+template <int TYPE, int RT>  // bytes of a wave
+constexpr int expand_lds = Expand<TYPE, false, 1, RT, may_be_wide<TYPE, RT>>::LDS;
+
 // y of a tile's columns blockIdx.y * cols .. from h in parts; the first columns' workgroups
 // store the sum of more than one part.
 template <int TYPE, int RT>
@@ -852,9 +942,8 @@ __global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float*
     }
     const Tile t = find_tile(b, tile);
     if (t.tokens == 0) return;
-    typedef Expand<TYPE, false, LE_THREADS / 64, RT, RT == 1> E;
     __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
-    __shared__ __attribute__((aligned(16))) uint8_t stage[LE_THREADS / 64 * E::LDS];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[LE_THREADS / 64 * expand_lds<TYPE, RT>];
     const int64_t n_lo = (int64_t) slice * cols;
     const float s = t.adapter >= 0 ? b.scale[t.adapter] : 1.f;
     float* const sums = n_lo == 0 ? h_sum : nullptr;
@@ -864,10 +953,13 @@ __global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float*
         stage_h<RT>(t, h, parts, b.T, R, s, sums, hs, LE_THREADS);
         e.run(hs);
     } else {
-        E e(t, wm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols, stage);
-        e.start();
-        stage_h<RT>(t, h, parts, b.T, R, s, sums, hs, LE_THREADS);
-        e.run(hs);
+        either_width<TYPE, RT>(R, [&](auto wide) {
+            Expand<TYPE, false, LE_THREADS / 64, RT, decltype(wide)::value, ALL> e(t, wm, R, base, base_nb1, N, out, out_nb1, n_lo,
+                                                                                    n_lo + cols, stage);
+            e.start();
+            stage_h<RT>(t, h, parts, b.T, R, s, sums, hs, LE_THREADS);
+            e.run(hs);
+        });
     }
 }
 
@@ -878,10 +970,9 @@ __global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix
                                                       float* __restrict__ h, int cols) {
     const Tile t = find_tile(b, (int) blockIdx.x);
     if (t.tokens == 0) return;
-    typedef Expand<TYPE, false, WAVES, RT, RT == 1> E;  // (there are registers for it)
     __shared__ union {
         ContractLds<TYPE, false, WAVES, RT> contract;
-        __attribute__((aligned(16))) uint8_t expand[WAVES * E::LDS];
+        __attribute__((aligned(16))) uint8_t expand[WAVES * expand_lds<TYPE, RT>];
     } lds;
     __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
     const int hrow = (R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4;
@@ -899,19 +990,22 @@ __global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix
         e.run(hs);
         return;
     }
-    E e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols, lds.expand);
-    e.start();
-    if (t.adapter < 0) {
-        if (blockIdx.y == 0) zero_h(t, R, 0, R, h, WAVES * 64);
-    } else {
-        for (int i = (int) threadIdx.x; i < LT * hrow; i += WAVES * 64) hs[i] = 0.f;
-        __syncthreads();
-        for (int r0 = 0; r0 < R; r0 += 16 * RT) {
-            contract_tile<TYPE, false, WAVES, RT>(t, x, am, R, r0, 0, x.n, lds.contract.stage, lds.contract.part, sink);
+    either_width<TYPE, RT>(R, [&](auto wide) {
+        Expand<TYPE, false, WAVES, RT, decltype(wide)::value, RT == 1 ? BASE : NOTHING> e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols,
+                                                                         lds.expand);
+        e.start();
+        if (t.adapter < 0) {
+            if (blockIdx.y == 0) zero_h(t, R, 0, R, h, WAVES * 64);
+        } else {
+            for (int i = (int) threadIdx.x; i < LT * hrow; i += WAVES * 64) hs[i] = 0.f;
             __syncthreads();
+            for (int r0 = 0; r0 < R; r0 += 16 * RT) {
+                contract_tile<TYPE, false, WAVES, RT>(t, x, am, R, r0, 0, x.n, lds.contract.stage, lds.contract.part, sink);
+                __syncthreads();
+            }
         }
-    }
-    e.run(hs);
+        e.run(hs);
+    });
 }
 
 // d(n, r) (+)= scale sum_t x[t][n] h[t][r] over the tokens of one adapter's requests:
@@ -1050,7 +1144,7 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
     const Tile t = find_tile(b, i / slices);
     if (t.tokens == 0) return;
     const int64_t n_lo = (int64_t) (i % slices) * cols;
-    typedef Expand<TYPE, true, LO_WAVES, RT, RT == 1> E;
+    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT == 1 ? ALL : NOTHING> E;
     E e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
     e.start();
     stage_h<RT>(t, g, 1, b.T, R, 1.f, nullptr, lds.hs, LO_WAVES * 64);
