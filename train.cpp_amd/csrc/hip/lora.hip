@@ -1042,43 +1042,52 @@ __device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R
 #pragma unroll
         for (int j = 0; j < RT; ++j) acc[c][j] = f4{0.f, 0.f, 0.f, 0.f};
     constexpr int U = 4;  // tokens of a lane that are loaded together
-    for (int q = 0; q < b.requests; ++q) {
-        if (b.ids[q] != adapter) continue;
-        const int64_t lo = max(min(max((int64_t) b.start[q], (int64_t) 0), b.T), t_lo);
-        const int64_t hi = min(max((int64_t) b.start[q + 1], lo), t_hi);
-        for (int64_t t0 = lo + 4 * U * wave; t0 < hi; t0 += 4 * U * LO_WAVES) {
-            // tokens past the last read it again, as zeros; columns past N read the last one
-            float xv[U][2], hv[U][RT];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t t = (uint32_t) min((int64_t) (4 * u + quad), hi - 1 - t0);
-                const uint8_t* const xb = o.x.p + t0 * o.x.nb1 + n0 * 4;
-                if (whole) {
-                    const f2u v = load_at<f2u>(xb, t * (uint32_t) o.x.nb1 + 8 * col);
-                    xv[u][0] = v[0], xv[u][1] = v[1];
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        xv[u][c] = load_at<float>(xb, t * (uint32_t) o.x.nb1 + 4 * (uint32_t) min((int64_t) (2 * col + c), N - 1 - n0));
-                }
-#pragma unroll
-                for (int j = 0; j < RT; ++j) hv[u][j] = load_at<float>(o.h + t0 * R, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
-            }
-            if (t0 + 4 * U > hi) {
+    int turn = wave;      // chunks of 4 U tokens until the wave's next
+    for (int q0 = 0; q0 < b.requests; q0 += 64) {
+        // each lane looks at a request; those of this adapter are taken in order
+        const int q = min(q0 + lane, b.requests - 1);
+        const int lo_q = (int) max(min(max((int64_t) b.start[q], (int64_t) 0), b.T), t_lo);
+        const int hi_q = (int) min(max((int64_t) b.start[q + 1], (int64_t) lo_q), t_hi);
+        uint64_t mine = __ballot(q0 + lane < b.requests && b.ids[q] == adapter && lo_q < hi_q);
+        for (; mine != 0; mine &= mine - 1) {
+            const int from = __builtin_ctzll(mine);
+            const int64_t lo = __builtin_amdgcn_readlane(lo_q, from), hi = __builtin_amdgcn_readlane(hi_q, from);
+            int64_t t0 = lo + 4 * U * turn;
+            for (; t0 < hi; t0 += 4 * U * LO_WAVES) {
+                // tokens past the last read it again, as zeros; columns past N read the last one
+                float xv[U][2], hv[U][RT];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const bool in = t0 + 4 * u + quad < hi;
-                    xv[u][0] = in ? xv[u][0] : 0.f, xv[u][1] = in ? xv[u][1] : 0.f;
+                    const uint32_t t = (uint32_t) min((int64_t) (4 * u + quad), hi - 1 - t0);
+                    const uint8_t* const xb = o.x.p + t0 * o.x.nb1 + n0 * 4;
+                    if (whole) {
+                        const f2u v = load_at<f2u>(xb, t * (uint32_t) o.x.nb1 + 8 * col);
+                        xv[u][0] = v[0], xv[u][1] = v[1];
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < RT; ++j) hv[u][j] = in ? hv[u][j] : 0.f;
+                        for (int c = 0; c < 2; ++c)
+                            xv[u][c] = load_at<float>(xb, t * (uint32_t) o.x.nb1 + 4 * (uint32_t) min((int64_t) (2 * col + c), N - 1 - n0));
+                    }
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) hv[u][j] = load_at<float>(o.h + t0 * R, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
                 }
+                if (t0 + 4 * U > hi) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const bool in = t0 + 4 * u + quad < hi;
+                        xv[u][0] = in ? xv[u][0] : 0.f, xv[u][1] = in ? xv[u][1] : 0.f;
+#pragma unroll
+                        for (int j = 0; j < RT; ++j) hv[u][j] = in ? hv[u][j] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < RT; ++j) acc[c][j] = mfma(xv[u][c], hv[u][j], acc[c][j]);
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < RT; ++j) acc[c][j] = mfma(xv[u][c], hv[u][j], acc[c][j]);
+            turn = (int) ((t0 - hi) / (4 * U));
         }
     }
     const float s = o.scaled ? b.scale[adapter] : 1.f;
@@ -1144,7 +1153,7 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
     const Tile t = find_tile(b, i / slices);
     if (t.tokens == 0) return;
     const int64_t n_lo = (int64_t) (i % slices) * cols;
-    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT == 1 ? ALL : NOTHING> E;
+    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT * sizeof(typename Wt<TYPE>::Elem) <= 8 ? ALL : NOTHING> E;
     E e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
     e.start();
     stage_h<RT>(t, g, 1, b.T, R, 1.f, nullptr, lds.hs, LO_WAVES * 64);
