@@ -230,6 +230,13 @@ def test_many_tokens(hip):
     check_backward(Problem("f32", 260, 520, 32, [3000, 1, 1100], [1, 0, 2]))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_single_tokens_of_high_ranks_over_a_long_axis(hip, kind):
+    announce(f"lora single tokens, high ranks {kind}")
+    check_forward(Problem(kind, 8200, 300, 200, [1, 1, 1, 2], [0, 2, -1, 1]))
+    check_forward(Problem(kind, 6000, 70, 67, [1], [1], pad=1, lead=1, adapter_pad=1))
+
+
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_gradients_of_one_small_adapter_over_many_tokens(hip, accumulate):
     """Few columns and thousands of tokens: the gradients' tokens are split, and the parts joined."""

@@ -904,7 +904,9 @@ __global__ __launch_bounds__(512) L_FOUR_WAVES void k_contract(Rows x, Matrix wm
     if (t.adapter < 0) {
         zero_h(t, R, r0, 16 * RT, out, 512);
     } else if (t.tokens == 1) {
-        if (r0 == 0) contract_one<TYPE, 8>(t, x, wm, R, lo, hi, (float*) lds.stage, sink);
+        wm.p = (const uint8_t*) wm.p + r0 * wm.row * (int64_t) sizeof(typename Wt<TYPE>::Elem);
+        contract_one<TYPE, 8>(t, x, wm, min(R - r0, 16 * RT), lo, hi, (float*) lds.stage,
+                              [&](int, int r, float v) { sink(0, r0 + r, v); });
     } else {
         contract_tile<TYPE, false, 8, RT>(t, x, wm, R, r0, lo, hi, lds.stage, lds.part, sink);
     }
@@ -1279,10 +1281,15 @@ int launch_lora(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hi
                 const trc_hip_tensor& dst, hipStream_t s) {
     const Call c = call_of(q, x.ne[1], s);
     const int64_t K = x.ne[0], M = dst.ne[0], tiles = c.tiles();
-    // One launch, every workgroup of a tile making h for itself, unless that is much to read.
-    const int64_t slices = std::max(std::min(device_cus() / tiles, (M + 255) / 256), (int64_t) 1);
-    const int64_t again = K * (c.R * (c.type == TRC_HIP_TYPE_F32 ? 4 : 2) + LT * 4);
-    if (slices > 1 && again > ((int64_t) 1 << 19)) return forward_apart(c, x, base, h, dst);
+    // One launch, every workgroup of a tile making h for itself, unless two let a workgroup read so much less (of A
+    // and x, split in parts; of base and y, where CUs were idle) that a second launch pays. Measured, in us, one and
+    // two launches: K = M = 4096, 64 tokens of as many adapters, R 16 (108 KB less) 7.8 and 9.6, R 32 (204 KB) 12.9 and
+    // 11.2; 256 tokens of 8 requests, R 8 (245 KB) 11.2 and 8.8; 2048 tokens, F32, R 16 (idle CUs) 29.4 and 26.7.
+    const int64_t cus = device_cus(), slices = std::max(std::min(cus / tiles, (M + 255) / 256), (int64_t) 1);
+    const int64_t tokens = std::min((c.batch.T + c.batch.requests - 1) / c.batch.requests, (int64_t) LT);  // of a tile
+    const int64_t again = K * (c.R * (c.type == TRC_HIP_TYPE_F32 ? 4 : 2) + tokens * 4);
+    const int64_t idle = std::max(cus - tiles * slices, (int64_t) 0);
+    if (again - again / contract_parts(c, K) + LT * 8 * M / slices * idle / cus > 200 << 10) return forward_apart(c, x, base, h, dst);
     const int cols = (int) round_up((M + slices - 1) / slices, LE_COLS);
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
