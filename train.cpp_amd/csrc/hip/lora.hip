@@ -9,7 +9,8 @@
 // Three steps make all six, on v_mfma_f32_16x16x4_f32 (products as exact as float
 // FMAs; adapters in 16 bits are widened). h and y of bfloat16 adapters are made on the bfloat16
 // instructions instead, the other factor in three parts, which is exact as well and takes a fifth of
-// the time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 43 us, 54 with the FP32 instructions.
+// the matrix cores' time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 43 us, 51 with the FP32
+// instructions.
 //   contract  h and g: a wide activation times a matrix of R rows or columns
 //   expand    y and dx: base plus a matrix times h or g
 //   outer     dA and dB: sums over tokens of outer products
@@ -262,12 +263,10 @@ __device__ __forceinline__ f4 mfma_bf16(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// elements of the long axis that a wave takes at a time: more where the weights' registers allow it
-template <bool OUTER, int RT>
-constexpr int chunk_of = OUTER && RT == 1 ? 64 : 32;
+constexpr int L_CHUNK = 32;  // elements of the long axis that a wave takes at a time
 // a wave's piece of LDS for contract_tile: x, then 16 columns of A
-template <class Elem, bool OUTER, int RT>
-constexpr int contract_lds = Rows16<float, chunk_of<OUTER, RT>>::BYTES + (OUTER ? 0 : Rows16<Elem, chunk_of<OUTER, RT>>::BYTES);
+template <class Elem, bool OUTER>
+constexpr int contract_lds = Rows16<float, L_CHUNK>::BYTES + (OUTER ? 0 : Rows16<Elem, L_CHUNK>::BYTES);
 
 // sum_n x[t][n] W(n, r) for the tile's tokens, n in lo .. hi-1 and r in r0 .. r0 + 16 RT - 1,
 // where W(n, r) is w[r][n] (A) or, with OUTER, w[n][r] (B); each sum goes to
@@ -279,13 +278,13 @@ __device__ __forceinline__ void contract_tile(const Tile& t, const Rows& x, cons
                                               int64_t hi, uint8_t* lds, Partial<WAVES, RT>& part, Sink&& sink) {
     typedef Wt<TYPE> W;
     typedef typename W::Elem Elem;
-    constexpr int CN = chunk_of<OUTER, RT>, U = CN / 16;
+    constexpr int CN = L_CHUNK, U = CN / 16;
     constexpr int ES = sizeof(Elem);
     typedef Rows16<float, CN> X;
     typedef Rows16<Elem, CN> A;
     const int lane = (int) threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
-    uint8_t* const xs = lds + wave * contract_lds<Elem, OUTER, RT>;
+    uint8_t* const xs = lds + wave * contract_lds<Elem, OUTER>;
     uint8_t* const ws = xs + X::BYTES;
     const uint8_t* const xb = x.p + (int64_t) t.lo * x.nb1;
     const uint32_t wrow = (uint32_t) wm.row * ES;
@@ -434,7 +433,8 @@ __device__ __forceinline__ void contract_tile(const Tile& t, const Rows& x, cons
     }
 }
 
-// The same of one token and A, without the matrix instructions, which would do 16 tokens' work: each
+// The same of one token and A, without the matrix instructions, which would do 16 tokens' work (64 tokens of as
+// many adapters, F16, K = M = 4096, R 16: 7.9 us, 12.0 by tiles): each
 // lane multiplies eight neighbours of n, a wave takes eight columns r at a time, and as many
 // waves as there are share a column's 512-element chunks. red: [wave][8].
 template <int TYPE, int WAVES, class Sink>
@@ -534,7 +534,8 @@ struct Expand {
     static constexpr int ES = sizeof(Elem);
     // A block is KB of the rank, as loaded. A: [k] is row r0 + 4 quad + k, columns 4 col .. + 3. B: [i] is row
     // 16 i + lane / 4 of the 64, r0 + F (lane % 4) .. + F-1; it is turned through LDS. A lane's F elements are
-    // 16 bytes for F32 and WIDE, else 8: a row's 64 bytes side by side are read at twice the rate of 32.
+    // 16 bytes for F32 and WIDE, else 8: a row's 64 bytes side by side are read at twice the rate of 32 (1001 tokens of 13
+    // requests, K 4096, M 14336, R 64: bfloat16 43 us, 49 without WIDE, F16 55 and 62).
     static constexpr int F = WIDE ? 8 : 4, KB = 4 * F;
     typedef Elem Four __attribute__((ext_vector_type(F)));
     typedef Elem FourU __attribute__((ext_vector_type(F), aligned(ES)));
@@ -590,8 +591,8 @@ struct Expand {
 #pragma unroll
         for (int k = 0; k < 4; ++k) s.w[k] = load_at<FourU>(OUTER ? w + n0 * ES + k * (int64_t) wrow : w + (n0 + 16 * k) * wrow, o);
     }
-    // base is read and the outputs are written once, past the caches (auxiliary bit 1): 4096 x 4096 outputs in 44 us
-    // where plain accesses take 50
+    // base is read and the outputs are written once, past the caches (auxiliary bit 1): 4096 tokens, K = M = 4096,
+    // R 16 in 37 us, with plain accesses 44
     __device__ __forceinline__ void load(Base& s, int64_t n0) const {
         const __amdgpu_buffer_rsrc_t m = span(bp + n0 * 4, based);
 #pragma unroll
@@ -883,7 +884,7 @@ __device__ __forceinline__ void zero_h(const Tile& t, int R, int r0, int rn, flo
 
 template <int TYPE, bool OUTER, int WAVES, int RT>
 union ContractLds {
-    __attribute__((aligned(16))) uint8_t stage[WAVES * contract_lds<typename Wt<TYPE>::Elem, OUTER, RT>];
+    __attribute__((aligned(16))) uint8_t stage[WAVES * contract_lds<typename Wt<TYPE>::Elem, OUTER>];
     Partial<WAVES, RT> part;
 };
 // floats of a tile's h in LDS
@@ -1020,7 +1021,7 @@ struct Outer {
     bool scaled, accumulate;
     int col_blocks, rank_blocks, splits;  // blocks: columns fastest, then ranks, adapters, splits
     int64_t split_len;                    // tokens
-    float* parts;                         // [split][adapter][n][r] where there is more than one split
+    float* parts;                         // [split][adapter], then as in d, where there is more than one split
     int64_t blocks(int adapters) const { return (int64_t) col_blocks * rank_blocks * adapters * splits; }
 };
 
@@ -1107,7 +1108,7 @@ __device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R
             const int64_t at = n0 + 2 * (4 * (l >> 4) + (e & 3)) + c;
             if (r >= R || at >= N) continue;
             if (o.splits > 1) {
-                p[at * R + r] = sum;
+                p[ROWS ? r * N + at : at * R + r] = sum;
             } else {
                 float* const q = d + (ROWS ? r * o.d_row + at : at * o.d_row + r);
                 *q = o.accumulate ? *q + sum * s : sum * s;
@@ -1162,16 +1163,24 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
     e.run(lds.hs);
 }
 
-// Gradients whose tokens were split: the parts in order.
-__global__ __launch_bounds__(256) void k_back_join(Outer o, bool rows, int R, Batch b) {
+// Gradients whose tokens were split: the parts in order. dB's are in `first` blocks, dA's in the others.
+__global__ __launch_bounds__(256) void k_back_join(Outer db, int first, Outer da, int R, Batch b) {
+    const bool rows = (int) blockIdx.x >= first;
+    const Outer o = rows ? da : db;
     const int64_t N = o.x.n, per = N * R, all = per * b.adapters;
-    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = (int64_t) (blockIdx.x - (rows ? first : 0)) * 256 + threadIdx.x;
     if (i >= all) return;
     float sum = 0.f;
-    for (int k = 0; k < o.splits; ++k) sum += o.parts[k * all + i];
-    const int64_t a = i / per, n = i % per / R, r = i % R;
+    for (int k0 = 0; k0 < o.splits; k0 += 8) {  // eight loads under way
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = o.parts[min(k0 + k, o.splits - 1) * all + i];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += k0 + k < o.splits ? x[k] : 0.f;
+    }
+    const int64_t a = i / per, row = i % per / (rows ? N : R), at = i % per % (rows ? N : R);
     if (o.scaled) sum *= b.scale[a];
-    float* const e = o.d + a * o.d_adapter + (rows ? r * o.d_row + n : n * o.d_row + r);
+    float* const e = o.d + a * o.d_adapter + row * o.d_row + at;
     *e = o.accumulate ? *e + sum : sum;
 }
 
@@ -1212,8 +1221,8 @@ int rank_blocks(int R) { return R <= 16 ? 1 : R <= 32 ? 1 : (R + LR - 1) / LR; }
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// The long axis in parts where the tiles leave CUs idle, of 1024 or more each; the
-// parts' sums are kept in the stream's workspace.
+// The long axis in parts where the tiles leave CUs idle, of 1024 or more each (512 or more takes as long); the
+// parts' sums are kept in the stream's workspace. 256 tokens, K 4096, M 14336, R 64: 20 us, in one part 28.
 int64_t contract_parts(const Call& c, int64_t N) {
     const int64_t blocks = c.tiles() * rank_blocks(c.R);
     int64_t parts = std::min(device_cus() / std::max(blocks, (int64_t) 1), N / 1024);
@@ -1242,7 +1251,8 @@ int forward_apart(const Call& c, const trc_hip_tensor& x, const trc_hip_tensor* 
     });
     int rc = check_launch("lora (contract)");
     if (rc != TRC_HIP_OK) return rc;
-    // four workgroups a CU at a time, of at least 256 columns (a step of each wave)
+    // four workgroups a CU at a time, of at least 256 columns (a step of each wave): 1001 tokens, K 4096, M 14336, R 64
+    // 43 us; two a CU 50, eight 43
     const int64_t slices = std::max(std::min(4 * device_cus() / c.tiles(), (M + 255) / 256), (int64_t) 1);
     const int cols = (int) round_up((M + slices - 1) / slices, 256);
     with_type(c.type, [&](auto type) {
@@ -1257,18 +1267,19 @@ int forward_apart(const Call& c, const trc_hip_tensor& x, const trc_hip_tensor* 
     return check_launch("lora (expand)");
 }
 
-// How a gradient's blocks are laid out: tokens split where there are few column blocks and an adapter has
-// 2048 tokens or more for each part (a launch to join them costs what some 1000 tokens take), while the parts fit
-// into `room` floats at `ws`.
+// How a gradient's blocks are laid out: tokens split in three or more, 512 of an adapter's or more each, where that
+// leaves half of the CUs to the other blocks of the launch, and while the parts fit into `room` floats at `ws`. One
+// adapter, bfloat16, R 16, us with and without: K = M = 512, 16384 tokens 44 and 119, 4096 19.3 and 35, 2048 15.8 and 18.9;
+// K = M = 2048, 4096 tokens in two parts 37 and 35.
 Outer outer_of(const Call& c, const trc_hip_tensor& x, const float* h, const trc_hip_tensor& d, bool scaled, bool accumulate,
                float* ws, int64_t room) {
     Outer o{rows_of(x), h, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate, 0, 0, 1, c.batch.T, ws};
     o.col_blocks = (int) ((x.ne[0] + LO_COLS - 1) / LO_COLS);
     o.rank_blocks = rank_blocks(c.R);
     const int64_t blocks = o.blocks(c.batch.adapters), T = c.batch.T;
-    int64_t n = std::min((int64_t) device_cus() / blocks, T / (2048 * c.batch.adapters));
+    int64_t n = std::min((int64_t) device_cus() / (2 * blocks), T / (512 * c.batch.adapters));
     n = std::min(n, room / (x.ne[0] * c.R * c.batch.adapters));
-    if (n > 1) {
+    if (n >= 3) {
         o.split_len = round_up((T + n - 1) / n, 64);
         o.splits = (int) ((T + o.split_len - 1) / o.split_len);
     }
@@ -1323,6 +1334,7 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
     }
     const int64_t nb = ob.blocks(c.batch.adapters), na = oa.blocks(c.batch.adapters);
     const int64_t ng = tiles * rank_blocks(c.R);
+    // two workgroups a CU, of 1024 columns or more: 2048 tokens, K = M = 4096, R 64 51 us; one a CU 54, four of 512 56
     const int64_t slices = std::max(std::min(2 * device_cus() / tiles, (K + 1023) / 1024), (int64_t) 1);
     const int cols = (int) round_up((K + slices - 1) / slices, LE_COLS);
     const int64_t nx = dx != nullptr ? tiles * ((K + cols - 1) / cols) : 0;
@@ -1346,14 +1358,11 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
         });
     });
     rc = check_launch("lora_back (dA, dx)");
-    for (int k = 0; k < 2 && rc == TRC_HIP_OK; ++k) {
-        const Outer& o = k == 0 ? ob : oa;
-        if (o.splits == 1) continue;
-        hipLaunchKernelGGL(k_back_join, dim3((unsigned) ((o.x.n * c.R * c.batch.adapters + 255) / 256)), dim3(256), 0, s, o, k == 1,
-                           c.R, c.batch);
-        rc = check_launch("lora_back (join)");
-    }
-    return rc;
+    if (rc != TRC_HIP_OK) return rc;
+    auto joins = [&](const Outer& o) { return o.splits > 1 ? (o.x.n * c.R * c.batch.adapters + 255) / 256 : 0; };
+    if (joins(ob) + joins(oa) == 0) return TRC_HIP_OK;
+    hipLaunchKernelGGL(k_back_join, dim3((unsigned) (joins(ob) + joins(oa))), dim3(256), 0, s, ob, (int) joins(ob), oa, c.R, c.batch);
+    return check_launch("lora_back (join)");
 }
 
 }  // namespace trc_hip
