@@ -237,6 +237,15 @@ def test_single_tokens_of_high_ranks_over_a_long_axis(hip, kind):
     check_forward(Problem(kind, 6000, 70, 67, [1], [1], pad=1, lead=1, adapter_pad=1))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_gradients_of_few_tokens_over_many_columns(hip, kind):
+    """g's sums are long and its tiles few: they meet in parts."""
+    announce(f"lora gradients, few tokens, many columns {kind}")
+    check_backward(Problem(kind, 300, 2100, 20, [40, 3, 1], [1, 0, -1]), accumulate=True)
+    check_backward(Problem(kind, 70, 1537, 16, [17], [2], pad=1))
+    check_backward(Problem(kind, 1100, 4111, 3, [1, 30], [0, 0]), in_place=True)
+
+
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_gradients_of_one_small_adapter_over_many_tokens(hip, accumulate):
     """Few columns and thousands of tokens: the gradients' tokens are split, and the parts joined."""

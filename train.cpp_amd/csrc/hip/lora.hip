@@ -34,6 +34,7 @@ constexpr int LO_WAVES = 16;       // waves of a workgroup of the backward pass
 constexpr int LE_THREADS = 256;    // k_expand
 constexpr int LE_COLS = 64;        // outputs a wave makes of each token at a time
 constexpr int LO_COLS = 32;        // outer: columns of a workgroup
+constexpr int L_G_PARTS = 4;       // parts of g where it has few tiles, at most
 constexpr int LR = 64;             // rank that is summed at a time, at most
 constexpr int L_MAX_RANK = TRC_HIP_LORA_MAX_RANK;
 
@@ -860,14 +861,13 @@ __device__ __forceinline__ void stage_h(const Tile& t, const float* __restrict__
         float v = 0.f;
         if (tok < t.tokens && r < R && t.adapter >= 0) {
             const float* const p = h + (int64_t) (t.lo + tok) * R + r;
-            int k = 0;
-            for (; k + 4 <= parts; k += 4) {
+            for (int k = 0; k < parts; k += 4) {  // (four loads under way)
                 float x[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = p[(k + j) * T * R];
-                v += ((x[0] + x[1]) + x[2]) + x[3];
+                for (int j = 0; j < 4; ++j) x[j] = p[min(k + j, parts - 1) * T * R];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v += k + j < parts ? x[j] : 0.f;
             }
-            for (; k < parts; ++k) v += p[k * T * R];
         }
         if (h_sum != nullptr && tok < t.tokens && r < R) h_sum[(int64_t) (t.lo + tok) * R + r] = v;
         hs[tok * (Rp + 4) + r] = v * s;
@@ -1016,6 +1016,7 @@ __global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix
 struct Outer {
     Rows x;
     const float* h;
+    int h_parts;  // h is the sum of so many, T R floats apart (dA only, and RT <= 2: L_G_PARTS at most)
     float* d;
     int64_t d_row, d_adapter;
     bool scaled, accumulate;
@@ -1074,6 +1075,28 @@ __device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R
 #pragma unroll
                     for (int j = 0; j < RT; ++j) hv[u][j] = load_at<float>(o.h + t0 * R, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
                 }
+                if constexpr (ROWS && RT <= 2) {
+                    if (o.h_parts > 1) {
+                        float more[L_G_PARTS - 1][U][RT];
+#pragma unroll
+                        for (int k = 1; k < L_G_PARTS; ++k) {
+                            const float* const hk = o.h + (min(k, o.h_parts - 1) * b.T + t0) * R;
+#pragma unroll
+                            for (int u = 0; u < U; ++u) {
+                                const uint32_t t = (uint32_t) min((int64_t) (4 * u + quad), hi - 1 - t0);
+#pragma unroll
+                                for (int j = 0; j < RT; ++j)
+                                    more[k - 1][u][j] = load_at<float>(hk, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
+                            }
+                        }
+#pragma unroll
+                        for (int k = 1; k < L_G_PARTS; ++k)
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int j = 0; j < RT; ++j) hv[u][j] += k < o.h_parts ? more[k - 1][u][j] : 0.f;
+                    }
+                }
                 if (t0 + 4 * U > hi) {
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
@@ -1117,33 +1140,35 @@ __device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R
     }
 }
 
-// The first launch of the backward pass: dB, then g = s B^T dy.
+// The first launch of the backward pass: dB, then g = s B^T dy in parts of the long axis.
 template <int TYPE, int RT>
-__global__ __launch_bounds__(LO_WAVES * 64) void k_back_b(Outer o, int outers, Rows dy, Matrix bm, int R, Batch b,
-                                                           float* __restrict__ g) {
+__global__ __launch_bounds__(LO_WAVES * 64) void k_back_b(Outer o, int outers, Rows dy, Matrix bm, int R, Batch b, int parts,
+                                                           int64_t part_len, float* __restrict__ g) {
     __shared__ ContractLds<TYPE, true, LO_WAVES, RT> lds;
     if ((int) blockIdx.x < outers) {
         outer_block<false, RT>(blockIdx.x, o, R, b, lds.part);
         return;
     }
     const int i = (int) blockIdx.x - outers, rank_blocks = (R + 16 * RT - 1) / (16 * RT);
-    const Tile t = find_tile(b, i / rank_blocks);
+    const Tile t = find_tile(b, i / rank_blocks / parts);
     if (t.tokens == 0) return;
-    const int r0 = i % rank_blocks * (16 * RT);
+    const int r0 = i % rank_blocks * (16 * RT), part = i / rank_blocks % parts;
+    const int64_t lo = part * part_len;
+    g += part * b.T * R;
     if (t.adapter < 0) {
         zero_h(t, R, r0, 16 * RT, g, LO_WAVES * 64);
         return;
     }
     const float s = b.scale[t.adapter];
-    contract_tile<TYPE, true, LO_WAVES, RT>(t, dy, bm, R, r0, 0, dy.n, lds.stage, lds.part,
+    contract_tile<TYPE, true, LO_WAVES, RT>(t, dy, bm, R, r0, lo, min(lo + part_len, dy.n), lds.stage, lds.part,
                                             [&](int tok, int r, float v) { g[(int64_t) (t.lo + tok) * R + r] = v * s; });
 }
 
-// The second: dA, then dx, `cols` columns of it a workgroup.
+// The second: dA, then dx, `cols` columns of it a workgroup; those of the first ones store g if it came in parts.
 template <int TYPE, int RT>
-__global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, const float* __restrict__ g, Matrix am, int R,
-                                                           Batch b, const uint8_t* base, size_t base_nb1, int64_t N,
-                                                           uint8_t* dx, size_t dx_nb1, int cols) {
+__global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, const float* __restrict__ g, int parts, Matrix am,
+                                                           int R, Batch b, const uint8_t* base, size_t base_nb1, int64_t N,
+                                                           uint8_t* dx, size_t dx_nb1, int cols, float* __restrict__ g_sum) {
     __shared__ union {
         Partial<LO_WAVES, RT> part;
         __attribute__((aligned(16))) float hs[h_floats<RT>];
@@ -1159,7 +1184,7 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
     typedef Expand<TYPE, true, LO_WAVES, RT, false, RT * sizeof(typename Wt<TYPE>::Elem) <= 8 ? ALL : NOTHING> E;
     E e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
     e.start();
-    stage_h<RT>(t, g, 1, b.T, R, 1.f, nullptr, lds.hs, LO_WAVES * 64);
+    stage_h<RT>(t, g, parts, b.T, R, 1.f, n_lo == 0 ? g_sum : nullptr, lds.hs, LO_WAVES * 64);
     e.run(lds.hs);
 }
 
@@ -1273,7 +1298,7 @@ int forward_apart(const Call& c, const trc_hip_tensor& x, const trc_hip_tensor* 
 // K = M = 2048, 4096 tokens in two parts 37 and 35.
 Outer outer_of(const Call& c, const trc_hip_tensor& x, const float* h, const trc_hip_tensor& d, bool scaled, bool accumulate,
                float* ws, int64_t room) {
-    Outer o{rows_of(x), h, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate, 0, 0, 1, c.batch.T, ws};
+    Outer o{rows_of(x), h, 1, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate, 0, 0, 1, c.batch.T, ws};
     o.col_blocks = (int) ((x.ne[0] + LO_COLS - 1) / LO_COLS);
     o.rank_blocks = rank_blocks(c.R);
     const int64_t blocks = o.blocks(c.batch.adapters), T = c.batch.T;
@@ -1333,7 +1358,24 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
         oa.parts = (float*) ws + half;
     }
     const int64_t nb = ob.blocks(c.batch.adapters), na = oa.blocks(c.batch.adapters);
-    const int64_t ng = tiles * rank_blocks(c.R);
+    // g in parts of 512 of the long axis or more, where CUs would be idle; they are summed where they are used. 512
+    // tokens, F32, K = M = 4096, R 16: 17 us in three parts, 22 in one.
+    int64_t ng = tiles * rank_blocks(c.R), parts = 1;
+    float* sums = (float*) g.data;
+    if (dx != nullptr && c.R <= 32 && ob.splits == 1 && oa.splits == 1 && nb < device_cus()) {
+        parts = std::min(std::min((device_cus() - nb) / ng, dy.ne[0] / 512), std::min((int64_t) L_G_PARTS, half / (c.batch.T * c.R)));
+        parts = std::max(parts, (int64_t) 1);
+    }
+    if (parts > 1) {
+        uint8_t* ws = nullptr;
+        const int rc = qm_stream_workspace(s, &ws);
+        if (rc != TRC_HIP_OK) return rc;
+        ng *= parts;
+        sums = (float*) ws;
+        oa.h = sums;
+        oa.h_parts = (int) parts;
+    }
+    const int64_t part_len = round_up((dy.ne[0] + parts - 1) / parts, 64);
     // two workgroups a CU, of 1024 columns or more: 2048 tokens, K = M = 4096, R 64 51 us; one a CU 54, four of 512 56
     const int64_t slices = std::max(std::min(2 * device_cus() / tiles, (K + 1023) / 1024), (int64_t) 1);
     const int cols = (int) round_up((K + slices - 1) / slices, LE_COLS);
@@ -1344,7 +1386,7 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
             hipLaunchKernelGGL((k_back_b<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (nb + ng)), dim3(LO_WAVES * 64), 0, s,
-                               ob, (int) nb, rows_of(dy), c.b, c.R, c.batch, (float*) g.data);
+                               ob, (int) nb, rows_of(dy), c.b, c.R, c.batch, (int) parts, part_len, sums);
         });
     });
     int rc = check_launch("lora_back (dB, g)");
@@ -1352,9 +1394,9 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
             hipLaunchKernelGGL((k_back_a<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (na + nx)), dim3(LO_WAVES * 64), 0, s,
-                               oa, (int) na, (const float*) g.data, c.a, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
+                               oa, (int) na, sums, (int) parts, c.a, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
                                base != nullptr ? base->nb[1] : (size_t) 0, K, dx != nullptr ? (uint8_t*) dx->data : nullptr,
-                               dx != nullptr ? dx->nb[1] : (size_t) 0, cols);
+                               dx != nullptr ? dx->nb[1] : (size_t) 0, cols, parts > 1 ? (float*) g.data : nullptr);
         });
     });
     rc = check_launch("lora_back (dA, dx)");
