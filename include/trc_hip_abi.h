@@ -205,8 +205,9 @@ int trc_hip_qmatvec(int type, const void* wq, int64_t K, int64_t M, size_t nb1_w
 /* Frees the x workspace trc_hip_qmatvec keeps for `stream` on the current
  * device, after waiting for the stream's queued work (hipStreamSynchronize).
  * Call it before hipStreamDestroy; a later call on the stream allocates a new
- * workspace. trc_hip_sum_f32 keeps its row sums in the same workspace, and
- * trc_hip_mul_mat_f32 its ticket words past its end.
+ * workspace. trc_hip_sum_f32 keeps its row sums in the same workspace, trc_hip_lora
+ * and trc_hip_lora_back sums in parts, trc_hip_preference_loss its rows' log-probabilities,
+ * and trc_hip_mul_mat_f32 its ticket words past its end.
  * hipStreamPerThread is keyed by the calling thread. Returns TRC_HIP_OK when
  * the stream has no workspace. No counterpart in the reference:
  * it bounds the memory of trc_hip_qmatvec's per-stream workspaces, like the
@@ -320,25 +321,27 @@ typedef struct trc_hip_lora_set {
  *   h[:,t] = A x[:,t]      dst[:,t] = base[:,t] + scale B h[:,t]
  * with A, B and scale of the adapter of token t's request. x is [K, T], base and dst
  * [M, T], h [R, T] contiguous; all F32 with nb[0] = 4 and rows at any 4-byte aligned stride
- * up to 128 MiB (16 MiB for the adapters') that keeps the written ones apart. base may be NULL (zeros) or dst itself. A token without
- * an adapter gets dst = base and h = 0. h is what trc_hip_lora_back needs of this call.
- * Sums are in 32 bits on the F32 matrix instructions, adapters in 16 bits widened, in an order
- * that only the sizes decide: the same from run to run. A batch of few tokens keeps partial sums in the
- * stream's workspace of trc_hip_qmatvec, which the first such call on a stream
- * allocates (make it before capturing that stream in global mode). start and adapter are read
- * on the device; wrong values in them give wrong results, and no access outside the tensors. */
+ * up to 128 MiB (16 MiB for the adapters') that keeps the written ones apart. base may be
+ * NULL (zeros) or dst itself. A token without an adapter gets dst = base and h = 0. h is what
+ * trc_hip_lora_back needs of this call. Adapters in 16 bits are not rounded further, nor is what they
+ * are multiplied by; sums are in 32 bits, in an order that only the sizes decide: the same from
+ * run to run. A batch of few tokens keeps partial sums in the stream's workspace of
+ * trc_hip_qmatvec, which the first such call on a stream allocates (make it before capturing that
+ * stream in global mode). start and adapter are read on the device; wrong values in them give
+ * wrong results, and no access outside the tensors. */
 int trc_hip_lora(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc_hip_tensor* base,
                  const trc_hip_tensor* h, const trc_hip_tensor* dst, void* stream);
 
 /* The gradients of trc_hip_lora for dy [M, T], with x and h of that call:
  *   g[:,t] = scale B^T dy[:,t]      dx[:,t] = base[:,t] + A^T g[:,t]
  *   da = sum over an adapter's tokens of g x^T ([K, R, n]), db = scale sum of dy h^T ([R, M, n])
- * g is [R, T] contiguous and scratch of the caller's. base (the gradient through the shared
+ * g is [R, T] contiguous; it is written whether or not the caller has a use for it. base (the gradient through the shared
  * projection) may be NULL (zeros) or dx itself; dx may be NULL where nothing before the
  * projection is trained (then base has to be NULL too). da and db are F32 whatever the adapters'
  * type, with nb[0] = 4; accumulate != 0 adds to them, as a graph's gradient accumulators
  * want it, 0 overwrites them. An adapter without tokens has gradients of 0. The sums' order is
- * fixed by the sizes and requests: no atomics. */
+ * fixed by the sizes and requests: no atomics. Few tokens over many columns, and many over
+ * few, keep partial sums in the stream's workspace (see trc_hip_lora). */
 int trc_hip_lora_back(const trc_hip_lora_set* set, const trc_hip_tensor* x, const trc_hip_tensor* h,
                       const trc_hip_tensor* dy, const trc_hip_tensor* g, const trc_hip_tensor* base,
                       const trc_hip_tensor* dx, const trc_hip_tensor* da, const trc_hip_tensor* db,
@@ -357,8 +360,8 @@ int trc_hip_lora_back(const trc_hip_lora_set* set, const trc_hip_tensor* x, cons
  * rows not counted), logp [2P], slope [P], loss [1]; lse and slope are what trc_hip_preference_loss_back
  * needs. All vectors contiguous. smoothing is in 0 .. 1. Rows are summed in 32 bits, sequences and
  * pairs in 64, in a fixed order. A logit of -inf is a token that cannot occur; a label of V or
- * more makes the loss NaN. Few rows keep partial sums in the stream's workspace (see
- * trc_hip_lora). */
+ * more makes the loss NaN. At most 2^20 rows (TRC_HIP_E_SHAPE beyond); what is held of them is in
+ * the stream's workspace (see trc_hip_lora). */
 int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* start,
                             const trc_hip_tensor* ref, float beta, float smoothing, const trc_hip_tensor* lse,
                             const trc_hip_tensor* logp, const trc_hip_tensor* slope, const trc_hip_tensor* loss,
@@ -367,7 +370,8 @@ int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* 
 /* The logits' gradient of trc_hip_preference_loss, for dloss [1] F32:
  *   dlogits[v,t] = dloss (+-beta / P) slope_i (1[v = label_t] - exp(logits[v,t] - lse[t]))
  * (+ for the chosen sequence), and 0 for rows that are not counted or in no sequence, whatever
- * their logits hold. dlogits has logits' type and shape and may be logits itself. */
+ * their logits hold. dlogits has logits' type and shape and may be logits itself. At most 2^20
+ * rows here too; no workspace. */
 int trc_hip_preference_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels,
                                  const trc_hip_tensor* start, const trc_hip_tensor* lse,
                                  const trc_hip_tensor* slope, const trc_hip_tensor* dloss, float beta,
