@@ -246,6 +246,13 @@ def test_gradients_of_few_tokens_over_many_columns(hip, kind):
     check_backward(Problem(kind, 1100, 4111, 3, [1, 30], [0, 0]), in_place=True)
 
 
+@pytest.mark.parametrize("use_base,in_place", [(True, False), (False, False), (True, True)])
+def test_many_tokens_without_an_adapter(hip, use_base, in_place):
+    """Their base is passed on, many columns of it to a workgroup."""
+    announce(f"lora many tokens without an adapter, base {use_base}, in place {in_place}")
+    check_forward(Problem("f16", 24, 3300, 8, [4200, 40], [-1, 1], n=2), use_base=use_base, in_place=in_place)
+
+
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_gradients_of_one_small_adapter_over_many_tokens(hip, accumulate):
     """Few columns and thousands of tokens: the gradients' tokens are split, and the parts joined."""

@@ -30,6 +30,7 @@ namespace trc_hip {
 namespace {
 
 constexpr int LT = 16;             // tokens of a tile
+constexpr int L_WAVES = 12;        // waves of a workgroup that makes h and y
 constexpr int LO_WAVES = 16;       // waves of a workgroup of the backward pass
 constexpr int LE_THREADS = 256;    // k_expand
 constexpr int LE_COLS = 64;        // outputs a wave makes of each token at a time
@@ -527,8 +528,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t span(const uint8_t* p, bool me
 // tokens, and base and out are read and written in runs of 256 bytes. Tokens past the tile's are left out
 // by their offsets, so no tile has a branch around its loads and stores: with one, a wait for
 // loads waits for all that is under way.
-constexpr int NOTHING = 0, BASE = 1, ALL = 2;  // what is loaded early
-template <int TYPE, bool OUTER, int WAVES, int RT, bool WIDE = false, int EARLY = NOTHING>
+template <int TYPE, bool OUTER, int WAVES, int RT, bool WIDE = false, bool EARLY = false>
 struct Expand {
     typedef Wt<TYPE> W;
     typedef typename W::Elem Elem;
@@ -557,7 +557,7 @@ struct Expand {
     uint32_t wrow;
     uint8_t* lds;
     int R, lane, col, quad, wave;
-    bool based;
+    bool based, in_place;  // in_place: base is out
     int64_t N, n_lo, steps;  // steps: whole ones
     uint32_t bo[4], oo[4];
     Weights window[D];
@@ -565,7 +565,7 @@ struct Expand {
 
     __device__ __forceinline__ Expand(const Tile& t, const Matrix& wm, int R, const uint8_t* base, size_t base_nb1, int64_t N,
                                       uint8_t* out, size_t out_nb1, int64_t n_lo, int64_t n_hi, uint8_t* all_lds)
-        : t(t), R(R), based(base != nullptr), N(min(n_hi, N)), n_lo(n_lo) {
+        : t(t), R(R), based(base != nullptr), in_place(base == out && base_nb1 == out_nb1), N(min(n_hi, N)), n_lo(n_lo) {
         lane = (int) threadIdx.x & 63;
         col = lane & 15;
         quad = lane >> 4;
@@ -594,13 +594,13 @@ struct Expand {
     }
     // base is read and the outputs are written once, past the caches (auxiliary bit 1): 4096 tokens, K = M = 4096,
     // R 16 in 37 us, with plain accesses 44
-    __device__ __forceinline__ void load(Base& s, int64_t n0) const {
-        const __amdgpu_buffer_rsrc_t m = span(bp + n0 * 4, based);
+    __device__ __forceinline__ void load(Base& s, int64_t n0, bool wanted = true) const {
+        const __amdgpu_buffer_rsrc_t m = span(bp + n0 * 4, based && wanted);
 #pragma unroll
         for (int v = 0; v < 4; ++v) s.b[v] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(m, bo[v], 0, 2));
     }
-    __device__ __forceinline__ void store(const f4 (&sum)[4], int64_t n0) const {
-        const __amdgpu_buffer_rsrc_t m = span(op + n0 * 4, true);
+    __device__ __forceinline__ void store(const f4 (&sum)[4], int64_t n0, bool wanted = true) const {
+        const __amdgpu_buffer_rsrc_t m = span(op + n0 * 4, wanted);
 #pragma unroll
         for (int v = 0; v < 4; ++v) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, sum[v]), m, oo[v], 0, 2);
     }
@@ -661,18 +661,17 @@ struct Expand {
         for (int v = 0; v < 4; ++v) b.b[v] += f4{acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
     }
 
-    // The wave's first columns: weights, then base, since loads arrive in the order they are waited for. All of
-    // it is loaded long before run(), or base alone, or nothing, by the registers that there are.
-    template <bool WEIGHTS, bool FIRST_BASE>
+    // The wave's first columns: weights, then base, since loads arrive in the order they are waited for.
     __device__ __forceinline__ void begin() {
         const int64_t n0 = n_lo + wave * LE_COLS;
 #pragma unroll
-        for (int j = 0; WEIGHTS && j < D; ++j) load(window[j], n0, KB * j);
-        if (FIRST_BASE) load(b, n0);
+        for (int j = 0; j < D; ++j) load(window[j], n0, KB * j);
+        load(b, n0);
     }
     __device__ __forceinline__ bool begins() const { return fours() && wave < steps; }
+    // With EARLY, they are loaded long before run().
     __device__ __forceinline__ void start() {
-        if (EARLY != NOTHING && begins()) begin<EARLY == ALL, true>();
+        if (EARLY && begins()) begin();
     }
     // 64 columns. A block's registers are loaded with the block D further on, of the next columns in the end; then
     // base of those.
@@ -707,7 +706,7 @@ struct Expand {
     __device__ __forceinline__ void whole_steps(const float* hrow) {
         constexpr int64_t S = WAVES * LE_COLS;
         int64_t n0 = n_lo + wave * LE_COLS;
-        begin<EARLY != ALL, EARLY == NOTHING>();
+        if (!EARLY) begin();
         for (int64_t left = (steps - 1 - wave) / WAVES; left > 0; --left, n0 += S) step<true>(hrow, n0, n0 + S);
         step<false>(hrow, n0, 0);
     }
@@ -756,11 +755,29 @@ struct Expand {
                 __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float) b.b[v][k]), to, in ? oo[v] + 4 * k : L_OUTSIDE, 0, 0);
         }
     }
+    // A tile without an adapter: base as it is, four steps under way. 4096 tokens, some of them without an adapter,
+    // K = M = 4096, R 8, F32: 44 us, step by step 45.
+    __device__ __forceinline__ void copy() const {
+        constexpr int64_t S = WAVES * LE_COLS;
+        for (int64_t i = wave; i < steps; i += 4 * WAVES) {
+            Base c[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load(c[u], n_lo + i * LE_COLS + u * S, i + u * WAVES < steps);
+            loads_stay();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) store(c[u].b, n_lo + i * LE_COLS + u * S, i + u * WAVES < steps);
+        }
+    }
     __device__ __forceinline__ void run(const float* hs) {
+        if (t.adapter < 0 && in_place) return;
         const float* const hrow = hs + col * ((R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4) + F * quad;
         int64_t i = wave;
         if (begins()) {
             whole_steps(hrow);
+            i += ((steps - 1 - wave) / WAVES + 1) * WAVES;
+        }
+        if (t.adapter < 0 && i < steps) {
+            copy();
             i += ((steps - 1 - wave) / WAVES + 1) * WAVES;
         }
         for (; n_lo + i * LE_COLS < N; i += WAVES) any_step(hrow, n_lo + i * LE_COLS);
@@ -957,7 +974,7 @@ __global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float*
         e.run(hs);
     } else {
         either_width<TYPE, RT>(R, [&](auto wide) {
-            Expand<TYPE, false, LE_THREADS / 64, RT, decltype(wide)::value, ALL> e(t, wm, R, base, base_nb1, N, out, out_nb1, n_lo,
+            Expand<TYPE, false, LE_THREADS / 64, RT, decltype(wide)::value, true> e(t, wm, R, base, base_nb1, N, out, out_nb1, n_lo,
                                                                                     n_lo + cols, stage);
             e.start();
             stage_h<RT>(t, h, parts, b.T, R, s, sums, hs, LE_THREADS);
@@ -966,16 +983,18 @@ __global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float*
     }
 }
 
-// Both in one launch: a workgroup makes h of its tile for itself, then y of `cols` columns.
-template <int TYPE, int WAVES, int RT>
-__global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix am, Matrix bm, int R, Batch b, const uint8_t* base,
+// Both in one launch: a workgroup makes h of its tile for itself, then y of `cols` columns. 12 waves, one workgroup a
+// CU: 4096 tokens, K = M = 4096, R 16, F32 36 us, with 16 waves 38; with 8, two workgroups a CU, 42 (but 42 instead of
+// 44 where the tiles are just more than the CUs).
+template <int TYPE, int RT>
+__global__ __launch_bounds__(L_WAVES * 64) void k_lora(Rows x, Matrix am, Matrix bm, int R, Batch b, const uint8_t* base,
                                                       size_t base_nb1, int64_t N, uint8_t* out, size_t out_nb1,
                                                       float* __restrict__ h, int cols) {
     const Tile t = find_tile(b, (int) blockIdx.x);
     if (t.tokens == 0) return;
     __shared__ union {
-        ContractLds<TYPE, false, WAVES, RT> contract;
-        __attribute__((aligned(16))) uint8_t expand[WAVES * expand_lds<TYPE, RT>];
+        ContractLds<TYPE, false, L_WAVES, RT> contract;
+        __attribute__((aligned(16))) uint8_t expand[L_WAVES * expand_lds<TYPE, RT>];
     } lds;
     __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
     const int hrow = (R + 16 * RT - 1) / (16 * RT) * (16 * RT) + 4;
@@ -986,24 +1005,23 @@ __global__ __launch_bounds__(WAVES * 64) L_FOUR_WAVES void k_lora(Rows x, Matrix
         if (blockIdx.y == 0) h[(int64_t) (t.lo + tok) * R + r] = v;
     };
     if (t.tokens == 1 && t.adapter >= 0) {
-        ExpandOne<TYPE, WAVES> e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols);
+        ExpandOne<TYPE, L_WAVES> e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols);
         e.start();
-        contract_one<TYPE, WAVES>(t, x, am, R, 0, x.n, (float*) lds.contract.stage, sink);
+        contract_one<TYPE, L_WAVES>(t, x, am, R, 0, x.n, (float*) lds.contract.stage, sink);
         __syncthreads();
         e.run(hs);
         return;
     }
     either_width<TYPE, RT>(R, [&](auto wide) {
-        Expand<TYPE, false, WAVES, RT, decltype(wide)::value, RT == 1 ? BASE : NOTHING> e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols,
+        Expand<TYPE, false, L_WAVES, RT, decltype(wide)::value> e(t, bm, R, base, base_nb1, N, out, out_nb1, n_lo, n_lo + cols,
                                                                          lds.expand);
-        e.start();
         if (t.adapter < 0) {
-            if (blockIdx.y == 0) zero_h(t, R, 0, R, h, WAVES * 64);
+            if (blockIdx.y == 0) zero_h(t, R, 0, R, h, L_WAVES * 64);
         } else {
-            for (int i = (int) threadIdx.x; i < LT * hrow; i += WAVES * 64) hs[i] = 0.f;
+            for (int i = (int) threadIdx.x; i < LT * hrow; i += L_WAVES * 64) hs[i] = 0.f;
             __syncthreads();
             for (int r0 = 0; r0 < R; r0 += 16 * RT) {
-                contract_tile<TYPE, false, WAVES, RT>(t, x, am, R, r0, 0, x.n, lds.contract.stage, lds.contract.part, sink);
+                contract_tile<TYPE, false, L_WAVES, RT>(t, x, am, R, r0, 0, x.n, lds.contract.stage, lds.contract.part, sink);
                 __syncthreads();
             }
         }
@@ -1181,7 +1199,7 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
     const Tile t = find_tile(b, i / slices);
     if (t.tokens == 0) return;
     const int64_t n_lo = (int64_t) (i % slices) * cols;
-    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT * sizeof(typename Wt<TYPE>::Elem) <= 8 ? ALL : NOTHING> E;
+    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT * sizeof(typename Wt<TYPE>::Elem) <= 8> E;
     E e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
     e.start();
     stage_h<RT>(t, g, parts, b.T, R, 1.f, n_lo == 0 ? g_sum : nullptr, lds.hs, LO_WAVES * 64);
@@ -1336,7 +1354,7 @@ int launch_lora(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hi
                                    base != nullptr ? base->nb[1] : (size_t) 0, M, (uint8_t*) dst.data, dst.nb[1], (float*) h.data,
                                    cols);
             };
-            go(k_lora<TYPE, 16, RT>, 1024);
+            go(k_lora<TYPE, RT>, L_WAVES * 64);
         });
     });
     return check_launch("lora");
