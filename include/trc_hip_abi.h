@@ -324,8 +324,8 @@ typedef struct trc_hip_lora_set {
  * up to 128 MiB (16 MiB for the adapters') that keeps the written ones apart. base may be
  * NULL (zeros) or dst itself. A token without an adapter gets dst = base and h = 0. h is what
  * trc_hip_lora_back needs of this call. Adapters in 16 bits are not rounded further, nor is what they
- * are multiplied by; sums are in 32 bits, in an order that only the sizes decide: the same from
- * run to run. A batch of few tokens keeps partial sums in the stream's workspace of
+ * are multiplied by (an infinite bfloat16 one gives infinity or NaN); sums are in 32 bits, in an
+ * order that only the sizes decide: the same from run to run. A batch of few tokens keeps partial sums in the stream's workspace of
  * trc_hip_qmatvec, which the first such call on a stream allocates (make it before capturing that
  * stream in global mode). start and adapter are read on the device; wrong values in them give
  * wrong results, and no access outside the tensors. */

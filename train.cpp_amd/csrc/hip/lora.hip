@@ -8,8 +8,8 @@
 //
 // Three steps make all six, on v_mfma_f32_16x16x4_f32 (products as exact as float
 // FMAs; adapters in 16 bits are widened). h and y of bfloat16 adapters are made on the bfloat16
-// instructions instead, the other factor in three parts, which is exact as well and takes a fifth of
-// the matrix cores' time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 43 us, 51 with the FP32
+// instructions instead, the other factor in three parts, which is exact as well (but an infinite
+// weight's products may be NaN: it meets a part that is 0) and takes a fifth of the matrix cores' time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 43 us, 51 with the FP32
 // instructions.
 //   contract  h and g: a wide activation times a matrix of R rows or columns
 //   expand    y and dx: base plus a matrix times h or g
@@ -1199,7 +1199,9 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
     const Tile t = find_tile(b, i / slices);
     if (t.tokens == 0) return;
     const int64_t n_lo = (int64_t) (i % slices) * cols;
-    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT * sizeof(typename Wt<TYPE>::Elem) <= 8> E;
+    // (512 tokens, K = M = 4096, R 16, F32: 17 us, 18 without the early loads; with more tiles of the rank they cost registers:
+    // R 32 20.0 us, 21.6 with them)
+    typedef Expand<TYPE, true, LO_WAVES, RT, false, RT == 1> E;
     E e(t, am, R, base, base_nb1, N, dx, dx_nb1, n_lo, n_lo + cols, nullptr);
     e.start();
     stage_h<RT>(t, g, parts, b.T, R, 1.f, n_lo == 0 ? g_sum : nullptr, lds.hs, LO_WAVES * 64);
