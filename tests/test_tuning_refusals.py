@@ -88,6 +88,13 @@ def test_lora_refuses(name, value, code):
     refused(forward, {**lora_args(), name: value}, code)
 
 
+def test_lora_refuses_more_tiles_than_one_launch_holds():
+    T = 6000000  # as many requests: a tile each, of 768 threads
+    shapes = dict(a=tensor(1, 1, 1, 1), b=tensor(2, 1, 1, 1), scale=tensor(3, 1), start=tensor(4, T + 1, type_=I32),
+                  adapter=tensor(5, T, type_=I32), x=tensor(6, 1, T), h=tensor(7, 1, T), base=tensor(8, 1, T), dst=tensor(9, 1, T))
+    refused(forward, {**lora_args(), **shapes}, H.E_SHAPE)
+
+
 def test_null_tensors():
     lib, q = H.load(), lora_args()
     s = H.lora_set(q["a"], q["b"], q["scale"], q["start"], q["adapter"])

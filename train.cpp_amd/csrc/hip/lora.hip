@@ -1337,6 +1337,9 @@ int launch_lora(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hi
                 const trc_hip_tensor& dst, hipStream_t s) {
     const Call c = call_of(q, x.ne[1], s);
     const int64_t K = x.ne[0], M = dst.ne[0], tiles = c.tiles();
+    if (tiles * rank_blocks(c.R) > max_groups(L_WAVES * 64)) {
+        return fail(TRC_HIP_E_SHAPE, "trc_hip_lora: %lld tiles of tokens", (long long) tiles);
+    }
     // One launch, every workgroup of a tile making h for itself, unless two let a workgroup read so much less (of A
     // and x, split in parts; of base and y, where CUs were idle) that a second launch pays. Measured, in us, one and
     // two launches: K = M = 4096, 64 tokens of as many adapters, R 16 (108 KB less) 7.8 and 9.6, R 32 (204 KB) 12.9 and
