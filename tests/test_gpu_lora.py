@@ -224,6 +224,16 @@ def test_many_requests(hip):
     check_backward(Problem("f16", 160, 200, 16, lens, ids, n=5))
 
 
+def test_more_requests_than_a_workgroup_has_lanes(hip):
+    announce("lora 1500 requests")
+    rng = np.random.default_rng(3)
+    lens = [int(v) for v in rng.choice([0, 1, 1, 1, 2, 18], 1500)]
+    ids = [int(v) for v in rng.integers(-1, 6, 1500)]
+    check_forward(Problem("f16", 60, 90, 8, lens, ids, n=5))
+    check_backward(Problem("f16", 60, 90, 8, lens, ids, n=5))
+    check_forward(Problem("f32", 2100, 1030, 40, [0] * 300 + [3, 0, 1], [0] * 301 + [1, 2]))
+
+
 def test_many_tokens(hip):
     announce("lora many tokens")
     check_forward(Problem("f32", 260, 520, 32, [3000, 1, 1100], [1, 0, 2]))

@@ -474,7 +474,7 @@ int check_lora_set(const char* who, const trc_hip_lora_set* set, int64_t T) {
     if (!is_float(a.type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of a is not F32, F16 or BF16", who, a.type);
     const int64_t K = a.ne[0], R = a.ne[1], n = a.ne[2], M = b.ne[1], requests = set->adapter.ne[0];
     if (K <= 0 || M <= 0 || T <= 0 || n <= 0 || n > 65535 || requests <= 0 || R <= 0 || R > TRC_HIP_LORA_MAX_RANK ||
-        requests > INT32_MAX || T > INT32_MAX || K > INT32_MAX || M > ((int64_t) 1 << 24) || K > ((int64_t) 1 << 24)) {
+        requests > (1 << 30) || T > INT32_MAX || M > (1 << 24) || K > (1 << 24)) {
         return fail(TRC_HIP_E_SHAPE,
                     "%s: K = %lld, M = %lld, T = %lld, rank %lld (at most %d), %lld adapters, %lld requests", who,
                     (long long) K, (long long) M, (long long) T, (long long) R, TRC_HIP_LORA_MAX_RANK, (long long) n,

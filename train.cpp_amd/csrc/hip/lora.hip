@@ -123,41 +123,71 @@ struct Tile {
     int adapter;  // -1: none
 };
 
-// Tile `index` of the batch, requests in order and each in tiles of LT tokens. Every lane
-// of a wave has to be here; the result is the same in all and held in scalar registers. What start
-// holds is only compared and clamped, so no value of it leads out of the T tokens.
-__device__ __forceinline__ Tile find_tile(const Batch& b, int index) {
-    const int lane = (int) threadIdx.x & 63, T = (int) b.T;
-    for (int q0 = 0; q0 < b.requests; q0 += 64) {
-        const int q = q0 + lane;
-        int lo = 0, hi = 0, id = -1;
+// Requests q0 .. q0+63: a lane's tokens and, in every lane, the tiles of the requests up to its own. What start holds
+// is only compared and clamped, so no value of it leads out of the T tokens (wrong ones may overflow the sums).
+struct Requests {
+    int lo, hi;
+    uint32_t mine, upto;
+    __device__ __forceinline__ Requests(const Batch& b, int q0) : lo(0), hi(0) {
+        const int q = q0 + ((int) threadIdx.x & 63), T = (int) b.T;
         if (q < b.requests) {
             lo = min(max(b.start[q], 0), T);
             hi = min(max(b.start[q + 1], lo), T);
-            id = b.ids[q];
         }
-        const int mine = (int) (((uint32_t) (hi - lo) + LT - 1) / LT);
-        // tiles of the requests up to this lane's (wrong starts may overflow it; what comes of that is clamped below)
-        uint32_t sum = (uint32_t) mine;
-        sum += (uint32_t) from_lane<DPP_SHR + 1>((int) sum);
-        sum += (uint32_t) from_lane<DPP_SHR + 2>((int) sum);
-        sum += (uint32_t) from_lane<DPP_SHR + 4>((int) sum);
-        sum += (uint32_t) from_lane<DPP_SHR + 8>((int) sum);
-        sum += (uint32_t) from_lane<DPP_BCAST15, 0xa>((int) sum);
-        sum += (uint32_t) from_lane<DPP_BCAST31, 0xc>((int) sum);
-        const int upto = (int) sum;
-        const uint64_t in = __ballot(index < upto && mine > 0);
+        mine = ((uint32_t) (hi - lo) + LT - 1) / LT;
+        upto = mine;
+        upto += (uint32_t) from_lane<DPP_SHR + 1>((int) upto);
+        upto += (uint32_t) from_lane<DPP_SHR + 2>((int) upto);
+        upto += (uint32_t) from_lane<DPP_SHR + 4>((int) upto);
+        upto += (uint32_t) from_lane<DPP_SHR + 8>((int) upto);
+        upto += (uint32_t) from_lane<DPP_BCAST15, 0xa>((int) upto);
+        upto += (uint32_t) from_lane<DPP_BCAST31, 0xc>((int) upto);
+    }
+    __device__ __forceinline__ uint32_t all() const { return (uint32_t) __builtin_amdgcn_readlane((int) upto, 63); }
+};
+
+// Tile `index` of the batch, requests in order and each in tiles of LT tokens. The whole workgroup has to be here;
+// the result is the same in all of it and held in scalar registers. Every wave goes through the requests, 64 at a time; of
+// more than 256 each wave counts the tiles of 64 first (1024 requests of a token, K = M = 256: 20 us, 23 otherwise;
+// 4096 113 and 188; but 256 6.5 and 6.0).
+template <int WAVES>
+__device__ __forceinline__ Tile find_tile(const Batch& b, uint32_t index) {
+    const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    int q0 = 0;
+    if (b.requests > 256) {
+        __shared__ uint32_t counts[WAVES];
+        bool found = false;
+        for (int at = 0; at < b.requests && !found; at += 64 * WAVES) {
+            const uint32_t mine = Requests(b, at + 64 * wave).all();  // (by all lanes, so before the branch)
+            if ((threadIdx.x & 63) == 0) counts[wave] = mine;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const uint32_t count = (uint32_t) __builtin_amdgcn_readfirstlane((int) counts[w]);
+                if (found) continue;
+                found = index < count;
+                if (found) q0 = at + 64 * w;
+                else index -= count;
+            }
+            __syncthreads();
+        }
+        if (!found) return {0, 0, -1};
+    }
+    for (; q0 < b.requests; q0 += 64) {
+        const int id = b.ids[min(q0 + ((int) threadIdx.x & 63), b.requests - 1)];
+        const Requests r(b, q0);
+        const uint32_t all = r.all();
+        const uint64_t in = __ballot(index < r.upto && r.mine > 0);
         if (in != 0) {
             const int src = __ffsll((unsigned long long) in) - 1;
-            lo = __builtin_amdgcn_readlane(lo, src);
-            hi = __builtin_amdgcn_readlane(hi, src);
-            id = __builtin_amdgcn_readlane(id, src);
-            const int before = __builtin_amdgcn_readlane((int) ((uint32_t) upto - (uint32_t) mine), src);
-            const int64_t first = lo + ((int64_t) index - before) * LT;
+            const int lo = __builtin_amdgcn_readlane(r.lo, src), hi = __builtin_amdgcn_readlane(r.hi, src);
+            const int a = __builtin_amdgcn_readlane(id, src);
+            const uint32_t before = (uint32_t) __builtin_amdgcn_readlane((int) (r.upto - r.mine), src);
+            const int64_t first = lo + (int64_t) (index - before) * LT;
             if (first < lo || first >= hi) return {0, 0, -1};
-            return {(int) first, min(hi - (int) first, LT), id >= 0 && id < b.adapters ? id : -1};
+            return {(int) first, min(hi - (int) first, LT), a >= 0 && a < b.adapters ? a : -1};
         }
-        index = (int) ((uint32_t) index - (uint32_t) __builtin_amdgcn_readlane(upto, 63));
+        index -= all;
     }
     return {0, 0, -1};
 }
@@ -912,7 +942,7 @@ constexpr int h_floats = LT * ((RT == 4 ? L_MAX_RANK : 16 * RT) + 4);
 template <int TYPE, int RT>
 __global__ __launch_bounds__(512) L_FOUR_WAVES void k_contract(Rows x, Matrix wm, int R, Batch b, int64_t part_len,
                                                                 float* __restrict__ out) {
-    const Tile t = find_tile(b, (int) blockIdx.x);
+    const Tile t = find_tile<8>(b, blockIdx.x);
     if (t.tokens == 0) return;
     __shared__ ContractLds<TYPE, false, 8, RT> lds;
     out += (int64_t) blockIdx.z * b.T * R;
@@ -960,7 +990,7 @@ __global__ __launch_bounds__(LE_THREADS) L_FOUR_WAVES void k_expand(const float*
         tile = id / 8 % tiles;
         slice = id / 8 / tiles * 8 + id % 8;
     }
-    const Tile t = find_tile(b, tile);
+    const Tile t = find_tile<LE_THREADS / 64>(b, tile);
     if (t.tokens == 0) return;
     __shared__ __attribute__((aligned(16))) float hs[h_floats<RT>];
     __shared__ __attribute__((aligned(16))) uint8_t stage[LE_THREADS / 64 * expand_lds<TYPE, RT>];
@@ -990,7 +1020,7 @@ template <int TYPE, int RT>
 __global__ __launch_bounds__(L_WAVES * 64) void k_lora(Rows x, Matrix am, Matrix bm, int R, Batch b, const uint8_t* base,
                                                       size_t base_nb1, int64_t N, uint8_t* out, size_t out_nb1,
                                                       float* __restrict__ h, int cols) {
-    const Tile t = find_tile(b, (int) blockIdx.x);
+    const Tile t = find_tile<L_WAVES>(b, blockIdx.x);
     if (t.tokens == 0) return;
     __shared__ union {
         ContractLds<TYPE, false, L_WAVES, RT> contract;
@@ -1168,7 +1198,7 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_b(Outer o, int outers, R
         return;
     }
     const int i = (int) blockIdx.x - outers, rank_blocks = (R + 16 * RT - 1) / (16 * RT);
-    const Tile t = find_tile(b, i / rank_blocks / parts);
+    const Tile t = find_tile<LO_WAVES>(b, i / rank_blocks / parts);
     if (t.tokens == 0) return;
     const int r0 = i % rank_blocks * (16 * RT), part = i / rank_blocks % parts;
     const int64_t lo = part * part_len;
@@ -1196,7 +1226,7 @@ __global__ __launch_bounds__(LO_WAVES * 64) void k_back_a(Outer o, int outers, c
         return;
     }
     const int i = (int) blockIdx.x - outers, slices = (int) ((N + cols - 1) / cols);
-    const Tile t = find_tile(b, i / slices);
+    const Tile t = find_tile<LO_WAVES>(b, i / slices);
     if (t.tokens == 0) return;
     const int64_t n_lo = (int64_t) (i % slices) * cols;
     // (512 tokens, K = M = 4096, R 16, F32: 17 us, 18 without the early loads; with more tiles of the rank they cost registers:
