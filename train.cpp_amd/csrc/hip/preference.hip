@@ -97,7 +97,8 @@ __device__ __forceinline__ Soft wave_join(Soft a) {
     for (int d = 32; d > 0; d >>= 1) a = join(a, {__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)});
     return a;
 }
-__device__ __forceinline__ float lse_of(Soft a) { return a.m + logf(a.s); }
+// A row's log-sum in 64 bits: the sums over a sequence's rows, and differences of them, would show its rounding.
+__device__ __forceinline__ double lse_of(Soft a) { return (double) a.m + log((double) a.s); }
 
 template <int N>
 __device__ __forceinline__ void take(Soft& a, const float (&x)[N]) {
@@ -174,13 +175,16 @@ __device__ __forceinline__ Soft share(const typename Row<TYPE>::Elem* p, int n) 
 template <int TYPE>
 __global__ __launch_bounds__(PF_THREADS) void k_pref_rows(const uint8_t* __restrict__ logits, size_t nb1, int64_t V,
                                                            const int32_t* __restrict__ labels, int64_t len,
-                                                           float* __restrict__ lse, float* __restrict__ lp,
+                                                           float* __restrict__ lse, double* __restrict__ lp,
                                                            Soft* __restrict__ parts) {
     typedef Row<TYPE> R;
     const int64_t row = blockIdx.x;
     const int32_t y = labels[row];
     if (y < 0) {
-        if (blockIdx.y == 0 && threadIdx.x == 0) lse[row] = lp[row] = 0.f;
+        if (blockIdx.y == 0 && threadIdx.x == 0) {
+            lse[row] = 0.f;
+            lp[row] = 0.0;
+        }
         return;
     }
     const typename R::Elem* const all = (const typename R::Elem*) (logits + row * nb1);
@@ -195,9 +199,9 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_rows(const uint8_t* __restr
 #pragma unroll
     for (int k = 1; k < PF_THREADS / 64; ++k) a = join(a, w[k]);
     if (gridDim.y == 1) {
-        const float e = lse_of(a);
-        lse[row] = e;
-        lp[row] = ly - e;
+        const double e = lse_of(a);
+        lse[row] = (float) e;
+        lp[row] = (double) ly - e;
     } else {
         parts[row * gridDim.y + blockIdx.y] = a;
         if (blockIdx.y == 0) lp[row] = ly;
@@ -211,30 +215,27 @@ __global__ __launch_bounds__(PF_WAVES * 64) void k_pref_pairs(int64_t T, const i
                                                                const int32_t* __restrict__ start, int64_t pairs,
                                                                const float* __restrict__ ref, float beta, float smooth,
                                                                int n_parts, const Soft* __restrict__ parts, float* lse,
-                                                               float* lp, float* __restrict__ logp,
+                                                               double* lp, float* __restrict__ logp,
                                                                float* __restrict__ slope, float* __restrict__ loss) {
     const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6;
     if (n_parts > 1) {
         for (int64_t t0 = wave; t0 < T; t0 += 4 * PF_WAVES) {
-            Soft a[4];
-            int32_t y[4];
-            float l[4];
+            Soft a[4], mine = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // (of rows not counted: whatever is there)
+                a[k] = parts[min(t0 + k * PF_WAVES, T - 1) * n_parts + min(lane, n_parts - 1)];
+            const int64_t t = t0 + lane * PF_WAVES;  // a row to each of four lanes
+            const bool own = lane < 4 && t < T && labels[t] >= 0;
+            const double l = own ? lp[t] : 0.0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int64_t t = min(t0 + k * PF_WAVES, T - 1);
-                y[k] = labels[t];
-                l[k] = lp[t];
-                a[k] = parts[t * n_parts + min(lane, n_parts - 1)];  // (of rows not counted: whatever is there)
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int64_t t = t0 + k * PF_WAVES;
                 const Soft all = wave_join(lane < n_parts ? a[k] : Soft{-INFINITY, 0.f});
-                if (lane == 0 && t < T && y[k] >= 0) {
-                    const float e = lse_of(all);
-                    lse[t] = e;
-                    lp[t] = l[k] - e;
-                }
+                if (lane == k) mine = all;
+            }
+            if (own) {
+                const double e = lse_of(mine);
+                lse[t] = (float) e;
+                lp[t] = l - e;
             }
         }
         __syncthreads();
@@ -247,11 +248,11 @@ __global__ __launch_bounds__(PF_WAVES * 64) void k_pref_pairs(int64_t T, const i
             const int64_t hi = min(max((int64_t) start[s0 + wave + 1], lo), T);
             double sum = 0.0;
             for (int64_t t = lo + lane; t < hi; t += 8 * 64) {
-                float x[8];
+                double x[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = t + 64 * k < hi ? lp[t + 64 * k] : 0.f;
+                for (int k = 0; k < 8; ++k) x[k] = t + 64 * k < hi ? lp[t + 64 * k] : 0.0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum += (double) x[k];
+                for (int k = 0; k < 8; ++k) sum += x[k];
             }
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
@@ -379,9 +380,9 @@ int forward(const trc_hip_tensor& l, const int32_t* labels, const int32_t* start
     uint8_t* ws = nullptr;
     int rc = qm_stream_workspace(s, &ws);
     if (rc != TRC_HIP_OK) return rc;
-    float* const lp = (float*) ws;
-    Soft* const parts = (Soft*) (ws + (size_t) (T + 1) / 2 * 8);
-    if ((size_t) (T + 1) / 2 * 8 + (n > 1 ? (size_t) (n * T) * sizeof(Soft) : 0) > qm_workspace_bytes()) {
+    double* const lp = (double*) ws;
+    Soft* const parts = (Soft*) (ws + (size_t) T * 8);
+    if ((size_t) T * 8 + (n > 1 ? (size_t) (n * T) * sizeof(Soft) : 0) > qm_workspace_bytes()) {
         return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss: %lld rows in %lld parts", (long long) T, (long long) n);
     }
     hipLaunchKernelGGL(k_pref_rows<TYPE>, dim3((unsigned) T, (unsigned) n), dim3(PF_THREADS), 0, s, (const uint8_t*) l.data,
