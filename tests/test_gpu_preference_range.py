@@ -1,0 +1,122 @@
+"""The preference loss's sums over logits of every size that a finite float has: rows most of
+which a finite value masks, and rows whose first tokens lie far from the others.
+
+Tolerance, per row: terms more than 100 below the row's largest are less than 1e-43 of it and do not
+count. Of the others each is an exponential whose argument is at most 100 in magnitude and rounded three
+times at most (the difference, its product, what a join adds), so off by 300 * 2^-24; the sum of V
+positive terms and its float have the (|lse| + log V + 4 + 8 sqrt(V)) 2^-24 of
+test_gpu_preference.py. The gradient's exponentials have the same arguments."""
+import numpy as np
+import pytest
+
+from conftest import announce
+from gpu_util import Dev
+from traincpp_amd import hip as H
+from tuning_util import TYPES, U32, Mat, decode, encode, vec
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+BETA, SMOOTHING, DLOSS = 0.2, 0.1, 0.7
+
+
+def check(kind, logits, labels, T):
+    """`logits` are the counted rows, a sequence each; the batch has T rows, of which the others are in no
+    sequence (they decide in how many parts a row is summed)."""
+    n, V = logits.shape
+    assert n % 2 == 0 and T >= n
+    held, l = encode(logits, kind)
+    whole = np.zeros((T, V), held.dtype)
+    whole[:n] = held
+    y = np.full(T, -1, np.int32)
+    y[:n] = labels
+    with np.errstate(under="ignore"):
+        top = l.max(1)
+        lse = top + np.log(np.exp(l - top[:, None]).sum(1))
+        prob = np.exp(l - lse[:, None])
+    logp = l[np.arange(n), labels] - lse
+    rng = np.random.default_rng(1)
+    ref = (logp + rng.standard_normal(n)).astype(np.float32)
+    z = BETA * ((logp - ref)[0::2] - (logp - ref)[1::2])
+    slope = SMOOTHING / (1 + np.exp(-z)) - (1 - SMOOTHING) / (1 + np.exp(z))
+    loss = np.mean((1 - SMOOTHING) * np.logaddexp(0, -z) + SMOOTHING * np.logaddexp(0, z))
+    unit = DLOSS * BETA / (n // 2)
+    w = unit * np.stack([slope, -slope], 1).reshape(-1, 1)
+    at = labels[:, None] == np.arange(V)
+    d = w * (at - prob)
+
+    t, keep = TYPES[kind], []
+
+    def v(x, type_=H.TYPE_F32):
+        dev, out = vec(x, type_)
+        keep.append(dev)
+        return dev, out
+
+    m, dl = Mat(whole, t), Mat(np.zeros_like(whole), t)
+    keep += [m, dl]
+    _, yt = v(y, H.TYPE_I32)
+    _, start = v(np.arange(n + 1, dtype=np.int32), H.TYPE_I32)
+    _, rt = v(ref)
+    _, dt = v(np.array([DLOSS], np.float32))
+    out = [v(np.full(k, np.nan, np.float32)) for k in (T, n, n // 2, 1)]
+    H.preference_loss(m.t, yt, start, rt, BETA, SMOOTHING, *(o[1] for o in out))
+    H.preference_loss_back(m.t, yt, start, out[0][1], out[2][1], dt, BETA, dl.t)
+    H.sync()
+    glse, glogp, gslope, gloss = (o[0].read() for o in out)
+    gd = dl.read()
+    for k in keep:
+        k.free()
+
+    sums = (300 + np.log(V) + 4 + 8 * np.sqrt(V)) * U32
+    e_lse = sums + np.abs(lse) * U32
+
+    def near(got, want, bound, what):
+        with np.errstate(invalid="ignore"):
+            over = np.abs(got.astype(np.float64) - want) / bound
+        bad = ~(over <= 1)
+        assert not bad.any(), f"{what}: {got[bad][:4]} for {want[bad][:4]} at {np.argwhere(bad)[:4].tolist()}"
+
+    near(glse[:n], lse, e_lse, "lse")
+    assert not glse[n:].any()
+    e_logp = e_lse + 2 * U32 * np.abs(logp)
+    near(glogp, logp, e_logp, "logp")
+    e_z = BETA * (e_logp[0::2] + e_logp[1::2]) + U32
+    near(gslope, slope, e_z / 4 + 4 * U32, "slope")
+    near(gloss, np.array([loss]), e_z.max() + 4 * U32 * abs(loss), "loss")
+    bound = (prob + at) * unit * (np.repeat(e_z, 2)[:, None] / 4 + 8 * U32 + e_lse[:, None] + 400 * U32) \
+        + HALF[kind] * np.abs(d) + (2.0 ** -25 if kind == "f16" else 1e-36)
+    near(decode(gd[:n], kind), d, bound, "dlogits")
+    assert not gd[n:].any()
+
+
+# (V, T) by type: a row in one part, and in several; in each a thread has its first loads and more
+ONE = {"f32": (8191, 40), "f16": (17000, 2048), "bf16": (17000, 2048)}
+PARTS = {"f32": (60000, 40), "f16": (60001, 512), "bf16": (60001, 512)}
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes", [ONE, PARTS], ids=["one", "parts"])
+def test_finite_masks(hip, kind, sizes):
+    """A finite value far below stands for a token that cannot occur, and covers all that a thread reads:
+    all but the last 40 tokens, or runs of a few thousand."""
+    V, T = sizes[kind]
+    announce(f"preference finite masks {kind} V={V} T={T}")
+    rng = np.random.default_rng(4)
+    masks = [-7e3, -1e6, -1e9, -3e10, -1e11, -1e12, -7e12, -1e15, -1e20, -1e25, -3e30, -1e38, -1.7e38, -2.2e38]
+    for runs in (False, True):
+        l = rng.standard_normal((len(masks), V)) * 2
+        out = np.arange(V) < V - 40 if not runs else (np.arange(V) // 3000) % 2 == 0
+        out[V - 1] = False
+        labels = np.where(rng.random(len(masks)) < 0.5, V - 1, np.flatnonzero(~out)[0]).astype(np.int32)
+        check(kind, np.where(out, np.array(masks)[:, None], l), labels, T)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_masked_but_for_their_label(hip, kind):
+    announce(f"preference rows of one token {kind}")
+    for V, T in (ONE[kind], PARTS[kind]):
+        masks = np.array([-1e4, -1e8, -1e10, -1e11, -1e12, -1e13, -1e16, -1e38])
+        l = np.repeat(masks[:, None], V, 1)
+        labels = np.array([0, V - 1, 5, V // 2, V - 3, 17, 4096, 1], np.int32)
+        l[np.arange(len(masks)), labels] = np.linspace(-4, 4, len(masks))
+        check(kind, l, labels, T)

@@ -131,7 +131,9 @@ __device__ __forceinline__ Soft careful_share(const typename Row<TYPE>::Elem* p,
 // The same, with the exponentials taken from the largest of the thread's first elements rather than from a
 // running maximum: their sum is as exact from any point that does not overflow, and an element costs a
 // multiply-add, an exponential and an add.
-// Sums that are not finite, or a start that is not, go the careful way.
+// A sum that is not finite goes the careful way, and so does a largest that is not finite or of 2^23 / LOG2E and more
+// in magnitude: what rounding leaves out of m LOG2E is up to half a unit of its last place, past 2^30 so much that
+// exp2 of it is 0 or an infinity where all that a thread reads is one far mask; under 2^23 it is 1/4 at most.
 template <int TYPE>
 __device__ __forceinline__ Soft share(const typename Row<TYPE>::Elem* p, int n) {
     typedef Row<TYPE> R;
@@ -164,7 +166,7 @@ __device__ __forceinline__ Soft share(const typename Row<TYPE>::Elem* p, int n) 
         if (i + u * STEP < whole) R::load(p + i + u * STEP, x + u * VEC);
     if (whole + (int) threadIdx.x < n) x[U * VEC - 1] = R::get(p[whole + threadIdx.x]);
     add();
-    if (!(s <= FLT_MAX) || !(fabsf(unit) <= FLT_MAX)) return careful_share<TYPE>(p, n);
+    if (!(s <= FLT_MAX) || !(fabsf(unit) < 0x1p23f)) return careful_share<TYPE>(p, n);
     // what rounding m LOG2E left out, taken back
     return {m, s * exp_of(fmaf(m, LOG2E, -unit) * -(1.f / LOG2E))};
 }
