@@ -120,3 +120,43 @@ def test_rows_masked_but_for_their_label(hip, kind):
         labels = np.array([0, V - 1, 5, V // 2, V - 3, 17, 4096, 1], np.int32)
         l[np.arange(len(masks)), labels] = np.linspace(-4, 4, len(masks))
         check(kind, l, labels, T)
+
+
+FAR = [60, 70] + list(range(76, 91)) + [100]
+FIRST = {"f32": 4096, "f16": 8192, "bf16": 8192}  # what a workgroup's first loads hold
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes", [ONE, PARTS], ids=["one", "parts"])
+@pytest.mark.parametrize("part", ["first", "half", "spread"])
+def test_first_tokens_far_below(hip, kind, sizes, part):
+    """A run of tokens at the row's start (what the first loads hold, or every second thread's share of it,
+    or such a run in every part), 60 to 100 below the others."""
+    V, T = sizes[kind]
+    announce(f"preference first tokens below {kind} V={V} T={T} {part}")
+    rng = np.random.default_rng(6)
+    l = rng.standard_normal((len(FAR), V))
+    i, lane = np.arange(V), 4 if kind == "f32" else 8
+    out = i < FIRST[kind] if part != "spread" else i % (FIRST[kind] * 3 // 2) < FIRST[kind]
+    if part == "half":
+        out &= (i // lane) % 2 == 0
+    l -= out * np.array(FAR, np.float64)[:, None]
+    labels = np.where(rng.random(len(FAR)) < 0.7, V - 1, 3).astype(np.int32)
+    check(kind, l, labels, T)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes", [ONE, PARTS], ids=["one", "parts"])
+def test_few_late_tokens_far_above(hip, kind, sizes):
+    """Rows of zeros with a few tokens, behind what the first loads hold, 40 to 89 above."""
+    V, T = sizes[kind]
+    announce(f"preference late tokens above {kind} V={V} T={T}")
+    rng = np.random.default_rng(7)
+    tops = [40, 60, 80, 84, 86, 87, 87.5, 88, 88.3, 88.6, 88.7, 89]
+    l = np.zeros((len(tops) * 2, V))
+    for r in range(len(l)):
+        at = FIRST[kind] + rng.choice(V - FIRST[kind], 8 if r % 2 else 64, replace=False)
+        l[r, at] = tops[r // 2]
+    labels = l.argmax(1).astype(np.int32)
+    labels[::5] = 0
+    check(kind, l, labels, T)

@@ -11,8 +11,6 @@
 // sum), one workgroup over the pairs, and the gradient (each row read and written once).
 // All three are bound by memory; the gradient cannot begin before the pair's last row is
 // summed, so the logits are read twice.
-#include <cfloat>
-
 #include "common.h"
 
 namespace trc_hip {
@@ -129,11 +127,13 @@ __device__ __forceinline__ Soft careful_share(const typename Row<TYPE>::Elem* p,
 }
 
 // The same, with the exponentials taken from the largest of the thread's first elements rather than from a
-// running maximum: their sum is as exact from any point that does not overflow, and an element costs a
+// running maximum: their sum is as exact from any point near enough, and an element costs a
 // multiply-add, an exponential and an add.
-// A sum that is not finite goes the careful way, and so does a largest that is not finite or of 2^23 / LOG2E and more
-// in magnitude: what rounding leaves out of m LOG2E is up to half a unit of its last place, past 2^30 so much that
-// exp2 of it is 0 or an infinity where all that a thread reads is one far mask; under 2^23 it is 1/4 at most.
+// The careful way go a sum over 2^64 (or not finite) and a largest of 2^23 / LOG2E or more in magnitude (or not finite):
+// - Joins add up to 2^14 sums (256 threads, 64 parts) and drop one whose maximum lies 126 bits under another's: 2^78 is
+//   finite, and 2^64 2^-126 nothing beside a sum that holds its maximum. A sum up to the largest float would be neither.
+// - What rounding leaves out of m LOG2E is up to half a unit of its last place, past 2^30 so much that exp2 of it
+//   is 0 or an infinity where all that a thread reads is one far mask. Under 2^23 it is 1/4 at most.
 template <int TYPE>
 __device__ __forceinline__ Soft share(const typename Row<TYPE>::Elem* p, int n) {
     typedef Row<TYPE> R;
@@ -166,7 +166,7 @@ __device__ __forceinline__ Soft share(const typename Row<TYPE>::Elem* p, int n) 
         if (i + u * STEP < whole) R::load(p + i + u * STEP, x + u * VEC);
     if (whole + (int) threadIdx.x < n) x[U * VEC - 1] = R::get(p[whole + threadIdx.x]);
     add();
-    if (!(s <= FLT_MAX) || !(fabsf(unit) < 0x1p23f)) return careful_share<TYPE>(p, n);
+    if (!(s <= 0x1p64f) || !(fabsf(unit) < 0x1p23f)) return careful_share<TYPE>(p, n);
     // what rounding m LOG2E left out, taken back
     return {m, s * exp_of(fmaf(m, LOG2E, -unit) * -(1.f / LOG2E))};
 }
