@@ -260,7 +260,8 @@ struct Rows16 {
 };
 
 // N floats, each the sum of three in bfloat16 that hold 8 bits of it each (down to 2^-126; an infinity or NaN
-// is in the first alone), so that products with numbers in bfloat16 are exact.
+// is in the first alone), so that products with numbers in bfloat16 are exact. A NaN is made quiet first: a signalling
+// one may have its payload in the lower half alone, and its upper half is an infinity's.
 template <int N>
 struct Thirds {
     typedef uint32_t Bits __attribute__((ext_vector_type(N / 2)));
@@ -269,9 +270,10 @@ struct Thirds {
         uint32_t a[N], b[N], c[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            a[k] = __builtin_bit_cast(uint32_t, x[k]);
-            const bool finite = __builtin_fabsf(x[k]) < __builtin_inff();
-            const float rest = finite ? x[k] - __builtin_bit_cast(float, a[k] & 0xffff0000u) : 0.f;
+            const float quiet = __builtin_canonicalizef(x[k]);
+            a[k] = __builtin_bit_cast(uint32_t, quiet);
+            const bool finite = __builtin_fabsf(quiet) < __builtin_inff();
+            const float rest = finite ? quiet - __builtin_bit_cast(float, a[k] & 0xffff0000u) : 0.f;
             b[k] = __builtin_bit_cast(uint32_t, rest);
             c[k] = __builtin_bit_cast(uint32_t, rest - __builtin_bit_cast(float, b[k] & 0xffff0000u));
         }
