@@ -199,6 +199,15 @@ def test_adamw_refuses(bits, change, code):
     assert e.value.code == code, str(e.value)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [(1 << 24) * 2048, (1 << 62), (1 << 63) - 2048, (1 << 63) - 1])
+def test_adamw_refuses_tensors_up_to_the_largest_size(bits, n):
+    """... the last of which overflow 64 bits if they are rounded up before they are divided."""
+    with pytest.raises(H.HipError) as e:
+        plan(bits, n=n)
+    assert e.value.code == H.E_SHAPE and "elements in one plan" in str(e.value), str(e.value)
+
+
 @pytest.mark.parametrize("entry,call", [
     ("trc_hip_lora", "R.forward(R.lora_args())"), ("trc_hip_lora_back", "R.backward(R.lora_args())"),
     ("trc_hip_preference_loss", "R.loss(R.loss_args())"), ("trc_hip_preference_loss_back", "R.loss_back(R.loss_args())"),

@@ -399,7 +399,7 @@ int adamw_create(const trc_hip_adamw_tensor* ts, int64_t count, int bits, void**
                         (long long) i);
         }
         readable = readable && t.m_out != nullptr && t.v_out != nullptr;
-        const int64_t c = (t.n + AW_CHUNK - 1) / AW_CHUNK;
+        const int64_t c = (t.n - 1) / AW_CHUNK + 1;
         if (chunks + c > max_groups(AW_THREADS)) {
             return fail(TRC_HIP_E_SHAPE, "%s: over %lld elements in one plan", who,
                         (long long) (max_groups(AW_THREADS) * AW_CHUNK));
