@@ -1,6 +1,6 @@
 """Builds the C++ test programs against libtraincpp_hip.so (the backend under test):
 tests/cpp/bin/test_hip_backend, the drop-in test, which is checked by oracle/liboracle.so,
-and tests/cpp/bin/test_tuning."""
+tests/cpp/bin/test_tuning and tests/cpp/bin/test_tuning_types."""
 import subprocess
 import sys
 from pathlib import Path
@@ -27,6 +27,7 @@ def build(name: str, oracle: bool) -> None:
 def main() -> None:
     build("test_hip_backend", oracle=True)
     build("test_tuning", oracle=False)
+    build("test_tuning_types", oracle=False)
 
 
 if __name__ == "__main__":
