@@ -1372,15 +1372,21 @@ int launch_lora(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hi
     if (tiles * rank_blocks(c.R) > max_groups(L_WAVES * 64)) {
         return fail(TRC_HIP_E_SHAPE, "trc_hip_lora: %lld tiles of tokens", (long long) tiles);
     }
-    // One launch, every workgroup of a tile making h for itself, unless two let a workgroup read so much less (of A
-    // and x, split in parts; of base and y, where CUs were idle) that a second launch pays. Measured, in us, one and
-    // two launches: K = M = 4096, 64 tokens of as many adapters, R 16 (108 KB less) 7.8 and 9.6, R 32 (204 KB) 12.9 and
-    // 11.2; 256 tokens of 8 requests, R 8 (245 KB) 11.2 and 8.8; 2048 tokens, F32, R 16 (idle CUs) 29.4 and 26.7.
+    // One launch, every workgroup of a tile making h for itself, unless two let a workgroup read so much less that a
+    // second launch pays: of A and x, which two take in parts, over 300 KB where tiles are single tokens and over 120 KB
+    // else (x counts as the 16 rows that a tile loads); of base and y, where CUs were idle, over 200 KB. Measured, in
+    // us, one and two launches, K = M = 4096 but where said:
+    //   64 single tokens, F16, R 24 (156 KB) 10.5 and 11.6, R 32 (204) 11.5 and 12.4, R 48 (300) 16.0 and 15.7
+    //   128 tokens of 8 requests, F16, K 2048, R 16 (96 KB) 8.0 and 8.7, R 32 (128) 11.1 and 10.9; K 4096, R 8 (240) 11.5
+    //   and 8.7; 64 of 32, R 8 (240) 11.1 and 9.5; but 512 of 2, M 2048, K 2048, R 16 (96) 10.4 and 9.3
+    //   one adapter, F32, R 16, idle CUs: 3300 tokens (96 KB) 36.3 and 39.7, 2700 (172) 31.9 and 32.1, 2300 (222) 31.2
+    //   and 29.4; but bfloat16, M 11008, 3300 tokens (258) 78 and 85
     const int64_t cus = device_cus(), slices = std::max(std::min(cus / tiles, (M + 255) / 256), (int64_t) 1);
-    const int64_t tokens = std::min((c.batch.T + c.batch.requests - 1) / c.batch.requests, (int64_t) LT);  // of a tile
-    const int64_t again = K * (c.R * (c.type == TRC_HIP_TYPE_F32 ? 4 : 2) + tokens * 4);
-    const int64_t idle = std::max(cus - tiles * slices, (int64_t) 0);
-    if (again - again / contract_parts(c, K) + LT * 8 * M / slices * idle / cus > 200 << 10) return forward_apart(c, x, base, h, dst);
+    const bool single = c.batch.T <= c.batch.requests;
+    const int64_t reads = K * (c.R * (c.type == TRC_HIP_TYPE_F32 ? 4 : 2) + (single ? 1 : LT) * 4);
+    const int64_t saved = reads - reads / contract_parts(c, K);
+    const int64_t idle = LT * 8 * M / slices * std::max(cus - tiles * slices, (int64_t) 0) / cus;
+    if ((single ? 2 : 5) * saved + 3 * idle > 600 << 10) return forward_apart(c, x, base, h, dst);
     const int cols = (int) round_up((M + slices - 1) / slices, LE_COLS);
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
