@@ -12,11 +12,13 @@
 // 8 bits: a block of 256 elements shares two float scales, its largest |m| and its
 // largest u = sqrt(v). The codes are square roots of the ratios to them,
 //   m = sm sign(c) (c / 127)^2, c in -127..127      u = su (c / 255)^2, c in 0..255
-// which gives small values finer steps (relative error 1 / c at most: 1 / 254 of the
-// largest value, 6 % at 1/254 of it), as block-wise non-linear codes do (Dettmers et al.,
-// "8-bit Optimizers via Block-wise Quantization", 2021). u is held rather than v
-// because it is what divides, and has twice the range: c is never 0 where u > 0, so a
-// small v never turns into 0 / eps. A block whose largest value is below the smallest
+// which gives small values finer steps, as block-wise non-linear codes do (Dettmers et al.,
+// "8-bit Optimizers via Block-wise Quantization", 2021). A value is off by half a step of its code
+// at most, (c + 1/4) / 127^2 of the block's largest |m| and (c + 1/4) / 255^2 of its largest u: of
+// values near the largest 1/127 and 1/255, of values near 1/254 of it up to 14 and 7 %. Values under the
+// first step (1/127^2 and 1/255^2 of the largest) have no relative bound: an m under a quarter of it is held as 0, a
+// u above 0 as the first step at least. u is held rather than v because it is what divides,
+// and has twice the range: c is never 0 where u > 0, so a small v never turns into 0 / eps. A block whose largest value is below the smallest
 // normal float is held as zeros; a block that meets a value that is not finite is not
 // finite from then on.
 #include <cmath>
@@ -65,8 +67,8 @@ struct Plan {
     uint32_t* owner;    // device: the tensor of each chunk
 };
 
-// A step reads and writes everything once, past the caches: the 243 million elements of a 4096-wide layer take
-// 1200 us, and 1270 with plain accesses.
+// A step reads and writes everything once, past the caches (but for k_adamw's gradients, which are read by plain loads):
+// the 243 million elements of a 4096-wide layer take 1200 us, and 1270 with plain accesses throughout.
 __device__ __forceinline__ f4u once(const f4u* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ h4u once(const h4u* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ uint32_t once(const u32u* p) { return __builtin_nontemporal_load(p); }

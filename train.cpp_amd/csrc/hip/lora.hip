@@ -7,10 +7,12 @@
 //   dA_a = sum_t g_t x_t^T      dB_a = s_a sum_t dy_t h_t^T
 //
 // Three steps make all six, on v_mfma_f32_16x16x4_f32 (products as exact as float
-// FMAs; adapters in 16 bits are widened). h and y of bfloat16 adapters are made on the bfloat16
-// instructions instead, the other factor in three parts, which is exact as well (but an infinite
-// weight's products may be NaN: it meets a part that is 0) and takes a fifth of the matrix cores' time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 43 us, 51 with the FP32
-// instructions.
+// FMAs; adapters in 16 bits are widened). h and y of bfloat16 adapters are made on the
+// bfloat16 instructions instead, the other factor in three parts, which is exact as well (but an
+// infinite weight's products may be NaN: it meets a part that is 0) and takes a fifth of the
+// matrix cores' time: 1001 tokens of 13 requests, K 4096, M 14336, R 64 in 42 us, 51 with the FP32
+// instructions. (y of ranks that are not whole fours, and of the last columns, stays on
+// those: see Expand::singly.)
 //   contract  h and g: a wide activation times a matrix of R rows or columns
 //   expand    y and dx: base plus a matrix times h or g
 //   outer     dA and dB: sums over tokens of outer products
@@ -622,7 +624,8 @@ struct Expand {
         const uint32_t r = (uint32_t) min(r0 + F * (OUTER ? quad : lane & 3), R - F);
         const uint32_t o = OUTER ? r * wrow + 4 * col * ES : (lane >> 2) * wrow + r * ES;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s.w[k] = load_at<FourU>(OUTER ? w + n0 * ES + k * (int64_t) wrow : w + (n0 + 16 * k) * wrow, o);
+        for (int k = 0; k < 4; ++k)
+            s.w[k] = load_at<FourU>(OUTER ? w + n0 * ES + k * (int64_t) wrow : w + (n0 + 16 * k) * wrow, o);
     }
     // base is read and the outputs are written once, past the caches (auxiliary bit 1): 4096 tokens, K = M = 4096,
     // R 16 in 37 us, with plain accesses 44
@@ -775,16 +778,20 @@ struct Expand {
         for (int k = 0; k < 4; ++k) {
             const bool in = n0 + 4 * col + k < N;
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                b.b[v][k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(from, in ? bo[v] + 4 * k : L_OUTSIDE, 0, 0));
+            for (int v = 0; v < 4; ++v) {
+                const uint32_t at = in ? bo[v] + 4 * k : L_OUTSIDE;
+                b.b[v][k] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0));
+            }
         }
         add(b, acc);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const bool in = n0 + 4 * col + k < N;
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float) b.b[v][k]), to, in ? oo[v] + 4 * k : L_OUTSIDE, 0, 0);
+            for (int v = 0; v < 4; ++v) {
+                const uint32_t at = in ? oo[v] + 4 * k : L_OUTSIDE;
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float) b.b[v][k]), to, at, 0, 0);
+            }
         }
     }
     // A tile without an adapter: base as it is, four steps under way. 4096 tokens, some of them without an adapter,
@@ -1119,11 +1126,14 @@ __device__ __forceinline__ void outer_block(int64_t block, const Outer& o, int R
                         xv[u][0] = v[0], xv[u][1] = v[1];
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            xv[u][c] = load_at<float>(xb, t * (uint32_t) o.x.nb1 + 4 * (uint32_t) min((int64_t) (2 * col + c), N - 1 - n0));
+                        for (int c = 0; c < 2; ++c) {
+                            const uint32_t at = (uint32_t) min((int64_t) (2 * col + c), N - 1 - n0);
+                            xv[u][c] = load_at<float>(xb, t * (uint32_t) o.x.nb1 + 4 * at);
+                        }
                     }
 #pragma unroll
-                    for (int j = 0; j < RT; ++j) hv[u][j] = load_at<float>(o.h + t0 * R, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
+                    for (int j = 0; j < RT; ++j)
+                        hv[u][j] = load_at<float>(o.h + t0 * R, 4 * (t * R + (uint32_t) min(r0 + 16 * j + col, R - 1)));
                 }
                 if constexpr (ROWS && RT <= 2) {
                     if (o.h_parts > 1) {
@@ -1350,7 +1360,8 @@ int forward_apart(const Call& c, const trc_hip_tensor& x, const trc_hip_tensor* 
 // K = M = 2048, 4096 tokens in two parts 37 and 35.
 Outer outer_of(const Call& c, const trc_hip_tensor& x, const float* h, const trc_hip_tensor& d, bool scaled, bool accumulate,
                float* ws, int64_t room) {
-    Outer o{rows_of(x), h, 1, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate, 0, 0, 1, c.batch.T, ws};
+    Outer o{rows_of(x), h, 1, (float*) d.data, (int64_t) (d.nb[1] / 4), (int64_t) (d.nb[2] / 4), scaled, accumulate,
+            0, 0, 1, c.batch.T, ws};
     o.col_blocks = (int) ((x.ne[0] + LO_COLS - 1) / LO_COLS);
     o.rank_blocks = rank_blocks(c.R);
     const int64_t blocks = o.blocks(c.batch.adapters), T = c.batch.T;
@@ -1391,13 +1402,11 @@ int launch_lora(const trc_hip_lora_set& q, const trc_hip_tensor& x, const trc_hi
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
             constexpr int TYPE = decltype(type)::value, RT = decltype(rt)::value;
-            auto go = [&](auto kernel, int threads) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned) tiles, (unsigned) ((M + cols - 1) / cols)), dim3((unsigned) threads), 0, s,
-                                   rows_of(x), c.a, c.b, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
-                                   base != nullptr ? base->nb[1] : (size_t) 0, M, (uint8_t*) dst.data, dst.nb[1], (float*) h.data,
-                                   cols);
-            };
-            go(k_lora<TYPE, RT>, L_WAVES * 64);
+            hipLaunchKernelGGL((k_lora<TYPE, RT>), dim3((unsigned) tiles, (unsigned) ((M + cols - 1) / cols)),
+                               dim3(L_WAVES * 64), 0, s, rows_of(x), c.a, c.b, c.R, c.batch,
+                               base != nullptr ? (const uint8_t*) base->data : nullptr,
+                               base != nullptr ? base->nb[1] : (size_t) 0, M, (uint8_t*) dst.data, dst.nb[1],
+                               (float*) h.data, cols);
         });
     });
     return check_launch("lora");
@@ -1424,7 +1433,8 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
     int64_t ng = tiles * rank_blocks(c.R), parts = 1;
     float* sums = (float*) g.data;
     if (dx != nullptr && c.R <= 32 && ob.splits == 1 && oa.splits == 1 && nb < device_cus()) {
-        parts = std::min(std::min((device_cus() - nb) / ng, dy.ne[0] / 512), std::min((int64_t) L_G_PARTS, half / (c.batch.T * c.R)));
+        parts = std::min((device_cus() - nb) / ng, dy.ne[0] / 512);
+        parts = std::min(parts, std::min((int64_t) L_G_PARTS, half / (c.batch.T * c.R)));
         parts = std::max(parts, (int64_t) 1);
     }
     if (parts > 1) {
@@ -1437,7 +1447,8 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
         oa.h_parts = (int) parts;
     }
     const int64_t part_len = round_up((dy.ne[0] + parts - 1) / parts, 64);
-    // two workgroups a CU, of 1024 columns or more: 2048 tokens, K = M = 4096, R 64 51 us; one a CU 54, four of 512 56
+    // two workgroups a CU, of 1024 columns or more: 2048 tokens of three requests (one without an adapter), bfloat16,
+    // K = M = 4096, R 64 51 us; one a CU 54, four of 512 56
     const int64_t slices = std::max(std::min(2 * device_cus() / tiles, (K + 1023) / 1024), (int64_t) 1);
     const int cols = (int) round_up((K + slices - 1) / slices, LE_COLS);
     const int64_t nx = dx != nullptr ? tiles * ((K + cols - 1) / cols) : 0;
@@ -1446,16 +1457,18 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
     }
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
-            hipLaunchKernelGGL((k_back_b<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (nb + ng)), dim3(LO_WAVES * 64), 0, s,
-                               ob, (int) nb, rows_of(dy), c.b, c.R, c.batch, (int) parts, part_len, sums);
+            hipLaunchKernelGGL((k_back_b<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (nb + ng)),
+                               dim3(LO_WAVES * 64), 0, s, ob, (int) nb, rows_of(dy), c.b, c.R, c.batch, (int) parts, part_len,
+                               sums);
         });
     });
     int rc = check_launch("lora_back (dB, g)");
     if (rc != TRC_HIP_OK) return rc;
     with_type(c.type, [&](auto type) {
         with_rank(c.R, [&](auto rt) {
-            hipLaunchKernelGGL((k_back_a<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (na + nx)), dim3(LO_WAVES * 64), 0, s,
-                               oa, (int) na, sums, (int) parts, c.a, c.R, c.batch, base != nullptr ? (const uint8_t*) base->data : nullptr,
+            hipLaunchKernelGGL((k_back_a<decltype(type)::value, decltype(rt)::value>), dim3((unsigned) (na + nx)),
+                               dim3(LO_WAVES * 64), 0, s, oa, (int) na, sums, (int) parts, c.a, c.R, c.batch,
+                               base != nullptr ? (const uint8_t*) base->data : nullptr,
                                base != nullptr ? base->nb[1] : (size_t) 0, K, dx != nullptr ? (uint8_t*) dx->data : nullptr,
                                dx != nullptr ? dx->nb[1] : (size_t) 0, cols, parts > 1 ? (float*) g.data : nullptr);
         });
@@ -1464,7 +1477,8 @@ int launch_lora_back(const trc_hip_lora_set& q, const trc_hip_tensor& x, const t
     if (rc != TRC_HIP_OK) return rc;
     auto joins = [&](const Outer& o) { return o.splits > 1 ? (o.x.n * c.R * c.batch.adapters + 255) / 256 : 0; };
     if (joins(ob) + joins(oa) == 0) return TRC_HIP_OK;
-    hipLaunchKernelGGL(k_back_join, dim3((unsigned) (joins(ob) + joins(oa))), dim3(256), 0, s, ob, (int) joins(ob), oa, c.R, c.batch);
+    hipLaunchKernelGGL(k_back_join, dim3((unsigned) (joins(ob) + joins(oa))), dim3(256), 0, s, ob, (int) joins(ob), oa, c.R,
+                       c.batch);
     return check_launch("lora_back (join)");
 }
 

@@ -266,7 +266,9 @@ __global__ __launch_bounds__(PF_WAVES * 64) void k_pref_pairs(int64_t T, const i
         __syncthreads();
         const int64_t i = s0 / 2 + threadIdx.x;
         if (threadIdx.x < PF_WAVES / 2 && i < pairs) {
-            const double z = (double) beta * ((L[2 * threadIdx.x] - (double) ref[2 * i]) - (L[2 * threadIdx.x + 1] - (double) ref[2 * i + 1]));
+            const double chosen = L[2 * threadIdx.x] - (double) ref[2 * i];
+            const double rejected = L[2 * threadIdx.x + 1] - (double) ref[2 * i + 1];
+            const double z = (double) beta * (chosen - rejected);
             const double e = (double) smooth, small = exp(-fabs(z)), tail = log1p(small);
             const double up = fmax(-z, 0.0) + tail, down = fmax(z, 0.0) + tail;  // -log sigma(z), -log sigma(-z)
             // (a weight of 0 takes no part of an infinite term)
@@ -412,7 +414,8 @@ int launch_preference_loss(const trc_hip_tensor& l, const int32_t* labels, const
                            const float* ref, float beta, float smooth, float* lse, float* logp, float* slope, float* loss,
                            hipStream_t s) {
     if (l.ne[1] > PF_MAX_ROWS) {
-        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss: %lld rows (at most %lld)", (long long) l.ne[1], (long long) PF_MAX_ROWS);
+        return fail(TRC_HIP_E_SHAPE, "trc_hip_preference_loss: %lld rows (at most %lld)", (long long) l.ne[1],
+                    (long long) PF_MAX_ROWS);
     }
     auto* const f = l.type == TRC_HIP_TYPE_F32   ? forward<TRC_HIP_TYPE_F32>
                     : l.type == TRC_HIP_TYPE_F16 ? forward<TRC_HIP_TYPE_F16>
