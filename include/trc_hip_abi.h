@@ -360,7 +360,7 @@ int trc_hip_lora_back(const trc_hip_lora_set* set, const trc_hip_tensor* x, cons
  * rows not counted), logp [2P], slope [P], loss [1]; lse and slope are what trc_hip_preference_loss_back
  * needs. All vectors contiguous. smoothing is in 0 .. 1. Rows are summed in 32 bits, sequences and
  * pairs in 64, in a fixed order. A logit of -inf is a token that cannot occur; a label of V or
- * more makes the loss NaN. At most 2^20 rows (TRC_HIP_E_SHAPE beyond); what is held of them is in
+ * more makes the loss NaN. At most 2^20 rows of 2^30 logits (TRC_HIP_E_SHAPE beyond); what is held of them is in
  * the stream's workspace (see trc_hip_lora). */
 int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* start,
                             const trc_hip_tensor* ref, float beta, float smoothing, const trc_hip_tensor* lse,
@@ -371,7 +371,7 @@ int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* 
  *   dlogits[v,t] = dloss (+-beta / P) slope_i (1[v = label_t] - exp(logits[v,t] - lse[t]))
  * (+ for the chosen sequence), and 0 for rows that are not counted or in no sequence, whatever
  * their logits hold. dlogits has logits' type and shape and may be logits itself. At most 2^20
- * rows here too; no workspace. */
+ * rows of 2^30 here too; no workspace. */
 int trc_hip_preference_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels,
                                  const trc_hip_tensor* start, const trc_hip_tensor* lse,
                                  const trc_hip_tensor* slope, const trc_hip_tensor* dloss, float beta,

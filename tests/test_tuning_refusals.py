@@ -181,6 +181,14 @@ def test_preference_refuses(call, name, value, code):
     refused(call, {**loss_args(), name: value}, code)
 
 
+@pytest.mark.parametrize("V", [(1 << 30) + 1, (1 << 31) - 16384, (1 << 31) - 1, 1 << 31])
+def test_preference_refuses_rows_that_32_bits_do_not_count(V):
+    """Rows that lie on one another, as a stride of 0 has them, fit memory however long they are."""
+    for call in (loss, loss_back):
+        refused(call, {**loss_args(), "logits": tensor(1, V, 9, type_=F16, nb={1: 0}), "dlogits": tensor(99, V, 9, type_=F16)},
+                H.E_SHAPE)
+
+
 def plan(bits=32, **change):
     t = dict(param=1 << 32, grad=2 << 32, m=3 << 32, v=4 << 32, m_scale=5 << 32, v_scale=6 << 32, n=100)
     t.update(change)

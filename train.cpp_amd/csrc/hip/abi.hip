@@ -520,7 +520,8 @@ int check_preference(const char* who, const trc_hip_tensor* logits, const trc_hi
     if (logits == nullptr || slope == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL tensor", who);
     if (!is_float(logits->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of logits is not F32, F16 or BF16", who, logits->type);
     const int64_t V = logits->ne[0], T = logits->ne[1], P = slope->ne[0];
-    if (V <= 0 || V > INT32_MAX || T <= 0 || T > INT32_MAX || P <= 0 || P > INT32_MAX / 2) {
+    // (the kernels count a row's elements in 32 bits, and some thousands past its end)
+    if (V <= 0 || V > (1 << 30) || T <= 0 || T > INT32_MAX || P <= 0 || P > INT32_MAX / 2) {
         return fail(TRC_HIP_E_SHAPE, "%s: V = %lld, T = %lld, %lld pairs", who, (long long) V, (long long) T, (long long) P);
     }
     if (!(beta == beta)) return fail(TRC_HIP_E_INVALID, "%s: beta is NaN", who);
