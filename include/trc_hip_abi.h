@@ -369,7 +369,8 @@ int trc_hip_preference_loss(const trc_hip_tensor* logits, const trc_hip_tensor* 
 
 /* The logits' gradient of trc_hip_preference_loss, for dloss [1] F32:
  *   dlogits[v,t] = dloss (+-beta / P) slope_i (1[v = label_t] - exp(logits[v,t] - lse[t]))
- * (+ for the chosen sequence), and 0 for rows that are not counted or in no sequence, whatever
+ * (+ for the chosen sequence; where lse is 1024 or more in magnitude, too far from 0 for its float to hold the row's
+ * sum, it is computed again), and 0 for rows that are not counted or in no sequence, whatever
  * their logits hold. dlogits has logits' type and shape and may be logits itself. At most 2^20
  * rows of 2^30 here too; no workspace. */
 int trc_hip_preference_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels,

@@ -20,9 +20,10 @@ HALF = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 BETA, SMOOTHING, DLOSS = 0.2, 0.1, 0.7
 
 
-def check(kind, logits, labels, T):
+def check(kind, logits, labels, T, far=False, in_place=False):
     """`logits` are the counted rows, a sequence each; the batch has T rows, of which the others are in no
-    sequence (they decide in how many parts a row is summed)."""
+    sequence (they decide in how many parts a row is summed). far: lse's own rounding to a float, |lse| 2^-24,
+    counts in full in lse alone, elsewhere as of 1024 at most."""
     n, V = logits.shape
     assert n % 2 == 0 and T >= n
     held, l = encode(logits, kind)
@@ -32,9 +33,10 @@ def check(kind, logits, labels, T):
     y[:n] = labels
     with np.errstate(under="ignore"):
         top = l.max(1)
-        lse = top + np.log(np.exp(l - top[:, None]).sum(1))
-        prob = np.exp(l - lse[:, None])
-    logp = l[np.arange(n), labels] - lse
+        log_s = np.log(np.exp(l - top[:, None]).sum(1))
+        prob = np.exp((l - top[:, None]) - log_s[:, None])
+    lse = top + log_s
+    logp = (l[np.arange(n), labels] - top) - log_s
     rng = np.random.default_rng(1)
     ref = (logp + rng.standard_normal(n)).astype(np.float32)
     z = BETA * ((logp - ref)[0::2] - (logp - ref)[1::2])
@@ -52,7 +54,8 @@ def check(kind, logits, labels, T):
         keep.append(dev)
         return dev, out
 
-    m, dl = Mat(whole, t), Mat(np.zeros_like(whole), t)
+    m = Mat(whole, t)
+    dl = m if in_place else Mat(np.zeros_like(whole), t)
     keep += [m, dl]
     _, yt = v(y, H.TYPE_I32)
     _, start = v(np.arange(n + 1, dtype=np.int32), H.TYPE_I32)
@@ -77,6 +80,8 @@ def check(kind, logits, labels, T):
         assert not bad.any(), f"{what}: {got[bad][:4]} for {want[bad][:4]} at {np.argwhere(bad)[:4].tolist()}"
 
     near(glse[:n], lse, e_lse, "lse")
+    if far:
+        e_lse = sums + np.minimum(np.abs(lse), 1024) * U32
     assert not glse[n:].any()
     e_logp = e_lse + 2 * U32 * np.abs(logp)
     near(glogp, logp, e_logp, "logp")
@@ -160,3 +165,26 @@ def test_few_late_tokens_far_above(hip, kind, sizes):
     labels = l.argmax(1).astype(np.int32)
     labels[::5] = 0
     check(kind, l, labels, T)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes", [ONE, PARTS, {k: (1000, 40) for k in TYPES}], ids=["one", "parts", "short"])
+def test_rows_far_from_zero(hip, kind, sizes, in_place):
+    """A row's log-sum may be so large that its float holds little of the sum, or nothing: rows all of whose
+    tokens a finite value masks, and rows moved as a whole. Their probabilities are those of the
+    differences between their logits."""
+    V, T = sizes[kind]
+    announce(f"preference far from zero {kind} V={V} T={T} in place {in_place}")
+    rng = np.random.default_rng(9)
+    at = np.array([2e3, -5e3, 3e4, -6e4] + ([] if kind == "f16" else [1e5, -1e6, -1e9, 3e12, -1e20, -1e30, 2e38, -3e38]))
+    even = np.repeat(at[:, None], V, 1)  # every token alike
+    moved = even + rng.standard_normal(even.shape) * 2
+    spread = even * (1 + (rng.random(even.shape) < 0.3) * 2.0 ** -6)
+    near_bound = 1024 + np.array([-60.0, -12, -11, -10, 2, 50])[:, None] + rng.standard_normal((6, V))
+    l = np.concatenate([even, moved, spread, near_bound])
+    labels = np.where(rng.random(len(l)) < 0.5, l.argmax(1), rng.integers(0, V, len(l))).astype(np.int32)
+    # (where the label lies far under the row's largest, the loss is that distance: not what is looked at here)
+    low = l[np.arange(len(l)), labels] < l.max(1) - 50
+    labels[low] = l.argmax(1)[low]
+    check(kind, l, labels, max(T, 64), far=True, in_place=in_place)

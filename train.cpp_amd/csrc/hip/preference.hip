@@ -22,6 +22,7 @@ constexpr int PF_WAVES = 16;       // of the join
 constexpr int PF_MAX_PARTS = 64;   // parts of a row: a lane each where they are joined
 constexpr int PF_LOADS = 4;        // 16-byte loads that a thread has under way
 constexpr int64_t PF_MAX_ROWS = (int64_t) 1 << 20;  // their log-probabilities fit the stream's workspace
+constexpr float PF_FAR = 1024.f;   // magnitude of a row's log-sum from which its float is not taken for the gradient
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // 16 bytes of a row whose address is only as aligned as one element
@@ -95,8 +96,17 @@ __device__ __forceinline__ Soft wave_join(Soft a) {
     for (int d = 32; d > 0; d >>= 1) a = join(a, {__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)});
     return a;
 }
-// A row's log-sum in 64 bits: the sums over a sequence's rows, and differences of them, would show its rounding.
-__device__ __forceinline__ double lse_of(Soft a) { return (double) a.m + log((double) a.s); }
+// A row's log-sum, and the log-probability of its label's logit ly, in 64 bits: the sums over a sequence's rows, and
+// differences of them, would show its rounding. The maximum goes first, or of rows far from 0 nothing would be left.
+struct RowSums {
+    float lse;
+    double lp;
+    __device__ __forceinline__ RowSums(Soft a, double ly) {
+        const double log_s = log((double) a.s);
+        lse = (float) ((double) a.m + log_s);
+        lp = (ly - (double) a.m) - log_s;
+    }
+};
 
 template <int N>
 __device__ __forceinline__ void take(Soft& a, const float (&x)[N]) {
@@ -201,9 +211,9 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_rows(const uint8_t* __restr
 #pragma unroll
     for (int k = 1; k < PF_THREADS / 64; ++k) a = join(a, w[k]);
     if (gridDim.y == 1) {
-        const double e = lse_of(a);
-        lse[row] = (float) e;
-        lp[row] = (double) ly - e;
+        const RowSums r(a, ly);
+        lse[row] = r.lse;
+        lp[row] = r.lp;
     } else {
         parts[row * gridDim.y + blockIdx.y] = a;
         if (blockIdx.y == 0) lp[row] = ly;
@@ -235,9 +245,9 @@ __global__ __launch_bounds__(PF_WAVES * 64) void k_pref_pairs(int64_t T, const i
                 if (lane == k) mine = all;
             }
             if (own) {
-                const double e = lse_of(mine);
-                lse[t] = (float) e;
-                lp[t] = l - e;
+                const RowSums r(mine, l);
+                lse[t] = r.lse;
+                lp[t] = r.lp;
             }
         }
         __syncthreads();
@@ -313,13 +323,32 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_back(const uint8_t* logits,
     constexpr int VEC = R::VEC, U = PF_LOADS, STEP = PF_THREADS * VEC;
     // The last rows first: they are what the caches still hold of the forward pass. With stores that do not stay
     // there either, 8192 rows of 32000 in 16 bits take 227 us both ways, and 275 in order with plain stores.
-    const int64_t row = gridDim.x - 1 - blockIdx.x, lo = (int64_t) blockIdx.y * len;
+    const int64_t row = gridDim.x - 1 - blockIdx.x;
     const int32_t y = labels[row];
     const int64_t seq = y < 0 ? -1 : sequence_of(start, 2 * pairs, row);
+    float base = lse[row], part = 1.f;  // a probability is exp(l - base) part
+    // A float is off by 2^-15 (3e-5 of every probability) at most under PF_FAR. Beyond, the row is summed again from its
+    // maximum: of logits around -1e9 the float holds nothing of log s. The row's first workgroup does it, and
+    // the whole row with it, since dlogits may be the logits and another would overwrite what it reads. 61 rows of 131071
+    // in F32 take 78 us both ways if all are so, 26 otherwise; 8192 of 32000 in 16 bits 265, 224 otherwise.
+    const bool far = seq >= 0 && fabsf(base) >= PF_FAR && fabsf(base) < INFINITY;
+    if (far && blockIdx.y != 0) return;
+    const int64_t lo = (int64_t) blockIdx.y * len;
     const typename R::Elem* const p = (const typename R::Elem*) (logits + row * nb1) + lo;
     typename R::Elem* const d = (typename R::Elem*) (dlogits + row * dnb1) + lo;
-    const int n = (int) (min(lo + len, V) - lo), whole = n / VEC * VEC;
+    const int n = (int) (far ? V : min(lo + len, V) - lo), whole = n / VEC * VEC;
     int i = (int) threadIdx.x * VEC;
+    if (far) {
+        __shared__ Soft sums[PF_THREADS / 64];
+        Soft a = wave_join(careful_share<TYPE>(p, n));
+        if (((int) threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = sums[0];
+#pragma unroll
+        for (int k = 1; k < PF_THREADS / 64; ++k) a = join(a, sums[k]);
+        base = a.m;
+        part = 1.f / a.s;
+    }
     if (seq < 0) {  // not counted: zeros, whatever the logits hold
         float z[VEC];
 #pragma unroll
@@ -329,7 +358,7 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_back(const uint8_t* logits,
         return;
     }
     const float w = (float) ((double) slope[seq >> 1] * (double) beta / (double) pairs) * dloss[0] * ((seq & 1) ? -1.f : 1.f);
-    const float base = lse[row];
+    const float wp = w * part;
     const int64_t label = y - lo;  // in this part
     // -w exp(l - lse), and w more at the label
     auto store = [&](int at, float* x) {
@@ -337,12 +366,12 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_back(const uint8_t* logits,
         for (int k = 0; k < VEC; ++k) x[k] = exp_of(x[k] - base);
         if (label >= at && label < at + VEC) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[k] = (label == at + k ? 1.f : 0.f) - x[k];
+            for (int k = 0; k < VEC; ++k) x[k] = (label == at + k ? 1.f : 0.f) - x[k] * part;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) x[k] *= w;
         } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[k] *= -w;
+            for (int k = 0; k < VEC; ++k) x[k] *= -wp;
         }
         R::store(d + at, x);
     };
@@ -362,7 +391,7 @@ __global__ __launch_bounds__(PF_THREADS) void k_pref_back(const uint8_t* logits,
 #pragma unroll
     for (int u = 0; u < U - 1; ++u)
         if (i + u * STEP < whole) store(i + u * STEP, x[u]);
-    if (last < n) d[last] = R::put(w * ((label == last ? 1.f : 0.f) - exp_of(x[U - 1][0] - base)));
+    if (last < n) d[last] = R::put(w * ((label == last ? 1.f : 0.f) - exp_of(x[U - 1][0] - base) * part));
 }
 
 // Parts of a row, and their length: whole rows while there are rows for every CU
