@@ -226,7 +226,7 @@ def prepare(case, seed):
     s["labels"][torch.tensor(_prompts(c), device=DEVICE)] = -1
     s["dloss"] = torch.ones(1, device=DEVICE)
     if own:
-        s["stats"], s["loss"] = torch.empty(T, 4, device=DEVICE), torch.empty(4, device=DEVICE)
+        s["stats"], s["loss"] = torch.empty(T, 5, device=DEVICE), torch.empty(4, device=DEVICE)
         s["dlogits"] = torch.empty_like(s["logits"])
         s["t"] = {n: _t(H, s[n]) for n in ("logits", "labels", "ids", "top", "stats", "loss", "dloss", "dlogits")}
     return s
