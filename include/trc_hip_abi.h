@@ -58,6 +58,7 @@ enum trc_hip_type {
     TRC_HIP_TYPE_Q5_0 = 6,
     TRC_HIP_TYPE_Q5_1 = 7,
     TRC_HIP_TYPE_Q8_0 = 8,
+    TRC_HIP_TYPE_I8   = 24,
     TRC_HIP_TYPE_I32  = 26,
     TRC_HIP_TYPE_BF16 = 30
 };
@@ -423,6 +424,83 @@ int trc_hip_adamw_moments(void* plan, void* stream);
 
 /* Frees the plan (not the tensors), after its work: synchronize first. NULL is allowed. */
 int trc_hip_adamw_destroy(void* plan);
+
+/* ------------------------------------------------------------------ 8-bit floating point
+ *
+ * Products with weights in 8-bit floating point: e4m3 (sign, 4 bits of exponent with a bias of 7, 3 of fraction;
+ * 448 is the largest value, 0x7F and 0xFF are NaN, there is no infinity), with a scale for each block of 128.
+ * No counterpart in the reference. */
+
+/* A matrix of K columns and R rows: value [k,r] = code [k,r] times its block's scale. */
+typedef struct trc_hip_fp8 {
+    trc_hip_tensor q;      /* [K, R] I8: the codes. data 16-byte aligned, nb[0] = 1, nb[1] (also of a single row) a
+                            * multiple of 128 up to 8 MiB: every row has room for whole blocks, and the bytes from K
+                            * to the end of its last block are zeros                                            */
+    trc_hip_tensor scale;  /* of each row:       [ceil(K / 128), R] I8
+                            * of 128 rows each:  [ceil(K / 128), ceil(R / 128)] I8 or F32
+                            * I8 holds a power of two: its exponent with 127 added, from 1 to 254. data 4-byte aligned,
+                            * nb[1] a multiple of 4; a row of bytes has room for a multiple of 4             */
+} trc_hip_fp8;
+
+/* Largest number of tokens of trc_hip_fp8_matvec. */
+#define TRC_HIP_FP8_MATVEC_MAX_N 64
+
+/* x [K, R] (F32, F16 or BF16; nb[0] the element size, rows at any aligned stride) as codes and scales of powers of
+ * two, either for each row (activations) or for 128 rows each (weights), as out.scale's shape has it: the smallest
+ * power that brings the block's largest magnitude to 448 or less, 2^-126 at least, and 1 for a block of zeros. All of it
+ * is exact but for the codes' rounding (to nearest, ties to even). A value that is not finite becomes NaN and takes no
+ * part in its block's scale. The rows' bytes up to whole blocks are written as zeros. */
+int trc_hip_fp8_quantize(const trc_hip_tensor* x, const trc_hip_fp8* out, void* stream);
+
+/* y [M, N] = mul_mat(w, x) of a weight w [K, M] with scales for 128 rows each and activations x [K, N] with scales (I8)
+ * for each row. y is F32, F16 or BF16 with nb[0] the element size and rows at any aligned stride, and overlaps
+ * neither. An F32 y is summed with exact products in 32 bits. For a y of 16 bits over more than TRC_HIP_FP8_MATVEC_MAX_N
+ * tokens the products go through the 8-bit matrix instruction, which adds eight of them with some 13 bits below
+ * the largest: off by up to 1e-4 of the sum of magnitudes, a fortieth of what rounding the activations to e4m3 may cost.
+ * The same bits from run to run. Products of few tiles keep sums in the stream's workspace of trc_hip_qmatvec, which
+ * the first such call on a stream allocates (make it before capturing that stream in global mode). */
+int trc_hip_fp8_mul_mat(const trc_hip_fp8* w, const trc_hip_fp8* x, const trc_hip_tensor* y, void* stream);
+
+/* The gradient of trc_hip_fp8_mul_mat by x: dx [K, N] = W^T dy for dy [M, N] with scales for each row. w is read as it
+ * is, there is no second copy of it. Types, sums and workspace as for trc_hip_fp8_mul_mat. */
+int trc_hip_fp8_mul_mat_back(const trc_hip_fp8* w, const trc_hip_fp8* dy, const trc_hip_tensor* dx, void* stream);
+
+/* y = mul_mat(w, x) for N <= TRC_HIP_FP8_MATVEC_MAX_N tokens whose activations x [K, N] are still F32, F16 or BF16: they
+ * are quantized on the way, as trc_hip_fp8_quantize does it, and y is what trc_hip_fp8_mul_mat makes of that, bit
+ * for bit. Beyond 4 tokens what is quantized is held in the stream's workspace (K N up to 8 million). */
+int trc_hip_fp8_matvec(const trc_hip_fp8* w, const trc_hip_tensor* x, const trc_hip_tensor* y, void* stream);
+
+/* ------------------------------------------------------------------ distillation */
+
+/* Most entries of a teacher's row. */
+#define TRC_HIP_DISTILL_MAX_TOP 1024
+
+/* The loss of a student's logits against a teacher's top logits, mixed with the labels' cross-entropy.
+ * logits is [V, T] of F32, F16 or BF16 (nb[0] the element size, rows at any aligned stride), labels [T] I32; a row whose
+ * label is negative is not counted and not read. ids [top, T] I32 and teacher [top, T] (F32, F16 or BF16) hold each
+ * row's tokens and the teacher's logits of them, both contiguous; an entry whose id is outside 0 .. V-1 is left out, and
+ * one token's entries may be several. With p = softmax(teacher / tau) over a row's entries, q = softmax(logits / tau):
+ *   KL_t = sum_j p_j (log p_j - log q[id_j])      CE_t = log sum_v exp(logits[v,t]) - logits[label,t]
+ *   loss[0] = mean_t alpha tau^2 KL_t + (1 - alpha) CE_t   over the n rows that are counted
+ * and loss [4] F32 holds that, the means of KL and CE, and n; of no rows all are 0. A row without entries has a KL of 0
+ * and no gradient of it. With alpha = 1 CE is not computed (0) and labels count only by their sign; with alpha = 0
+ * KL is not. tau > 0, alpha in 0 .. 1. stats [5, T] F32 contiguous is what trc_hip_distill_loss_back needs: the row's
+ * largest logit, one over its sums of exponentials from there at 1 and at tau, the teacher's largest and one over its sum.
+ * Sums of a row are in 32 bits from its maximum, their logarithms and all sums over rows in 64, in a fixed order. A label of V or
+ * more, where alpha < 1, makes the loss NaN. At most 2^19 rows of 2^30 logits; rows' terms are in the stream's workspace
+ * (see trc_hip_lora). */
+int trc_hip_distill_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
+                         const trc_hip_tensor* teacher, float tau, float alpha, const trc_hip_tensor* stats,
+                         const trc_hip_tensor* loss, void* stream);
+
+/* The logits' gradient of trc_hip_distill_loss, with stats and loss of that call, for dloss [1] F32:
+ *   dlogits[v,t] = dloss / n (alpha tau (q_v - sum of p_j with id_j = v) + (1 - alpha) (softmax(logits)_v - 1[v = label_t]))
+ * and 0 for rows that are not counted, whatever their logits hold. dlogits has logits' type and shape and may be
+ * logits itself. No workspace. */
+int trc_hip_distill_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
+                              const trc_hip_tensor* teacher, const trc_hip_tensor* stats, const trc_hip_tensor* loss,
+                              const trc_hip_tensor* dloss, float tau, float alpha, const trc_hip_tensor* dlogits,
+                              void* stream);
 
 #ifdef __cplusplus
 }

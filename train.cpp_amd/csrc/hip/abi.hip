@@ -1,8 +1,9 @@
 // extern "C" entry points of libtrc_hip.so (declared in include/trc_hip_abi.h):
 // argument validation, error reporting and the HIP runtime calls. Kernels live
 // in dequant.hip, qmatvec.hip, qmm.hip, mul_mat.hip, elementwise.hip, copy.hip, lora.hip,
-// preference.hip and adamw.hip.
+// preference.hip, adamw.hip, fp8.hip, fp8_mm.hip and distill.hip.
 #include "common.h"
+#include "fp8.h"
 
 #include <cstdarg>
 #include <cstdio>
@@ -672,6 +673,220 @@ int trc_hip_adamw_moments(void* plan, void* stream) {
 int trc_hip_adamw_destroy(void* plan) {
     TRC_FORCED("trc_hip_adamw_destroy");
     return plan != nullptr ? adamw_destroy(plan) : TRC_HIP_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// A matrix in 8-bit floating point and what is read of it: whole blocks of its rows, whole words of its rows of bytes
+// of scales. per_row: its scales are its rows'; else those of 128 rows each.
+int check_fp8(const char* who, const char* name, const trc_hip_fp8* m, int64_t K, int64_t R, bool per_row) {
+    const trc_hip_tensor &q = m->q, &s = m->scale;
+    const int64_t kb = (K + 127) / 128, groups = per_row ? R : (R + 127) / 128;
+    TRC_TRY(check_shape(who, name, &q, TRC_HIP_TYPE_I8, K, R, 1, false));
+    if ((uintptr_t) q.data % 16 != 0 || q.nb[1] % 128 != 0) {
+        return fail(TRC_HIP_E_ALIGN, "%s: codes of %s must be 16-byte aligned, rows whole blocks of 128 bytes", who, name);
+    }
+    if (q.nb[1] < (size_t) kb * 128 || q.nb[1] > ((size_t) 1 << 23)) {
+        return fail(TRC_HIP_E_SHAPE, "%s: rows of %s are %zu bytes apart (whole blocks, 8 MiB at most)", who, name, q.nb[1]);
+    }
+    if (s.type != TRC_HIP_TYPE_I8 && (per_row || s.type != TRC_HIP_TYPE_F32)) {
+        return fail(TRC_HIP_E_INVALID, "%s: type %d of %s's scales", who, s.type, name);
+    }
+    TRC_TRY(check_shape(who, name, &s, s.type, kb, groups, 1, true));
+    if ((uintptr_t) s.data % 4 != 0 || (groups > 1 && s.nb[1] % 4 != 0)) {
+        return fail(TRC_HIP_E_ALIGN, "%s: scales of %s must be 4-byte aligned, their rows too", who, name);
+    }
+    // (a row of bytes has room for whole words, since rows are whole words apart and do not overlap)
+    if (groups > 1 && s.nb[1] > ((size_t) 1 << 22)) {
+        return fail(TRC_HIP_E_SHAPE, "%s: scales of %s's rows over 4 MiB apart", who, name);
+    }
+    return TRC_HIP_OK;
+}
+
+// What a matrix in 8 bits covers, whole blocks and words included, as contiguous bytes.
+trc_hip_tensor bytes_of(const trc_hip_tensor& t, int64_t whole) {
+    const int64_t es = (int64_t) basic_type_size(t.type), row = (t.ne[0] * es + whole - 1) / whole * whole;
+    const int64_t n = (t.ne[1] - 1) * (int64_t) t.nb[1] + row;
+    trc_hip_tensor b{};
+    b.data = t.data;
+    b.type = TRC_HIP_TYPE_I8;
+    b.ne[0] = n;
+    b.ne[1] = b.ne[2] = b.ne[3] = 1;
+    b.nb[0] = 1;
+    return b;
+}
+int check_fp8_apart(const char* who, const trc_hip_tensor* out, const char* name, const trc_hip_fp8* m, const char* other) {
+    const trc_hip_tensor q = bytes_of(m->q, 128), s = bytes_of(m->scale, 4);
+    TRC_TRY(check_apart(who, out, name, &q, other, false));
+    return check_apart(who, out, name, &s, other, false);
+}
+
+// The sizes that the kernels' 32-bit offsets and counts allow for.
+int check_fp8_sizes(const char* who, int64_t K, int64_t M, int64_t N) {
+    if (K <= 0 || M <= 0 || N <= 0 || K > (1 << 23) || M > (1 << 23) || N > (1 << 23)) {
+        return fail(TRC_HIP_E_SHAPE, "%s: K = %lld, M = %lld, N = %lld (1 to 2^23 each)", who, (long long) K, (long long) M, (long long) N);
+    }
+    return TRC_HIP_OK;
+}
+
+// y, rows x N in any float type, apart from the weight; `in` are its columns.
+int check_fp8_out(const char* who, const char* name, const trc_hip_tensor* y, int64_t rows, int64_t N, const trc_hip_fp8* w) {
+    if (y == nullptr) return fail(TRC_HIP_E_INVALID, "%s: %s is NULL", who, name);
+    if (!is_float(y->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of %s is not F32, F16 or BF16", who, y->type, name);
+    TRC_TRY(check_shape(who, name, y, y->type, rows, N, 1, true));
+    return check_fp8_apart(who, y, name, w, "w");
+}
+
+F8Args fp8_args(const trc_hip_fp8& w, const trc_hip_tensor& y, int64_t N) {
+    F8Args a{};
+    a.w = (const uint8_t*) w.q.data;
+    a.w_nb1 = (int64_t) w.q.nb[1];
+    a.K = w.q.ne[0];
+    a.M = w.q.ne[1];
+    a.N = N;
+    a.ws = (const uint8_t*) w.scale.data;
+    a.ws_nb1 = (int64_t) w.scale.nb[1];
+    a.ws_float = w.scale.type == TRC_HIP_TYPE_F32;
+    a.y = (uint8_t*) y.data;
+    a.y_nb1 = (int64_t) y.nb[1];
+    a.y_type = y.type;
+    return a;
+}
+
+// The product and its gradient by x: back sums over w's rows.
+int fp8_product(const char* who, const trc_hip_fp8* w, const trc_hip_fp8* x, const trc_hip_tensor* y, bool back, hipStream_t s) {
+    if (w == nullptr || x == nullptr || y == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL argument", who);
+    const int64_t K = w->q.ne[0], M = w->q.ne[1], N = x->q.ne[1];
+    const char *const xn = back ? "dy" : "x", *const yn = back ? "dx" : "y";
+    TRC_TRY(check_fp8_sizes(who, K, M, N));
+    TRC_TRY(check_fp8(who, "w", w, K, M, false));
+    TRC_TRY(check_fp8(who, xn, x, back ? M : K, N, true));
+    TRC_TRY(check_fp8_out(who, yn, y, back ? K : M, N, w));
+    TRC_TRY(check_fp8_apart(who, y, yn, x, xn));
+    F8Args a = fp8_args(*w, *y, N);
+    a.x = (const uint8_t*) x->q.data;
+    a.x_nb1 = (int64_t) x->q.nb[1];
+    a.xs = (const uint8_t*) x->scale.data;
+    a.xs_nb1 = (int64_t) x->scale.nb[1];
+    if (!back && N <= TRC_HIP_FP8_MATVEC_MAX_N) return launch_f8_skinny(a, nullptr, s);
+    return launch_f8_tiles(a, back, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int trc_hip_fp8_quantize(const trc_hip_tensor* x, const trc_hip_fp8* out, void* stream) {
+    const char* const who = "trc_hip_fp8_quantize";
+    TRC_FORCED("trc_hip_fp8_quantize");
+    if (x == nullptr || out == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL argument", who);
+    if (!is_float(x->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of x is not F32, F16 or BF16", who, x->type);
+    const int64_t K = x->ne[0], R = x->ne[1];
+    TRC_TRY(check_fp8_sizes(who, K, R, 1));
+    TRC_TRY(check_shape(who, "x", x, x->type, K, R, 1, false));
+    TRC_TRY(check_fp8(who, "out", out, K, R, out->scale.ne[1] == R));
+    if (out->scale.type != TRC_HIP_TYPE_I8) return fail(TRC_HIP_E_INVALID, "%s: the scales must be I8", who);
+    // (a workgroup of 256 for each 128 x 128, or for four pieces of 512 of a row)
+    if ((out->scale.ne[1] == R ? R * ((K + 511) / 512) / 4 : ((R + 127) / 128) * ((K + 127) / 128)) >= max_groups(256)) {
+        return fail(TRC_HIP_E_SHAPE, "%s: %lld rows of %lld", who, (long long) R, (long long) K);
+    }
+    const trc_hip_tensor q = bytes_of(out->q, 128), s = bytes_of(out->scale, 4);
+    TRC_TRY(check_apart(who, &q, "out", x, "x", false));
+    TRC_TRY(check_apart(who, &s, "out's scale", x, "x", false));
+    TRC_TRY(check_apart(who, &q, "out", &s, "its scale", false));
+    return launch_f8_quantize(*x, *out, (hipStream_t) stream);
+}
+
+int trc_hip_fp8_mul_mat(const trc_hip_fp8* w, const trc_hip_fp8* x, const trc_hip_tensor* y, void* stream) {
+    TRC_FORCED("trc_hip_fp8_mul_mat");
+    return fp8_product("trc_hip_fp8_mul_mat", w, x, y, false, (hipStream_t) stream);
+}
+
+int trc_hip_fp8_mul_mat_back(const trc_hip_fp8* w, const trc_hip_fp8* dy, const trc_hip_tensor* dx, void* stream) {
+    TRC_FORCED("trc_hip_fp8_mul_mat_back");
+    return fp8_product("trc_hip_fp8_mul_mat_back", w, dy, dx, true, (hipStream_t) stream);
+}
+
+int trc_hip_fp8_matvec(const trc_hip_fp8* w, const trc_hip_tensor* x, const trc_hip_tensor* y, void* stream) {
+    const char* const who = "trc_hip_fp8_matvec";
+    TRC_FORCED("trc_hip_fp8_matvec");
+    if (w == nullptr || x == nullptr || y == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL argument", who);
+    const int64_t K = w->q.ne[0], M = w->q.ne[1], N = x->ne[1];
+    TRC_TRY(check_fp8_sizes(who, K, M, N));
+    if (N > TRC_HIP_FP8_MATVEC_MAX_N) {
+        return fail(TRC_HIP_E_SHAPE, "%s: %lld tokens (at most %d)", who, (long long) N, TRC_HIP_FP8_MATVEC_MAX_N);
+    }
+    if (!is_float(x->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of x is not F32, F16 or BF16", who, x->type);
+    TRC_TRY(check_fp8(who, "w", w, K, M, false));
+    TRC_TRY(check_shape(who, "x", x, x->type, K, N, 1, false));
+    TRC_TRY(check_fp8_out(who, "y", y, M, N, w));
+    TRC_TRY(check_apart(who, y, "y", x, "x", false));
+    return launch_f8_skinny(fp8_args(*w, *y, N), x, (hipStream_t) stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+// The rules that the distillation loss and its gradient share.
+int check_distill(const char* who, const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
+                  const trc_hip_tensor* teacher, const trc_hip_tensor* stats, const trc_hip_tensor* loss, float tau, float alpha) {
+    if (logits == nullptr || ids == nullptr || teacher == nullptr) return fail(TRC_HIP_E_INVALID, "%s: NULL tensor", who);
+    if (!is_float(logits->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of logits is not F32, F16 or BF16", who, logits->type);
+    if (!is_float(teacher->type)) return fail(TRC_HIP_E_INVALID, "%s: type %d of teacher is not F32, F16 or BF16", who, teacher->type);
+    const int64_t V = logits->ne[0], T = logits->ne[1], top = ids->ne[0];
+    // (the kernels count a row's elements in 32 bits, and some thousands past its end)
+    if (V <= 0 || V > (1 << 30) || T <= 0 || T > INT32_MAX || top <= 0 || top > TRC_HIP_DISTILL_MAX_TOP) {
+        return fail(TRC_HIP_E_SHAPE, "%s: V = %lld, T = %lld, %lld entries (at most %d)", who, (long long) V, (long long) T,
+                    (long long) top, TRC_HIP_DISTILL_MAX_TOP);
+    }
+    if (!(tau > 0.f) || !(1.f / tau > 0.f) || !(1.f / tau < INFINITY)) return fail(TRC_HIP_E_INVALID, "%s: tau = %g", who, tau);
+    if (!(alpha >= 0.f && alpha <= 1.f)) return fail(TRC_HIP_E_INVALID, "%s: alpha = %g is not in 0 .. 1", who, alpha);
+    TRC_TRY(check_shape(who, "logits", logits, logits->type, V, T, 1, false));
+    TRC_TRY(check_shape(who, "labels", labels, TRC_HIP_TYPE_I32, T, 1, 1, false));
+    TRC_TRY(check_shape(who, "ids", ids, TRC_HIP_TYPE_I32, top, T, 1, false));
+    TRC_TRY(check_packed(who, "ids", ids));
+    TRC_TRY(check_shape(who, "teacher", teacher, teacher->type, top, T, 1, false));
+    TRC_TRY(check_packed(who, "teacher", teacher));
+    TRC_TRY(check_shape(who, "stats", stats, TRC_HIP_TYPE_F32, 5, T, 1, false));
+    TRC_TRY(check_packed(who, "stats", stats));
+    return check_shape(who, "loss", loss, TRC_HIP_TYPE_F32, 4, 1, 1, false);
+}
+
+}  // namespace
+
+extern "C" {
+
+int trc_hip_distill_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
+                         const trc_hip_tensor* teacher, float tau, float alpha, const trc_hip_tensor* stats,
+                         const trc_hip_tensor* loss, void* stream) {
+    const char* const who = "trc_hip_distill_loss";
+    TRC_FORCED("trc_hip_distill_loss");
+    TRC_TRY(check_distill(who, logits, labels, ids, teacher, stats, loss, tau, alpha));
+    const trc_hip_tensor* const all[6] = {stats, loss, logits, labels, ids, teacher};
+    const char* const names[6] = {"stats", "loss", "logits", "labels", "ids", "teacher"};
+    for (int i = 0; i < 2; ++i) {
+        for (int j = i + 1; j < 6; ++j) TRC_TRY(check_apart(who, all[i], names[i], all[j], names[j], false));
+    }
+    return launch_distill_loss(*logits, (const int32_t*) labels->data, *ids, *teacher, tau, alpha, (float*) stats->data,
+                               (float*) loss->data, (hipStream_t) stream);
+}
+
+int trc_hip_distill_loss_back(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
+                              const trc_hip_tensor* teacher, const trc_hip_tensor* stats, const trc_hip_tensor* loss,
+                              const trc_hip_tensor* dloss, float tau, float alpha, const trc_hip_tensor* dlogits, void* stream) {
+    const char* const who = "trc_hip_distill_loss_back";
+    TRC_FORCED("trc_hip_distill_loss_back");
+    TRC_TRY(check_distill(who, logits, labels, ids, teacher, stats, loss, tau, alpha));
+    TRC_TRY(check_shape(who, "dloss", dloss, TRC_HIP_TYPE_F32, 1, 1, 1, false));
+    TRC_TRY(check_shape(who, "dlogits", dlogits, logits->type, logits->ne[0], logits->ne[1], 1, true));
+    const trc_hip_tensor* const all[7] = {logits, labels, ids, teacher, stats, loss, dloss};
+    const char* const names[7] = {"logits", "labels", "ids", "teacher", "stats", "loss", "dloss"};
+    for (int j = 0; j < 7; ++j) TRC_TRY(check_apart(who, dlogits, "dlogits", all[j], names[j], j == 0));
+    return launch_distill_loss_back(*logits, (const int32_t*) labels->data, *ids, *teacher, (const float*) stats->data,
+                                    (const float*) loss->data, (const float*) dloss->data, tau, alpha, *dlogits, (hipStream_t) stream);
 }
 
 }  // extern "C"

@@ -183,6 +183,11 @@ int launch_preference_loss(const trc_hip_tensor& logits, const int32_t* labels, 
 int launch_preference_loss_back(const trc_hip_tensor& logits, const int32_t* labels, const int32_t* start, int64_t pairs,
                                 const float* lse, const float* slope, const float* dloss, float beta,
                                 const trc_hip_tensor& dlogits, hipStream_t stream);
+int launch_distill_loss(const trc_hip_tensor& logits, const int32_t* labels, const trc_hip_tensor& ids,
+                        const trc_hip_tensor& teacher, float tau, float alpha, float* stats, float* loss, hipStream_t stream);
+int launch_distill_loss_back(const trc_hip_tensor& logits, const int32_t* labels, const trc_hip_tensor& ids,
+                             const trc_hip_tensor& teacher, const float* stats, const float* loss, const float* dloss, float tau,
+                             float alpha, const trc_hip_tensor& dlogits, hipStream_t stream);
 // AdamW plans (adamw.hip). adamw_create may throw std::bad_alloc.
 int adamw_create(const trc_hip_adamw_tensor* tensors, int64_t count, int bits, void** plan);
 int adamw_step(void* plan, const trc_hip_adamw_hyper& hyper, hipStream_t stream);

@@ -1,0 +1,98 @@
+// y = W x and dx = W^T dy for a weight in 8-bit floating point with a scale for each 128 x 128 block and activations (or
+// gradients) quantized the same way, each token's in blocks of 128:
+//
+//   y[m,n]  = sum_b ws[m/128,b] 2^e[n,b] sum_{k in block b} w[m,k] x[n,k]
+//   dx[k,n] = sum_b ws[b,k/128] 2^e[n,b] sum_{m in block b} w[m,k] g[n,m]
+#include "fp8_mm.h"
+
+namespace trc_hip {
+
+#define F8_DECLARE(BM, BN, WM, WN, TRANS, FAST, POW2) \
+    template <>                                       \
+    void f8_tiles_launch<BM, BN, WM, WN, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
+#define F8_DECLARE_ALL(BM, BN, WM, WN, FAST)       \
+    F8_DECLARE(BM, BN, WM, WN, false, FAST, false) \
+    F8_DECLARE(BM, BN, WM, WN, false, FAST, true)  \
+    F8_DECLARE(BM, BN, WM, WN, true, FAST, false)  \
+    F8_DECLARE(BM, BN, WM, WN, true, FAST, true)
+F8_DECLARE_ALL(256, 256, 2, 4, true)
+F8_DECLARE_ALL(128, 128, 2, 2, true)
+F8_DECLARE_ALL(128, 128, 2, 2, false)
+F8_DECLARE_ALL(64, 64, 2, 2, true)
+F8_DECLARE_ALL(64, 64, 2, 2, false)
+
+namespace {
+
+constexpr int JOIN_THREADS = 256;
+
+// The parts' sums added in their order, four rows of a token per thread.
+__global__ __launch_bounds__(JOIN_THREADS) void k_f8_join(const float* __restrict__ sums, int64_t nb1, int64_t N, int64_t rows, int parts,
+                                                           uint32_t quads, uint8_t* __restrict__ y, int64_t y_nb1, int y_type) {
+    const uint32_t at = blockIdx.x * JOIN_THREADS + threadIdx.x, n = at / quads, r = (at - n * quads) * 4;
+    if (n >= N) return;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; ++p) v += *(const f4*) (sums + ((int64_t) p * N + n) * nb1 + r);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (r + k >= rows) break;
+        if (y_type == TRC_HIP_TYPE_F32) ((float*) (y + n * y_nb1))[r + k] = v[k];
+        else ((uint16_t*) (y + n * y_nb1))[r + k] = f8_bits(y_type, v[k]);
+    }
+}
+
+template <int BM, int BN, int WM, int WN, bool FAST>
+void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
+    const bool pow2 = !t.a.ws_float;
+    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, true, FAST, true> : f8_tiles_launch<BM, BN, WM, WN, true, FAST, false>)
+                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, false, FAST, true> : f8_tiles_launch<BM, BN, WM, WN, false, FAST, false>);
+    f(t, parts, s);
+}
+
+}  // namespace
+
+int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s) {
+    F8Tiles t{};
+    t.a = a;
+    t.rows = trans ? a.K : a.M;
+    t.steps = (int) (((trans ? a.M : a.K) + F8_BLOCK - 1) / F8_BLOCK);
+    const bool fast = a.y_type != TRC_HIP_TYPE_F32;
+    const int64_t cus = device_cus();
+    auto tiles = [&](int64_t b) { return ((t.rows + b - 1) / b) * ((a.N + b - 1) / b); };
+    const int edge = fast && tiles(256) >= cus ? 256 : tiles(128) >= cus ? 128 : 64;
+    if (tiles(edge) > max_groups(512) - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
+    t.tm = (int) ((t.rows + edge - 1) / edge);
+    t.tn = (int) ((a.N + edge - 1) / edge);
+    // few tiles: the sum in parts
+    int64_t parts = 1;
+    if (edge == 64 && tiles(64) * 2 <= cus) {
+        t.sums_nb1 = (t.rows + 3) / 4 * 4;
+        const int64_t fit = (int64_t) (qm_workspace_bytes() / 4) / (a.N * t.sums_nb1);
+        parts = cus / tiles(64);
+        if (parts > (t.steps + 3) / 4) parts = (t.steps + 3) / 4;
+        if (parts > fit) parts = fit;
+        if (parts < 1) parts = 1;
+    }
+    t.part_steps = t.steps;
+    if (parts > 1) {
+        t.part_steps = (int) (((t.steps + parts - 1) / parts + 3) / 4 * 4);
+        parts = (t.steps + t.part_steps - 1) / t.part_steps;
+    }
+    if (parts > 1) {
+        uint8_t* ws = nullptr;
+        const int rc = qm_stream_workspace(s, &ws);
+        if (rc != TRC_HIP_OK) return rc;
+        t.sums = (float*) ws;
+    }
+    const unsigned p = (unsigned) parts;
+    if (edge == 256) launch<256, 256, 2, 4, true>(t, trans, p, s);
+    else if (edge == 128) fast ? launch<128, 128, 2, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, false>(t, trans, p, s);
+    else fast ? launch<64, 64, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, false>(t, trans, p, s);
+    const int rc = check_launch("fp8_mul_mat");
+    if (rc != TRC_HIP_OK || parts == 1) return rc;
+    const int64_t quads = t.sums_nb1 / 4;
+    hipLaunchKernelGGL(k_f8_join, dim3((unsigned) ((a.N * quads + JOIN_THREADS - 1) / JOIN_THREADS)), dim3(JOIN_THREADS), 0, s, t.sums,
+                       t.sums_nb1, a.N, t.rows, (int) parts, (uint32_t) quads, a.y, a.y_nb1, a.y_type);
+    return check_launch("fp8_mul_mat (join)");
+}
+
+}  // namespace trc_hip

@@ -13,12 +13,14 @@ LIB_DIR = Path(__file__).resolve().parent / "lib"
 LIB_PATH = LIB_DIR / "libtrc_hip.so"
 
 TYPE_F32, TYPE_Q4_0, TYPE_Q4_1, TYPE_Q5_0, TYPE_Q5_1, TYPE_Q8_0 = 0, 2, 3, 6, 7, 8
-TYPE_F16, TYPE_I32, TYPE_BF16 = 1, 26, 30
+TYPE_F16, TYPE_I8, TYPE_I32, TYPE_BF16 = 1, 24, 26, 30
 QUANT_TYPES = {"q4_0": TYPE_Q4_0, "q4_1": TYPE_Q4_1, "q5_0": TYPE_Q5_0, "q5_1": TYPE_Q5_1, "q8_0": TYPE_Q8_0}
 BLOCK_BYTES = {TYPE_Q4_0: 18, TYPE_Q4_1: 20, TYPE_Q5_0: 22, TYPE_Q5_1: 24, TYPE_Q8_0: 34}
 QMATVEC_MAX_N = 64
 LORA_MAX_RANK = 256
 ADAMW_BLOCK = 256
+FP8_MATVEC_MAX_N = 64
+DISTILL_MAX_TOP = 1024
 
 OK, E_INVALID, E_SHAPE, E_ALIGN, E_NO_DEVICE, E_FORCED = 0, -1, -2, -3, -4, -5
 
@@ -31,6 +33,8 @@ EXPORTS = (
     "trc_hip_mul_mat_acc_f32", "trc_hip_sqr_f32", "trc_hip_scale_f32",
     "trc_hip_lora", "trc_hip_lora_back", "trc_hip_preference_loss", "trc_hip_preference_loss_back",
     "trc_hip_adamw_create", "trc_hip_adamw_step", "trc_hip_adamw_moments", "trc_hip_adamw_destroy",
+    "trc_hip_fp8_quantize", "trc_hip_fp8_mul_mat", "trc_hip_fp8_mul_mat_back", "trc_hip_fp8_matvec",
+    "trc_hip_distill_loss", "trc_hip_distill_loss_back",
 )
 
 
@@ -51,6 +55,10 @@ class Tensor(C.Structure):
 
 class LoraSet(C.Structure):
     _fields_ = [("a", Tensor), ("b", Tensor), ("scale", Tensor), ("start", Tensor), ("adapter", Tensor)]
+
+
+class Fp8(C.Structure):
+    _fields_ = [("q", Tensor), ("scale", Tensor)]
 
 
 class AdamWTensor(C.Structure):
@@ -138,6 +146,12 @@ def load() -> C.CDLL:
         "trc_hip_adamw_step": ([P, C.POINTER(AdamWHyper), P], I),
         "trc_hip_adamw_moments": ([P, P], I),
         "trc_hip_adamw_destroy": ([P], I),
+        "trc_hip_fp8_quantize": ([C.POINTER(Tensor), C.POINTER(Fp8), P], I),
+        "trc_hip_fp8_mul_mat": ([C.POINTER(Fp8), C.POINTER(Fp8), C.POINTER(Tensor), P], I),
+        "trc_hip_fp8_mul_mat_back": ([C.POINTER(Fp8), C.POINTER(Fp8), C.POINTER(Tensor), P], I),
+        "trc_hip_fp8_matvec": ([C.POINTER(Fp8), C.POINTER(Tensor), C.POINTER(Tensor), P], I),
+        "trc_hip_distill_loss": ([C.POINTER(Tensor)] * 4 + [F, F] + [C.POINTER(Tensor)] * 2 + [P], I),
+        "trc_hip_distill_loss_back": ([C.POINTER(Tensor)] * 7 + [F, F, C.POINTER(Tensor), P], I),
     }
     for name, (args, ret) in sig.items():
         fn = getattr(lib, name)
@@ -276,6 +290,43 @@ def preference_loss_back(logits: Tensor, labels: Tensor, start: Tensor, lse: Ten
                          beta: float, dlogits: Tensor, stream: int | None = None) -> None:
     check(load().trc_hip_preference_loss_back(C.byref(logits), C.byref(labels), C.byref(start), C.byref(lse),
                                               C.byref(slope), C.byref(dloss), beta, C.byref(dlogits), stream))
+
+
+def fp8(q: Tensor, scale: Tensor) -> Fp8:
+    """A matrix in 8-bit floating point: codes and scales (trc_hip_fp8)."""
+    return Fp8(q, scale)
+
+
+def fp8_quantize(x: Tensor, out: Fp8, stream: int | None = None) -> None:
+    check(load().trc_hip_fp8_quantize(C.byref(x), C.byref(out), stream))
+
+
+def fp8_mul_mat(w: Fp8, x: Fp8, y: Tensor, stream: int | None = None) -> None:
+    """y = mul_mat(w, x) (trc_hip_fp8_mul_mat)."""
+    check(load().trc_hip_fp8_mul_mat(C.byref(w), C.byref(x), C.byref(y), stream))
+
+
+def fp8_mul_mat_back(w: Fp8, dy: Fp8, dx: Tensor, stream: int | None = None) -> None:
+    """dx = W^T dy (trc_hip_fp8_mul_mat_back)."""
+    check(load().trc_hip_fp8_mul_mat_back(C.byref(w), C.byref(dy), C.byref(dx), stream))
+
+
+def fp8_matvec(w: Fp8, x: Tensor, y: Tensor, stream: int | None = None) -> None:
+    """y = mul_mat(w, x) for up to FP8_MATVEC_MAX_N tokens, x quantized on the way (trc_hip_fp8_matvec)."""
+    check(load().trc_hip_fp8_matvec(C.byref(w), C.byref(x), C.byref(y), stream))
+
+
+def distill_loss(logits: Tensor, labels: Tensor, ids: Tensor, teacher: Tensor, tau: float, alpha: float, stats: Tensor,
+                 loss: Tensor, stream: int | None = None) -> None:
+    check(load().trc_hip_distill_loss(C.byref(logits), C.byref(labels), C.byref(ids), C.byref(teacher), tau, alpha,
+                                      C.byref(stats), C.byref(loss), stream))
+
+
+def distill_loss_back(logits: Tensor, labels: Tensor, ids: Tensor, teacher: Tensor, stats: Tensor, loss: Tensor,
+                      dloss: Tensor, tau: float, alpha: float, dlogits: Tensor, stream: int | None = None) -> None:
+    check(load().trc_hip_distill_loss_back(C.byref(logits), C.byref(labels), C.byref(ids), C.byref(teacher),
+                                           C.byref(stats), C.byref(loss), C.byref(dloss), tau, alpha, C.byref(dlogits),
+                                           stream))
 
 
 class AdamW:
