@@ -30,23 +30,25 @@ union F8Frag {
     i8v all;
 };
 
-// The same as four 16 x 32 operands in binary16, which holds every e4m3 value.
+// Eight codes in binary16, which holds every e4m3 value.
+__device__ __forceinline__ h8v f8_half8(u2v c) {
+    union {
+        h2v h[4];
+        h8v all;
+    } o;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        o.h[2 * w] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[w], 1.f, false);
+        o.h[2 * w + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[w], 1.f, true);
+    }
+    return o.all;
+}
+// An operand as four of 16 x 32.
 struct F8Half {
     h8v part[4];
     __device__ __forceinline__ explicit F8Half(const F8Frag& f) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            union {
-                h2v h[4];
-                h8v all;
-            } o;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                o.h[2 * w] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f.quarter[q][w], 1.f, false);
-                o.h[2 * w + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f.quarter[q][w], 1.f, true);
-            }
-            part[q] = o.all;
-        }
+        for (int q = 0; q < 4; ++q) part[q] = f8_half8(f.quarter[q]);
     }
 };
 

@@ -74,10 +74,11 @@ constexpr int SK_PITCH = 512 + 16;      // of their codes in LDS: 8 rows' 16 byt
 constexpr uint32_t SK_RSRC = 0x00027000;
 
 // Up to 16 NT tokens: a workgroup takes 16 of the weight's rows, its waves share K out in groups of four blocks and
-// join their sums in LDS. The weight goes from memory to registers, a group ahead; bound by its bytes.
+// join their sums in LDS. The weight goes from memory to registers; bound by its bytes, of which as many are under way as
+// waves fit a CU: they are held to few registers, operands turned to binary16 a quarter at a time.
 // FUSED: x holds floats (of type XTYPE), and every wave quantizes what it multiplies: N <= SK_FUSED.
 template <int NT, int XTYPE>
-__global__ __launch_bounds__(SK_WAVES * 64) void k_f8_skinny(F8Args a, const uint8_t* __restrict__ xf, size_t xf_nb1) {
+__global__ __launch_bounds__(SK_WAVES * 64, NT == 1 ? 6 : 4) void k_f8_skinny(F8Args a, const uint8_t* __restrict__ xf, size_t xf_nb1) {
     constexpr bool FUSED = XTYPE >= 0;
     const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6, waves = (int) blockDim.x >> 6;
     const int r16 = lane & 15, chunk = lane >> 4;
@@ -99,33 +100,27 @@ __global__ __launch_bounds__(SK_WAVES * 64) void k_f8_skinny(F8Args a, const uin
     f4 acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j] = {0.f, 0.f, 0.f, 0.f};
-    F8Frag next[4];
-    auto load_w = [&](int g) {
+    for (int g = wave; g < groups; g += waves) {
+        F8Frag w[4];
+        float ws[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const uint32_t at = (uint32_t) (4 * g + b) * F8_BLOCK;
-            if (4 * g + b < kb) {
-                next[b].half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w_off, at, 0));
-                next[b].half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w_off + 64, at, 0));
-            }
+            // (past K the last block again, which is not used)
+            const int at = min(4 * g + b, kb - 1);
+            w[b].half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w_off, (uint32_t) at * F8_BLOCK, 0));
+            w[b].half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w_off + 64, (uint32_t) at * F8_BLOCK, 0));
+            ws[b] = a.ws_float ? ((const float*) wsr)[at] : f8_scale(wsr[at]);
         }
-    };
-    if (wave < groups) load_w(wave);
-    for (int g = wave; g < groups; g += waves) {
         uint32_t scale[NT];
         if constexpr (FUSED) {
             uint8_t* const mine = codes + wave * SK_FUSED * SK_PITCH;
-            float v[SK_FUSED][8];
-#pragma unroll
-            for (int t = 0; t < SK_FUSED; ++t)
-                if (t < a.N) f8_load8<XTYPE>(xf + t * xf_nb1, (int64_t) g * 512 + lane * 8, a.K, v[t]);
-#pragma unroll
-            for (int t = 0; t < SK_FUSED; ++t)
-                if (t < a.N) {
-                    const uint32_t e = f8_exponent(f8_max16(f8_amax8(v[t])));
-                    *(u2v*) (mine + t * SK_PITCH + lane * 8) = f8_codes(v[t], f8_inverse(e));
-                    if (r16 == 0) ((uint8_t*) (words + wave * SK_FUSED + t))[chunk] = (uint8_t) e;
-                }
+            for (int t = 0; t < a.N; ++t) {
+                float v[8];
+                f8_load8<XTYPE>(xf + t * xf_nb1, (int64_t) g * 512 + lane * 8, a.K, v);
+                const uint32_t e = f8_exponent(f8_max16(f8_amax8(v)));
+                *(u2v*) (mine + t * SK_PITCH + lane * 8) = f8_codes(v, f8_inverse(e));
+                if (r16 == 0) ((uint8_t*) (words + wave * SK_FUSED + t))[chunk] = (uint8_t) e;
+            }
             // a wave's own LDS accesses are carried out in their order
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             scale[0] = words[wave * SK_FUSED + min(r16, (int) a.N - 1)];
@@ -134,31 +129,36 @@ __global__ __launch_bounds__(SK_WAVES * 64) void k_f8_skinny(F8Args a, const uin
             for (int j = 0; j < NT; ++j)
                 scale[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, (uint32_t) ((16 * j + r16) * a.xs_nb1) + 4 * g, 0, 0);
         }
-        F8Frag w[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[b] = next[b];
-        if (g + waves < groups) load_w(g + waves);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             if (4 * g + b >= kb) break;
-            const float ws = a.ws_float ? ((const float*) wsr)[4 * g + b] : f8_scale(wsr[4 * g + b]);
-            const F8Half wh(w[b]);
+            F8Frag x[NT];
+            f4 part[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                F8Frag x;
                 if constexpr (FUSED) {
                     const uint8_t* const p = codes + (wave * SK_FUSED + min(r16, (int) a.N - 1)) * SK_PITCH + b * F8_BLOCK + chunk * 16;
-                    x.half[0] = *(const u4v*) p;
-                    x.half[1] = *(const u4v*) (p + 64);
+                    x[j].half[0] = *(const u4v*) p;
+                    x[j].half[1] = *(const u4v*) (p + 64);
                 } else {
                     const uint32_t at = (uint32_t) ((16 * j + r16) * a.x_nb1) + (4 * g + b) * F8_BLOCK + chunk * 16;
-                    x.half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 0, 0));
-                    x.half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at + 64, 0, 0));
+                    x[j].half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 0, 0));
+                    x[j].half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at + 64, 0, 0));
                 }
-                const f4 part = f8_dot(wh, F8Half(x));
+                part[j] = {0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const h8v wq = f8_half8(w[b].quarter[q]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wq, f8_half8(x[j].quarter[q]), part[j], 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
                 const float s = f8_scale((scale[j] >> (8 * b)) & 255u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[i] * s, ws, acc[j][i]);
+                for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[j][i] * s, ws[b], acc[j][i]);
             }
         }
         if constexpr (FUSED) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -11,249 +11,429 @@ struct F8Tiles {
     int steps;          // blocks of 128 summed over
     int part_steps;     // of one part of the sum, a multiple of 4 where there are several
     int tm, tn;         // tiles along rows and tokens
+    int whole;          // of an XCD's tiles: those that are not halved
     float* sums;        // several parts: their sums, [part][token][rows]; else null
     int64_t sums_nb1;   // floats from token to token
 };
 
 // FAST: the 8-bit matrix instruction, or binary16 with sums in 32 bits (fp8_mm.hip says when). POW2: the weight's
 // scales are bytes.
-template <int BM, int BN, int WM, int WN, bool TRANS, bool FAST, bool POW2>
+template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool FAST, bool POW2>
 void f8_tiles_launch(const F8Tiles& t, unsigned parts, hipStream_t s);
 
 namespace {
 
 constexpr uint32_t F8_RSRC = 0x00027000;
+constexpr int F8_TOUCHED = 256;  // bytes of LDS for what is loaded only to have it in the L2
 
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef int i2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i2v lds_i2v;
 
-// 16-byte chunks of a tile's row in LDS lie at slots chunk ^ f8_turn(row), so that eight rows' reads fall on
-// different banks. CH: chunks of a row.
-template <int CH>
+// 16-byte chunks of a tile's row in LDS lie at slots chunk ^ f8_turn(row), so that what is read together falls on
+// different banks (64 of 4 bytes). Rows of 128 bytes read 16 bytes a lane: eight rows, one chunk. A weight that is read
+// turned, 32 lanes at once: rows m to m + 7 and m + 16 to m + 23, 16 bytes of each (by rows of CH chunks; with row & 7
+// there every such read took two passes).
+template <bool TURNED, int CH>
 __device__ __forceinline__ int f8_turn(int row) {
-    return CH == 4 ? (row >> 1) & 3 : row & 7;
+    if (!TURNED) return row & 7;
+    if (CH == 16) return (row & 7) | ((row >> 4) & 1) << 3;
+    if (CH == 8) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
+    return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
 }
 
-// One operand's tile of a step, ROWS rows of 16 CH bytes, from memory to LDS without a way through registers: piece
-// p of a thread lands 16 THREADS bytes after piece p - 1, and the slots' turn is in the address it is read from.
-template <int ROWS, int CH, int THREADS>
+// One operand's tile of a step, ROWS rows of 16 CH bytes, from memory to LDS without a way through registers, in pieces of
+// 16 bytes a thread: piece p lands 16 THREADS bytes after piece p - 1, and the slots' turn is in the address it is read
+// from.
+template <int ROWS, int CH, int THREADS, bool TURNED>
 struct F8Slab {
     static constexpr int PIECES = ROWS * CH / THREADS, PER = THREADS / CH;  // rows of a piece
     static constexpr int BYTES = ROWS * CH * 16;
-    static_assert(PIECES * THREADS == ROWS * CH && PER % 8 == 0, "whole pieces, the same turn in each");
+    static_assert(PIECES * THREADS == ROWS * CH && PER % 32 == 0, "whole pieces, the same turn in each");
     uint32_t off;
     __device__ __forceinline__ F8Slab(int tid, int64_t nb1) {
         const int row = tid / CH, slot = tid % CH;
-        off = (uint32_t) (row * nb1) + (uint32_t) (slot ^ f8_turn<CH>(row)) * 16;
+        off = (uint32_t) (row * nb1) + (uint32_t) (slot ^ f8_turn<TURNED, CH>(row)) * 16;
     }
-    __device__ __forceinline__ void load(const uint8_t* base, int64_t bytes, int64_t nb1, lds_byte* lds, int wave) const {
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc((void*) base, (short) 0, (int) (uint32_t) bytes, F8_RSRC);
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*) (lds + (p * THREADS + wave * 64) * 16), 16, off,
-                                                     (uint32_t) (p * PER * nb1), 0, 0);
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int p, int64_t nb1, lds_byte* lds, int wave) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*) (lds + (p * THREADS + wave * 64) * 16), 16, off,
+                                                 (uint32_t) (p * PER * nb1), 0, 0);
     }
 };
 
-template <int BM, int BN, int WM, int WN, bool TRANS, bool FAST, bool POW2>
-__global__ __launch_bounds__(WM * WN * 64, 2) void k_f8_tiles(F8Tiles t) {
-    constexpr int THREADS = WM * WN * 64, TM = BM / WM, TN = BN / WN, IT = TM / 16, JT = TN / 16;
-    constexpr int ACH = TRANS ? BM / 16 : 8;
+// Waves of a SIMD: a workgroup's, twice where its stages leave room in LDS for another workgroup.
+constexpr int f8_waves(int bm, int bn, int waves, int stages) {
+    return (waves + 3) / 4 * (stages * ((bm + bn) * F8_BLOCK + 4 * bn) <= 80 * 1024 ? 2 : 1);
+}
+
+// A wave waits until `n` of its loads from memory at most are under way, and for its accesses to LDS.
+template <int N>
+__device__ __forceinline__ void f8_wait() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+}
+
+// A workgroup's tile: where it lies, its operands' way to LDS and from there, and its results' to memory.
+template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool POW2>
+struct F8Tile {
+    static constexpr int THREADS = WM * WN * 64, TM = BM / WM, TN = BN / WN, IT = TM / 16, JT = TN / 16;
+    static constexpr int ACH = TRANS ? BM / 16 : 8;
     static_assert(TM <= F8_BLOCK && F8_BLOCK % TM == 0, "a wave's rows share their scales");
-    typedef F8Slab<TRANS ? F8_BLOCK : BM, ACH, THREADS> ASlab;
-    typedef F8Slab<BN, 8, THREADS> BSlab;
-    __shared__ __attribute__((aligned(128))) uint8_t lds_all[2 * (ASlab::BYTES + BSlab::BYTES)];
-    lds_byte* const lds = (lds_byte*) lds_all;
+    typedef F8Slab<TRANS ? F8_BLOCK : BM, ACH, THREADS, TRANS> ASlab;
+    typedef F8Slab<BN, 8, THREADS, false> BSlab;
+    static constexpr int ACROSS = TRANS && BM > 128 ? BM / 128 : 1;  // lines of 128 bytes of a row in the weight's tile
+    static constexpr int ALINES = (TRANS ? F8_BLOCK : BM) * ACROSS;
+    static constexpr int STAGE = ASlab::BYTES + BSlab::BYTES + BN * 4, LOADS = ASlab::PIECES + BSlab::PIECES + 1;
 
-    const int per_xcd = (t.tm * t.tn + 7) / 8;
-    const int tile = (int) (blockIdx.x & 7) * per_xcd + (int) (blockIdx.x >> 3);
-    if (tile >= t.tm * t.tn) return;
-    // four tiles of rows by all of the tokens', then the next four: neighbours on an XCD share operands in its L2
-    const int in = tile % (4 * t.tn), first = tile / (4 * t.tn) * 4, high = min(4, t.tm - first);
-    const int64_t row0 = (int64_t) (first + in % high) * BM, n0 = (int64_t) (in / high) * BN;
+    const F8Tiles& t;
+    lds_byte* const lds;
+    const int lane, wave, wm, wn, r16, chunk;
+    int64_t row0, n0, a_rows, b_rows, pitch;
+    const ASlab slab_a;
+    const BSlab slab_b;
+    const uint8_t* x0;
+    __amdgpu_buffer_rsrc_t rs;  // the tokens' exponents, a word of four steps of each
+    uint32_t e_off, touch_off;
+    uint64_t ws;
+    int64_t ws_step;
 
-    const int tid = (int) threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave % WM, wn = wave / WM, r16 = lane & 15, chunk = lane >> 4;
-    const F8Args& a = t.a;
-    const int s0 = (int) blockIdx.y * t.part_steps, s1 = min(s0 + t.part_steps, t.steps);
-
-    const ASlab slab_a(tid, a.w_nb1);
-    const BSlab slab_b(tid, a.x_nb1);
-    const int64_t pitch = (a.K + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK;
-    const int64_t a_rows = min((int64_t) BM, a.M - row0), b_rows = min((int64_t) BN, a.N - n0);
-    const uint8_t* const x0 = a.x + n0 * a.x_nb1;
-    // rows past an operand are read as zeros (on the way back: the weight's last rows of a step)
-    auto load = [&](int s, int buf) {
-        lds_byte* const at = lds + buf * (ASlab::BYTES + BSlab::BYTES);
-        if constexpr (TRANS) {
-            const int64_t left = min((int64_t) F8_BLOCK, a.M - (int64_t) s * F8_BLOCK);
-            slab_a.load(a.w + (int64_t) s * F8_BLOCK * a.w_nb1 + row0, (left - 1) * a.w_nb1 + pitch - row0, a.w_nb1, at, wave);
-        } else {
-            slab_a.load(a.w + row0 * a.w_nb1 + (int64_t) s * F8_BLOCK, (a_rows - 1) * a.w_nb1 + F8_BLOCK, a.w_nb1, at, wave);
+    // tile: its number in a grid of tiles over `wide` tokens each, of which this takes BN, `part` times BN on
+    __device__ __forceinline__ F8Tile(const F8Tiles& tiles, uint8_t* shared, int tile, int wide, int part)
+        : t(tiles), lds((lds_byte*) shared), lane((int) threadIdx.x & 63),
+          wave(__builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6)), wm(wave % WM), wn(wave / WM), r16(lane & 15),
+          chunk(lane >> 4), slab_a((int) threadIdx.x, tiles.a.w_nb1), slab_b((int) threadIdx.x, tiles.a.x_nb1) {
+        const F8Args& a = t.a;
+        // four tiles of rows by all of the tokens', then the next four: neighbours on an XCD share operands in its L2
+        const int in = tile % (4 * t.tn), first = tile / (4 * t.tn) * 4, high = min(4, t.tm - first);
+        row0 = (int64_t) (first + in % high) * BM;
+        n0 = (int64_t) (in / high) * wide + part * BN;
+        pitch = (a.K + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK;
+        a_rows = min((int64_t) BM, a.M - row0);
+        b_rows = min((int64_t) BN, a.N - n0);
+        x0 = a.x + n0 * a.x_nb1;
+        rs = __builtin_amdgcn_make_buffer_rsrc((void*) (a.xs + n0 * a.xs_nb1), (short) 0,
+                                               (int) ((b_rows - 1) * a.xs_nb1 + (t.steps + 3) / 4 * 4), F8_RSRC);
+        e_off = (uint32_t) (((int) threadIdx.x % BN) * a.xs_nb1);
+        // The lines of a later step that this workgroup brings into the XCD's L2: its share of what it has in common with
+        // its neighbours there.
+        const int sa = min(8, t.tn), sb = min(4, high), tid = (int) threadIdx.x;
+        touch_off = 0xFFFFFF00u;
+        if (tid < ALINES) {
+            if (tid * sa / ALINES == in / high % sa)
+                touch_off = (uint32_t) (tid / ACROSS * a.w_nb1) + tid % ACROSS * 128;
+        } else if (tid - ALINES < BN) {
+            if ((tid - ALINES) * sb / BN == in % high % sb) touch_off = (uint32_t) ((tid - ALINES) * a.x_nb1);
         }
-        slab_b.load(x0 + (int64_t) s * F8_BLOCK, (b_rows - 1) * a.x_nb1 + F8_BLOCK, a.x_nb1, at + ASlab::BYTES, wave);
+        const int64_t rb = min((row0 + wm * TM) / F8_BLOCK, (t.rows - 1) / F8_BLOCK);
+        ws = (uint64_t) (a.ws + (TRANS ? rb * (POW2 ? 1 : 4) : rb * a.ws_nb1));
+        ws_step = TRANS ? a.ws_nb1 : (POW2 ? 1 : 4);
+    }
+    // Where a step's tiles lie. Rows past an operand are read as zeros (on the way back: the weight's last rows of a step),
+    // and so is all of a step from `end` on: what is loaded ahead needs no branch.
+    struct Source {
+        __amdgpu_buffer_rsrc_t a, b;
+        int word;
     };
-    // the tokens' exponents, four steps in a word
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*) (a.xs + n0 * a.xs_nb1), (short) 0, (int) ((b_rows - 1) * a.xs_nb1 + (t.steps + 3) / 4 * 4), F8_RSRC);
-    uint32_t exps[JT], more[JT];
-    auto load_exps = [&](int s) {
+    __device__ __forceinline__ Source source(int s, int end) const {
+        const F8Args& g = t.a;
+        const bool some = s < end;
+        s = min(s, end - 1);
+        const uint8_t* const w = TRANS ? g.w + (int64_t) s * F8_BLOCK * g.w_nb1 + row0 : g.w + row0 * g.w_nb1 + (int64_t) s * F8_BLOCK;
+        const int64_t left = TRANS ? min((int64_t) F8_BLOCK, g.M - (int64_t) s * F8_BLOCK) : a_rows, width = TRANS ? pitch - row0 : F8_BLOCK;
+        return {__builtin_amdgcn_make_buffer_rsrc((void*) w, (short) 0, some ? (int) (uint32_t) ((left - 1) * g.w_nb1 + width) : 0, F8_RSRC),
+                __builtin_amdgcn_make_buffer_rsrc((void*) (x0 + (int64_t) s * F8_BLOCK), (short) 0,
+                                                  some ? (int) (uint32_t) ((b_rows - 1) * g.x_nb1 + F8_BLOCK) : 0, F8_RSRC),
+                s & ~3};
+    }
+    // piece p of LOADS on its way to a stage
+    __device__ __forceinline__ void load(const Source& from, int stage, int p) const {
+        lds_byte* const at = lds + stage * STAGE;
+        if (p < ASlab::PIECES) slab_a.load(from.a, p, t.a.w_nb1, at, wave);
+        else if (p < LOADS - 1) slab_b.load(from.b, p - ASlab::PIECES, t.a.x_nb1, at + ASlab::BYTES, wave);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rs, (__attribute__((address_space(3))) void*) (at + ASlab::BYTES + BSlab::BYTES + (wave * 64 % BN) * 4), 4, e_off, from.word, 0, 0);
+    }
+    __device__ __forceinline__ void touch(const Source& from) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wave * 64 < ALINES ? from.a : from.b, (__attribute__((address_space(3))) void*) (lds + 2 * STAGE), 4,
+                                                 touch_off, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(int s, int stage) const {
+        const Source from = source(s, s + 1);
 #pragma unroll
-        for (int j = 0; j < JT; ++j)
-            more[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, (uint32_t) ((wn * TN + j * 16 + r16) * a.xs_nb1) + s, 0, 0);
-    };
-    // the weight's scale of a step
-    const int64_t rb = min((row0 + wm * TM) / F8_BLOCK, (t.rows - 1) / F8_BLOCK);
-    const uint8_t* ws = a.ws + (TRANS ? rb * (POW2 ? 1 : 4) : rb * a.ws_nb1);
-    const int64_t ws_step = TRANS ? a.ws_nb1 : (POW2 ? 1 : 4);
+        for (int p = 0; p < LOADS; ++p) load(from, stage, p);
+    }
+    // the weight's scale of a step, by the scalar unit
+    __device__ __forceinline__ uint32_t scale(int s) const {
+        typedef const __attribute__((address_space(4))) uint32_t scalar_word;
+        const uint64_t at = ws + (uint64_t) (s * ws_step);
+        const uint32_t word = *(scalar_word*) (at & ~(uint64_t) 3);
+        return POW2 ? word >> (8 * (at & 3)) & 255u : word;
+    }
+    __device__ __forceinline__ F8Frag rows_of(const lds_byte* base, int row) const {
+        F8Frag f;
+        const lds_byte* const p = base + row * 128;
+        const int turn = f8_turn<false, 8>(row);
+        f.half[0] = *(const __attribute__((address_space(3))) u4v*) (p + ((chunk ^ turn) * 16));
+        f.half[1] = *(const __attribute__((address_space(3))) u4v*) (p + (((chunk + 4) ^ turn) * 16));
+        return f;
+    }
+    // Fragment i of the weight. Turned: eight of its rows by 16 of its columns at a time; lane l of 16 gives the address of
+    // half a row and gets a column.
+    __device__ __forceinline__ F8Frag weight(int stage, int i) const {
+        const lds_byte* const base = lds + stage * STAGE;
+        if constexpr (!TRANS) return rows_of(base, wm * TM + i * 16 + r16);
+        F8Frag f;
+        const int col = (wm * TM + i * 16) >> 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int m = 16 * chunk + 8 * (q & 1) + 64 * (q >> 1) + (r16 >> 1);
+            const lds_byte* const p = base + m * BM + ((col ^ f8_turn<true, ACH>(m)) * 16) + (r16 & 1) * 8;
+            f.quarter[q] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2v*) p));
+        }
+        return f;
+    }
+    __device__ __forceinline__ F8Frag token(int stage, int j) const {
+        return rows_of(lds + stage * STAGE + ASlab::BYTES, wn * TN + j * 16 + r16);
+    }
+    __device__ __forceinline__ uint32_t exponent(int s, int stage, int j) const {
+        const lds_byte* const p = lds + stage * STAGE + ASlab::BYTES + BSlab::BYTES;
+        return ((const __attribute__((address_space(3))) uint32_t*) p)[wn * TN + j * 16 + r16] >> (8 * (s & 3)) & 255u;
+    }
+    // a lane holds four neighbouring rows of one token
+    __device__ __forceinline__ void store(const f4 (&acc)[IT][JT]) const {
+        const F8Args& a = t.a;
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+            const int64_t n = n0 + wn * TN + j * 16 + r16;
+            if (n >= a.N) continue;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int64_t r = row0 + wm * TM + i * 16 + chunk * 4;
+                if (r >= t.rows) continue;
+                const int left = (int) min((int64_t) 4, t.rows - r);
+                if (t.sums != nullptr || a.y_type == TRC_HIP_TYPE_F32) {
+                    float* const p = t.sums != nullptr ? t.sums + ((int64_t) blockIdx.y * a.N + n) * t.sums_nb1 + r
+                                                       : (float*) (a.y + n * a.y_nb1) + r;
+                    if (left == 4) *(f4a4*) p = acc[i][j];
+                    else
+                        for (int k = 0; k < left; ++k) p[k] = acc[i][j][k];
+                } else {
+                    uint16_t* const p = (uint16_t*) (a.y + n * a.y_nb1) + r;
+                    uint16_t v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = f8_bits(a.y_type, acc[i][j][k]);
+                    if (left == 4) {
+                        typedef uint32_t u2a2 __attribute__((ext_vector_type(2), aligned(2)));
+                        *(u2a2*) p = (u2a2){(uint32_t) v[0] | (uint32_t) v[1] << 16, (uint32_t) v[2] | (uint32_t) v[3] << 16};
+                    } else {
+                        for (int k = 0; k < left; ++k) p[k] = v[k];
+                    }
+                }
+            }
+        }
+    }
+};
 
+// Products in binary16.
+template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool POW2>
+__device__ __forceinline__ void f8_exact(const F8Tiles& t, uint8_t* shared, int tile, int wide, int part) {
+    typedef F8Tile<BM, BN, WM, WN, STAGES, TRANS, POW2> Tile;
+    // (pieces from memory at once: all of them in the first two rounds of products)
+    constexpr int IT = Tile::IT, JT = Tile::JT, EACH = (Tile::LOADS + 1) / 2;
+    const Tile w(t, shared, tile, wide, part);
+    if (w.n0 >= t.a.N) return;
+    const int s0 = (int) blockIdx.y * t.part_steps, s1 = min(s0 + t.part_steps, t.steps);
     f4 acc[IT][JT];
 #pragma unroll
     for (int i = 0; i < IT; ++i)
 #pragma unroll
         for (int j = 0; j < JT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
-
-    // (loaded a step ahead and taken after the wait below, so that the loads to LDS are waited for there only)
-    uint32_t wbits, wnext = 0;
-    auto load_ws = [&](int s) {
-        if constexpr (POW2) wnext = ws[s * ws_step];
-        else wnext = *(const uint32_t*) (ws + s * ws_step);
-    };
-    if (s0 < s1) {
-        load_exps(s0);
-        load_ws(s0);
-        load(s0, 0);
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) {
+        const typename Tile::Source from = w.source(s0 + k, s1);
+#pragma unroll
+        for (int p = 0; p < Tile::LOADS; ++p) w.load(from, k, p);
     }
+    uint32_t wnext = w.scale(s0);
+    int stage = 0;
     for (int s = s0; s < s1; ++s) {
-        // this step's tiles have landed, and every wave has read the last one's
-        __builtin_amdgcn_s_waitcnt(0);
+        // this step's tiles have landed (the next STAGES - 2 may not have), and every wave has read the last step's
+        f8_wait<Tile::LOADS * (STAGES - 2)>();
         __builtin_amdgcn_s_barrier();
-        const int buf = (s - s0) & 1;
-        if ((s & 3) == 0 || s == s0) {
+        const float wscale = POW2 ? f8_scale(wnext) : __builtin_bit_cast(float, wnext);
+        if (s + 1 < s1) wnext = w.scale(s + 1);
+        const typename Tile::Source from = w.source(s + STAGES - 1, s1);
+        const int into = stage == 0 ? STAGES - 1 : stage - 1;
+        h8v wh[IT][4], x[4];
+        auto half = [](const F8Frag& f, h8v (&h)[4]) {
 #pragma unroll
-            for (int j = 0; j < JT; ++j) exps[j] = more[j] >> (8 * (s & 3));
-            if ((s | 3) + 1 < s1) load_exps((s | 3) + 1);
-        } else {
-#pragma unroll
-            for (int j = 0; j < JT; ++j) exps[j] >>= 8;
-        }
-        wbits = wnext;
-        if (s + 1 < s1) {
-            load_ws(s + 1);
-            load(s + 1, buf ^ 1);
-        }
-
-        const lds_byte* const la = lds + buf * (ASlab::BYTES + BSlab::BYTES);
-        const lds_byte* const lb = la + ASlab::BYTES;
-        auto read = [&](const lds_byte* base, int row) {
-            F8Frag f;
-            const lds_byte* const p = base + row * 128;
-            f.half[0] = *(const __attribute__((address_space(3))) u4v*) (p + ((chunk ^ f8_turn<8>(row)) * 16));
-            f.half[1] = *(const __attribute__((address_space(3))) u4v*) (p + (((chunk + 4) ^ f8_turn<8>(row)) * 16));
-            return f;
+            for (int q = 0; q < 4; ++q) h[q] = f8_half8(f.quarter[q]);
         };
-        // The weight turned: eight of its rows by 16 of its columns at a time. Lane l of 16 gives the address of half
-        // a row and gets a column.
-        auto read_turned = [&](int col) {
-            F8Frag f;
-            const int half = r16 >> 1;
+        half(w.token(stage, 0), x);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int m = 16 * chunk + 8 * (q & 1) + 64 * (q >> 1) + half;
-                const lds_byte* const p = la + m * BM + (((col >> 4) ^ f8_turn<ACH>(m)) * 16) + (r16 & 1) * 8;
-                f.quarter[q] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2v*) p));
-            }
-            return f;
+        for (int i = 0; i < IT; ++i) half(w.weight(stage, i), wh[i]);
+        f4 part[2][IT];
+        float scale[2];
+        auto add = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(part[j & 1][i][k], scale[j & 1], acc[i][j][k]);
         };
-        if constexpr (FAST) {
-            F8Frag b[JT];
 #pragma unroll
-            for (int j = 0; j < JT; ++j) b[j] = read(lb, wn * TN + j * 16 + r16);
+        for (int j = 0; j < JT; ++j) {
+            h8v next[4];
+            scale[j & 1] = f8_scale(w.exponent(s, stage, j)) * wscale;
 #pragma unroll
-            for (int i = 0; i < IT; ++i) {
-                F8Frag f;
-                if constexpr (TRANS) f = read_turned(wm * TM + i * 16);
-                else f = read(la, wm * TM + i * 16 + r16);
-#pragma unroll
-                for (int j = 0; j < JT; ++j) {
-                    if constexpr (POW2) {
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.all, b[j].all, acc[i][j], 0, 0, 0, (int) wbits, 0,
-                                                                                    (int) exps[j]);
-                    } else {
-                        const f4 zero = {0.f, 0.f, 0.f, 0.f};
-                        const f4 part =
-                            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.all, b[j].all, zero, 0, 0, 0, 127, 0, (int) exps[j]);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            acc[i][j][k] = fmaf(part[k], __builtin_bit_cast(float, wbits), acc[i][j][k]);
-                    }
-                }
-            }
-        } else {
-            const float wscale = POW2 ? f8_scale(wbits) : __builtin_bit_cast(float, wbits);
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-                const F8Half b(read(lb, wn * TN + j * 16 + r16));
-                const float scale = f8_scale(exps[j] & 255u);
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int i = 0; i < IT; ++i) {
-                    F8Frag f;
-                    if constexpr (TRANS) f = read_turned(wm * TM + i * 16);
-                    else f = read(la, wm * TM + i * 16 + r16);
-                    const f4 part = f8_dot(F8Half(f), b);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(part[k] * scale, wscale, acc[i][j][k]);
+                    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+                    part[j & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[i][q], x[q], q == 0 ? zero : part[j & 1][i], 0, 0, 0);
                 }
+            if (j + 1 < JT) half(w.token(stage, j + 1), next);
+            if (j > 0) add(j - 1);
+#pragma unroll
+            for (int p = j * EACH; p < (j + 1) * EACH && p < Tile::LOADS; ++p) w.load(from, into, p);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = next[q];
+        }
+        add(JT - 1);
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+    f8_wait<0>();  // (what was loaded ahead: zeros, to LDS that another workgroup may have next)
+    w.store(acc);
+}
+
+// Products on the 8-bit instruction, two stages. The barrier comes before a step's last two rows of fragments are
+// multiplied: meanwhile the next step's first two come from LDS, each token's fragment as soon as the last product with the
+// one whose registers it takes is under way. The step after that comes from memory from then on, a piece after every
+// second product: all at once, a wave's products would wait until the loads before them have been taken.
+template <int BM, int BN, int WM, int WN, bool TRANS, bool POW2>
+__device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int tile, int wide, int part) {
+    typedef F8Tile<BM, BN, WM, WN, 2, TRANS, POW2> Tile;
+    constexpr int IT = Tile::IT, JT = Tile::JT;
+    const Tile w(t, shared, tile, wide, part);
+    if (w.n0 >= t.a.N) return;
+    const int s0 = (int) blockIdx.y * t.part_steps, s1 = min(s0 + t.part_steps, t.steps);
+    f4 acc[IT][JT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int j = 0; j < JT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+    // pieces loaded between the barrier and the next step, the others' distance there in products
+    constexpr int ROOM = (IT - 2) * JT, EARLY = ROOM < Tile::LOADS - JT ? Tile::LOADS : JT < Tile::LOADS ? JT : Tile::LOADS;
+    constexpr int AHEAD = 3;
+    constexpr int EVERY = ROOM >= 4 * (Tile::LOADS - EARLY) ? 2 : 1;
+    F8Frag token[JT], a[2];
+    uint32_t exps[JT], scale = 0;
+    auto multiply = [&](int i, int j, const F8Frag& f) {
+        if constexpr (POW2) {
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.all, token[j].all, acc[i][j], 0, 0, 0, (int) scale, 0, (int) exps[j]);
+        } else {
+            const f4 zero = {0.f, 0.f, 0.f, 0.f};
+            const f4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.all, token[j].all, zero, 0, 0, 0, 127, 0, (int) exps[j]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(part[k], __builtin_bit_cast(float, scale), acc[i][j][k]);
+        }
+    };
+    if (s0 < s1) {
+        w.load(s0, 0);
+        typename Tile::Source from = w.source(s0 + 1, s1);
+        f8_wait<0>();
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int p = 0; p < EARLY; ++p) w.load(from, 1, p);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = w.weight(0, i);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+            token[j] = w.token(0, j);
+            exps[j] = w.exponent(s0, 0, j);
+        }
+        scale = w.scale(s0);
+        int stage = 0;
+        for (int s = s0; s < s1; ++s) {
+            // the pieces of the next step that were not loaded after the barrier
+            int piece = EARLY;
+#pragma unroll
+            for (int i = 0; i + 2 < IT; i += 2) {
+                const F8Frag b[2] = {w.weight(stage, i + 2), w.weight(stage, i + 3)};
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int j = 0; j < JT; ++j) {
+                        multiply(i + k, j, a[k]);
+                        if (((k * JT + j) % EVERY) == EVERY - 1 && piece < Tile::LOADS) {
+                            w.load(from, stage ^ 1, piece);
+                            ++piece;
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                a[0] = b[0], a[1] = b[1];
             }
+            // this wave has read all of the step's stage, and its share of the next one has landed
+            w.touch(w.source(s + AHEAD, s1));
+            __builtin_amdgcn_sched_barrier(0);
+            f8_wait<1>();
+            __builtin_amdgcn_s_barrier();
+            from = w.source(s + 2, s1);
+            const int n = min(s + 1, s1 - 1);  // (past the last step what is there is read, and not used)
+            const F8Frag next[2] = {w.weight(stage ^ 1, 0), w.weight(stage ^ 1, 1)};
+            const uint32_t scale_next = w.scale(n);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+                multiply(IT - 2, j, a[0]);
+                multiply(IT - 1, j, a[1]);
+                token[j] = w.token(stage ^ 1, j);
+                exps[j] = w.exponent(n, stage ^ 1, j);
+                if (j < EARLY) w.load(from, stage, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int p = JT; p < EARLY; ++p) w.load(from, stage, p);
+            stage ^= 1;
+            a[0] = next[0], a[1] = next[1];
+            scale = scale_next;
         }
     }
+    f8_wait<0>();  // (what was loaded ahead: zeros, to LDS that another workgroup may have next)
+    w.store(acc);
+}
 
-    // a lane holds four neighbouring rows of one token
-#pragma unroll
-    for (int j = 0; j < JT; ++j) {
-        const int64_t n = n0 + wn * TN + j * 16 + r16;
-        if (n >= a.N) continue;
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int64_t r = row0 + wm * TM + i * 16 + chunk * 4;
-            if (r >= t.rows) continue;
-            const int left = (int) min((int64_t) 4, t.rows - r);
-            if (t.sums != nullptr || a.y_type == TRC_HIP_TYPE_F32) {
-                float* const p = t.sums != nullptr ? t.sums + ((int64_t) blockIdx.y * a.N + n) * t.sums_nb1 + r
-                                                   : (float*) (a.y + n * a.y_nb1) + r;
-                if (left == 4) *(f4a4*) p = acc[i][j];
-                else
-                    for (int k = 0; k < left; ++k) p[k] = acc[i][j][k];
-            } else {
-                uint16_t* const p = (uint16_t*) (a.y + n * a.y_nb1) + r;
-                uint16_t v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = f8_bits(a.y_type, acc[i][j][k]);
-                if (left == 4) {
-                    typedef uint32_t u2a2 __attribute__((ext_vector_type(2), aligned(2)));
-                    *(u2a2*) p = (u2a2){(uint32_t) v[0] | (uint32_t) v[1] << 16, (uint32_t) v[2] | (uint32_t) v[3] << 16};
-                } else {
-                    for (int k = 0; k < left; ++k) p[k] = v[k];
-                }
-            }
+// An XCD (workgroup b is on XCD b % 8) takes neighbouring tiles: t.whole as they are and the rest, the last round
+// of its CUs where that is half of one or less, in two halves of the tokens by a workgroup each.
+template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool FAST, bool POW2>
+__global__ __launch_bounds__(WM * WN * 64, f8_waves(BM, BN, WM * WN, STAGES)) void k_f8_tiles(F8Tiles t) {
+    __shared__ __attribute__((aligned(128))) uint8_t
+        shared[STAGES * F8Tile<BM, BN, WM, WN, STAGES, TRANS, POW2>::STAGE + (FAST ? F8_TOUCHED : 0)];
+    const int per_xcd = (t.tm * t.tn + 7) / 8, at = (int) (blockIdx.x >> 3);
+    const int tile = (int) (blockIdx.x & 7) * per_xcd + (at < t.whole ? at : t.whole + (at - t.whole) / 2);
+    if (tile >= t.tm * t.tn) return;
+    if constexpr (FAST) {
+        if constexpr (BN == 256) {
+            if (at >= t.whole) return f8_fast<BM, BN / 2, WM, WN, TRANS, POW2>(t, shared, tile, BN, (at - t.whole) & 1);
         }
+        f8_fast<BM, BN, WM, WN, TRANS, POW2>(t, shared, tile, BN, 0);
+    } else {
+        f8_exact<BM, BN, WM, WN, STAGES, TRANS, POW2>(t, shared, tile, BN, 0);
     }
 }
 
 }  // namespace
 
-#define F8_INSTANCE(BM, BN, WM, WN, TRANS, FAST, POW2)                                                                \
-    template <>                                                                                                       \
-    void f8_tiles_launch<BM, BN, WM, WN, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s) {        \
-        hipLaunchKernelGGL((k_f8_tiles<BM, BN, WM, WN, TRANS, FAST, POW2>), dim3((unsigned) ((t.tm * t.tn + 7) / 8 * 8), parts), \
-                           dim3(WM * WN * 64), 0, s, t);                                                              \
+#define F8_INSTANCE(BM, BN, WM, WN, STAGES, TRANS, FAST, POW2)                                                         \
+    template <>                                                                                                        \
+    void f8_tiles_launch<BM, BN, WM, WN, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s) { \
+        hipLaunchKernelGGL((k_f8_tiles<BM, BN, WM, WN, STAGES, TRANS, FAST, POW2>),                                    \
+                           dim3((unsigned) (8 * (2 * ((t.tm * t.tn + 7) / 8) - t.whole)), parts), dim3(WM * WN * 64), 0, s, t); \
     }
-#define F8_INSTANCES(BM, BN, WM, WN, FAST)          \
-    F8_INSTANCE(BM, BN, WM, WN, false, FAST, false) \
-    F8_INSTANCE(BM, BN, WM, WN, false, FAST, true)  \
-    F8_INSTANCE(BM, BN, WM, WN, true, FAST, false)  \
-    F8_INSTANCE(BM, BN, WM, WN, true, FAST, true)
+#define F8_INSTANCES(BM, BN, WM, WN, STAGES, FAST)          \
+    F8_INSTANCE(BM, BN, WM, WN, STAGES, false, FAST, false) \
+    F8_INSTANCE(BM, BN, WM, WN, STAGES, false, FAST, true)  \
+    F8_INSTANCE(BM, BN, WM, WN, STAGES, true, FAST, false)  \
+    F8_INSTANCE(BM, BN, WM, WN, STAGES, true, FAST, true)
 
 }  // namespace trc_hip

@@ -7,19 +7,20 @@
 
 namespace trc_hip {
 
-#define F8_DECLARE(BM, BN, WM, WN, TRANS, FAST, POW2) \
-    template <>                                       \
-    void f8_tiles_launch<BM, BN, WM, WN, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
-#define F8_DECLARE_ALL(BM, BN, WM, WN, FAST)       \
-    F8_DECLARE(BM, BN, WM, WN, false, FAST, false) \
-    F8_DECLARE(BM, BN, WM, WN, false, FAST, true)  \
-    F8_DECLARE(BM, BN, WM, WN, true, FAST, false)  \
-    F8_DECLARE(BM, BN, WM, WN, true, FAST, true)
-F8_DECLARE_ALL(256, 256, 2, 4, true)
-F8_DECLARE_ALL(128, 128, 2, 2, true)
-F8_DECLARE_ALL(128, 128, 2, 2, false)
-F8_DECLARE_ALL(64, 64, 2, 2, true)
-F8_DECLARE_ALL(64, 64, 2, 2, false)
+#define F8_DECLARE(BM, BN, WM, WN, STAGES, TRANS, FAST, POW2) \
+    template <>                                               \
+    void f8_tiles_launch<BM, BN, WM, WN, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
+#define F8_DECLARE_ALL(BM, BN, WM, WN, STAGES, FAST)       \
+    F8_DECLARE(BM, BN, WM, WN, STAGES, false, FAST, false) \
+    F8_DECLARE(BM, BN, WM, WN, STAGES, false, FAST, true)  \
+    F8_DECLARE(BM, BN, WM, WN, STAGES, true, FAST, false)  \
+    F8_DECLARE(BM, BN, WM, WN, STAGES, true, FAST, true)
+
+F8_DECLARE_ALL(256, 256, 2, 4, 2, true)
+F8_DECLARE_ALL(128, 128, 2, 2, 2, true)
+F8_DECLARE_ALL(128, 128, 2, 2, 2, false)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, true)
+F8_DECLARE_ALL(64, 64, 2, 2, 3, false)
 
 namespace {
 
@@ -40,11 +41,13 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_f8_join(const float* __restric
     }
 }
 
-template <int BM, int BN, int WM, int WN, bool FAST>
+template <int BM, int BN, int WM, int WN, int STAGES, bool FAST>
 void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
     const bool pow2 = !t.a.ws_float;
-    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, true, FAST, true> : f8_tiles_launch<BM, BN, WM, WN, true, FAST, false>)
-                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, false, FAST, true> : f8_tiles_launch<BM, BN, WM, WN, false, FAST, false>);
+    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, STAGES, true, FAST, true>
+                                  : f8_tiles_launch<BM, BN, WM, WN, STAGES, true, FAST, false>)
+                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, STAGES, false, FAST, true>
+                                  : f8_tiles_launch<BM, BN, WM, WN, STAGES, false, FAST, false>);
     f(t, parts, s);
 }
 
@@ -57,11 +60,14 @@ int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s) {
     t.steps = (int) (((trans ? a.M : a.K) + F8_BLOCK - 1) / F8_BLOCK);
     const bool fast = a.y_type != TRC_HIP_TYPE_F32;
     const int64_t cus = device_cus();
-    auto tiles = [&](int64_t b) { return ((t.rows + b - 1) / b) * ((a.N + b - 1) / b); };
+    auto tiles = [&](int64_t edge) { return ((t.rows + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
     const int edge = fast && tiles(256) >= cus ? 256 : tiles(128) >= cus ? 128 : 64;
-    if (tiles(edge) > max_groups(512) - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
+    if (tiles(edge) > max_groups(512) / 2 - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
     t.tm = (int) ((t.rows + edge - 1) / edge);
     t.tn = (int) ((a.N + edge - 1) / edge);
+    t.whole = (t.tm * t.tn + 7) / 8;
+    const int per_xcd = (int) (cus / 8), last = edge == 256 && per_xcd > 0 ? t.whole % per_xcd : 0;
+    if (last * 2 <= per_xcd) t.whole -= last;
     // few tiles: the sum in parts
     int64_t parts = 1;
     if (edge == 64 && tiles(64) * 2 <= cus) {
@@ -84,9 +90,9 @@ int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s) {
         t.sums = (float*) ws;
     }
     const unsigned p = (unsigned) parts;
-    if (edge == 256) launch<256, 256, 2, 4, true>(t, trans, p, s);
-    else if (edge == 128) fast ? launch<128, 128, 2, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, false>(t, trans, p, s);
-    else fast ? launch<64, 64, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, false>(t, trans, p, s);
+    if (edge == 256) launch<256, 256, 2, 4, 2, true>(t, trans, p, s);
+    else if (edge == 128) fast ? launch<128, 128, 2, 2, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, 2, false>(t, trans, p, s);
+    else fast ? launch<64, 64, 2, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, 3, false>(t, trans, p, s);
     const int rc = check_launch("fp8_mul_mat");
     if (rc != TRC_HIP_OK || parts == 1) return rc;
     const int64_t quads = t.sums_nb1 / 4;

@@ -1,7 +1,7 @@
-// Tiles of 128 x 128 (fp8_mm.h), 4 waves of 64 rows by 64 tokens.
+// Tiles of 128 rows (fp8_mm.h).
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(128, 128, 2, 2, true)
-F8_INSTANCES(128, 128, 2, 2, false)
+F8_INSTANCES(128, 128, 2, 2, 2, true)
+F8_INSTANCES(128, 128, 2, 2, 2, false)
 }  // namespace trc_hip

@@ -1,6 +1,6 @@
-// Tiles of 256 x 256 (fp8_mm.h), 8 waves of 128 rows by 64 tokens.
+// Tiles of 256 rows (fp8_mm.h).
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(256, 256, 2, 4, true)
+F8_INSTANCES(256, 256, 2, 4, 2, true)
 }  // namespace trc_hip
