@@ -249,6 +249,27 @@ def test_matvec(hip, kind, xkind, K, M, N):
             b.free()
 
 
+@pytest.mark.parametrize("K,M,N", [(5000, 100, 1), (14336, 48, 2), (30000, 20, 1), (30000, 33, 2), (4096, 4104, 50), (4096, 4104, 64),
+                                   (2048, 14340, 20)])
+def test_matvec_of_long_rows_and_large_weights(hip, K, M, N):
+    """Several groups of K a wave, activations that do not fit LDS, tiles in parts for few tokens: as above, bit for bit."""
+    announce(f"fp8 matvec K={K} M={M} N={N}")
+    w, ws, x, xs = problem(K, M, N, "float", K + M + N, whole=True)
+    p = Product(w, ws, x, xs, K, M, "f32")
+    p.run()
+    assert np.array_equal(p.read(), p.want()[0].astype(np.float32))
+    rng = np.random.default_rng(N)
+    raw = rng.standard_normal((N, K)).astype(np.float32)
+    m, y = Mat(raw), Mat(np.zeros((N, M), np.float32))
+    H.fp8_quantize(m.t, p.x.t)
+    p.run()
+    H.fp8_matvec(p.w.t, m.t, y.t)
+    H.sync()
+    assert np.array_equal(y.read(), p.read())
+    for b in (p, m, y):
+        b.free()
+
+
 def test_values_that_are_not_finite(hip):
     """A NaN of a token reaches every result of that token and no other; one of the weight every token's result of its row."""
     announce("fp8 not finite")

@@ -770,8 +770,7 @@ int fp8_product(const char* who, const trc_hip_fp8* w, const trc_hip_fp8* x, con
     a.x_nb1 = (int64_t) x->q.nb[1];
     a.xs = (const uint8_t*) x->scale.data;
     a.xs_nb1 = (int64_t) x->scale.nb[1];
-    if (!back && N <= TRC_HIP_FP8_MATVEC_MAX_N) return launch_f8_skinny(a, nullptr, s);
-    return launch_f8_tiles(a, back, s);
+    return launch_f8_product(a, back, 0, s);
 }
 
 }  // namespace
@@ -823,7 +822,7 @@ int trc_hip_fp8_matvec(const trc_hip_fp8* w, const trc_hip_tensor* x, const trc_
     TRC_TRY(check_shape(who, "x", x, x->type, K, N, 1, false));
     TRC_TRY(check_fp8_out(who, "y", y, M, N, w));
     TRC_TRY(check_apart(who, y, "y", x, "x", false));
-    return launch_f8_skinny(fp8_args(*w, *y, N), x, (hipStream_t) stream);
+    return launch_f8_matvec(fp8_args(*w, *y, N), *x, (hipStream_t) stream);
 }
 
 }  // extern "C"

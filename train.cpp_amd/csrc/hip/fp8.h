@@ -151,10 +151,13 @@ struct F8Args {
     int64_t y_nb1;
     int y_type;
 };
-// fp8.hip
+// fp8.hip: the quantizer; the products of few tokens that are still floats; those of up to 64 in 8 bits, without a
+// workspace
 int launch_f8_quantize(const trc_hip_tensor& x, const trc_hip_fp8& q, hipStream_t s);
-int launch_f8_skinny(const F8Args& a, const trc_hip_tensor* x, hipStream_t s);
-// fp8_mm.hip
-int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s);
+int launch_f8_matvec(const F8Args& a, const trc_hip_tensor& x, hipStream_t s);
+int launch_f8_skinny(const F8Args& a, hipStream_t s);
+// fp8_mm.hip: W x, or W^T x with `back`, of operands in 8 bits. The first `used` bytes of the stream's workspace are
+// the caller's.
+int launch_f8_product(const F8Args& a, bool back, size_t used, hipStream_t s);
 
 }  // namespace trc_hip

@@ -68,113 +68,209 @@ __global__ __launch_bounds__(Q_THREADS) void k_f8_blocks(const uint8_t* __restri
     if (threadIdx.x == 0) sc[bj * sc_nb1 + bi] = (uint8_t) e;
 }
 
-constexpr int SK_WAVES = 8;
-constexpr int SK_FUSED = 4;             // tokens whose activations a wave quantizes for itself
-constexpr int SK_PITCH = 512 + 16;      // of their codes in LDS: 8 rows' 16 bytes fall on different banks
+constexpr int SK_WAVES = 16;            // most of a workgroup
+constexpr int SK_FUSED = 2;             // tokens whose activations a workgroup quantizes for itself
+constexpr int SK_LDS = 48 * 1024;       // most bytes that it keeps of them (three workgroups fit a CU)
 constexpr uint32_t SK_RSRC = 0x00027000;
 
-// Up to 16 NT tokens: a workgroup takes 16 of the weight's rows, its waves share K out in groups of four blocks and
-// join their sums in LDS. The weight goes from memory to registers; bound by its bytes, of which as many are under way as
-// waves fit a CU: they are held to few registers, operands turned to binary16 a quarter at a time.
-// FUSED: x holds floats (of type XTYPE), and every wave quantizes what it multiplies: N <= SK_FUSED.
-template <int NT, int XTYPE>
-__global__ __launch_bounds__(SK_WAVES * 64, NT == 1 ? 6 : 4) void k_f8_skinny(F8Args a, const uint8_t* __restrict__ xf, size_t xf_nb1) {
-    constexpr bool FUSED = XTYPE >= 0;
-    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6, waves = (int) blockDim.x >> 6;
-    const int r16 = lane & 15, chunk = lane >> 4;
-    const int64_t row0 = (int64_t) blockIdx.x * 16;
-    const int kb = (int) ((a.K + F8_BLOCK - 1) / F8_BLOCK), groups = (kb + 3) / 4;
-    const int rows = (int) min((int64_t) 16, a.M - row0);
-    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
-        (void*) (a.w + row0 * a.w_nb1), (short) 0, (int) ((rows - 1) * a.w_nb1 + (int64_t) kb * F8_BLOCK), SK_RSRC);
-    const uint32_t w_off = (uint32_t) (r16 * a.w_nb1) + chunk * 16;
-    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
-        (void*) a.x, (short) 0, FUSED ? 0 : (int) ((a.N - 1) * a.x_nb1 + (int64_t) kb * F8_BLOCK), SK_RSRC);
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*) a.xs, (short) 0, FUSED ? 0 : (int) ((a.N - 1) * a.xs_nb1 + (int64_t) groups * 4), SK_RSRC);
-    __shared__ __attribute__((aligned(16))) uint8_t codes[FUSED ? SK_WAVES * SK_FUSED * SK_PITCH : 16];
-    __shared__ uint32_t words[FUSED ? SK_WAVES * SK_FUSED : 1];
-    __shared__ __attribute__((aligned(16))) float red[SK_WAVES * 16 * NT * 16];
-    const uint8_t* const wsr = a.ws + (row0 / F8_BLOCK) * a.ws_nb1;
+// The weight's rows of a workgroup, 16 at a time (every gridDim.x-th 16), as its waves read them: groups of four blocks of K in
+// turn, from memory to registers.
+struct SkWeight {
+    const F8Args& a;
+    const int lane, wave, waves;
+    const int kb, groups;
+    __device__ __forceinline__ explicit SkWeight(const F8Args& args)
+        : a(args), lane((int) threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6)),
+          waves((int) blockDim.x >> 6), kb((int) ((args.K + F8_BLOCK - 1) / F8_BLOCK)), groups((kb + 3) / 4) {}
+    // (rows past the weight are read as zeros; past K the last block again, which is not used)
+    __device__ __forceinline__ void load(int64_t tile, int g, F8Frag (&w)[4]) const {
+        const int64_t row0 = tile * 16;
+        const int64_t rows = min((int64_t) 16, a.M - row0);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            (void*) (a.w + row0 * a.w_nb1), (short) 0, (int) ((rows - 1) * a.w_nb1 + (int64_t) kb * F8_BLOCK), SK_RSRC);
+        const uint32_t off = (uint32_t) ((lane & 15) * a.w_nb1) + (lane >> 4) * 16;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const uint32_t at = (uint32_t) min(4 * g + b, kb - 1) * F8_BLOCK;
+            w[b].half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(r, off, at, 0));
+            w[b].half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(r, off + 64, at, 0));
+        }
+    }
+    // a group's scales, by the scalar unit (a byte within its word; a vector load would wait for the weight's before it)
+    __device__ __forceinline__ void scales(int64_t tile, int g, float (&s)[4]) const {
+        typedef const __attribute__((address_space(4))) uint32_t scalar_word;
+        const uint64_t row = (uint64_t) (a.ws + tile / 8 * a.ws_nb1);
+        if (a.ws_float) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) s[b] = __builtin_bit_cast(float, ((scalar_word*) row)[min(4 * g + b, kb - 1)]);
+        } else {
+            const uint32_t word = ((scalar_word*) row)[g];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) s[b] = f8_scale(word >> (8 * b) & 255u);
+        }
+    }
+};
 
+// A block's products of one fragment of the weight with NT of tokens, added to acc.
+template <int NT>
+__device__ __forceinline__ void sk_block(const F8Frag& w, float ws, const F8Frag (&x)[NT], const float (&xs)[NT], f4 (&acc)[NT]) {
+    f4 part[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[j] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const h8v h = f8_half8(w.quarter[q]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, f8_half8(x[j].quarter[q]), part[j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[j][i], xs[j] * ws, acc[j][i]);
+}
+
+// The waves' sums of a tile, joined in their order and stored.
+template <int NT>
+__device__ __forceinline__ void sk_store(const SkWeight& w, int64_t tile, const f4 (&acc)[NT], float* red) {
+    const int r16 = w.lane & 15, chunk = w.lane >> 4;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *(f4*) (red + ((w.wave * NT + j) * 16 + r16) * 16 + chunk * 4) = acc[j];
+    // (a bare barrier: loads from memory stay under way)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    for (int e = (int) threadIdx.x; e < 256 * NT; e += (int) blockDim.x) {
+        const int token = e >> 4;
+        const int64_t r = tile * 16 + (e & 15);
+        if (token >= w.a.N || r >= w.a.M) continue;
+        float s = 0.f;
+        for (int k = 0; k < w.waves; ++k) s += red[k * NT * 256 + e];
+        uint8_t* const y = w.a.y + token * w.a.y_nb1;
+        if (w.a.y_type == TRC_HIP_TYPE_F32) ((float*) y)[r] = s;
+        else ((uint16_t*) y)[r] = f8_bits(w.a.y_type, s);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+}
+
+// N tokens, up to SK_FUSED, whose activations are still floats (of type XTYPE): every wave first quantizes what it will
+// multiply, into LDS, while its first weights come. DEEP: several groups a wave, two of them under way in turn; else one, in as
+// few registers as let three workgroups share a CU. A workgroup a tile: fewer that take several each were slower
+// (14336 rows of 4096: 16.4 us, 15.4 so), what is under way from the start counts for more.
+template <int N, int XTYPE, bool DEEP>
+__global__ __launch_bounds__(DEEP ? SK_WAVES * 64 : 512, DEEP ? 4 : 6) void k_f8_few(F8Args a, const uint8_t* __restrict__ xf, size_t xf_nb1) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t codes[];  // tokens' rows, then their exponents' words
+    __shared__ __attribute__((aligned(16))) float red[(DEEP ? SK_WAVES : 8) * 256];
+    const SkWeight w(a);
+    const int lane = w.lane, r16 = lane & 15, chunk = lane >> 4;
+    const int pitch = w.groups * 512 + 16;
+    uint32_t* const words = (uint32_t*) (codes + N * pitch);
+    auto load_x = [&](int g, float (&x)[N][8]) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) f8_load8<XTYPE>(xf + t * xf_nb1, (int64_t) g * 512 + lane * 8, a.K, x[t]);
+    };
+    // (the activations before the weight: loads arrive in their order)
+    float v[N][8];
+    load_x(w.wave, v);
+    struct Group {
+        F8Frag w[4];
+        float scale[4];
+    } even, odd;
+    auto load_w = [&](int g, Group& into) {
+        w.load(blockIdx.x, g, into.w);
+        w.scales(blockIdx.x, g, into.scale);
+    };
+    load_w(w.wave, even);
+    if (DEEP && w.wave + w.waves < w.groups) load_w(w.wave + w.waves, odd);
+    for (int g = w.wave; g < w.groups; g += w.waves) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            const uint32_t e = f8_exponent(f8_max16(f8_amax8(v[t])));
+            *(u2v*) (codes + t * pitch + g * 512 + lane * 8) = f8_codes(v[t], f8_inverse(e));
+            if (r16 == 0) ((uint8_t*) (words + t * w.groups + g))[chunk] = (uint8_t) e;
+        }
+        if (!DEEP) break;
+        if (g + w.waves < w.groups) load_x(g + w.waves, v);
+    }
+    // a wave's own LDS accesses are carried out in their order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int token = min(r16, N - 1);
+    f4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
+    auto multiply = [&](int g, const Group& f) {
+        const uint32_t word = words[token * w.groups + g];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if (4 * g + b >= w.kb) break;
+            F8Frag x[1];
+            const uint8_t* const p = codes + token * pitch + g * 512 + b * F8_BLOCK + chunk * 16;
+            x[0].half[0] = *(const u4v*) p;
+            x[0].half[1] = *(const u4v*) (p + 64);
+            const float xs[1] = {f8_scale(word >> (8 * b) & 255u)};
+            sk_block<1>(f.w[b], f.scale[b], x, xs, acc);
+        }
+    };
+    if (!DEEP) {
+        multiply(w.wave, even);
+    } else {
+        for (int g = w.wave; g < w.groups; g += 2 * w.waves) {
+            multiply(g, even);
+            if (g + 2 * w.waves < w.groups) load_w(g + 2 * w.waves, even);
+            if (g + w.waves >= w.groups) break;
+            multiply(g + w.waves, odd);
+            if (g + 3 * w.waves < w.groups) load_w(g + 3 * w.waves, odd);
+        }
+    }
+    sk_store<1>(w, blockIdx.x, acc, red);
+}
+
+// Up to 16 NT tokens in 8 bits: a workgroup a tile.
+template <int NT>
+__global__ __launch_bounds__(SK_WAVES * 64, 4) void k_f8_skinny(F8Args a) {
+    __shared__ __attribute__((aligned(16))) float red[SK_WAVES * 256 * NT];
+    const SkWeight w(a);
+    const int r16 = w.lane & 15, chunk = w.lane >> 4;
+    const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+        (void*) a.x, (short) 0, (int) ((a.N - 1) * a.x_nb1 + (int64_t) w.kb * F8_BLOCK), SK_RSRC);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*) a.xs, (short) 0, (int) ((a.N - 1) * a.xs_nb1 + (int64_t) w.groups * 4), SK_RSRC);
+    const int64_t tile = blockIdx.x;
     f4 acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j] = {0.f, 0.f, 0.f, 0.f};
-    for (int g = wave; g < groups; g += waves) {
-        F8Frag w[4];
+    for (int g = w.wave; g < w.groups; g += w.waves) {
+        auto token = [&](int b, int j) {
+            F8Frag x;
+            const uint32_t at = (uint32_t) ((16 * j + r16) * a.x_nb1) + min(4 * g + b, w.kb - 1) * F8_BLOCK + chunk * 16;
+            x.half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 0, 0));
+            x.half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at + 64, 0, 0));
+            return x;
+        };
+        // (the tokens before the weight: loads arrive in their order)
+        uint32_t words[NT];
+        F8Frag x[NT], now[4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            words[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, (uint32_t) ((16 * j + r16) * a.xs_nb1) + 4 * g, 0, 0);
+            x[j] = token(0, j);
+        }
+        w.load(tile, g, now);
         float ws[4];
+        w.scales(tile, g, ws);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            // (past K the last block again, which is not used)
-            const int at = min(4 * g + b, kb - 1);
-            w[b].half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w_off, (uint32_t) at * F8_BLOCK, 0));
-            w[b].half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rw, w_off + 64, (uint32_t) at * F8_BLOCK, 0));
-            ws[b] = a.ws_float ? ((const float*) wsr)[at] : f8_scale(wsr[at]);
-        }
-        uint32_t scale[NT];
-        if constexpr (FUSED) {
-            uint8_t* const mine = codes + wave * SK_FUSED * SK_PITCH;
-            for (int t = 0; t < a.N; ++t) {
-                float v[8];
-                f8_load8<XTYPE>(xf + t * xf_nb1, (int64_t) g * 512 + lane * 8, a.K, v);
-                const uint32_t e = f8_exponent(f8_max16(f8_amax8(v)));
-                *(u2v*) (mine + t * SK_PITCH + lane * 8) = f8_codes(v, f8_inverse(e));
-                if (r16 == 0) ((uint8_t*) (words + wave * SK_FUSED + t))[chunk] = (uint8_t) e;
-            }
-            // a wave's own LDS accesses are carried out in their order
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            scale[0] = words[wave * SK_FUSED + min(r16, (int) a.N - 1)];
-        } else {
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                scale[j] = __builtin_amdgcn_raw_buffer_load_b32(rs, (uint32_t) ((16 * j + r16) * a.xs_nb1) + 4 * g, 0, 0);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            if (4 * g + b >= kb) break;
-            F8Frag x[NT];
-            f4 part[NT];
+            if (4 * g + b >= w.kb) break;
+            F8Frag more[NT];
+            float xs[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                if constexpr (FUSED) {
-                    const uint8_t* const p = codes + (wave * SK_FUSED + min(r16, (int) a.N - 1)) * SK_PITCH + b * F8_BLOCK + chunk * 16;
-                    x[j].half[0] = *(const u4v*) p;
-                    x[j].half[1] = *(const u4v*) (p + 64);
-                } else {
-                    const uint32_t at = (uint32_t) ((16 * j + r16) * a.x_nb1) + (4 * g + b) * F8_BLOCK + chunk * 16;
-                    x[j].half[0] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at, 0, 0));
-                    x[j].half[1] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rx, at + 64, 0, 0));
-                }
-                part[j] = {0.f, 0.f, 0.f, 0.f};
+                if (b < 3) more[j] = token(b + 1, j);
+                xs[j] = f8_scale(words[j] >> (8 * b) & 255u);
             }
+            sk_block<NT>(now[b], ws[b], x, xs, acc);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const h8v wq = f8_half8(w[b].quarter[q]);
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wq, f8_half8(x[j].quarter[q]), part[j], 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const float s = f8_scale((scale[j] >> (8 * b)) & 255u);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(part[j][i] * s, ws[b], acc[j][i]);
-            }
+            for (int j = 0; j < NT; ++j) x[j] = more[j];
         }
-        if constexpr (FUSED) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) *(f4*) (red + ((wave * NT + j) * 16 + r16) * 16 + chunk * 4) = acc[j];
-    __syncthreads();
-    for (int e = (int) threadIdx.x; e < 256 * NT; e += (int) blockDim.x) {
-        const int token = e >> 4, r = e & 15;
-        if (token >= a.N || r >= rows) continue;
-        float s = 0.f;
-        for (int w = 0; w < waves; ++w) s += red[w * NT * 256 + e];
-        uint8_t* const y = a.y + token * a.y_nb1;
-        if (a.y_type == TRC_HIP_TYPE_F32) ((float*) y)[row0 + r] = s;
-        else ((uint16_t*) y)[row0 + r] = f8_bits(a.y_type, s);
-    }
+    sk_store<NT>(w, tile, acc, red);
 }
 
 template <int TYPE>
@@ -197,15 +293,23 @@ int blocks_of(const trc_hip_tensor& x, const trc_hip_fp8& q, hipStream_t s) {
     return check_launch("fp8_quantize (blocks)");
 }
 
+int64_t sk_groups(int64_t K) { return (K + 4 * F8_BLOCK - 1) / (4 * F8_BLOCK); }
+// A wave a group up to 8, then two each: the same in both kernels, so that their sums are.
+unsigned sk_threads(int64_t K) {
+    const int64_t groups = sk_groups(K), waves = groups <= 8 ? groups : (groups + 1) / 2;
+    return 64 * (unsigned) (waves < SK_WAVES ? waves : SK_WAVES);
+}
+size_t few_bytes(int64_t K, int64_t N) {
+    return (size_t) (N * (sk_groups(K) * 516 + 16));
+}
 template <int XTYPE>
-int skinny(const F8Args& a, const uint8_t* xf, size_t xf_nb1, hipStream_t s) {
-    const int64_t wgs = (a.M + 15) / 16, groups = (a.K + 4 * F8_BLOCK - 1) / (4 * F8_BLOCK);
-    const unsigned threads = 64 * (unsigned) (groups < SK_WAVES ? groups : SK_WAVES);
-    auto* k = k_f8_skinny<1, XTYPE>;
-    if constexpr (XTYPE < 0) {
-        if (a.N > 16) k = a.N <= 32 ? k_f8_skinny<2, -1> : a.N <= 48 ? k_f8_skinny<3, -1> : k_f8_skinny<4, -1>;
-    }
-    hipLaunchKernelGGL(k, dim3((unsigned) wgs), dim3(threads), 0, s, a, xf, xf_nb1);
+int few(const F8Args& a, const trc_hip_tensor& x, hipStream_t s) {
+    static_assert(SK_FUSED == 2, "a kernel for each");
+    const bool deep = sk_groups(a.K) > 8;
+    auto* const k = a.N == 1 ? (deep ? k_f8_few<1, XTYPE, true> : k_f8_few<1, XTYPE, false>)
+                             : (deep ? k_f8_few<2, XTYPE, true> : k_f8_few<2, XTYPE, false>);
+    hipLaunchKernelGGL(k, dim3((unsigned) ((a.M + 15) / 16)), dim3(sk_threads(a.K)), few_bytes(a.K, a.N), s, a,
+                       (const uint8_t*) x.data, x.nb[1]);
     return check_launch("fp8 (few tokens)");
 }
 
@@ -218,14 +322,16 @@ int launch_f8_quantize(const trc_hip_tensor& x, const trc_hip_fp8& q, hipStream_
     return rows ? rows_of<TRC_HIP_TYPE_BF16>(x, q, s) : blocks_of<TRC_HIP_TYPE_BF16>(x, q, s);
 }
 
-// x: activations to be quantized on the way, or null where a holds codes.
-int launch_f8_skinny(const F8Args& a, const trc_hip_tensor* x, hipStream_t s) {
-    if (x == nullptr) return skinny<-1>(a, nullptr, 0, s);
-    if (a.N <= SK_FUSED) {
-        const uint8_t* const p = (const uint8_t*) x->data;
-        if (x->type == TRC_HIP_TYPE_F32) return skinny<TRC_HIP_TYPE_F32>(a, p, x->nb[1], s);
-        if (x->type == TRC_HIP_TYPE_F16) return skinny<TRC_HIP_TYPE_F16>(a, p, x->nb[1], s);
-        return skinny<TRC_HIP_TYPE_BF16>(a, p, x->nb[1], s);
+int launch_f8_skinny(const F8Args& a, hipStream_t s) {
+    auto* const k = a.N <= 16 ? k_f8_skinny<1> : a.N <= 32 ? k_f8_skinny<2> : a.N <= 48 ? k_f8_skinny<3> : k_f8_skinny<4>;
+    hipLaunchKernelGGL(k, dim3((unsigned) ((a.M + 15) / 16)), dim3(sk_threads(a.K)), 0, s, a);
+    return check_launch("fp8 (few tokens)");
+}
+
+int launch_f8_matvec(const F8Args& a, const trc_hip_tensor& x, hipStream_t s) {
+    if (a.N <= SK_FUSED && few_bytes(a.K, a.N) <= SK_LDS) {
+        if (x.type == TRC_HIP_TYPE_F32) return few<TRC_HIP_TYPE_F32>(a, x, s);
+        return x.type == TRC_HIP_TYPE_F16 ? few<TRC_HIP_TYPE_F16>(a, x, s) : few<TRC_HIP_TYPE_BF16>(a, x, s);
     }
     // codes and exponents in the stream's workspace
     const int64_t kb = (a.K + F8_BLOCK - 1) / F8_BLOCK, pitch = kb * F8_BLOCK, words = (kb + 3) / 4 * 4;
@@ -242,14 +348,14 @@ int launch_f8_skinny(const F8Args& a, const trc_hip_tensor* x, hipStream_t s) {
     q.scale.data = wsp + a.N * pitch;
     q.scale.nb[1] = (size_t) words;
     q.scale.ne[1] = a.N;
-    rc = launch_f8_quantize(*x, q, s);
+    rc = launch_f8_quantize(x, q, s);
     if (rc != TRC_HIP_OK) return rc;
     F8Args b = a;
     b.x = wsp;
     b.x_nb1 = pitch;
     b.xs = wsp + a.N * pitch;
     b.xs_nb1 = words;
-    return skinny<-1>(b, nullptr, 0, s);
+    return launch_f8_product(b, false, (size_t) (a.N * (pitch + words)), s);
 }
 
 }  // namespace trc_hip

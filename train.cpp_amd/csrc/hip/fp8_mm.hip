@@ -53,12 +53,17 @@ void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
 
 }  // namespace
 
-int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s) {
+int launch_f8_product(const F8Args& a, bool trans, size_t used, hipStream_t s) {
+    // Up to 64 tokens a workgroup with 16 of the weight's rows has all of K, and reads all tokens: from about 700 million
+    // products beyond the first 16 tokens' on that costs more than tiles and their sums' joining (K, M, tokens, us so and in
+    // tiles: 4096, 4096, 48 10.8 and 11.5, 64 13.7 and 11.9; 4096, 14336, 16 18.9 and 18.3, 32 26.1 and 18.9; 14336, 4096,
+    // 16 15.6 and 19.9, 32 21.8 and 20.6; 1000, 777, 64 6.2 and 8.1).
+    if (!trans && a.N <= TRC_HIP_FP8_MATVEC_MAX_N && ((a.N + 15) / 16 - 1) * 16 * a.K * a.M <= 700000000) return launch_f8_skinny(a, s);
     F8Tiles t{};
     t.a = a;
     t.rows = trans ? a.K : a.M;
     t.steps = (int) (((trans ? a.M : a.K) + F8_BLOCK - 1) / F8_BLOCK);
-    const bool fast = a.y_type != TRC_HIP_TYPE_F32;
+    const bool fast = a.y_type != TRC_HIP_TYPE_F32 && a.N > TRC_HIP_FP8_MATVEC_MAX_N;
     const int64_t cus = device_cus();
     auto tiles = [&](int64_t edge) { return ((t.rows + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
     const int edge = fast && tiles(256) >= cus ? 256 : tiles(128) >= cus ? 128 : 64;
@@ -72,7 +77,8 @@ int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s) {
     int64_t parts = 1;
     if (edge == 64 && tiles(64) * 2 <= cus) {
         t.sums_nb1 = (t.rows + 3) / 4 * 4;
-        const int64_t fit = (int64_t) (qm_workspace_bytes() / 4) / (a.N * t.sums_nb1);
+        used = (used + 255) / 256 * 256;
+        const int64_t fit = (int64_t) ((qm_workspace_bytes() - used) / 4) / (a.N * t.sums_nb1);
         parts = cus / tiles(64);
         if (parts > (t.steps + 3) / 4) parts = (t.steps + 3) / 4;
         if (parts > fit) parts = fit;
@@ -87,7 +93,7 @@ int launch_f8_tiles(const F8Args& a, bool trans, hipStream_t s) {
         uint8_t* ws = nullptr;
         const int rc = qm_stream_workspace(s, &ws);
         if (rc != TRC_HIP_OK) return rc;
-        t.sums = (float*) ws;
+        t.sums = (float*) (ws + used);
     }
     const unsigned p = (unsigned) parts;
     if (edge == 256) launch<256, 256, 2, 4, 2, true>(t, trans, p, s);
