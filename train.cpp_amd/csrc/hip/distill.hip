@@ -6,9 +6,10 @@
 //   loss = mean_t  alpha tau^2 KL_t + (1 - alpha) CE_t
 //   dl_tv = dloss / n (alpha tau (q_v - sum_{id_j = v} p_j) + (1 - alpha) (r_v - 1[v = label]))
 //
-// The rows' sums (each row read once), the rows' terms with the teacher's entries, a wave a row, and their mean by one
-// workgroup; the gradient reads and writes each row once more. Bound by memory, and by the exponentials where
-// both temperatures are summed.
+// Two launches for the loss, the rows and one workgroup for what comes of them, and one for the gradient, which reads and writes
+// each row once more. Bound by memory, and by the exponentials where both temperatures are summed. (A single launch,
+// whose last workgroups to arrive finish a row and the loss, was slower: each of its steps waits for a trip to memory
+// that all XCDs see. 61 rows of 131071: 18.8 us, 12 so.)
 #include "logit_rows.h"
 
 namespace trc_hip {
@@ -147,34 +148,6 @@ __device__ __forceinline__ Sums share(const typename Row<TYPE>::Elem* p, int n, 
     return {m, sa * (MODE == DI_SQUARE ? fb * fb : exp2_of(-fmaf(m, c.a, -ua))), MODE == DI_ONE ? 0.f : sb * fb};
 }
 
-// Rows that are not counted are not read. gridDim.y parts of `len` elements each: one writes the sums where the row's
-// statistics will be, several to parts.
-template <int TYPE, int MODE>
-__global__ __launch_bounds__(DI_THREADS) void k_distill_rows(const uint8_t* __restrict__ logits, size_t nb1, int64_t V,
-                                                              const int32_t* __restrict__ labels, Factors c, int64_t len,
-                                                              float* __restrict__ stats, Sums* __restrict__ parts) {
-    typedef Row<TYPE> R;
-    const int64_t row = blockIdx.x;
-    if (labels[row] < 0) return;
-    const int64_t lo = (int64_t) blockIdx.y * len;
-    const typename R::Elem* const p = (const typename R::Elem*) (logits + row * nb1) + lo;
-    Sums s = wave_join<MODE>(share<TYPE, MODE>(p, (int) (min(lo + len, V) - lo), c), c);
-    __shared__ Sums w[DI_THREADS / 64];
-    if (((int) threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-#pragma unroll
-    for (int k = 1; k < DI_THREADS / 64; ++k) s = join<MODE>(s, w[k], c);
-    if (gridDim.y == 1) {
-        float* const out = stats + row * DI_STATS;
-        out[0] = s.m;
-        out[1] = s.a;
-        out[2] = s.b;
-    } else {
-        parts[row * gridDim.y + blockIdx.y] = s;
-    }
-}
-
 // Where the teacher's entries of a row lie.
 struct Teacher {
     const int32_t* ids;
@@ -187,92 +160,158 @@ struct Teacher {
     }
 };
 
+// One of a row's entries: the teacher's logit and the student's.
+struct Entry {
+    float z, l;
+    bool in;
+};
+
 struct Term {
     double kl, ce;
 };
 
-// A wave a row: the parts of its sums joined, the teacher's softmax, and the row's terms, in 64 bits from the sums on.
+// What a row's terms need of its entries and its label: with e_j = exp((z_j - zmax) / tau) and the student's logits taken from
+// `ref`, the largest of what was summed beside them: sum e (0: no entries), sum e (z_j - zmax) / tau, sum e (l_j - ref), l_label - ref.
+struct Entries {
+    double e, ez, el, label;
+    float ref, zmax;
+    // sum_j p_j (log p_j - log q_j) and -log r_label for the sums of the whole row
+    __device__ __forceinline__ Term term(const Sums& s, float tau, float alpha) const {
+        const double off = (double) ref - (double) s.m;
+        return {alpha > 0.f && e != 0.0 ? (ez - (el + e * off) / (double) tau) / e - log(e) + log((double) s.b) : 0.0,
+                alpha < 1.f ? log((double) s.a) - (label + off) : 0.0};
+    }
+};
+
+// What the gradient needs of a row.
+__device__ __forceinline__ void put_stats(float* st, const Sums& s, const Entries& q) {
+    st[0] = base_of(s.m);
+    st[1] = 1.f / s.a;
+    st[2] = 1.f / s.b;
+    st[3] = q.zmax;
+    st[4] = q.e == 0.0 ? 0.f : (float) (1.0 / q.e);
+}
+
+// Rows that are not counted are not read. gridDim.y parts of `len` elements each; the first one's first wave has the entries,
+// on their way while the row is summed. One part makes the row's terms, several leave sums and what comes of the entries.
 template <int TYPE, int MODE>
-__global__ __launch_bounds__(DI_THREADS) void k_distill_terms(const uint8_t* __restrict__ logits, size_t nb1, int64_t V, int64_t T,
-                                                               const int32_t* __restrict__ labels, Teacher teacher, Factors c,
-                                                               float tau, float alpha, int n_parts, const Sums* __restrict__ parts,
-                                                               float* __restrict__ stats, Term* __restrict__ terms) {
+__global__ __launch_bounds__(DI_THREADS) void k_distill_rows(const uint8_t* __restrict__ logits, size_t nb1, int64_t V,
+                                                              const int32_t* __restrict__ labels, Teacher teacher, Factors c,
+                                                              float tau, float alpha, int64_t len, float* __restrict__ stats,
+                                                              Term* __restrict__ terms, Sums* __restrict__ parts,
+                                                              Entries* __restrict__ of_entries) {
     typedef Row<TYPE> R;
-    const int lane = (int) threadIdx.x & 63;
-    const int64_t row = (int64_t) blockIdx.x * (DI_THREADS / 64) + (threadIdx.x >> 6);
-    if (row >= T) return;
-    float* const out = stats + row * DI_STATS;
+    const int64_t row = blockIdx.x;
+    const int lane = (int) threadIdx.x & 63, wave = (int) threadIdx.x >> 6;
     const int32_t y = labels[row];
     if (y < 0) {
-        if (lane < DI_STATS) out[lane] = 0.f;
-        if (lane == 0) terms[row] = {0.0, 0.0};
+        if (blockIdx.y == 0 && threadIdx.x < DI_STATS) stats[row * DI_STATS + threadIdx.x] = 0.f;
+        if (blockIdx.y == 0 && threadIdx.x == 0) terms[row] = {0.0, 0.0};
         return;
     }
-    Sums s;
-    if (n_parts > 1) {
-        s = wave_join<MODE>(lane < n_parts ? parts[row * n_parts + lane] : Sums{-INFINITY, 0.f, 0.f}, c);
-    } else {
-        s = {out[0], out[1], out[2]};
-    }
-    if (MODE == DI_ONE) s.b = s.a;  // the only sum, whichever is wanted
     const typename R::Elem* const l = (const typename R::Elem*) (logits + row * nb1);
-    float zmax = 0.f, inv = 0.f;
-    Term t = {0.0, 0.0};
-    if (alpha > 0.f) {
-        const int64_t at = row * teacher.top;
-        float m = -INFINITY;
-        int entries = 0;
-        for (int j = lane; j < teacher.top; j += 64) {
-            const int32_t id = teacher.ids[at + j];
-            if (id < 0 || id >= V) continue;
-            m = fmaxf(m, teacher.logit(at + j));
-            entries = 1;
+    const int64_t at = row * teacher.top;
+    auto entry = [&](int j) {
+        const int32_t id = j < teacher.top ? teacher.ids[at + j] : -1;
+        const bool in = id >= 0 && id < V;
+        return Entry{in ? teacher.logit(at + j) : -INFINITY, in ? R::get(l[id]) : 0.f, in};
+    };
+    const bool kl = alpha > 0.f, mine = wave == 0 && blockIdx.y == 0;
+    Entry first = {-INFINITY, 0.f, false};
+    float ly = 0.f;
+    if (kl && mine) first = entry(lane);
+    if (alpha < 1.f && mine) ly = y < V ? R::get(l[y]) : NAN;
+    const int64_t lo = (int64_t) blockIdx.y * len;
+    Sums s = wave_join<MODE>(share<TYPE, MODE>(l + lo, (int) (min(lo + len, V) - lo), c), c);
+    __shared__ Sums w[DI_THREADS / 64];
+    if (lane == 0) w[wave] = s;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int k = 0; k < DI_THREADS / 64; ++k) s = k == 0 ? w[0] : join<MODE>(s, w[k], c);
+    if (gridDim.y > 1 && lane == 0) parts[row * gridDim.y + blockIdx.y] = s;
+    if (!mine) return;
+    if (MODE == DI_ONE) s.b = s.a;  // the only sum, whichever is wanted
+    Entries q = {0.0, 0.0, 0.0, 0.0, base_of(s.m), 0.f};
+    q.label = (double) ly - (double) q.ref;
+    if (kl) {
+        float m = first.z;
+        bool some = first.in;
+        for (int j = lane + 64; j < teacher.top; j += 64) {
+            const Entry e = entry(j);
+            m = fmaxf(m, e.z);
+            some = some || e.in;
         }
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-        if (__any(entries)) {
-            // sum_j e_j (x_j - y_j) / S - log S + log s, with e_j = exp(x_j), x_j and y_j the teacher's and the student's
-            // logit from their maxima over tau
-            const float base = base_of(m);
-            double sum = 0.0, dot = 0.0;
-            for (int j = lane; j < teacher.top; j += 64) {
-                const int32_t id = teacher.ids[at + j];
-                if (id < 0 || id >= V) continue;
-                const double x = ((double) teacher.logit(at + j) - (double) base) / (double) tau, e = exp(x);
-                const double d = x - ((double) R::get(l[id]) - (double) s.m) / (double) tau;
-                sum += e;
-                dot += e == 0.0 ? 0.0 : e * d;
-            }
+        q.zmax = base_of(m);
+        auto take = [&](const Entry& n) {
+            if (!n.in) return;
+            const double x = (double) (n.z - q.zmax) / (double) tau, e = (double) exp2_of((float) (x * (double) LOG2E));
+            if (e == 0.0) return;
+            q.e += e;
+            q.ez += e * x;
+            q.el += e * ((double) n.l - (double) q.ref);
+        };
+        take(first);
+        for (int j = lane + 64; j < teacher.top; j += 64) take(entry(j));
 #pragma unroll
-            for (int d = 32; d > 0; d >>= 1) {
-                sum += __shfl_xor(sum, d, 64);
-                dot += __shfl_xor(dot, d, 64);
-            }
-            t.kl = dot / sum - log(sum) + log((double) s.b);
-            zmax = base;
-            inv = (float) (1.0 / sum);
+        for (int d = 32; d > 0; d >>= 1) {
+            q.e += __shfl_xor(q.e, d, 64);
+            q.ez += __shfl_xor(q.ez, d, 64);
+            q.el += __shfl_xor(q.el, d, 64);
         }
+        if (q.e == 0.0 && __any(some)) q.e = NAN;  // (a teacher to whom every entry is impossible)
     }
-    if (alpha < 1.f) t.ce = y < V ? log((double) s.a) - ((double) R::get(l[y]) - (double) s.m) : (double) NAN;
-    if (lane == 0) {
-        out[0] = base_of(s.m);
-        out[1] = 1.f / s.a;
-        out[2] = 1.f / s.b;
-        out[3] = zmax;
-        out[4] = inv;
-        terms[row] = t;
+    if (lane != 0) return;
+    if (gridDim.y > 1) {
+        of_entries[row] = q;
+    } else {
+        put_stats(stats + row * DI_STATS, s, q);
+        terms[row] = q.term(s, tau, alpha);
     }
 }
 
-// One workgroup: the terms' means, each thread's rows and then the threads in a fixed order.
-__global__ __launch_bounds__(DI_JOIN) void k_distill_mean(const Term* __restrict__ terms, const int32_t* __restrict__ labels, int64_t T,
-                                                           float tau, float alpha, float* __restrict__ loss) {
+// One workgroup: the sums of rows in parts, `each` threads (a power of two up to 64) a row, then the terms' means, each
+// thread's rows and then the threads in a fixed order.
+template <int MODE>
+__global__ __launch_bounds__(DI_JOIN) void k_distill_mean(const int32_t* __restrict__ labels, int64_t T, Factors c, float tau, float alpha,
+                                                           int n_parts, int each, const Sums* __restrict__ parts,
+                                                           const Entries* __restrict__ of_entries,
+                                                           const Term* __restrict__ terms, float* __restrict__ stats, float* __restrict__ loss) {
     double kl = 0.0, ce = 0.0;
     int n = 0;
-    for (int64_t t = threadIdx.x; t < T; t += DI_JOIN) {
-        kl += terms[t].kl;
-        ce += terms[t].ce;
-        n += labels[t] >= 0;
+    const int sub = (int) threadIdx.x & (each - 1);
+    for (int64_t t0 = 0; t0 < T; t0 += DI_JOIN / each) {
+        const int64_t t = t0 + threadIdx.x / each;
+        const bool counted = t < T && labels[t] >= 0;
+        Term q = {0.0, 0.0};
+        if (n_parts > 1) {
+            // (read whether or not the row is counted, so as not to wait for its label first)
+            const int64_t row = min(t, T - 1);
+            const Entries e = of_entries[row];
+            const Sums* const p = parts + row * n_parts;
+            Sums s = {-INFINITY, 0.f, 0.f};
+            for (int i = sub; i < n_parts; i += 4 * each) {
+                Sums x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = p[min(i + k * each, n_parts - 1)];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i + k * each < n_parts) s = join<MODE>(s, x[k], c);
+            }
+            for (int d = 1; d < each; d <<= 1) s = join<MODE>(s, {__shfl_xor(s.m, d, 64), __shfl_xor(s.a, d, 64), __shfl_xor(s.b, d, 64)}, c);
+            if (MODE == DI_ONE) s.b = s.a;
+            if (counted && sub == 0) {
+                put_stats(stats + t * DI_STATS, s, e);
+                q = e.term(s, tau, alpha);
+            }
+        } else if (counted) {
+            q = terms[t];
+        }
+        kl += q.kl;
+        ce += q.ce;
+        n += counted && sub == 0;
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -298,7 +337,7 @@ __global__ __launch_bounds__(DI_JOIN) void k_distill_mean(const Term* __restrict
         kl /= n;
         ce /= n;
     }
-    // (a weight of 0 takes no part of an infinite term: such a one was not computed)
+    // (a term of weight 0 was not computed, so that it is 0 and not infinite)
     loss[0] = (float) ((double) alpha * tau * tau * kl + (1.0 - (double) alpha) * ce);
     loss[1] = (float) kl;
     loss[2] = (float) ce;
@@ -412,20 +451,18 @@ int forward(const Call& q, float* stats, float* loss, hipStream_t s) {
     int rc = qm_stream_workspace(s, &ws);
     if (rc != TRC_HIP_OK) return rc;
     Term* const terms = (Term*) ws;
-    Sums* const parts = (Sums*) (ws + (size_t) T * sizeof(Term));
-    if ((size_t) T * sizeof(Term) + (n > 1 ? (size_t) (n * T) * sizeof(Sums) : 0) > qm_workspace_bytes()) {
+    Entries* const of_entries = (Entries*) (terms + T);
+    Sums* const parts = (Sums*) (of_entries + (n > 1 ? T : 0));
+    if ((size_t) T * sizeof(Term) + (n > 1 ? (size_t) T * sizeof(Entries) + (size_t) (n * T) * sizeof(Sums) : 0) > qm_workspace_bytes()) {
         return fail(TRC_HIP_E_SHAPE, "trc_hip_distill_loss: %lld rows in %lld parts", (long long) T, (long long) n);
     }
     hipLaunchKernelGGL((k_distill_rows<TYPE, MODE>), dim3((unsigned) T, (unsigned) n), dim3(DI_THREADS), 0, s, (const uint8_t*) q.l->data,
-                       q.l->nb[1], V, q.labels, q.c, len, stats, parts);
+                       q.l->nb[1], V, q.labels, q.teacher, q.c, q.tau, q.alpha, len, stats, terms, parts, of_entries);
     rc = check_launch("distill_loss (rows)");
     if (rc != TRC_HIP_OK) return rc;
-    const int64_t per = DI_THREADS / 64;
-    hipLaunchKernelGGL((k_distill_terms<TYPE, MODE>), dim3((unsigned) ((T + per - 1) / per)), dim3(DI_THREADS), 0, s,
-                       (const uint8_t*) q.l->data, q.l->nb[1], V, T, q.labels, q.teacher, q.c, q.tau, q.alpha, (int) n, parts, stats, terms);
-    rc = check_launch("distill_loss (terms)");
-    if (rc != TRC_HIP_OK) return rc;
-    hipLaunchKernelGGL(k_distill_mean, dim3(1), dim3(DI_JOIN), 0, s, terms, q.labels, T, q.tau, q.alpha, loss);
+    const int each = n == 1 || T > 256 ? 1 : T > 64 ? 4 : 16;  // (few rows have many parts)
+    hipLaunchKernelGGL(k_distill_mean<MODE>, dim3(1), dim3(DI_JOIN), 0, s, q.labels, T, q.c, q.tau, q.alpha, (int) n, each,
+                       parts, of_entries, terms, stats, loss);
     return check_launch("distill_loss (mean)");
 }
 

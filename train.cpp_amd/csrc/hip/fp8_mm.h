@@ -18,7 +18,7 @@ struct F8Tiles {
 
 // FAST: the 8-bit matrix instruction, or binary16 with sums in 32 bits (fp8_mm.hip says when). POW2: the weight's
 // scales are bytes.
-template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool FAST, bool POW2>
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool FAST, bool POW2>
 void f8_tiles_launch(const F8Tiles& t, unsigned parts, hipStream_t s);
 
 namespace {
@@ -62,8 +62,8 @@ struct F8Slab {
 };
 
 // Waves of a SIMD: a workgroup's, twice where its stages leave room in LDS for another workgroup.
-constexpr int f8_waves(int bm, int bn, int waves, int stages) {
-    return (waves + 3) / 4 * (stages * ((bm + bn) * F8_BLOCK + 4 * bn) <= 80 * 1024 ? 2 : 1);
+constexpr int f8_waves(int bm, int bn, int waves, int groups, int stages) {
+    return (waves * groups + 3) / 4 * (groups * (stages * ((bm + bn) * F8_BLOCK + 4 * bn) + F8_TOUCHED) <= 80 * 1024 ? 2 : 1);
 }
 
 // A wave waits until `n` of its loads from memory at most are under way, and for its accesses to LDS.
@@ -72,8 +72,16 @@ __device__ __forceinline__ void f8_wait() {
     __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
 }
 
-// A workgroup's tile: where it lies, its operands' way to LDS and from there, and its results' to memory.
-template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool POW2>
+// A bare barrier: __syncthreads' fence would wait for the loads that are to stay under way.
+__device__ __forceinline__ void f8_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A tile: where it lies, its operands' way to LDS and from there, and its results' to memory. KG groups of WM WN waves take
+// every KG-th step each, with stages of their own.
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool POW2>
 struct F8Tile {
     static constexpr int THREADS = WM * WN * 64, TM = BM / WM, TN = BN / WN, IT = TM / 16, JT = TN / 16;
     static constexpr int ACH = TRANS ? BM / 16 : 8;
@@ -83,10 +91,12 @@ struct F8Tile {
     static constexpr int ACROSS = TRANS && BM > 128 ? BM / 128 : 1;  // lines of 128 bytes of a row in the weight's tile
     static constexpr int ALINES = (TRANS ? F8_BLOCK : BM) * ACROSS;
     static constexpr int STAGE = ASlab::BYTES + BSlab::BYTES + BN * 4, LOADS = ASlab::PIECES + BSlab::PIECES + 1;
+    static constexpr int GROUP = STAGES * STAGE + F8_TOUCHED;  // bytes of LDS
 
     const F8Tiles& t;
+    const int tid, kg, lane, wave;  // (tid and wave: within the group)
     lds_byte* const lds;
-    const int lane, wave, wm, wn, r16, chunk;
+    const int wm, wn, r16, chunk;
     int64_t row0, n0, a_rows, b_rows, pitch;
     const ASlab slab_a;
     const BSlab slab_b;
@@ -98,9 +108,9 @@ struct F8Tile {
 
     // tile: its number in a grid of tiles over `wide` tokens each, of which this takes BN, `part` times BN on
     __device__ __forceinline__ F8Tile(const F8Tiles& tiles, uint8_t* shared, int tile, int wide, int part)
-        : t(tiles), lds((lds_byte*) shared), lane((int) threadIdx.x & 63),
-          wave(__builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6)), wm(wave % WM), wn(wave / WM), r16(lane & 15),
-          chunk(lane >> 4), slab_a((int) threadIdx.x, tiles.a.w_nb1), slab_b((int) threadIdx.x, tiles.a.x_nb1) {
+        : t(tiles), tid((int) threadIdx.x % THREADS), kg(KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((int) threadIdx.x / THREADS)),
+          lane(tid & 63), wave(__builtin_amdgcn_readfirstlane(tid >> 6)), lds((lds_byte*) shared + kg * GROUP), wm(wave % WM),
+          wn(wave / WM), r16(lane & 15), chunk(lane >> 4), slab_a(tid, tiles.a.w_nb1), slab_b(tid, tiles.a.x_nb1) {
         const F8Args& a = t.a;
         // four tiles of rows by all of the tokens', then the next four: neighbours on an XCD share operands in its L2
         const int in = tile % (4 * t.tn), first = tile / (4 * t.tn) * 4, high = min(4, t.tm - first);
@@ -112,10 +122,10 @@ struct F8Tile {
         x0 = a.x + n0 * a.x_nb1;
         rs = __builtin_amdgcn_make_buffer_rsrc((void*) (a.xs + n0 * a.xs_nb1), (short) 0,
                                                (int) ((b_rows - 1) * a.xs_nb1 + (t.steps + 3) / 4 * 4), F8_RSRC);
-        e_off = (uint32_t) (((int) threadIdx.x % BN) * a.xs_nb1);
+        e_off = (uint32_t) ((tid % BN) * a.xs_nb1);
         // The lines of a later step that this workgroup brings into the XCD's L2: its share of what it has in common with
         // its neighbours there.
-        const int sa = min(8, t.tn), sb = min(4, high), tid = (int) threadIdx.x;
+        const int sa = min(8, t.tn), sb = min(4, high);
         touch_off = 0xFFFFFF00u;
         if (tid < ALINES) {
             if (tid * sa / ALINES == in / high % sa)
@@ -154,7 +164,7 @@ struct F8Tile {
                 rs, (__attribute__((address_space(3))) void*) (at + ASlab::BYTES + BSlab::BYTES + (wave * 64 % BN) * 4), 4, e_off, from.word, 0, 0);
     }
     __device__ __forceinline__ void touch(const Source& from) const {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(wave * 64 < ALINES ? from.a : from.b, (__attribute__((address_space(3))) void*) (lds + 2 * STAGE), 4,
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wave * 64 < ALINES ? from.a : from.b, (__attribute__((address_space(3))) void*) (lds + STAGES * STAGE), 4,
                                                  touch_off, 0, 0, 0);
     }
     __device__ __forceinline__ void load(int s, int stage) const {
@@ -163,7 +173,8 @@ struct F8Tile {
         for (int p = 0; p < LOADS; ++p) load(from, stage, p);
     }
     // the weight's scale of a step, by the scalar unit
-    __device__ __forceinline__ uint32_t scale(int s) const {
+    __device__ __forceinline__ uint32_t scale(int s, int end) const {
+        s = min(s, end - 1);
         typedef const __attribute__((address_space(4))) uint32_t scalar_word;
         const uint64_t at = ws + (uint64_t) (s * ws_step);
         const uint32_t word = *(scalar_word*) (at & ~(uint64_t) 3);
@@ -199,9 +210,32 @@ struct F8Tile {
         const lds_byte* const p = lds + stage * STAGE + ASlab::BYTES + BSlab::BYTES;
         return ((const __attribute__((address_space(3))) uint32_t*) p)[wn * TN + j * 16 + r16] >> (8 * (s & 3)) & 255u;
     }
-    // a lane holds four neighbouring rows of one token
-    __device__ __forceinline__ void store(const f4 (&acc)[IT][JT]) const {
+    // The groups' sums added in their order, and stored: a lane holds four neighbouring rows of one token.
+    __device__ __forceinline__ void store(f4 (&acc)[IT][JT]) const {
         const F8Args& a = t.a;
+        f8_wait<0>();  // (what was loaded ahead: zeros, to LDS that this or another workgroup has another use for)
+        if constexpr (KG > 1) {
+            static_assert(KG == 2 && IT * JT * THREADS * 16 <= GROUP, "the other group's sums fit its stages");
+            typedef __attribute__((address_space(3))) f4 lds_f4;
+            lds_f4* const sums = (lds_f4*) (lds - kg * GROUP + GROUP);
+            if (kg == 1) {
+                // (its waves have read their stages' last, but not all at once)
+                f8_barrier();
+#pragma unroll
+                for (int i = 0; i < IT; ++i)
+#pragma unroll
+                    for (int j = 0; j < JT; ++j) sums[(i * JT + j) * THREADS + tid] = acc[i][j];
+                f8_wait<0>();
+                f8_barrier();
+                return;
+            }
+            f8_barrier();
+            f8_barrier();
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int j = 0; j < JT; ++j) acc[i][j] += sums[(i * JT + j) * THREADS + tid];
+        }
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
             const int64_t n = n0 + wn * TN + j * 16 + r16;
@@ -235,14 +269,15 @@ struct F8Tile {
 };
 
 // Products in binary16.
-template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool POW2>
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool POW2>
 __device__ __forceinline__ void f8_exact(const F8Tiles& t, uint8_t* shared, int tile, int wide, int part) {
-    typedef F8Tile<BM, BN, WM, WN, STAGES, TRANS, POW2> Tile;
+    typedef F8Tile<BM, BN, WM, WN, KG, STAGES, TRANS, POW2> Tile;
     // (pieces from memory at once: all of them in the first two rounds of products)
     constexpr int IT = Tile::IT, JT = Tile::JT, EACH = (Tile::LOADS + 1) / 2;
     const Tile w(t, shared, tile, wide, part);
     if (w.n0 >= t.a.N) return;
-    const int s0 = (int) blockIdx.y * t.part_steps, s1 = min(s0 + t.part_steps, t.steps);
+    const int first = (int) blockIdx.y * t.part_steps, s1 = min(first + t.part_steps, t.steps), s0 = first + w.kg;
+    const int rounds = (s1 - first + KG - 1) / KG;  // (a step from s1 on is one of zeros)
     f4 acc[IT][JT];
 #pragma unroll
     for (int i = 0; i < IT; ++i)
@@ -250,19 +285,19 @@ __device__ __forceinline__ void f8_exact(const F8Tiles& t, uint8_t* shared, int 
         for (int j = 0; j < JT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < STAGES - 1; ++k) {
-        const typename Tile::Source from = w.source(s0 + k, s1);
+        const typename Tile::Source from = w.source(s0 + k * KG, s1);
 #pragma unroll
         for (int p = 0; p < Tile::LOADS; ++p) w.load(from, k, p);
     }
-    uint32_t wnext = w.scale(s0);
-    int stage = 0;
-    for (int s = s0; s < s1; ++s) {
+    uint32_t wnext = w.scale(s0, s1);
+    int stage = 0, s = s0;
+    for (int round = 0; round < rounds; ++round, s += KG) {
         // this step's tiles have landed (the next STAGES - 2 may not have), and every wave has read the last step's
         f8_wait<Tile::LOADS * (STAGES - 2)>();
-        __builtin_amdgcn_s_barrier();
+        f8_barrier();
         const float wscale = POW2 ? f8_scale(wnext) : __builtin_bit_cast(float, wnext);
-        if (s + 1 < s1) wnext = w.scale(s + 1);
-        const typename Tile::Source from = w.source(s + STAGES - 1, s1);
+        wnext = w.scale(s + KG, s1);
+        const typename Tile::Source from = w.source(s + (STAGES - 1) * KG, s1);
         const int into = stage == 0 ? STAGES - 1 : stage - 1;
         h8v wh[IT][4], x[4];
         auto half = [](const F8Frag& f, h8v (&h)[4]) {
@@ -302,21 +337,21 @@ __device__ __forceinline__ void f8_exact(const F8Tiles& t, uint8_t* shared, int 
         add(JT - 1);
         stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
-    f8_wait<0>();  // (what was loaded ahead: zeros, to LDS that another workgroup may have next)
     w.store(acc);
 }
 
-// Products on the 8-bit instruction, two stages. The barrier comes before a step's last two rows of fragments are
+// Products on the 8-bit instruction. The barrier comes before a step's last two rows of fragments are
 // multiplied: meanwhile the next step's first two come from LDS, each token's fragment as soon as the last product with the
 // one whose registers it takes is under way. The step after that comes from memory from then on, a piece after every
 // second product: all at once, a wave's products would wait until the loads before them have been taken.
-template <int BM, int BN, int WM, int WN, bool TRANS, bool POW2>
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool POW2>
 __device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int tile, int wide, int part) {
-    typedef F8Tile<BM, BN, WM, WN, 2, TRANS, POW2> Tile;
+    typedef F8Tile<BM, BN, WM, WN, KG, STAGES, TRANS, POW2> Tile;
     constexpr int IT = Tile::IT, JT = Tile::JT;
     const Tile w(t, shared, tile, wide, part);
     if (w.n0 >= t.a.N) return;
-    const int s0 = (int) blockIdx.y * t.part_steps, s1 = min(s0 + t.part_steps, t.steps);
+    const int first = (int) blockIdx.y * t.part_steps, s1 = min(first + t.part_steps, t.steps), s0 = first + w.kg;
+    const int rounds = (s1 - first + KG - 1) / KG;  // (a step from s1 on is one of zeros)
     f4 acc[IT][JT];
 #pragma unroll
     for (int i = 0; i < IT; ++i)
@@ -324,7 +359,7 @@ __device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int t
         for (int j = 0; j < JT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
     // pieces loaded between the barrier and the next step, the others' distance there in products
     constexpr int ROOM = (IT - 2) * JT, EARLY = ROOM < Tile::LOADS - JT ? Tile::LOADS : JT < Tile::LOADS ? JT : Tile::LOADS;
-    constexpr int AHEAD = 3;
+    constexpr int AHEAD = STAGES + 1;  // steps that the L2 has a line before it is wanted there
     constexpr int EVERY = ROOM >= 4 * (Tile::LOADS - EARLY) ? 2 : 1;
     F8Frag token[JT], a[2];
     uint32_t exps[JT], scale = 0;
@@ -338,13 +373,18 @@ __device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int t
             for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(part[k], __builtin_bit_cast(float, scale), acc[i][j][k]);
         }
     };
-    if (s0 < s1) {
-        w.load(s0, 0);
-        typename Tile::Source from = w.source(s0 + 1, s1);
-        f8_wait<0>();
-        __builtin_amdgcn_s_barrier();
+    if (rounds > 0) {
 #pragma unroll
-        for (int p = 0; p < EARLY; ++p) w.load(from, 1, p);
+        for (int k = 0; k < STAGES - 1; ++k) {
+            const typename Tile::Source from = w.source(s0 + k * KG, s1);
+#pragma unroll
+            for (int p = 0; p < Tile::LOADS; ++p) w.load(from, k, p);
+        }
+        typename Tile::Source from = w.source(s0 + (STAGES - 1) * KG, s1);
+        f8_wait<Tile::LOADS * (STAGES - 2)>();
+        f8_barrier();
+#pragma unroll
+        for (int p = 0; p < EARLY; ++p) w.load(from, STAGES - 1, p);
 #pragma unroll
         for (int i = 0; i < 2; ++i) a[i] = w.weight(0, i);
 #pragma unroll
@@ -352,10 +392,11 @@ __device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int t
             token[j] = w.token(0, j);
             exps[j] = w.exponent(s0, 0, j);
         }
-        scale = w.scale(s0);
-        int stage = 0;
-        for (int s = s0; s < s1; ++s) {
-            // the pieces of the next step that were not loaded after the barrier
+        scale = w.scale(s0, s1);
+        int stage = 0, s = s0;
+        for (int round = 0; round < rounds; ++round, s += KG) {
+            const int before = stage == 0 ? STAGES - 1 : stage - 1, after = stage == STAGES - 1 ? 0 : stage + 1;
+            // the pieces that were not loaded after the barrier
             int piece = EARLY;
 #pragma unroll
             for (int i = 0; i + 2 < IT; i += 2) {
@@ -366,7 +407,7 @@ __device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int t
                     for (int j = 0; j < JT; ++j) {
                         multiply(i + k, j, a[k]);
                         if (((k * JT + j) % EVERY) == EVERY - 1 && piece < Tile::LOADS) {
-                            w.load(from, stage ^ 1, piece);
+                            w.load(from, before, piece);
                             ++piece;
                             __builtin_amdgcn_sched_barrier(0);
                         }
@@ -374,66 +415,64 @@ __device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int t
                 a[0] = b[0], a[1] = b[1];
             }
             // this wave has read all of the step's stage, and its share of the next one has landed
-            w.touch(w.source(s + AHEAD, s1));
+            w.touch(w.source(s + AHEAD * KG, s1));
             __builtin_amdgcn_sched_barrier(0);
-            f8_wait<1>();
-            __builtin_amdgcn_s_barrier();
-            from = w.source(s + 2, s1);
-            const int n = min(s + 1, s1 - 1);  // (past the last step what is there is read, and not used)
-            const F8Frag next[2] = {w.weight(stage ^ 1, 0), w.weight(stage ^ 1, 1)};
-            const uint32_t scale_next = w.scale(n);
+            f8_wait<Tile::LOADS * (STAGES - 2) + 1>();
+            f8_barrier();
+            from = w.source(s + STAGES * KG, s1);
+            const int n = s + KG;  // (past the last step what is there is read, and not used)
+            const F8Frag next[2] = {w.weight(after, 0), w.weight(after, 1)};
+            const uint32_t scale_next = w.scale(n, s1);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
                 multiply(IT - 2, j, a[0]);
                 multiply(IT - 1, j, a[1]);
-                token[j] = w.token(stage ^ 1, j);
-                exps[j] = w.exponent(n, stage ^ 1, j);
+                token[j] = w.token(after, j);
+                exps[j] = w.exponent(n, after, j);
                 if (j < EARLY) w.load(from, stage, j);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int p = JT; p < EARLY; ++p) w.load(from, stage, p);
-            stage ^= 1;
+            stage = after;
             a[0] = next[0], a[1] = next[1];
             scale = scale_next;
         }
     }
-    f8_wait<0>();  // (what was loaded ahead: zeros, to LDS that another workgroup may have next)
     w.store(acc);
 }
 
 // An XCD (workgroup b is on XCD b % 8) takes neighbouring tiles: t.whole as they are and the rest, the last round
 // of its CUs where that is half of one or less, in two halves of the tokens by a workgroup each.
-template <int BM, int BN, int WM, int WN, int STAGES, bool TRANS, bool FAST, bool POW2>
-__global__ __launch_bounds__(WM * WN * 64, f8_waves(BM, BN, WM * WN, STAGES)) void k_f8_tiles(F8Tiles t) {
-    __shared__ __attribute__((aligned(128))) uint8_t
-        shared[STAGES * F8Tile<BM, BN, WM, WN, STAGES, TRANS, POW2>::STAGE + (FAST ? F8_TOUCHED : 0)];
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool FAST, bool POW2>
+__global__ __launch_bounds__(WM * WN * KG * 64, f8_waves(BM, BN, WM * WN, KG, STAGES)) void k_f8_tiles(F8Tiles t) {
+    __shared__ __attribute__((aligned(128))) uint8_t shared[KG * F8Tile<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>::GROUP];
     const int per_xcd = (t.tm * t.tn + 7) / 8, at = (int) (blockIdx.x >> 3);
     const int tile = (int) (blockIdx.x & 7) * per_xcd + (at < t.whole ? at : t.whole + (at - t.whole) / 2);
     if (tile >= t.tm * t.tn) return;
     if constexpr (FAST) {
         if constexpr (BN == 256) {
-            if (at >= t.whole) return f8_fast<BM, BN / 2, WM, WN, TRANS, POW2>(t, shared, tile, BN, (at - t.whole) & 1);
+            if (at >= t.whole) return f8_fast<BM, BN / 2, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile, BN, (at - t.whole) & 1);
         }
-        f8_fast<BM, BN, WM, WN, TRANS, POW2>(t, shared, tile, BN, 0);
+        f8_fast<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile, BN, 0);
     } else {
-        f8_exact<BM, BN, WM, WN, STAGES, TRANS, POW2>(t, shared, tile, BN, 0);
+        f8_exact<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile, BN, 0);
     }
 }
 
 }  // namespace
 
-#define F8_INSTANCE(BM, BN, WM, WN, STAGES, TRANS, FAST, POW2)                                                         \
+#define F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2)                                                         \
     template <>                                                                                                        \
-    void f8_tiles_launch<BM, BN, WM, WN, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s) { \
-        hipLaunchKernelGGL((k_f8_tiles<BM, BN, WM, WN, STAGES, TRANS, FAST, POW2>),                                    \
-                           dim3((unsigned) (8 * (2 * ((t.tm * t.tn + 7) / 8) - t.whole)), parts), dim3(WM * WN * 64), 0, s, t); \
+    void f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s) { \
+        hipLaunchKernelGGL((k_f8_tiles<BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2>),                                    \
+                           dim3((unsigned) (8 * (2 * ((t.tm * t.tn + 7) / 8) - t.whole)), parts), dim3(WM * WN * KG * 64), 0, s, t); \
     }
-#define F8_INSTANCES(BM, BN, WM, WN, STAGES, FAST)          \
-    F8_INSTANCE(BM, BN, WM, WN, STAGES, false, FAST, false) \
-    F8_INSTANCE(BM, BN, WM, WN, STAGES, false, FAST, true)  \
-    F8_INSTANCE(BM, BN, WM, WN, STAGES, true, FAST, false)  \
-    F8_INSTANCE(BM, BN, WM, WN, STAGES, true, FAST, true)
+#define F8_INSTANCES(BM, BN, WM, WN, KG, STAGES, FAST)          \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, false, FAST, false) \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, false, FAST, true)  \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, true, FAST, false)  \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, true, FAST, true)
 
 }  // namespace trc_hip

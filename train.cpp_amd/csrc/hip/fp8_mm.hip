@@ -7,20 +7,22 @@
 
 namespace trc_hip {
 
-#define F8_DECLARE(BM, BN, WM, WN, STAGES, TRANS, FAST, POW2) \
+#define F8_DECLARE(BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2) \
     template <>                                               \
-    void f8_tiles_launch<BM, BN, WM, WN, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
-#define F8_DECLARE_ALL(BM, BN, WM, WN, STAGES, FAST)       \
-    F8_DECLARE(BM, BN, WM, WN, STAGES, false, FAST, false) \
-    F8_DECLARE(BM, BN, WM, WN, STAGES, false, FAST, true)  \
-    F8_DECLARE(BM, BN, WM, WN, STAGES, true, FAST, false)  \
-    F8_DECLARE(BM, BN, WM, WN, STAGES, true, FAST, true)
+    void f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
+#define F8_DECLARE_ALL(BM, BN, WM, WN, KG, STAGES, FAST)       \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, false, FAST, false) \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, false, FAST, true)  \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, true, FAST, false)  \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, true, FAST, true)
 
-F8_DECLARE_ALL(256, 256, 2, 4, 2, true)
-F8_DECLARE_ALL(128, 128, 2, 2, 2, true)
-F8_DECLARE_ALL(128, 128, 2, 2, 2, false)
-F8_DECLARE_ALL(64, 64, 2, 2, 2, true)
-F8_DECLARE_ALL(64, 64, 2, 2, 3, false)
+F8_DECLARE_ALL(256, 256, 2, 4, 1, 2, true)
+F8_DECLARE_ALL(128, 128, 2, 2, 1, 2, true)
+F8_DECLARE_ALL(128, 128, 2, 2, 1, 2, false)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, 2, true)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, 2, false)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, 3, true)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, 3, false)
 
 namespace {
 
@@ -41,30 +43,31 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_f8_join(const float* __restric
     }
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, bool FAST>
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool FAST>
 void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
     const bool pow2 = !t.a.ws_float;
-    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, STAGES, true, FAST, true>
-                                  : f8_tiles_launch<BM, BN, WM, WN, STAGES, true, FAST, false>)
-                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, STAGES, false, FAST, true>
-                                  : f8_tiles_launch<BM, BN, WM, WN, STAGES, false, FAST, false>);
+    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, true, FAST, true>
+                                  : f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, true, FAST, false>)
+                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, false, FAST, true>
+                                  : f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, false, FAST, false>);
     f(t, parts, s);
 }
 
 }  // namespace
 
 int launch_f8_product(const F8Args& a, bool trans, size_t used, hipStream_t s) {
-    // Up to 64 tokens a workgroup with 16 of the weight's rows has all of K, and reads all tokens: from about 700 million
-    // products beyond the first 16 tokens' on that costs more than tiles and their sums' joining (K, M, tokens, us so and in
-    // tiles: 4096, 4096, 48 10.8 and 11.5, 64 13.7 and 11.9; 4096, 14336, 16 18.9 and 18.3, 32 26.1 and 18.9; 14336, 4096,
-    // 16 15.6 and 19.9, 32 21.8 and 20.6; 1000, 777, 64 6.2 and 8.1).
-    if (!trans && a.N <= TRC_HIP_FP8_MATVEC_MAX_N && ((a.N + 15) / 16 - 1) * 16 * a.K * a.M <= 700000000) return launch_f8_skinny(a, s);
+    // Up to 64 tokens a workgroup with 16 of the weight's rows has all of K, and reads all tokens: from some 850 million
+    // products on (of 16, 32, 48 or 64 tokens) that costs more than tiles do, which few tokens and rows leave to be summed
+    // in parts (K, M, tokens, us so and in tiles: 4096, 4096, 48 10.8 and 11.5, 64 13.7 and 12.3; 4096, 14336, 16 18.9
+    // and 15.5, 64 42 and 16.3; 14336, 4096, 16 15.7 and 17.5, 32 21.8 and 18.2; 1000, 777, 64 6.2 and 8.1).
+    const int64_t cus = device_cus(), n16 = (a.N + 15) / 16 * 16;
+    const bool many = n16 * a.K * a.M > 850000000 && (n16 > 16 || (a.M + 63) / 64 * 2 > cus);
+    if (!trans && a.N <= TRC_HIP_FP8_MATVEC_MAX_N && !many) return launch_f8_skinny(a, s);
     F8Tiles t{};
     t.a = a;
     t.rows = trans ? a.K : a.M;
     t.steps = (int) (((trans ? a.M : a.K) + F8_BLOCK - 1) / F8_BLOCK);
     const bool fast = a.y_type != TRC_HIP_TYPE_F32 && a.N > TRC_HIP_FP8_MATVEC_MAX_N;
-    const int64_t cus = device_cus();
     auto tiles = [&](int64_t edge) { return ((t.rows + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
     const int edge = fast && tiles(256) >= cus ? 256 : tiles(128) >= cus ? 128 : 64;
     if (tiles(edge) > max_groups(512) / 2 - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
@@ -96,9 +99,10 @@ int launch_f8_product(const F8Args& a, bool trans, size_t used, hipStream_t s) {
         t.sums = (float*) (ws + used);
     }
     const unsigned p = (unsigned) parts;
-    if (edge == 256) launch<256, 256, 2, 4, 2, true>(t, trans, p, s);
-    else if (edge == 128) fast ? launch<128, 128, 2, 2, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, 2, false>(t, trans, p, s);
-    else fast ? launch<64, 64, 2, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, 3, false>(t, trans, p, s);
+    if (edge == 256) launch<256, 256, 2, 4, 1, 2, true>(t, trans, p, s);
+    else if (edge == 128) fast ? launch<128, 128, 2, 2, 1, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, 1, 2, false>(t, trans, p, s);
+    else if (t.tm * t.tn > cus) fast ? launch<64, 64, 2, 2, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 2, false>(t, trans, p, s);
+    else fast ? launch<64, 64, 2, 2, 2, 3, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 3, false>(t, trans, p, s);
     const int rc = check_launch("fp8_mul_mat");
     if (rc != TRC_HIP_OK || parts == 1) return rc;
     const int64_t quads = t.sums_nb1 / 4;

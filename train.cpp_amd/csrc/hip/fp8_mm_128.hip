@@ -2,6 +2,6 @@
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(128, 128, 2, 2, 2, true)
-F8_INSTANCES(128, 128, 2, 2, 2, false)
+F8_INSTANCES(128, 128, 2, 2, 1, 2, true)
+F8_INSTANCES(128, 128, 2, 2, 1, 2, false)
 }  // namespace trc_hip

@@ -2,5 +2,5 @@
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(256, 256, 2, 4, 2, true)
+F8_INSTANCES(256, 256, 2, 4, 1, 2, true)
 }  // namespace trc_hip
