@@ -270,6 +270,26 @@ def test_matvec_of_long_rows_and_large_weights(hip, K, M, N):
         b.free()
 
 
+@pytest.mark.parametrize("K,M,N", [(4096, 14336, 1), (4096, 14336, 2), (4096, 14336, 3), (4100, 14336, 16), (33000, 700, 2), (70000, 64, 64),
+                                   (130000, 70, 60)])
+def test_matvec_adds_in_the_products_order(hip, K, M, N):
+    """Sums that do depend on their order: weights of many rows, and activations that take most of the workspace."""
+    announce(f"fp8 order K={K} M={M} N={N}")
+    rng = np.random.default_rng(K + M + N)
+    kb = -(-K // 128)
+    w = rng.integers(0, 127, (M, K), dtype=np.uint8) | rng.integers(0, 2, (M, K), dtype=np.uint8) << 7
+    ws = rng.uniform(0.6, 1.4, (-(-M // 128), kb)).astype(np.float32)
+    p = Product(w, ws, np.zeros((N, K), np.uint8), np.full((N, kb), 127, np.uint8), K, M, "f32")
+    m, y = Mat(rng.standard_normal((N, K)).astype(np.float32)), Mat(np.zeros((N, M), np.float32))
+    H.fp8_quantize(m.t, p.x.t)
+    p.run()
+    H.fp8_matvec(p.w.t, m.t, y.t)
+    H.sync()
+    assert np.array_equal(y.read(), p.read())
+    for b in (p, m, y):
+        b.free()
+
+
 def test_values_that_are_not_finite(hip):
     """A NaN of a token reaches every result of that token and no other; one of the weight every token's result of its row."""
     announce("fp8 not finite")

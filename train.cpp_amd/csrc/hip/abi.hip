@@ -770,7 +770,7 @@ int fp8_product(const char* who, const trc_hip_fp8* w, const trc_hip_fp8* x, con
     a.x_nb1 = (int64_t) x->q.nb[1];
     a.xs = (const uint8_t*) x->scale.data;
     a.xs_nb1 = (int64_t) x->scale.nb[1];
-    return launch_f8_product(a, back, 0, s);
+    return launch_f8_product(a, back, s);
 }
 
 }  // namespace

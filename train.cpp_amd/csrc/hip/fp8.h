@@ -156,8 +156,15 @@ struct F8Args {
 int launch_f8_quantize(const trc_hip_tensor& x, const trc_hip_fp8& q, hipStream_t s);
 int launch_f8_matvec(const F8Args& a, const trc_hip_tensor& x, hipStream_t s);
 int launch_f8_skinny(const F8Args& a, hipStream_t s);
-// fp8_mm.hip: W x, or W^T x with `back`, of operands in 8 bits. The first `used` bytes of the stream's workspace are
-// the caller's.
-int launch_f8_product(const F8Args& a, bool back, size_t used, hipStream_t s);
+// fp8_mm.hip: W x, or W^T x with `back`, of operands in 8 bits. Up to 64 tokens the first f8_held bytes of the stream's
+// workspace are left as they are.
+int launch_f8_product(const F8Args& a, bool back, hipStream_t s);
+
+constexpr int F8_FUSED = 2;  // most tokens whose activations a product's workgroups quantize for themselves
+// bytes of the workspace with N tokens' codes and exponents
+constexpr size_t f8_held(int64_t K, int64_t N) {
+    const int64_t kb = (K + 127) / 128;
+    return (size_t) (N * (kb * 128 + (kb + 3) / 4 * 4));
+}
 
 }  // namespace trc_hip

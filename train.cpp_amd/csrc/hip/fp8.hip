@@ -69,7 +69,6 @@ __global__ __launch_bounds__(Q_THREADS) void k_f8_blocks(const uint8_t* __restri
 }
 
 constexpr int SK_WAVES = 16;            // most of a workgroup
-constexpr int SK_FUSED = 2;             // tokens whose activations a workgroup quantizes for itself
 constexpr int SK_LDS = 48 * 1024;       // most bytes that it keeps of them (three workgroups fit a CU)
 constexpr uint32_t SK_RSRC = 0x00027000;
 
@@ -152,7 +151,7 @@ __device__ __forceinline__ void sk_store(const SkWeight& w, int64_t tile, const 
     __builtin_amdgcn_s_barrier();
 }
 
-// N tokens, up to SK_FUSED, whose activations are still floats (of type XTYPE): every wave first quantizes what it will
+// N tokens, up to F8_FUSED, whose activations are still floats (of type XTYPE): every wave first quantizes what it will
 // multiply, into LDS, while its first weights come. DEEP: several groups a wave, two of them under way in turn; else one, in as
 // few registers as let three workgroups share a CU. A workgroup a tile: fewer that take several each were slower
 // (14336 rows of 4096: 16.4 us, 15.4 so), what is under way from the start counts for more.
@@ -304,7 +303,7 @@ size_t few_bytes(int64_t K, int64_t N) {
 }
 template <int XTYPE>
 int few(const F8Args& a, const trc_hip_tensor& x, hipStream_t s) {
-    static_assert(SK_FUSED == 2, "a kernel for each");
+    static_assert(F8_FUSED == 2, "a kernel for each");
     const bool deep = sk_groups(a.K) > 8;
     auto* const k = a.N == 1 ? (deep ? k_f8_few<1, XTYPE, true> : k_f8_few<1, XTYPE, false>)
                              : (deep ? k_f8_few<2, XTYPE, true> : k_f8_few<2, XTYPE, false>);
@@ -329,13 +328,13 @@ int launch_f8_skinny(const F8Args& a, hipStream_t s) {
 }
 
 int launch_f8_matvec(const F8Args& a, const trc_hip_tensor& x, hipStream_t s) {
-    if (a.N <= SK_FUSED && few_bytes(a.K, a.N) <= SK_LDS) {
+    if (a.N <= F8_FUSED && few_bytes(a.K, a.N) <= SK_LDS) {
         if (x.type == TRC_HIP_TYPE_F32) return few<TRC_HIP_TYPE_F32>(a, x, s);
         return x.type == TRC_HIP_TYPE_F16 ? few<TRC_HIP_TYPE_F16>(a, x, s) : few<TRC_HIP_TYPE_BF16>(a, x, s);
     }
     // codes and exponents in the stream's workspace
     const int64_t kb = (a.K + F8_BLOCK - 1) / F8_BLOCK, pitch = kb * F8_BLOCK, words = (kb + 3) / 4 * 4;
-    if ((size_t) (a.N * (pitch + words)) > qm_workspace_bytes()) {
+    if (f8_held(a.K, a.N) > qm_workspace_bytes()) {
         return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_matvec: %lld tokens of %lld do not fit the workspace", (long long) a.N,
                     (long long) a.K);
     }
@@ -355,7 +354,7 @@ int launch_f8_matvec(const F8Args& a, const trc_hip_tensor& x, hipStream_t s) {
     b.x_nb1 = pitch;
     b.xs = wsp + a.N * pitch;
     b.xs_nb1 = words;
-    return launch_f8_product(b, false, (size_t) (a.N * (pitch + words)), s);
+    return launch_f8_product(b, false, s);
 }
 
 }  // namespace trc_hip

@@ -55,13 +55,16 @@ void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
 
 }  // namespace
 
-int launch_f8_product(const F8Args& a, bool trans, size_t used, hipStream_t s) {
-    // Up to 64 tokens a workgroup with 16 of the weight's rows has all of K, and reads all tokens: from some 850 million
-    // products on (of 16, 32, 48 or 64 tokens) that costs more than tiles do, which few tokens and rows leave to be summed
-    // in parts (K, M, tokens, us so and in tiles: 4096, 4096, 48 10.8 and 11.5, 64 13.7 and 12.3; 4096, 14336, 16 18.9
-    // and 15.5, 64 42 and 16.3; 14336, 4096, 16 15.7 and 17.5, 32 21.8 and 18.2; 1000, 777, 64 6.2 and 8.1).
-    const int64_t cus = device_cus(), n16 = (a.N + 15) / 16 * 16;
-    const bool many = n16 * a.K * a.M > 850000000 && (n16 > 16 || (a.M + 63) / 64 * 2 > cus);
+int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
+    // Up to 64 tokens a workgroup with 16 of the weight's rows has all of K, and reads all tokens: its time grows with
+    // K and tokens, and with the rounds of workgroups. Tiles of 64 rows read them less often, but few of them leave the sum
+    // in parts, to be joined; 16 tokens or fewer are worth that only where there is nothing to join. F8_FUSED tokens are
+    // added up as by the kernel that quantizes them itself (K, M, tokens, us so and in tiles: 4096, 4096, 48 10.8 and
+    // 11.2, 64 13.7 and 11.5; 2048, 6000, 32 8.3 and 9.6, 48 10.4 and 9.9, 64 12.8 and 10.2; 4096, 14336, 8 17.0 and 14.2,
+    // 16 19.0 and 14.4; 14336, 4096, 16 15.7 and 16.2, 32 22.0 and 16.8; 8192, 8192, 8 15.9 and 17.5, 16 18.2 and 17.5;
+    // 1000, 777, 64 6.1 and 7.7).
+    const int64_t cus = device_cus(), n16 = (a.N + 15) / 16 * 16, rounds = ((a.M + 15) / 16 + cus - 1) / cus;
+    const bool many = a.N > F8_FUSED && rounds * a.K * n16 > 240000 && (n16 > 16 || (a.M + 63) / 64 * 2 > cus);
     if (!trans && a.N <= TRC_HIP_FP8_MATVEC_MAX_N && !many) return launch_f8_skinny(a, s);
     F8Tiles t{};
     t.a = a;
@@ -78,10 +81,13 @@ int launch_f8_product(const F8Args& a, bool trans, size_t used, hipStream_t s) {
     if (last * 2 <= per_xcd) t.whole -= last;
     // few tiles: the sum in parts
     int64_t parts = 1;
+    size_t used = 0;
     if (edge == 64 && tiles(64) * 2 <= cus) {
         t.sums_nb1 = (t.rows + 3) / 4 * 4;
-        used = (used + 255) / 256 * 256;
-        const int64_t fit = (int64_t) ((qm_workspace_bytes() - used) / 4) / (a.N * t.sums_nb1);
+        // (activations that trc_hip_fp8_matvec holds there, room for them in every call: as many parts, the same bits)
+        used = trans || a.N > TRC_HIP_FP8_MATVEC_MAX_N ? 0 : (f8_held(a.K, a.N) + 255) / 256 * 256;
+        const size_t room = qm_workspace_bytes();
+        const int64_t fit = (int64_t) ((used < room ? room - used : 0) / 4) / (a.N * t.sums_nb1);
         parts = cus / tiles(64);
         if (parts > (t.steps + 3) / 4) parts = (t.steps + 3) / 4;
         if (parts > fit) parts = fit;
@@ -102,6 +108,7 @@ int launch_f8_product(const F8Args& a, bool trans, size_t used, hipStream_t s) {
     if (edge == 256) launch<256, 256, 2, 4, 1, 2, true>(t, trans, p, s);
     else if (edge == 128) fast ? launch<128, 128, 2, 2, 1, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, 1, 2, false>(t, trans, p, s);
     else if (t.tm * t.tn > cus) fast ? launch<64, 64, 2, 2, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 2, false>(t, trans, p, s);
+    // (three stages where a CU has one workgroup: four took 2 to 5 % longer at 1 to 64 tokens of K and M from 777 to 14336)
     else fast ? launch<64, 64, 2, 2, 2, 3, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 3, false>(t, trans, p, s);
     const int rc = check_launch("fp8_mul_mat");
     if (rc != TRC_HIP_OK || parts == 1) return rc;
