@@ -85,6 +85,37 @@ void hip_preference_loss(const HipPreference& p);
 // The logits' gradient for the loss's gradient dloss [1]; dlogits may be the logits themselves.
 void hip_preference_loss_back(const HipPreference& p, const Tensor* dloss, Tensor* dlogits);
 
+// ---- weights and activations in 8-bit floating point, and learning from a teacher ----
+
+// Rows of e4m3 codes with a scale for every 128 elements (trc_hip_fp8 of trc_hip_abi.h).
+struct HipFp8 {
+    Tensor* q = nullptr;      // [K, R] I8, a view of rows with room for whole blocks
+    Tensor* scale = nullptr;  // I8 (powers of two): of each row, or of 128 rows each (also F32)
+};
+// Tensors for R rows of K, without memory yet: a weight's (scales for 128 rows each) or activations'.
+HipFp8 hip_fp8_new(Context* ctx, int64_t K, int64_t R, bool weight);
+void   hip_fp8_quantize(const Tensor* x, const HipFp8& out);
+// y = mul_mat(w, x); dx = W^T dy.
+void   hip_fp8_mul_mat(const HipFp8& w, const HipFp8& x, Tensor* y);
+void   hip_fp8_mul_mat_back(const HipFp8& w, const HipFp8& dy, Tensor* dx);
+// y = mul_mat(w, quantized x) for up to 64 tokens.
+void   hip_fp8_matvec(const HipFp8& w, const Tensor* x, Tensor* y);
+
+// The loss of logits [V, T] against a teacher's top logits, mixed with the labels' cross-entropy.
+struct HipDistillation {
+    Tensor* logits = nullptr;   // [V, T] F32, F16 or BF16
+    Tensor* labels = nullptr;   // [T] I32, negative: not counted
+    Tensor* ids = nullptr;      // [top, T] I32: the teacher's tokens, outside 0 .. V-1: left out
+    Tensor* teacher = nullptr;  // [top, T] F32, F16 or BF16: their logits
+    Tensor* stats = nullptr;    // [5, T] F32, written
+    Tensor* loss = nullptr;     // [4] F32, written: the loss, its two parts' means, the rows counted
+    float tau = 2.0f;
+    float alpha = 0.5f;         // the teacher's share
+};
+void hip_distill_loss(const HipDistillation& d);
+// The logits' gradient for the loss's gradient dloss [1]; dlogits may be the logits themselves.
+void hip_distill_loss_back(const HipDistillation& d, const Tensor* dloss, Tensor* dlogits);
+
 // One AdamW step over many tensors in one launch (the reference's AdamW, src/optim/trc_optim.cpp), its moments as floats
 // or in 8 bits. The moments belong to the optimizer and start as zeros; the parameters (F32) and gradients
 // (F32, F16 or BF16) are contiguous, keep their places and outlive it.

@@ -1,6 +1,6 @@
 """Builds the C++ test programs against libtraincpp_hip.so (the backend under test):
 tests/cpp/bin/test_hip_backend, the drop-in test, which is checked by oracle/liboracle.so,
-tests/cpp/bin/test_tuning and tests/cpp/bin/test_tuning_types."""
+tests/cpp/bin/test_tuning, tests/cpp/bin/test_tuning_types and tests/cpp/bin/test_distillation."""
 import subprocess
 import sys
 from pathlib import Path
@@ -28,6 +28,7 @@ def main() -> None:
     build("test_hip_backend", oracle=True)
     build("test_tuning", oracle=False)
     build("test_tuning_types", oracle=False)
+    build("test_distillation", oracle=False)
 
 
 if __name__ == "__main__":

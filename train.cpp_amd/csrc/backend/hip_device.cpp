@@ -780,6 +780,53 @@ void hip_preference_loss_back(const HipPreference& p, const Tensor* dloss, Tenso
     check(trc_hip_preference_loss_back(&l, &y, &s, &e, &sl, &d, p.beta, &dl, nullptr), "hip_preference_loss_back");
 }
 
+HipFp8 hip_fp8_new(Context* ctx, int64_t K, int64_t R, bool weight) {
+    const int64_t blocks = (K + 127) / 128, rows = weight ? (R + 127) / 128 : R;
+    return {view_2d(ctx, new_tensor_2d(ctx, TYPE_I8, blocks * 128, R), K, R, 0),
+            view_2d(ctx, new_tensor_2d(ctx, TYPE_I8, (blocks + 3) / 4 * 4, rows), blocks, rows, 0)};
+}
+
+void hip_fp8_quantize(const Tensor* x, const HipFp8& out) {
+    Operands at("hip_fp8_quantize");
+    const trc_hip_tensor t = at(x);
+    const trc_hip_fp8 o{at(out.q), at(out.scale)};
+    check(trc_hip_fp8_quantize(&t, &o, nullptr), "hip_fp8_quantize");
+}
+
+void hip_fp8_mul_mat(const HipFp8& w, const HipFp8& x, Tensor* y) {
+    Operands at("hip_fp8_mul_mat");
+    const trc_hip_fp8 tw{at(w.q), at(w.scale)}, tx{at(x.q), at(x.scale)};
+    const trc_hip_tensor ty = at(y);
+    check(trc_hip_fp8_mul_mat(&tw, &tx, &ty, nullptr), "hip_fp8_mul_mat");
+}
+
+void hip_fp8_mul_mat_back(const HipFp8& w, const HipFp8& dy, Tensor* dx) {
+    Operands at("hip_fp8_mul_mat_back");
+    const trc_hip_fp8 tw{at(w.q), at(w.scale)}, ty{at(dy.q), at(dy.scale)};
+    const trc_hip_tensor tx = at(dx);
+    check(trc_hip_fp8_mul_mat_back(&tw, &ty, &tx, nullptr), "hip_fp8_mul_mat_back");
+}
+
+void hip_fp8_matvec(const HipFp8& w, const Tensor* x, Tensor* y) {
+    Operands at("hip_fp8_matvec");
+    const trc_hip_fp8 tw{at(w.q), at(w.scale)};
+    const trc_hip_tensor tx = at(x), ty = at(y);
+    check(trc_hip_fp8_matvec(&tw, &tx, &ty, nullptr), "hip_fp8_matvec");
+}
+
+void hip_distill_loss(const HipDistillation& d) {
+    Operands at("hip_distill_loss");
+    const trc_hip_tensor l = at(d.logits), y = at(d.labels), i = at(d.ids), z = at(d.teacher), s = at(d.stats), lo = at(d.loss);
+    check(trc_hip_distill_loss(&l, &y, &i, &z, d.tau, d.alpha, &s, &lo, nullptr), "hip_distill_loss");
+}
+
+void hip_distill_loss_back(const HipDistillation& d, const Tensor* dloss, Tensor* dlogits) {
+    Operands at("hip_distill_loss_back");
+    const trc_hip_tensor l = at(d.logits), y = at(d.labels), i = at(d.ids), z = at(d.teacher), s = at(d.stats), lo = at(d.loss),
+                         g = at(dloss), dl = at(dlogits);
+    check(trc_hip_distill_loss_back(&l, &y, &i, &z, &s, &lo, &g, d.tau, d.alpha, &dl, nullptr), "hip_distill_loss_back");
+}
+
 struct HipAdamW::State {
     std::vector<trc_hip_adamw_tensor> tensors;
     int bits = 32;
