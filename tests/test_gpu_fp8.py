@@ -209,6 +209,29 @@ def test_products(hip, K, M, N, kind, scales, back):
     p.free()
 
 
+@pytest.mark.parametrize("scales", ["pow2", "float"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("K,M,N", [(500, 2000, 600), (300, 4097, 1030), (700, 6000, 400), (130, 4225, 250), (1, 2050, 520)])
+@pytest.mark.parametrize("back", [False, True])
+def test_numbers_of_tiles(hip, K, M, N, kind, scales, back):
+    """From one tile of 64 x 64 a CU to one of 128 x 128, with gaps between rows: whole numbers bit for bit, then others."""
+    if back:
+        K, M = M, K
+    announce(f"fp8 tiles K={K} M={M} N={N} {kind} {scales} back={back}")
+    for whole, (extra, lead, pad) in ((True, (0, 0, 0)), (False, (1, 1, 3))):
+        w, ws, x, xs = problem(K, M, N, scales, K + 2 * M + N, whole=whole)
+        if back:
+            _, _, x, xs = problem(M, 1, N, "pow2", K + N, whole=whole)
+        p = Product(w, ws, x, xs, K, M, kind, back, extra, lead, pad)
+        if whole:
+            p.run()
+            assert np.array_equal(decode(p.read(), kind), encode(p.want()[0], kind)[1])
+        else:
+            check(p, is_fast(p))
+            p.w.q.read(), p.x.q.read()
+        p.free()
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("back", [False, True])
 @pytest.mark.parametrize("N", [3, 40, 80, 300])

@@ -19,7 +19,8 @@ namespace trc_hip {
 F8_DECLARE_ALL(256, 256, 2, 4, 1, 2, true)
 F8_DECLARE_ALL(128, 128, 2, 2, 1, 2, true)
 F8_DECLARE_ALL(128, 128, 2, 2, 1, 2, false)
-F8_DECLARE_ALL(64, 64, 2, 2, 2, 2, true)
+F8_DECLARE_ALL(128, 64, 2, 2, 2, 3, true)
+F8_DECLARE_ALL(128, 64, 2, 2, 2, 3, false)
 F8_DECLARE_ALL(64, 64, 2, 2, 2, 2, false)
 F8_DECLARE_ALL(64, 64, 2, 2, 2, 3, true)
 F8_DECLARE_ALL(64, 64, 2, 2, 2, 3, false)
@@ -72,9 +73,19 @@ int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
     t.steps = (int) (((trans ? a.M : a.K) + F8_BLOCK - 1) / F8_BLOCK);
     const bool fast = a.y_type != TRC_HIP_TYPE_F32 && a.N > TRC_HIP_FP8_MATVEC_MAX_N;
     auto tiles = [&](int64_t edge) { return ((t.rows + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
-    const int edge = fast && tiles(256) >= cus ? 256 : tiles(128) >= cus ? 128 : 64;
+    // Which tiles: 64 x 64 up to one a CU, else 128 x 64 up to one a CU, else 128 x 128 (of exact products 64 x 64 again
+    // while three CUs in four would not have one), and 256 x 256 once those of 128 are more than two a CU. K, M, tokens, us
+    // in tiles of 64, 128 x 64 and 128: exact 4096, 4096, 512 26.2, 24.2, 37.9, 777 45.0, 41.1, 38.1, 1000, 6000, 400 13.6,
+    // 17.2, 14.3; on the 8-bit instruction 22.4, 17.6, 28.6, 38.4, 31.4, 28.4 and 12.8, 15.2, 12.0. In tiles of 128 and 256:
+    // 4096, 4096, 2560 66.5 and 49.2; 4096, 14336, 700 70.2 and 52.0; 1024, 8192, 1400 23.4 and 21.8.
+    const int64_t high = (t.rows + 127) / 128 * ((a.N + 63) / 64);
+    const bool by_128 = tiles(64) > cus && high <= cus;
+    const int edge = tiles(64) <= cus || by_128              ? 64
+                     : fast && tiles(128) > 2 * cus          ? 256
+                     : fast || tiles(128) * 4 >= cus * 3     ? 128
+                                                             : 64;
     if (tiles(edge) > max_groups(512) / 2 - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
-    t.tm = (int) ((t.rows + edge - 1) / edge);
+    t.tm = by_128 ? (int) ((t.rows + 127) / 128) : (int) ((t.rows + edge - 1) / edge);
     t.tn = (int) ((a.N + edge - 1) / edge);
     t.whole = (t.tm * t.tn + 7) / 8;
     const int per_xcd = (int) (cus / 8), last = edge == 256 && per_xcd > 0 ? t.whole % per_xcd : 0;
@@ -107,7 +118,8 @@ int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
     const unsigned p = (unsigned) parts;
     if (edge == 256) launch<256, 256, 2, 4, 1, 2, true>(t, trans, p, s);
     else if (edge == 128) fast ? launch<128, 128, 2, 2, 1, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, 1, 2, false>(t, trans, p, s);
-    else if (t.tm * t.tn > cus) fast ? launch<64, 64, 2, 2, 2, 2, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 2, false>(t, trans, p, s);
+    else if (by_128) fast ? launch<128, 64, 2, 2, 2, 3, true>(t, trans, p, s) : launch<128, 64, 2, 2, 2, 3, false>(t, trans, p, s);
+    else if (t.tm * t.tn > cus) launch<64, 64, 2, 2, 2, 2, false>(t, trans, p, s);
     // (three stages where a CU has one workgroup: four took 2 to 5 % longer at 1 to 64 tokens of K and M from 777 to 14336)
     else fast ? launch<64, 64, 2, 2, 2, 3, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 3, false>(t, trans, p, s);
     const int rc = check_launch("fp8_mul_mat");
