@@ -167,11 +167,6 @@ struct F8Tile {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(wave * 64 < ALINES ? from.a : from.b, (__attribute__((address_space(3))) void*) (lds + STAGES * STAGE), 4,
                                                  touch_off, 0, 0, 0);
     }
-    __device__ __forceinline__ void load(int s, int stage) const {
-        const Source from = source(s, s + 1);
-#pragma unroll
-        for (int p = 0; p < LOADS; ++p) load(from, stage, p);
-    }
     // the weight's scale of a step, by the scalar unit
     __device__ __forceinline__ uint32_t scale(int s, int end) const {
         s = min(s, end - 1);
@@ -236,32 +231,42 @@ struct F8Tile {
 #pragma unroll
                 for (int j = 0; j < JT; ++j) acc[i][j] += sums[(i * JT + j) * THREADS + tid];
         }
+        const int64_t first = row0 + wm * TM;
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
             const int64_t n = n0 + wn * TN + j * 16 + r16;
-            if (n >= a.N) continue;
+            if (t.sums != nullptr || a.y_type == TRC_HIP_TYPE_F32) {
+                if (n >= a.N) continue;
+                float* const p = t.sums != nullptr ? t.sums + ((int64_t) blockIdx.y * a.N + n) * t.sums_nb1 : (float*) (a.y + n * a.y_nb1);
 #pragma unroll
-            for (int i = 0; i < IT; ++i) {
-                const int64_t r = row0 + wm * TM + i * 16 + chunk * 4;
-                if (r >= t.rows) continue;
-                const int left = (int) min((int64_t) 4, t.rows - r);
-                if (t.sums != nullptr || a.y_type == TRC_HIP_TYPE_F32) {
-                    float* const p = t.sums != nullptr ? t.sums + ((int64_t) blockIdx.y * a.N + n) * t.sums_nb1 + r
-                                                       : (float*) (a.y + n * a.y_nb1) + r;
-                    if (left == 4) *(f4a4*) p = acc[i][j];
+                for (int i = 0; i < IT; ++i) {
+                    const int64_t r = first + i * 16 + chunk * 4;
+                    if (r + 4 <= t.rows) *(f4a4*) (p + r) = acc[i][j];
                     else
-                        for (int k = 0; k < left; ++k) p[k] = acc[i][j][k];
-                } else {
-                    uint16_t* const p = (uint16_t*) (a.y + n * a.y_nb1) + r;
-                    uint16_t v[4];
+                        for (int k = 0; r + k < t.rows; ++k) p[r + k] = acc[i][j][k];
+                }
+            } else {
+                // Of two fragments' rows a lane has four each; it changes one four with its neighbour 16 lanes on, and has
+                // eight of one: 64 bytes of a token are stored at once (33 MB took 17 us in pieces of 32 bytes, 9 so).
+                uint16_t* const p = (uint16_t*) (a.y + n * a.y_nb1);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = f8_bits(a.y_type, acc[i][j][k]);
-                    if (left == 4) {
-                        typedef uint32_t u2a2 __attribute__((ext_vector_type(2), aligned(2)));
-                        *(u2a2*) p = (u2a2){(uint32_t) v[0] | (uint32_t) v[1] << 16, (uint32_t) v[2] | (uint32_t) v[3] << 16};
-                    } else {
-                        for (int k = 0; k < left; ++k) p[k] = v[k];
+                for (int i = 0; i < IT; i += 2) {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        auto two = [&](const f4& x) {
+                            return (uint32_t) f8_bits(a.y_type, x[2 * k]) | (uint32_t) f8_bits(a.y_type, x[2 * k + 1]) << 16;
+                        };
+                        const auto s = __builtin_amdgcn_permlane16_swap(two(acc[i][j]), two(acc[i + 1][j]), false, false);
+                        v[k] = s[0];
+                        v[k + 2] = s[1];
                     }
+                    const int64_t r = first + (i + (chunk & 1)) * 16 + (chunk >> 1) * 8;
+                    if (n >= a.N) continue;
+                    typedef uint32_t u4a2 __attribute__((ext_vector_type(4), aligned(2)));
+                    if (r + 8 <= t.rows) *(u4a2*) (p + r) = (u4a2){v[0], v[1], v[2], v[3]};
+                    else
+                        for (int k = 0; r + k < t.rows && k < 8; ++k) p[r + k] = (uint16_t) (v[k / 2] >> (16 * (k & 1)));
                 }
             }
         }
