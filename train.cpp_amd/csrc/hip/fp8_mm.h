@@ -103,6 +103,7 @@ struct F8Tile {
     const uint8_t* x0;
     __amdgpu_buffer_rsrc_t rs;  // the tokens' exponents, a word of four steps of each
     uint32_t e_off, touch_off;
+    int a_bytes, a_last, b_bytes;  // of a step's tiles from their first byte on; of the weight's last step, on the way back
     uint64_t ws;
     int64_t ws_step;
 
@@ -120,6 +121,10 @@ struct F8Tile {
         a_rows = min((int64_t) BM, a.M - row0);
         b_rows = min((int64_t) BN, a.N - n0);
         x0 = a.x + n0 * a.x_nb1;
+        const int64_t width = TRANS ? pitch - row0 : F8_BLOCK;
+        a_bytes = (int) (uint32_t) (((TRANS ? min((int64_t) F8_BLOCK, a.M) : a_rows) - 1) * a.w_nb1 + width);
+        a_last = TRANS ? (int) (uint32_t) ((a.M - 1) % F8_BLOCK * a.w_nb1 + width) : a_bytes;
+        b_bytes = (int) (uint32_t) ((b_rows - 1) * a.x_nb1 + F8_BLOCK);
         rs = __builtin_amdgcn_make_buffer_rsrc((void*) (a.xs + n0 * a.xs_nb1), (short) 0,
                                                (int) ((b_rows - 1) * a.xs_nb1 + (t.steps + 3) / 4 * 4), F8_RSRC);
         e_off = (uint32_t) ((tid % BN) * a.xs_nb1);
@@ -148,10 +153,10 @@ struct F8Tile {
         const bool some = s < end;
         s = min(s, end - 1);
         const uint8_t* const w = TRANS ? g.w + (int64_t) s * F8_BLOCK * g.w_nb1 + row0 : g.w + row0 * g.w_nb1 + (int64_t) s * F8_BLOCK;
-        const int64_t left = TRANS ? min((int64_t) F8_BLOCK, g.M - (int64_t) s * F8_BLOCK) : a_rows, width = TRANS ? pitch - row0 : F8_BLOCK;
-        return {__builtin_amdgcn_make_buffer_rsrc((void*) w, (short) 0, some ? (int) (uint32_t) ((left - 1) * g.w_nb1 + width) : 0, F8_RSRC),
-                __builtin_amdgcn_make_buffer_rsrc((void*) (x0 + (int64_t) s * F8_BLOCK), (short) 0,
-                                                  some ? (int) (uint32_t) ((b_rows - 1) * g.x_nb1 + F8_BLOCK) : 0, F8_RSRC),
+        // (selections, without a branch: it would keep the products before it apart from those behind it)
+        const int bytes = TRANS && s == t.steps - 1 ? a_last : a_bytes;
+        return {__builtin_amdgcn_make_buffer_rsrc((void*) w, (short) 0, some ? bytes : 0, F8_RSRC),
+                __builtin_amdgcn_make_buffer_rsrc((void*) (x0 + (int64_t) s * F8_BLOCK), (short) 0, some ? b_bytes : 0, F8_RSRC),
                 s & ~3};
     }
     // piece p of LOADS on its way to a stage
