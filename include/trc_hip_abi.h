@@ -208,6 +208,7 @@ int trc_hip_qmatvec(int type, const void* wq, int64_t K, int64_t M, size_t nb1_w
  * Call it before hipStreamDestroy; a later call on the stream allocates a new
  * workspace. trc_hip_sum_f32 keeps its row sums in the same workspace, trc_hip_lora
  * and trc_hip_lora_back sums in parts, trc_hip_preference_loss its rows' log-probabilities,
+ * trc_hip_fp8_mul_mat and its kin sums in parts and quantized tokens, trc_hip_distill_loss its rows' terms,
  * and trc_hip_mul_mat_f32 its ticket words past its end.
  * hipStreamPerThread is keyed by the calling thread. Returns TRC_HIP_OK when
  * the stream has no workspace. No counterpart in the reference:
@@ -454,9 +455,10 @@ int trc_hip_fp8_quantize(const trc_hip_tensor* x, const trc_hip_fp8* out, void* 
 
 /* y [M, N] = mul_mat(w, x) of a weight w [K, M] with scales for 128 rows each and activations x [K, N] with scales (I8)
  * for each row. y is F32, F16 or BF16 with nb[0] the element size and rows at any aligned stride, and overlaps
- * neither. An F32 y is summed with exact products in 32 bits. For a y of 16 bits over more than TRC_HIP_FP8_MATVEC_MAX_N
- * tokens the products go through the 8-bit matrix instruction, which adds eight of them with some 13 bits below
- * the largest: off by up to 1e-4 of the sum of magnitudes, a fortieth of what rounding the activations to e4m3 may cost.
+ * neither. The two scales' product is formed in 32 bits. An F32 y, and any y of up to TRC_HIP_FP8_MATVEC_MAX_N tokens, is
+ * summed with exact products in 32 bits. For a y of 16 bits over more tokens the products go through the 8-bit
+ * matrix instruction, which adds eight of them with some 12 bits below the largest: off by up to 1e-4 of the sum of
+ * magnitudes, by 1e-5 on normal data.
  * The same bits from run to run. Products of few tiles keep sums in the stream's workspace of trc_hip_qmatvec, which
  * the first such call on a stream allocates (make it before capturing that stream in global mode). */
 int trc_hip_fp8_mul_mat(const trc_hip_fp8* w, const trc_hip_fp8* x, const trc_hip_tensor* y, void* stream);
@@ -467,7 +469,8 @@ int trc_hip_fp8_mul_mat_back(const trc_hip_fp8* w, const trc_hip_fp8* dy, const 
 
 /* y = mul_mat(w, x) for N <= TRC_HIP_FP8_MATVEC_MAX_N tokens whose activations x [K, N] are still F32, F16 or BF16: they
  * are quantized on the way, as trc_hip_fp8_quantize does it, and y is what trc_hip_fp8_mul_mat makes of that, bit
- * for bit. Beyond 4 tokens what is quantized is held in the stream's workspace (K N up to 8 million). */
+ * for bit. Beyond two tokens, or where their rows' codes take more than 48 KiB, what is quantized is held in the
+ * stream's workspace (8.3 MiB: K N up to 8 million). */
 int trc_hip_fp8_matvec(const trc_hip_fp8* w, const trc_hip_tensor* x, const trc_hip_tensor* y, void* stream);
 
 /* ------------------------------------------------------------------ distillation */
