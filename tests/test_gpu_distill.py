@@ -158,6 +158,28 @@ def test_in_place(hip, V):
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("V,top", [(600, 1024), (40000, 1024), (40000, 300), (70000, 33)])
+def test_many_repeated_entries(hip, kind, V, top):
+    """All of a row's entries one token, pairs, runs, tokens that differ by powers of two, the label among them or not."""
+    announce(f"distill many repeated {kind} V={V} top={top}")
+    for alpha in (1.0, 0.6):
+        p = Problem(kind, V, 9, top, 2.0, alpha, skip=0.0)
+        j = np.arange(top)
+        p.ids[0] = 17
+        p.ids[1] = j // 2 % V
+        p.ids[2] = j % 7
+        p.ids[3] = (j * 256) % V
+        p.ids[4] = np.where(j % 3 == 0, V - 1, j % V)
+        p.ids[5] = np.where(j % 2 == 0, -1, V)
+        p.ids[6] = np.where(j < top - 2, j % V, p.ids[6, 0])
+        p.labels[:7] = [17, 3, 20, 256 % V, V - 1, 5, V // 2]
+        a = p.run()
+        check(p, a)
+        b = p.run(in_place=True)
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
 @pytest.mark.parametrize("V", [500, 50000])
 def test_repeated_and_missing_entries(hip, V):
     """One token several times in a row, ids outside of the vocabulary, rows without any entry."""
