@@ -11,31 +11,24 @@ namespace {
 constexpr int Q_THREADS = 256;
 
 // Rows. A wave takes four blocks of a row: 16 lanes each, 8 elements a lane, and writes their exponents as one word.
-// Bound by memory: 4096 x 4096 of bfloat16 in 12.7 us (50 MB, 4.0 TB/s). UNITS such pieces of a wave are under way together.
-template <int TYPE, int UNITS>
+// Bound by memory: 4096 x 4096 of bfloat16 12 us (4.2 TB/s), 14336 x 8192 65 (5.5). Two or four such pieces a wave, their loads
+// under way together, were slower (13 and 16 us, 71 and 95): fewer waves hide less.
+template <int TYPE>
 __global__ __launch_bounds__(Q_THREADS) void k_f8_rows(const uint8_t* __restrict__ x, size_t x_nb1, int64_t K, int64_t units,
                                                         FastDiv groups, uint8_t* __restrict__ q, size_t q_nb1,
                                                         uint8_t* __restrict__ sc, size_t sc_nb1) {
     const int lane = (int) threadIdx.x & 63;
-    const int64_t u0 = ((int64_t) blockIdx.x * (Q_THREADS / 64) + (threadIdx.x >> 6)) * UNITS;
-    float v[UNITS][8];
-    uint32_t row[UNITS], g[UNITS];
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        const uint32_t unit = (uint32_t) min(u0 + u, units - 1);  // (a piece may be done twice, with the same result)
-        row[u] = div_by(unit, groups);
-        g[u] = unit - row[u] * groups.d;
-        f8_load8<TYPE>(x + row[u] * x_nb1, (int64_t) g[u] * 512 + lane * 8, K, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        const uint32_t e = f8_exponent(f8_max16(f8_amax8(v[u])));
-        const int64_t at = (int64_t) g[u] * 512 + lane * 8;
-        if (at / F8_BLOCK * F8_BLOCK < K) *(u2v*) (q + row[u] * q_nb1 + at) = f8_codes(v[u], f8_inverse(e));
-        const uint32_t word = __builtin_amdgcn_readlane(e, 0) | __builtin_amdgcn_readlane(e, 16) << 8 |
-                              __builtin_amdgcn_readlane(e, 32) << 16 | __builtin_amdgcn_readlane(e, 48) << 24;
-        if (lane == 0) *(uint32_t*) (sc + row[u] * sc_nb1 + 4 * g[u]) = word;
-    }
+    // (the last piece may be done more than once, with the same result)
+    const uint32_t unit = (uint32_t) min((int64_t) blockIdx.x * (Q_THREADS / 64) + (threadIdx.x >> 6), units - 1);
+    const uint32_t row = div_by(unit, groups), g = unit - row * groups.d;
+    const int64_t at = (int64_t) g * 512 + lane * 8;
+    float v[8];
+    f8_load8<TYPE>(x + row * x_nb1, at, K, v);
+    const uint32_t e = f8_exponent(f8_max16(f8_amax8(v)));
+    if (at / F8_BLOCK * F8_BLOCK < K) *(u2v*) (q + row * q_nb1 + at) = f8_codes(v, f8_inverse(e));
+    const uint32_t word = __builtin_amdgcn_readlane(e, 0) | __builtin_amdgcn_readlane(e, 16) << 8 |
+                          __builtin_amdgcn_readlane(e, 32) << 16 | __builtin_amdgcn_readlane(e, 48) << 24;
+    if (lane == 0) *(uint32_t*) (sc + row * sc_nb1 + 4 * g) = word;
 }
 
 // Blocks of 128 x 128: a workgroup holds one in registers.
@@ -278,10 +271,7 @@ __global__ __launch_bounds__(SK_WAVES * 64, 4) void k_f8_skinny(F8Args a) {
 template <int TYPE>
 int rows_of(const trc_hip_tensor& x, const trc_hip_fp8& q, hipStream_t s) {
     const int64_t K = x.ne[0], R = x.ne[1], groups = (K + 4 * F8_BLOCK - 1) / (4 * F8_BLOCK), units = R * groups;
-    // four pieces a wave from 16 waves a SIMD on
-    const int n = units >= (int64_t) device_cus() * 64 * 4 ? 4 : 1;
-    const int64_t per = (Q_THREADS / 64) * n, wgs = (units + per - 1) / per;
-    hipLaunchKernelGGL(n == 4 ? (k_f8_rows<TYPE, 4>) : (k_f8_rows<TYPE, 1>), dim3((unsigned) wgs), dim3(Q_THREADS), 0, s,
+    hipLaunchKernelGGL(k_f8_rows<TYPE>, dim3((unsigned) ((units + Q_THREADS / 64 - 1) / (Q_THREADS / 64))), dim3(Q_THREADS), 0, s,
                        (const uint8_t*) x.data, x.nb[1], K, units, fast_div(groups), (uint8_t*) q.q.data, q.q.nb[1],
                        (uint8_t*) q.scale.data, q.scale.nb[1]);
     return check_launch("fp8_quantize");
