@@ -70,14 +70,15 @@ void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
 
 int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
     // Up to 64 tokens a workgroup with 16 of the weight's rows has all of K, and reads all tokens: its time grows with
-    // K and tokens, and with the rounds of workgroups. Tiles of 64 rows read them less often, but few of them leave the sum
-    // in parts, to be joined; 16 tokens or fewer are worth that only where there is nothing to join. F8_FUSED tokens are
-    // added up as by the kernel that quantizes them itself (K, M, tokens, us so and in tiles: 4096, 4096, 48 10.8 and
-    // 11.2, 64 13.7 and 11.5; 2048, 6000, 32 8.3 and 9.6, 48 10.4 and 9.9, 64 12.8 and 10.2; 4096, 14336, 8 17.0 and 14.2,
-    // 16 19.0 and 14.4; 14336, 4096, 16 15.7 and 16.2, 32 22.0 and 16.8; 8192, 8192, 8 15.9 and 17.5, 16 18.2 and 17.5;
-    // 1000, 777, 64 6.1 and 7.7).
+    // K, with tokens and with the rounds of workgroups. Tiles of 64 rows read the tokens less often; where few of them leave a
+    // long sum in parts, joining those costs some 14 steps. F8_FUSED tokens are added up as by the kernel that quantizes them
+    // itself (K, M, tokens, us so and in tiles; joined: 4096, 4096, 48 10.8 and 10.9, 64 13.7 and 11.4, 14336, 4096, 16 15.8 and
+    // 16.6, 32 22.0 and 16.9, 8192, 8192, 8 15.9 and 17.5, 16 18.2 and 17.7, 32 25.7 and 18.2; not joined: 2048, 2048, 64 8.0 and
+    // 8.7, 1024, 8192, 32 5.8 and 6.1, 48 7.2 and 6.2, 2048, 6000, 32 8.3 and 8.7, 48 10.4 and 8.8, 4096, 14336, 4 16.1 and 14.2,
+    // 16 18.9 and 14.3, 1000, 777, 64 6.1 and 6.2).
     const int64_t cus = device_cus(), n16 = (a.N + 15) / 16 * 16, rounds = ((a.M + 15) / 16 + cus - 1) / cus;
-    const bool many = a.N > F8_FUSED && rounds * a.K * n16 > 240000 && (n16 > 16 || (a.M + 63) / 64 * 2 > cus);
+    const bool joined = (a.M + 63) / 64 * 2 <= cus && a.K > 21 * F8_BLOCK;
+    const bool many = a.N > F8_FUSED && (joined ? n16 > 16 && rounds * a.K * n16 > 240000 : rounds * n16 > 64 || rounds > 3);
     if (!trans && a.N <= TRC_HIP_FP8_MATVEC_MAX_N && !many) return launch_f8_skinny(a, s);
     F8Tiles t{};
     t.a = a;
@@ -102,7 +103,10 @@ int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
     t.whole = (t.tm * t.tn + 7) / 8;
     const int per_xcd = (int) (cus / 8), last = edge == 256 && per_xcd > 0 ? t.whole % per_xcd : 0;
     if (last * 2 <= per_xcd) t.whole -= last;
-    // few tiles: the sum in parts
+    // Few tiles: the sum in parts of 8 steps or more, where each is 14 steps or more short of the whole, which is what joining
+    // them takes (tiles, steps, us whole and in parts, exact: 26, 8 6.0 and 7.5, 16 8.6 and 8.3, 24 11.2 and 9.2, 112 39.7 and 13.8;
+    // 128, 24 11.5 and 11.6, 32 14.3 and 13.1; on the 8-bit instruction 26, 16 7.7 and 8.3, 24 9.5 and 8.7, 128, 24 9.8
+    // and 11.2, 32 12.4 and 12.5).
     int64_t parts = 1;
     size_t used = 0;
     if (edge == 64 && tiles(64) * 2 <= cus) {
@@ -112,15 +116,13 @@ int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
         const size_t room = qm_workspace_bytes();
         const int64_t fit = (int64_t) ((used < room ? room - used : 0) / 4) / (a.N * t.sums_nb1);
         parts = cus / tiles(64);
-        if (parts > (t.steps + 3) / 4) parts = (t.steps + 3) / 4;
+        if (parts > (t.steps + 7) / 8) parts = (t.steps + 7) / 8;
         if (parts > fit) parts = fit;
         if (parts < 1) parts = 1;
     }
-    t.part_steps = t.steps;
-    if (parts > 1) {
-        t.part_steps = (int) (((t.steps + parts - 1) / parts + 3) / 4 * 4);
-        parts = (t.steps + t.part_steps - 1) / t.part_steps;
-    }
+    t.part_steps = (int) (((t.steps + parts - 1) / parts + 3) / 4 * 4);
+    if (t.steps - t.part_steps < 14) t.part_steps = t.steps;
+    parts = (t.steps + t.part_steps - 1) / t.part_steps;
     if (parts > 1) {
         uint8_t* ws = nullptr;
         const int rc = qm_stream_workspace(s, &ws);
