@@ -43,23 +43,6 @@ __device__ __forceinline__ h8v f8_half8(u2v c) {
     }
     return o.all;
 }
-// An operand as four of 16 x 32.
-struct F8Half {
-    h8v part[4];
-    __device__ __forceinline__ explicit F8Half(const F8Frag& f) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) part[q] = f8_half8(f.quarter[q]);
-    }
-};
-
-// 16 x 16 sums over 128 k, from 0, in binary16 with every product exact and sums in 32 bits.
-__device__ __forceinline__ f4 f8_dot(const F8Half& a, const F8Half& b) {
-    f4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.part[q], b.part[q], s, 0, 0, 0);
-    return s;
-}
-
 __device__ __forceinline__ float f8_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
 // A block's exponent byte from its largest finite magnitude: the smallest power of two by which it falls to 448 =
