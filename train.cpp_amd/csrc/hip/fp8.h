@@ -4,8 +4,8 @@
 //
 // A value is code x scale. Activations have a scale for each 128 neighbours of a row, a power
 // of two held as its exponent's byte (127 added); weights one for each 128 x 128, such a byte or a float. A
-// power of two costs an e4m3 value nothing but range (its spacing is relative), makes quantizing exact but
-// for the code's own rounding, and is what the matrix instruction takes as an operand's scale.
+// power of two costs an e4m3 value nothing but range (its spacing is relative), and makes quantizing exact but
+// for the code's own rounding.
 #pragma once
 
 #include "common.h"
@@ -15,7 +15,6 @@ namespace {
 
 constexpr int F8_BLOCK = 128;
 
-typedef int i8v __attribute__((ext_vector_type(8)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
@@ -27,7 +26,6 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 union F8Frag {
     u4v half[2];
     u2v quarter[4];
-    i8v all;
 };
 
 // Eight codes in binary16, which holds every e4m3 value.

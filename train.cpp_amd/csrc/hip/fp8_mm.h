@@ -11,20 +11,17 @@ struct F8Tiles {
     int steps;          // blocks of 128 summed over
     int part_steps;     // of one part of the sum, a multiple of 4 where there are several
     int tm, tn;         // tiles along rows and tokens
-    int whole;          // of an XCD's tiles: those that are not halved
     float* sums;        // several parts: their sums, [part][token][rows]; else null
     int64_t sums_nb1;   // floats from token to token
 };
 
-// FAST: the 8-bit matrix instruction, or binary16 with sums in 32 bits (fp8_mm.hip says when). POW2: the weight's
-// scales are bytes.
-template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool FAST, bool POW2>
+// POW2: the weight's scales are bytes.
+template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool POW2>
 void f8_tiles_launch(const F8Tiles& t, unsigned parts, hipStream_t s);
 
 namespace {
 
 constexpr uint32_t F8_RSRC = 0x00027000;
-constexpr int F8_TOUCHED = 256;  // bytes of LDS for what is loaded only to have it in the L2
 
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef int i2v __attribute__((ext_vector_type(2)));
@@ -37,7 +34,6 @@ typedef __attribute__((address_space(3))) i2v lds_i2v;
 template <bool TURNED, int CH>
 __device__ __forceinline__ int f8_turn(int row) {
     if (!TURNED) return row & 7;
-    if (CH == 16) return (row & 7) | ((row >> 4) & 1) << 3;
     if (CH == 8) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
     return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
 }
@@ -63,7 +59,7 @@ struct F8Slab {
 
 // Waves of a SIMD: a workgroup's, twice where its stages leave room in LDS for another workgroup.
 constexpr int f8_waves(int bm, int bn, int waves, int groups, int stages) {
-    return (waves * groups + 3) / 4 * (groups * (stages * ((bm + bn) * F8_BLOCK + 4 * bn) + F8_TOUCHED) <= 80 * 1024 ? 2 : 1);
+    return (waves * groups + 3) / 4 * (groups * stages * ((bm + bn) * F8_BLOCK + 4 * bn) <= 80 * 1024 ? 2 : 1);
 }
 
 // A wave waits until `n` of its loads from memory at most are under way, and for its accesses to LDS.
@@ -88,10 +84,8 @@ struct F8Tile {
     static_assert(TM <= F8_BLOCK && F8_BLOCK % TM == 0, "a wave's rows share their scales");
     typedef F8Slab<TRANS ? F8_BLOCK : BM, ACH, THREADS, TRANS> ASlab;
     typedef F8Slab<BN, 8, THREADS, false> BSlab;
-    static constexpr int ACROSS = TRANS && BM > 128 ? BM / 128 : 1;  // lines of 128 bytes of a row in the weight's tile
-    static constexpr int ALINES = (TRANS ? F8_BLOCK : BM) * ACROSS;
     static constexpr int STAGE = ASlab::BYTES + BSlab::BYTES + BN * 4, LOADS = ASlab::PIECES + BSlab::PIECES + 1;
-    static constexpr int GROUP = STAGES * STAGE + F8_TOUCHED;  // bytes of LDS
+    static constexpr int GROUP = STAGES * STAGE;  // bytes of LDS
 
     const F8Tiles& t;
     const int tid, kg, lane, wave;  // (tid and wave: within the group)
@@ -102,13 +96,12 @@ struct F8Tile {
     const BSlab slab_b;
     const uint8_t* x0;
     __amdgpu_buffer_rsrc_t rs;  // the tokens' exponents, a word of four steps of each
-    uint32_t e_off, touch_off;
+    uint32_t e_off;
     int a_bytes, a_last, b_bytes;  // of a step's tiles from their first byte on; of the weight's last step, on the way back
     uint64_t ws;
     int64_t ws_step;
 
-    // tile: its number in a grid of tiles over `wide` tokens each, of which this takes BN, `part` times BN on
-    __device__ __forceinline__ F8Tile(const F8Tiles& tiles, uint8_t* shared, int tile, int wide, int part)
+    __device__ __forceinline__ F8Tile(const F8Tiles& tiles, uint8_t* shared, int tile)
         : t(tiles), tid((int) threadIdx.x % THREADS), kg(KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((int) threadIdx.x / THREADS)),
           lane(tid & 63), wave(__builtin_amdgcn_readfirstlane(tid >> 6)), lds((lds_byte*) shared + kg * GROUP), wm(wave % WM),
           wn(wave / WM), r16(lane & 15), chunk(lane >> 4), slab_a(tid, tiles.a.w_nb1), slab_b(tid, tiles.a.x_nb1) {
@@ -116,7 +109,7 @@ struct F8Tile {
         // four tiles of rows by all of the tokens', then the next four: neighbours on an XCD share operands in its L2
         const int in = tile % (4 * t.tn), first = tile / (4 * t.tn) * 4, high = min(4, t.tm - first);
         row0 = (int64_t) (first + in % high) * BM;
-        n0 = (int64_t) (in / high) * wide + part * BN;
+        n0 = (int64_t) (in / high) * BN;
         pitch = (a.K + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK;
         a_rows = min((int64_t) BM, a.M - row0);
         b_rows = min((int64_t) BN, a.N - n0);
@@ -128,16 +121,6 @@ struct F8Tile {
         rs = __builtin_amdgcn_make_buffer_rsrc((void*) (a.xs + n0 * a.xs_nb1), (short) 0,
                                                (int) ((b_rows - 1) * a.xs_nb1 + (t.steps + 3) / 4 * 4), F8_RSRC);
         e_off = (uint32_t) ((tid % BN) * a.xs_nb1);
-        // The lines of a later step that this workgroup brings into the XCD's L2: its share of what it has in common with
-        // its neighbours there.
-        const int sa = min(8, t.tn), sb = min(4, high);
-        touch_off = 0xFFFFFF00u;
-        if (tid < ALINES) {
-            if (tid * sa / ALINES == in / high % sa)
-                touch_off = (uint32_t) (tid / ACROSS * a.w_nb1) + tid % ACROSS * 128;
-        } else if (tid - ALINES < BN) {
-            if ((tid - ALINES) * sb / BN == in % high % sb) touch_off = (uint32_t) ((tid - ALINES) * a.x_nb1);
-        }
         const int64_t rb = min((row0 + wm * TM) / F8_BLOCK, (t.rows - 1) / F8_BLOCK);
         ws = (uint64_t) (a.ws + (TRANS ? rb * (POW2 ? 1 : 4) : rb * a.ws_nb1));
         ws_step = TRANS ? a.ws_nb1 : (POW2 ? 1 : 4);
@@ -167,10 +150,6 @@ struct F8Tile {
         else
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rs, (__attribute__((address_space(3))) void*) (at + ASlab::BYTES + BSlab::BYTES + (wave * 64 % BN) * 4), 4, e_off, from.word, 0, 0);
-    }
-    __device__ __forceinline__ void touch(const Source& from) const {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(wave * 64 < ALINES ? from.a : from.b, (__attribute__((address_space(3))) void*) (lds + STAGES * STAGE), 4,
-                                                 touch_off, 0, 0, 0);
     }
     // the weight's scale of a step, by the scalar unit
     __device__ __forceinline__ uint32_t scale(int s, int end) const {
@@ -280,12 +259,11 @@ struct F8Tile {
 
 // Products in binary16.
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool POW2>
-__device__ __forceinline__ void f8_exact(const F8Tiles& t, uint8_t* shared, int tile, int wide, int part) {
+__device__ __forceinline__ void f8_multiply(const F8Tiles& t, uint8_t* shared, int tile) {
     typedef F8Tile<BM, BN, WM, WN, KG, STAGES, TRANS, POW2> Tile;
     // (pieces from memory at once: all of them in the first two rounds of products)
     constexpr int IT = Tile::IT, JT = Tile::JT, EACH = (Tile::LOADS + 1) / 2;
-    const Tile w(t, shared, tile, wide, part);
-    if (w.n0 >= t.a.N) return;
+    const Tile w(t, shared, tile);
     const int first = (int) blockIdx.y * t.part_steps, s1 = min(first + t.part_steps, t.steps), s0 = first + w.kg;
     const int rounds = (s1 - first + KG - 1) / KG;  // (a step from s1 on is one of zeros)
     f4 acc[IT][JT];
@@ -350,139 +328,26 @@ __device__ __forceinline__ void f8_exact(const F8Tiles& t, uint8_t* shared, int 
     w.store(acc);
 }
 
-// Products on the 8-bit instruction. The barrier comes before a step's last two rows of fragments are
-// multiplied: meanwhile the next step's first two come from LDS, each token's fragment as soon as the last product with the
-// one whose registers it takes is under way. The step after that comes from memory from then on, a piece after every
-// second product: all at once, a wave's products would wait until the loads before them have been taken.
+// An XCD (workgroup b is on XCD b % 8) takes neighbouring tiles.
 template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool POW2>
-__device__ __forceinline__ void f8_fast(const F8Tiles& t, uint8_t* shared, int tile, int wide, int part) {
-    typedef F8Tile<BM, BN, WM, WN, KG, STAGES, TRANS, POW2> Tile;
-    constexpr int IT = Tile::IT, JT = Tile::JT;
-    const Tile w(t, shared, tile, wide, part);
-    if (w.n0 >= t.a.N) return;
-    const int first = (int) blockIdx.y * t.part_steps, s1 = min(first + t.part_steps, t.steps), s0 = first + w.kg;
-    const int rounds = (s1 - first + KG - 1) / KG;  // (a step from s1 on is one of zeros)
-    f4 acc[IT][JT];
-#pragma unroll
-    for (int i = 0; i < IT; ++i)
-#pragma unroll
-        for (int j = 0; j < JT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
-    // pieces loaded between the barrier and the next step, the others' distance there in products
-    constexpr int ROOM = (IT - 2) * JT, EARLY = ROOM < Tile::LOADS - JT ? Tile::LOADS : JT < Tile::LOADS ? JT : Tile::LOADS;
-    constexpr int AHEAD = STAGES + 1;  // steps that the L2 has a line before it is wanted there
-    constexpr int EVERY = ROOM >= 4 * (Tile::LOADS - EARLY) ? 2 : 1;
-    F8Frag token[JT], a[2];
-    uint32_t exps[JT], scale = 0;
-    auto multiply = [&](int i, int j, const F8Frag& f) {
-        if constexpr (POW2) {
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.all, token[j].all, acc[i][j], 0, 0, 0, (int) scale, 0, (int) exps[j]);
-        } else {
-            const f4 zero = {0.f, 0.f, 0.f, 0.f};
-            const f4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.all, token[j].all, zero, 0, 0, 0, 127, 0, (int) exps[j]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(part[k], __builtin_bit_cast(float, scale), acc[i][j][k]);
-        }
-    };
-    if (rounds > 0) {
-#pragma unroll
-        for (int k = 0; k < STAGES - 1; ++k) {
-            const typename Tile::Source from = w.source(s0 + k * KG, s1);
-#pragma unroll
-            for (int p = 0; p < Tile::LOADS; ++p) w.load(from, k, p);
-        }
-        typename Tile::Source from = w.source(s0 + (STAGES - 1) * KG, s1);
-        f8_wait<Tile::LOADS * (STAGES - 2)>();
-        f8_barrier();
-#pragma unroll
-        for (int p = 0; p < EARLY; ++p) w.load(from, STAGES - 1, p);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) a[i] = w.weight(0, i);
-#pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            token[j] = w.token(0, j);
-            exps[j] = w.exponent(s0, 0, j);
-        }
-        scale = w.scale(s0, s1);
-        int stage = 0, s = s0;
-        for (int round = 0; round < rounds; ++round, s += KG) {
-            const int before = stage == 0 ? STAGES - 1 : stage - 1, after = stage == STAGES - 1 ? 0 : stage + 1;
-            // the pieces that were not loaded after the barrier
-            int piece = EARLY;
-#pragma unroll
-            for (int i = 0; i + 2 < IT; i += 2) {
-                const F8Frag b[2] = {w.weight(stage, i + 2), w.weight(stage, i + 3)};
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                    for (int j = 0; j < JT; ++j) {
-                        multiply(i + k, j, a[k]);
-                        if (((k * JT + j) % EVERY) == EVERY - 1 && piece < Tile::LOADS) {
-                            w.load(from, before, piece);
-                            ++piece;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                a[0] = b[0], a[1] = b[1];
-            }
-            // this wave has read all of the step's stage, and its share of the next one has landed
-            w.touch(w.source(s + AHEAD * KG, s1));
-            __builtin_amdgcn_sched_barrier(0);
-            f8_wait<Tile::LOADS * (STAGES - 2) + 1>();
-            f8_barrier();
-            from = w.source(s + STAGES * KG, s1);
-            const int n = s + KG;  // (past the last step what is there is read, and not used)
-            const F8Frag next[2] = {w.weight(after, 0), w.weight(after, 1)};
-            const uint32_t scale_next = w.scale(n, s1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-                multiply(IT - 2, j, a[0]);
-                multiply(IT - 1, j, a[1]);
-                token[j] = w.token(after, j);
-                exps[j] = w.exponent(n, after, j);
-                if (j < EARLY) w.load(from, stage, j);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int p = JT; p < EARLY; ++p) w.load(from, stage, p);
-            stage = after;
-            a[0] = next[0], a[1] = next[1];
-            scale = scale_next;
-        }
-    }
-    w.store(acc);
-}
-
-// An XCD (workgroup b is on XCD b % 8) takes neighbouring tiles: t.whole as they are and the rest, the last round
-// of its CUs where that is half of one or less, in two halves of the tokens by a workgroup each.
-template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool TRANS, bool FAST, bool POW2>
 __global__ __launch_bounds__(WM * WN * KG * 64, f8_waves(BM, BN, WM * WN, KG, STAGES)) void k_f8_tiles(F8Tiles t) {
     __shared__ __attribute__((aligned(128))) uint8_t shared[KG * F8Tile<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>::GROUP];
-    const int per_xcd = (t.tm * t.tn + 7) / 8, at = (int) (blockIdx.x >> 3);
-    const int tile = (int) (blockIdx.x & 7) * per_xcd + (at < t.whole ? at : t.whole + (at - t.whole) / 2);
-    if (tile >= t.tm * t.tn) return;
-    if constexpr (FAST) {
-        if constexpr (BN == 256) {
-            if (at >= t.whole) return f8_fast<BM, BN / 2, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile, BN, (at - t.whole) & 1);
-        }
-        f8_fast<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile, BN, 0);
-    } else {
-        f8_exact<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile, BN, 0);
-    }
+    const int tile = (int) (blockIdx.x & 7) * ((t.tm * t.tn + 7) / 8) + (int) (blockIdx.x >> 3);
+    if (tile < t.tm * t.tn) f8_multiply<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(t, shared, tile);
 }
 
 }  // namespace
 
-#define F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2)                                                         \
+#define F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, TRANS, POW2)                                                                \
     template <>                                                                                                        \
-    void f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s) { \
-        hipLaunchKernelGGL((k_f8_tiles<BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2>),                                    \
-                           dim3((unsigned) (8 * (2 * ((t.tm * t.tn + 7) / 8) - t.whole)), parts), dim3(WM * WN * KG * 64), 0, s, t); \
+    void f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s) {       \
+        hipLaunchKernelGGL((k_f8_tiles<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>),                                          \
+                           dim3((unsigned) (8 * ((t.tm * t.tn + 7) / 8)), parts), dim3(WM * WN * KG * 64), 0, s, t);       \
     }
-#define F8_INSTANCES(BM, BN, WM, WN, KG, STAGES, FAST)          \
-    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, false, FAST, false) \
-    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, false, FAST, true)  \
-    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, true, FAST, false)  \
-    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, true, FAST, true)
+#define F8_INSTANCES(BM, BN, WM, WN, KG, STAGES)          \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, false, false) \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, false, true)  \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, true, false)  \
+    F8_INSTANCE(BM, BN, WM, WN, KG, STAGES, true, true)
 
 }  // namespace trc_hip

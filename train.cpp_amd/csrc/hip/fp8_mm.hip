@@ -4,38 +4,31 @@
 //   y[m,n]  = sum_b ws[m/128,b] 2^e[n,b] sum_{k in block b} w[m,k] x[n,k]
 //   dx[k,n] = sum_b ws[b,k/128] 2^e[n,b] sum_{m in block b} w[m,k] g[n,m]
 //
-// Two ways to multiply. The 8-bit matrix instruction (16 x 16 x 128, which takes powers of two as its operands' scales) adds
-// eight products with some 12 bits below the largest: 1e-5 of a sum's magnitudes on normal data, 1e-4 at most in a search.
-// Results of 16 bits do not show that. Those of 32 bits, and up to 64 tokens all, go through binary16, which holds every
-// code and whose products are exact, with sums in 32 bits: 1e-7 off, at less than half the rate (1.87 PFLOP/s of the
-// instruction alone on normal data, 4.11 in 8 bits, where the clock falls with power: 4.5 to 5 on zeros). A block's sum is scaled in
-// 32 bits: by the instruction where both scales are powers of two, else by a multiply-add.
+// Codes are multiplied in binary16, which holds all of them and whose products are exact, with sums in 32 bits: 1e-7 off. (The
+// 8-bit matrix instructions are twice as fast, or as fast, but add eight products with some 12 bits below the largest:
+// 6e-4 of a sum's magnitudes in a search, which a result of 16 bits shows.) A block's sum is scaled in 32 bits.
 //
 // A weight's scales lie on its rows' blocks both ways, so the way back reads the same bytes, turned on their way from LDS
-// (ds_read_tr8). Bound by the matrix units, power and what does not overlap: 4096 tokens 4096 -> 14336 with bfloat16 results 205 us
-// (2.3 PFLOP/s; the vendor library's product, without scales for blocks, 169 to 190), back 236; F32 results, 2048 tokens
-// 4096 -> 4096, 64 us (1.07 PFLOP/s; the products and the reads from LDS alone took 51).
+// (ds_read_tr8). Bound by the matrix units, power and what does not overlap: 4096 tokens 4096 -> 14336 with bfloat16 results 417 us
+// (1.15 PFLOP/s; the vendor library's large 16-bit products reach 1.24), back 2048 tokens 14336 <- 4096 220 (1.09); F32 results,
+// 2048 tokens 4096 -> 4096, 64 (1.07; the products and the reads from LDS alone took 51).
 #include "fp8_mm.h"
 
 namespace trc_hip {
 
-#define F8_DECLARE(BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2) \
-    template <>                                               \
-    void f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, TRANS, FAST, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
-#define F8_DECLARE_ALL(BM, BN, WM, WN, KG, STAGES, FAST)       \
-    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, false, FAST, false) \
-    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, false, FAST, true)  \
-    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, true, FAST, false)  \
-    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, true, FAST, true)
+#define F8_DECLARE(BM, BN, WM, WN, KG, STAGES, TRANS, POW2) \
+    template <>                                         \
+    void f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, TRANS, POW2>(const F8Tiles& t, unsigned parts, hipStream_t s);
+#define F8_DECLARE_ALL(BM, BN, WM, WN, KG, STAGES)       \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, false, false) \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, false, true)  \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, true, false)  \
+    F8_DECLARE(BM, BN, WM, WN, KG, STAGES, true, true)
 
-F8_DECLARE_ALL(256, 256, 2, 4, 1, 2, true)
-F8_DECLARE_ALL(128, 128, 2, 2, 1, 2, true)
-F8_DECLARE_ALL(128, 128, 2, 2, 1, 2, false)
-F8_DECLARE_ALL(128, 64, 2, 2, 2, 3, true)
-F8_DECLARE_ALL(128, 64, 2, 2, 2, 3, false)
-F8_DECLARE_ALL(64, 64, 2, 2, 2, 2, false)
-F8_DECLARE_ALL(64, 64, 2, 2, 2, 3, true)
-F8_DECLARE_ALL(64, 64, 2, 2, 2, 3, false)
+F8_DECLARE_ALL(128, 128, 2, 2, 1, 2)
+F8_DECLARE_ALL(128, 64, 2, 2, 2, 3)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, 2)
+F8_DECLARE_ALL(64, 64, 2, 2, 2, 3)
 
 namespace {
 
@@ -56,13 +49,12 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_f8_join(const float* __restric
     }
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int STAGES, bool FAST>
+template <int BM, int BN, int WM, int WN, int KG, int STAGES>
 void launch(const F8Tiles& t, bool trans, unsigned parts, hipStream_t s) {
     const bool pow2 = !t.a.ws_float;
-    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, true, FAST, true>
-                                  : f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, true, FAST, false>)
-                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, false, FAST, true>
-                                  : f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, false, FAST, false>);
+    auto* const f = trans ? (pow2 ? f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, true, true> : f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, true, false>)
+                          : (pow2 ? f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, false, true>
+                                  : f8_tiles_launch<BM, BN, WM, WN, KG, STAGES, false, false>);
     f(t, parts, s);
 }
 
@@ -84,29 +76,19 @@ int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
     t.a = a;
     t.rows = trans ? a.K : a.M;
     t.steps = (int) (((trans ? a.M : a.K) + F8_BLOCK - 1) / F8_BLOCK);
-    const bool fast = a.y_type != TRC_HIP_TYPE_F32 && a.N > TRC_HIP_FP8_MATVEC_MAX_N;
     auto tiles = [&](int64_t edge) { return ((t.rows + edge - 1) / edge) * ((a.N + edge - 1) / edge); };
-    // Which tiles: 64 x 64 up to one a CU, else 128 x 64 up to one a CU, else 128 x 128 (of exact products 64 x 64 again
-    // while three CUs in four would not have one), and 256 x 256 once those of 128 are more than two a CU. K, M, tokens, us
-    // in tiles of 64, 128 x 64 and 128: exact 4096, 4096, 512 26.2, 24.2, 37.9, 777 45.0, 41.1, 38.1, 1000, 6000, 400 13.6,
-    // 17.2, 14.3; on the 8-bit instruction 22.4, 17.6, 28.6, 38.4, 31.4, 28.4 and 12.8, 15.2, 12.0. In tiles of 128 and 256:
-    // 4096, 4096, 2560 66.5 and 49.2; 4096, 14336, 700 70.2 and 52.0; 1024, 8192, 1400 23.4 and 21.8.
+    // Which tiles: 64 x 64 up to one a CU, else 128 x 64 up to one a CU, else 128 x 128, but 64 x 64 again while three CUs
+    // in four would not have one of those (K, M, tokens, us in tiles of 64, 128 x 64 and 128: 4096, 4096, 512 26.2, 24.2, 37.9,
+    // 777 45.0, 41.1, 38.1, 1000, 6000, 400 13.6, 17.2, 14.3).
     const int64_t high = (t.rows + 127) / 128 * ((a.N + 63) / 64);
     const bool by_128 = tiles(64) > cus && high <= cus;
-    const int edge = tiles(64) <= cus || by_128              ? 64
-                     : fast && tiles(128) > 2 * cus          ? 256
-                     : fast || tiles(128) * 4 >= cus * 3     ? 128
-                                                             : 64;
-    if (tiles(edge) > max_groups(512) / 2 - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
+    const int edge = tiles(64) <= cus || by_128 || tiles(128) * 4 < cus * 3 ? 64 : 128;
+    if (tiles(edge) > max_groups(512) - 8) return fail(TRC_HIP_E_SHAPE, "trc_hip_fp8_mul_mat: %lld tiles", (long long) tiles(edge));
     t.tm = by_128 ? (int) ((t.rows + 127) / 128) : (int) ((t.rows + edge - 1) / edge);
     t.tn = (int) ((a.N + edge - 1) / edge);
-    t.whole = (t.tm * t.tn + 7) / 8;
-    const int per_xcd = (int) (cus / 8), last = edge == 256 && per_xcd > 0 ? t.whole % per_xcd : 0;
-    if (last * 2 <= per_xcd) t.whole -= last;
     // Few tiles: the sum in parts of 8 steps or more, where each is 14 steps or more short of the whole, which is what joining
-    // them takes (tiles, steps, us whole and in parts, exact: 26, 8 6.0 and 7.5, 16 8.6 and 8.3, 24 11.2 and 9.2, 112 39.7 and 13.8;
-    // 128, 24 11.5 and 11.6, 32 14.3 and 13.1; on the 8-bit instruction 26, 16 7.7 and 8.3, 24 9.5 and 8.7, 128, 24 9.8
-    // and 11.2, 32 12.4 and 12.5).
+    // them takes (tiles, steps, us whole and in parts: 26, 8 6.0 and 7.5, 16 8.6 and 8.3, 24 11.2 and 9.2, 112 39.7 and 13.8;
+    // 128, 24 11.5 and 11.6, 32 14.3 and 13.1).
     int64_t parts = 1;
     size_t used = 0;
     if (edge == 64 && tiles(64) * 2 <= cus) {
@@ -130,12 +112,11 @@ int launch_f8_product(const F8Args& a, bool trans, hipStream_t s) {
         t.sums = (float*) (ws + used);
     }
     const unsigned p = (unsigned) parts;
-    if (edge == 256) launch<256, 256, 2, 4, 1, 2, true>(t, trans, p, s);
-    else if (edge == 128) fast ? launch<128, 128, 2, 2, 1, 2, true>(t, trans, p, s) : launch<128, 128, 2, 2, 1, 2, false>(t, trans, p, s);
-    else if (by_128) fast ? launch<128, 64, 2, 2, 2, 3, true>(t, trans, p, s) : launch<128, 64, 2, 2, 2, 3, false>(t, trans, p, s);
-    else if (t.tm * t.tn > cus) launch<64, 64, 2, 2, 2, 2, false>(t, trans, p, s);
+    if (edge == 128) launch<128, 128, 2, 2, 1, 2>(t, trans, p, s);
+    else if (by_128) launch<128, 64, 2, 2, 2, 3>(t, trans, p, s);
+    else if (t.tm * t.tn > cus) launch<64, 64, 2, 2, 2, 2>(t, trans, p, s);
     // (three stages where a CU has one workgroup: four took 2 to 5 % longer at 1 to 64 tokens of K and M from 777 to 14336)
-    else fast ? launch<64, 64, 2, 2, 2, 3, true>(t, trans, p, s) : launch<64, 64, 2, 2, 2, 3, false>(t, trans, p, s);
+    else launch<64, 64, 2, 2, 2, 3>(t, trans, p, s);
     const int rc = check_launch("fp8_mul_mat");
     if (rc != TRC_HIP_OK || parts == 1) return rc;
     const int64_t quads = t.sums_nb1 / 4;

@@ -2,6 +2,5 @@
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(128, 128, 2, 2, 1, 2, true)
-F8_INSTANCES(128, 128, 2, 2, 1, 2, false)
+F8_INSTANCES(128, 128, 2, 2, 1, 2)
 }  // namespace trc_hip

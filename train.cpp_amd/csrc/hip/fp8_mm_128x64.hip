@@ -2,6 +2,5 @@
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(128, 64, 2, 2, 2, 3, true)
-F8_INSTANCES(128, 64, 2, 2, 2, 3, false)
+F8_INSTANCES(128, 64, 2, 2, 2, 3)
 }  // namespace trc_hip

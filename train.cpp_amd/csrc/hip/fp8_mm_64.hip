@@ -2,7 +2,6 @@
 #include "fp8_mm.h"
 
 namespace trc_hip {
-F8_INSTANCES(64, 64, 2, 2, 2, 2, false)
-F8_INSTANCES(64, 64, 2, 2, 2, 3, true)
-F8_INSTANCES(64, 64, 2, 2, 2, 3, false)
+F8_INSTANCES(64, 64, 2, 2, 2, 2)
+F8_INSTANCES(64, 64, 2, 2, 2, 3)
 }  // namespace trc_hip
