@@ -18,16 +18,18 @@ def fill_room(b, used, value):
     b.dev.buf.upload(raw)
 
 
-# blocks summed over: 1, 5, 17 (two groups of waves share an odd number of steps), and numbers that divide by 4; tiles of
-# 64 x 64, one a CU and more (700 x 2600 and 900 x 1000), and of 128 x 64 (4300 x 600)
-@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+# Numbers of blocks summed over that two groups of waves share unevenly (1, 3, 5, 17) and evenly (4, 32); a few tokens, tiles of
+# 64 x 64 in parts, one a CU and more of them, and of 128 x 64.
+CASES = [(rows, N, summed, kind) for rows, N in ((190, 3), (190, 70), (300, 333)) for summed in (100, 300, 512, 2050)
+         for kind in ("f32", "f16")]
+CASES += [(190, 70, 640, "bf16"), (190, 70, 4096, "f32"), (4300, 600, 300, "bf16"), (4300, 600, 2050, "f32"), (900, 1000, 640, "f32"),
+          (700, 2600, 300, "f32")]
+
+
 @pytest.mark.parametrize("scales", ["pow2", "float"])
-@pytest.mark.parametrize("summed", [100, 300, 512, 640, 2050, 2176])
-@pytest.mark.parametrize("rows,N", [(190, 3), (190, 70), (300, 333), (4300, 600), (900, 1000), (700, 2600)])
+@pytest.mark.parametrize("rows,N,summed,kind", CASES)
 @pytest.mark.parametrize("back", [False, True])
 def test_bytes_behind_the_scales(hip, rows, N, summed, scales, kind, back):
-    if N > 1000 and kind != "f32":
-        pytest.skip("one type is enough for the largest")
     announce(f"fp8 room rows={rows} N={N} summed={summed} {scales} {kind} back={back}")
     K, M = (rows, summed) if back else (summed, rows)
     w, ws, x, xs = problem(K, M, N, scales, summed + rows)

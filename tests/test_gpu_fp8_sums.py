@@ -16,7 +16,7 @@ from tuning_util import decode, encode
 pytestmark = pytest.mark.gpu
 
 # tiles of 64 x 64, the same in parts, of 128 x 64 and 128 x 128; rows and tokens that fill none; K, M, N
-SHAPES = [(32, 70, 65), (128, 200, 100), (2050, 199, 333), (4096, 130, 65), (4096, 4096, 512), (1000, 4300, 600), (1024, 4096, 1100)]
+SHAPES = [(32, 70, 65), (128, 200, 100), (2050, 199, 333), (4096, 130, 65), (640, 4096, 512), (300, 4300, 600), (640, 4096, 1100)]
 
 
 def spiky(rng, rows, cols):

@@ -185,7 +185,10 @@ struct F8Tile {
     __device__ __forceinline__ F8Frag token(int stage, int j) const {
         return rows_of(lds + stage * STAGE + ASlab::BYTES, wn * TN + j * 16 + r16);
     }
-    __device__ __forceinline__ uint32_t exponent(int s, int stage, int j) const {
+    // (of a step of zeros from `end` on the last step's: what lies behind a row's exponents may be anything, and 0 times the
+    // infinity or NaN that it stands for would be NaN)
+    __device__ __forceinline__ uint32_t exponent(int s, int end, int stage, int j) const {
+        s = min(s, end - 1);
         const lds_byte* const p = lds + stage * STAGE + ASlab::BYTES + BSlab::BYTES;
         return ((const __attribute__((address_space(3))) uint32_t*) p)[wn * TN + j * 16 + r16] >> (8 * (s & 3)) & 255u;
     }
@@ -306,7 +309,7 @@ __device__ __forceinline__ void f8_multiply(const F8Tiles& t, uint8_t* shared, i
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
             h8v next[4];
-            scale[j & 1] = f8_scale(w.exponent(s, stage, j)) * wscale;
+            scale[j & 1] = f8_scale(w.exponent(s, s1, stage, j)) * wscale;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
