@@ -488,7 +488,7 @@ int trc_hip_fp8_matvec(const trc_hip_fp8* w, const trc_hip_tensor* x, const trc_
  * KL is not. tau > 0, alpha in 0 .. 1. stats [5, T] F32 contiguous is what trc_hip_distill_loss_back needs: the row's
  * largest logit, one over its sums of exponentials from there at 1 and at tau, the teacher's largest and one over its sum.
  * Sums of a row are in 32 bits from its maximum, their logarithms and all sums over rows in 64, in a fixed order. A label of V or
- * more, where alpha < 1, makes the loss NaN. At most 2^19 rows of 2^30 logits; rows' terms are in the stream's workspace
+ * more, where alpha < 1, makes the loss NaN, and its row's gradient. At most 2^19 rows of 2^30 logits; rows' terms are in the stream's workspace
  * (see trc_hip_lora). */
 int trc_hip_distill_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
                          const trc_hip_tensor* teacher, float tau, float alpha, const trc_hip_tensor* stats,

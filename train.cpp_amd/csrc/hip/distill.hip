@@ -389,7 +389,8 @@ __global__ __launch_bounds__(DI_THREADS) void k_distill_back(const uint8_t* logi
     }
     const float* const st = stats + row * DI_STATS;
     const float m = st[0], unit = dloss[0] / loss[3];
-    const float wk = alpha > 0.f && st[4] != 0.f ? unit * alpha * tau : 0.f, wc = alpha < 1.f ? unit * (1.f - alpha) : 0.f;
+    const float wk = alpha > 0.f && st[4] != 0.f ? unit * alpha * tau : 0.f;
+    const float wc = alpha < 1.f ? (y < V ? unit * (1.f - alpha) : NAN) : 0.f;  // (a label past the vocabulary: NaN, as the loss is)
     // factors on the exponentials of `both`
     const float qb = wk * st[2], qa = wc != 0.f ? wc * st[1] : 0.f;
     const int top = wk != 0.f ? teacher.top : 0;
