@@ -841,7 +841,8 @@ int check_distill(const char* who, const trc_hip_tensor* logits, const trc_hip_t
         return fail(TRC_HIP_E_SHAPE, "%s: V = %lld, T = %lld, %lld entries (at most %d)", who, (long long) V, (long long) T,
                     (long long) top, TRC_HIP_DISTILL_MAX_TOP);
     }
-    if (!(tau > 0.f) || !(1.f / tau > 0.f) || !(1.f / tau < INFINITY)) return fail(TRC_HIP_E_INVALID, "%s: tau = %g", who, tau);
+    // (the kernels take log2 e / tau as a factor)
+    if (!(tau > 0.f) || !(1.f / tau > 0.f) || !(1.44269504f / tau < INFINITY)) return fail(TRC_HIP_E_INVALID, "%s: tau = %g", who, tau);
     if (!(alpha >= 0.f && alpha <= 1.f)) return fail(TRC_HIP_E_INVALID, "%s: alpha = %g is not in 0 .. 1", who, alpha);
     TRC_TRY(check_shape(who, "logits", logits, logits->type, V, T, 1, false));
     TRC_TRY(check_shape(who, "labels", labels, TRC_HIP_TYPE_I32, T, 1, 1, false));
