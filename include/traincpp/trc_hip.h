@@ -92,8 +92,8 @@ struct HipFp8 {
     Tensor* q = nullptr;      // [K, R] I8, a view of rows with room for whole blocks
     Tensor* scale = nullptr;  // I8 (powers of two): of each row, or of 128 rows each (also F32)
 };
-// Tensors for R rows of K, without memory yet: a weight's (scales for 128 rows each) or activations'.
-HipFp8 hip_fp8_new(Context* ctx, int64_t K, int64_t R, bool weight);
+// Tensors for R rows of K, without memory yet: a weight's (scales for 128 rows each, of type I8 or F32) or activations' (I8).
+HipFp8 hip_fp8_new(Context* ctx, int64_t K, int64_t R, bool weight, Type scales = TYPE_I8);
 void   hip_fp8_quantize(const Tensor* x, const HipFp8& out);
 // y = mul_mat(w, x); dx = W^T dy.
 void   hip_fp8_mul_mat(const HipFp8& w, const HipFp8& x, Tensor* y);

@@ -1,6 +1,6 @@
 """Builds the C++ test programs against libtraincpp_hip.so (the backend under test):
 tests/cpp/bin/test_hip_backend, the drop-in test, which is checked by oracle/liboracle.so,
-tests/cpp/bin/test_tuning, tests/cpp/bin/test_tuning_types and tests/cpp/bin/test_distillation."""
+tests/cpp/bin/test_tuning, tests/cpp/bin/test_tuning_types, tests/cpp/bin/test_distillation and tests/cpp/bin/test_fp8_scales."""
 import subprocess
 import sys
 from pathlib import Path
@@ -29,6 +29,7 @@ def main() -> None:
     build("test_tuning", oracle=False)
     build("test_tuning_types", oracle=False)
     build("test_distillation", oracle=False)
+    build("test_fp8_scales", oracle=False)
 
 
 if __name__ == "__main__":

@@ -780,10 +780,15 @@ void hip_preference_loss_back(const HipPreference& p, const Tensor* dloss, Tenso
     check(trc_hip_preference_loss_back(&l, &y, &s, &e, &sl, &d, p.beta, &dl, nullptr), "hip_preference_loss_back");
 }
 
-HipFp8 hip_fp8_new(Context* ctx, int64_t K, int64_t R, bool weight) {
+HipFp8 hip_fp8_new(Context* ctx, int64_t K, int64_t R, bool weight, Type scales) {
+    if (scales != TYPE_I8 && !(weight && scales == TYPE_F32)) {
+        std::fprintf(stderr, "[traincpp-hip][FATAL] hip_fp8_new: scales of type %d (I8, or F32 of a weight)\n", (int) scales);
+        std::abort();
+    }
     const int64_t blocks = (K + 127) / 128, rows = weight ? (R + 127) / 128 : R;
     return {view_2d(ctx, new_tensor_2d(ctx, TYPE_I8, blocks * 128, R), K, R, 0),
-            view_2d(ctx, new_tensor_2d(ctx, TYPE_I8, (blocks + 3) / 4 * 4, rows), blocks, rows, 0)};
+            scales == TYPE_F32 ? new_tensor_2d(ctx, TYPE_F32, blocks, rows)
+                               : view_2d(ctx, new_tensor_2d(ctx, TYPE_I8, (blocks + 3) / 4 * 4, rows), blocks, rows, 0)};
 }
 
 void hip_fp8_quantize(const Tensor* x, const HipFp8& out) {
