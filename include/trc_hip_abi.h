@@ -485,11 +485,12 @@ int trc_hip_fp8_matvec(const trc_hip_fp8* w, const trc_hip_tensor* x, const trc_
  *   loss[0] = mean_t alpha tau^2 KL_t + (1 - alpha) CE_t   over the n rows that are counted
  * and loss [4] F32 holds that, the means of KL and CE, and n; of no rows all are 0. A row without entries has a KL of 0
  * and no gradient of it. With alpha = 1 CE is not computed (0) and labels count only by their sign; with alpha = 0
- * KL is not. tau > 0, alpha in 0 .. 1. stats [5, T] F32 contiguous is what trc_hip_distill_loss_back needs: the row's
- * largest logit, one over its sums of exponentials from there at 1 and at tau, the teacher's largest and one over its sum.
- * Sums of a row are in 32 bits from its maximum, their logarithms and all sums over rows in 64, in a fixed order. A label of V or
- * more, where alpha < 1, makes the loss NaN, and its row's gradient. At most 2^19 rows of 2^30 logits; rows' terms are in the stream's workspace
- * (see trc_hip_lora). */
+ * KL is not. tau > 0 (finite, 4.3e-39 at least), alpha in 0 .. 1. stats [5, T] F32 contiguous is what
+ * trc_hip_distill_loss_back needs: a point near the row's largest logit (the largest of some of them), one over its sums
+ * of exponentials from there at 1 and at tau, the teacher's largest and one over its sum.
+ * Sums of a row are in 32 bits, their logarithms and all sums over rows in 64, in a fixed order. A label of V or more, where
+ * alpha < 1, makes the loss NaN, and its row's gradient. At most 2^19 rows of 2^30 logits; rows' terms are in the
+ * stream's workspace (see trc_hip_lora). */
 int trc_hip_distill_loss(const trc_hip_tensor* logits, const trc_hip_tensor* labels, const trc_hip_tensor* ids,
                          const trc_hip_tensor* teacher, float tau, float alpha, const trc_hip_tensor* stats,
                          const trc_hip_tensor* loss, void* stream);

@@ -30,7 +30,8 @@ constexpr float LOG2E = 1.44269504088896340736f;
 // is 2 and the one is the other's square.
 constexpr int DI_ONE = 0, DI_BOTH = 1, DI_SQUARE = 2;
 
-// A maximum and the sums from it, at temperature 1 (or the only one) and at tau.
+// A point m near the largest of what is summed (its maximum, or the largest of some of it) and the sums of exponentials from
+// there, at temperature 1 (or the only one) and at tau.
 struct Sums {
     float m, a, b;
 };
@@ -173,7 +174,7 @@ struct Term {
 };
 
 // What a row's terms need of its entries and its label: with e_j = exp((z_j - zmax) / tau) and the student's logits taken from
-// `ref`, the largest of what was summed beside them: sum e (0: no entries), sum e (z_j - zmax) / tau, sum e (l_j - ref), l_label - ref.
+// `ref`, the point m of what was summed beside them: sum e (0: no entries), sum e (z_j - zmax) / tau, sum e (l_j - ref), l_label - ref.
 struct Entries {
     double e, ez, el, label;
     float ref, zmax;

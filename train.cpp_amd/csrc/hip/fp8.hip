@@ -62,11 +62,11 @@ __global__ __launch_bounds__(Q_THREADS) void k_f8_blocks(const uint8_t* __restri
 }
 
 constexpr int SK_WAVES = 16;            // most of a workgroup
-constexpr int SK_LDS = 48 * 1024;       // most bytes that it keeps of them (three workgroups fit a CU)
+constexpr int SK_LDS = 48 * 1024;       // most bytes of tokens that it holds (with its waves' sums two workgroups fit a CU)
 constexpr uint32_t SK_RSRC = 0x00027000;
 
-// The weight's rows of a workgroup, 16 at a time (every gridDim.x-th 16), as its waves read them: groups of four blocks of K in
-// turn, from memory to registers.
+// The 16 rows of the weight that a workgroup takes, as its waves read them: groups of four blocks of K in turn, from memory to
+// registers.
 struct SkWeight {
     const F8Args& a;
     const int lane, wave, waves;
@@ -140,8 +140,6 @@ __device__ __forceinline__ void sk_store(const SkWeight& w, int64_t tile, const 
         if (w.a.y_type == TRC_HIP_TYPE_F32) ((float*) y)[r] = s;
         else ((uint16_t*) y)[r] = f8_bits(w.a.y_type, s);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
 }
 
 // N tokens, up to F8_FUSED, whose activations are still floats (of type XTYPE): every wave first quantizes what it will
