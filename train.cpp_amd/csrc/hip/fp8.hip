@@ -11,8 +11,8 @@ namespace {
 constexpr int Q_THREADS = 256;
 
 // Rows. A wave takes four blocks of a row: 16 lanes each, 8 elements a lane, and writes their exponents as one word.
-// Bound by memory: 4096 x 4096 of bfloat16 12 us (4.2 TB/s), 14336 x 8192 65 (5.5). Two or four such pieces a wave, their loads
-// under way together, were slower (13 and 16 us, 71 and 95): fewer waves hide less.
+// Bound by memory: 4096 x 4096 of bfloat16 10 us (4.9 TB/s), 14336 x 8192 64 (5.5). Two or four such pieces a wave, their loads
+// under way together, were slower (13 and 16 us where one took 12, 71 and 95 where it took 65): fewer waves hide less.
 template <int TYPE>
 __global__ __launch_bounds__(Q_THREADS) void k_f8_rows(const uint8_t* __restrict__ x, size_t x_nb1, int64_t K, int64_t units,
                                                         FastDiv groups, uint8_t* __restrict__ q, size_t q_nb1,
@@ -31,7 +31,9 @@ __global__ __launch_bounds__(Q_THREADS) void k_f8_rows(const uint8_t* __restrict
     if (lane == 0) *(uint32_t*) (sc + row * sc_nb1 + 4 * g) = word;
 }
 
-// Blocks of 128 x 128: a workgroup holds one in registers.
+// Blocks of 128 x 128: a workgroup holds one in registers, so that the matrix is read once; one a workgroup keeps every CU
+// busy from 4 M elements on. Bound by memory: 4096 x 4096 of bfloat16 11 us (4.6 TB/s), 14336 x 8192 70 (5.0), of floats 102 (5.7);
+// smaller ones have few workgroups (1999 x 2050: 272, 7.6 us where rows take 4.7).
 template <int TYPE>
 __global__ __launch_bounds__(Q_THREADS) void k_f8_blocks(const uint8_t* __restrict__ x, size_t x_nb1, int64_t K, int64_t R,
                                                           uint32_t kb, uint8_t* __restrict__ q, size_t q_nb1,

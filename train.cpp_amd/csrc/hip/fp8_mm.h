@@ -234,7 +234,7 @@ struct F8Tile {
                 }
             } else {
                 // Of two fragments' rows a lane has four each; it changes one four with its neighbour 16 lanes on, and has
-                // eight of one: 64 bytes of a token are stored at once (33 MB took 17 us in pieces of 32 bytes, 9 so).
+                // eight of one: 64 bytes of a token are stored at once (from larger tiles 33 MB took 17 us in pieces of 32 bytes, 9 so).
                 uint16_t* const p = (uint16_t*) (a.y + n * a.y_nb1);
 #pragma unroll
                 for (int i = 0; i < IT; i += 2) {

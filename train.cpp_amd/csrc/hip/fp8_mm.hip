@@ -10,8 +10,9 @@
 //
 // A weight's scales lie on its rows' blocks both ways, so the way back reads the same bytes, turned on their way from LDS
 // (ds_read_tr8). Bound by the matrix units, power and what does not overlap: 4096 tokens 4096 -> 14336 with bfloat16 results 417 us
-// (1.15 PFLOP/s; the vendor library's large 16-bit products reach 1.24), back 2048 tokens 14336 <- 4096 220 (1.09); F32 results,
-// 2048 tokens 4096 -> 4096, 64 (1.07; the products and the reads from LDS alone took 51).
+// (1.15 PFLOP/s; 437 at least and 470 in the median under the profiler, where the clock falls; the vendor library's bfloat16
+// product of that size 390 to 405, 1.38 PFLOP/s at 8192 x 8192 x 8192), back 2048 tokens 14336 <- 4096 218 (1.10); F32 results, 2048
+// tokens 4096 -> 4096, 65 (1.06; 70 under the profiler; the products and the reads from LDS alone took 51).
 #include "fp8_mm.h"
 
 namespace trc_hip {
